@@ -328,6 +328,118 @@ int swq_attention_token(const swq_attention_layer *layer, const swq_qlinear *pro
                         float norm_eps, void *cache, size_t cache_bytes, int64_t position, float *scratch,
                         size_t scratch_floats, float *out, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- attention over a KV cache held in 4 bits ---------------------------- */
+
+/* A cache of `sequences` sequences in one device buffer, 256-byte aligned and
+ * of at least swq_q4_cache_bytes bytes.  R = max_positions rounded up to 32;
+ * three parts, each at a 256-byte boundary:
+ *   k codes  uint32 [sequences][KVH][R][hd / 8]: word j of a row holds its
+ *            dims 8 j .. 8 j + 7, lowest bits first;
+ *   v codes  uint32 [sequences][KVH][R / 8][hd]: word d of a block holds dim d
+ *            of rows 8 i .. 8 i + 7, lowest bits first (the matrix cores'
+ *            operand order, so that the reader transposes nothing);
+ *   params   f16 [sequences][KVH][4][hd / 64][R]: k scale, k bias, v scale and
+ *            v bias of each 64 dims of a row.
+ * A row's value is scale * code + bias: hd + hd / 8 bytes per row and kv head,
+ * k and v together, against 8 hd of swq_attention_step's f32 cache.
+ * What rows that were never written hold is not read as a value. */
+typedef struct swq_q4_cache {
+    void *data;             /* device */
+    size_t bytes;
+    int32_t sequences;
+    int32_t num_kv_heads;
+    int32_t head_dim;       /* 64, 128 or 256 */
+    int32_t max_positions;  /* rows of one sequence */
+} swq_q4_cache;
+
+/* 0 on bad input. */
+size_t swq_q4_cache_bytes(int sequences, int num_kv_heads, int head_dim, int max_positions);
+
+/* The tokens of one call, sequence after sequence: sequence b of the cache
+ * brings T_b tokens, the first of them for row rows[b].  A sequence may bring
+ * none.  Arrays on the device are read by the kernels, so the same call may be
+ * captured and replayed as they change. */
+typedef struct swq_q4_batch {
+    int32_t sequences;        /* at most the cache's                          */
+    int32_t tokens;           /* of all sequences together                    */
+    int32_t max_tokens;       /* no sequence brings more; starts NULL: not read */
+    int32_t max_rows;         /* rows that a sequence has after the call, about:
+                                 sets how the work is split, not what is read;
+                                 0: the cache's max_positions                 */
+    const int32_t *starts;    /* device [sequences + 1]: T_b = starts[b + 1] -
+                                 starts[b]; NULL: tokens / sequences each     */
+    const int32_t *rows;      /* device [sequences]: rows before this call    */
+    const int32_t *positions; /* device [sequences]: rotary position of each
+                                 sequence's first token (after rows were
+                                 evicted it is larger than the row); NULL: rows */
+    const float *rope;        /* device [rope_positions][rotary_dims / 2][2]:
+                                 cos and sin; swq_q4_rope_table gives
+                                 swq_attention_step's.  NULL if rotary_dims 0 */
+    int32_t rope_positions;   /* positions past the table take its last entry */
+    int32_t reserved;         /* must be 0                                    */
+} swq_q4_batch;
+
+/* Host: cos and sin of positions first .. first + count - 1 into
+ * out [count][rotary_dims / 2][2], the values that swq_attention_step turns by. */
+int swq_q4_rope_table(int rotary_dims, float rope_theta, int64_t first, int count, float *out);
+
+/* The tokens' k and v [tokens][KVH * hd] of dtype (SWQ_F32 / SWQ_BF16) into
+ * the cache: k RMS-normalised with layer->k_norm_weight and rotated as in
+ * swq_attention_step, v as it is, both clamped to +-65504 with NaN as 0 (the
+ * cache holds finite values only).  Per 64 dims bias = f16(min) and scale =
+ * f16((max - min) / 15), each rounded to f32 first; code = (x - bias) / scale
+ * rounded to nearest even, 0 .. 15.  All in 64 bits up to these roundings, so
+ * that a value next to a border falls to the same side everywhere.  Rows from
+ * max_positions on are not written.  layer->max_positions is not read. */
+int swq_q4_append(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
+                  const void *k_proj, const void *v_proj, int dtype, void *stream);
+
+/* Workspace bytes of swq_attention_q4 for calls of up to batch->tokens tokens,
+ * batch->max_tokens per sequence and any rows; weights: whether they are asked
+ * for.  Only the sizes of batch are read.  0 on bad input. */
+size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const swq_q4_cache *cache,
+                                        const swq_q4_batch *batch, int weights);
+
+/* Gated causal attention of the tokens over the cache, swq_attention_step for
+ * many tokens and sequences: q_proj [tokens][H][2 * hd] (per head the query,
+ * then the output gate), k_proj / v_proj [tokens][KVH * hd] of dtype.  k and v
+ * are appended first (swq_q4_append); both NULL: they are in the cache already
+ * (a layer that shares another's).  Token i of sequence b attends over rows
+ * 0 .. rows[b] + i as the cache holds them, its own included, with scale
+ * 1/sqrt(hd); out [tokens][H * hd] of out_dtype = attention * sigmoid(gate).
+ * weights, if not NULL: f32 [sequences][KVH][max_positions], the attention that
+ * each row has gathered, summed over tokens and the kv head's query heads:
+ * added to for rows below rows[b], set for the call's rows; others are left as
+ * they are.  Scores, softmax and sums in 32 bits; f32 outputs and weights are
+ * exact to about 1e-6, bf16 ones to their rounding.  Repeatable bit for bit.
+ * One token per sequence: split over the rows, two launches; more: tiles of
+ * queries on the matrix cores.  The workspace needs no preparation. */
+int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
+                     const void *q_proj, const void *k_proj, const void *v_proj, int dtype, float *weights,
+                     void *out, int out_dtype, void *ws, size_t ws_bytes, void *stream);
+
+/* Rows as the values they stand for, as swq_dequantize does for weights: of
+ * each of `sequences` sequences the rows first[b] .. into k and v of dtype
+ * (either may be NULL).  starts NULL: `count` rows each, [sequences][count][KVH]
+ * [hd]; else starts[b + 1] - starts[b] of them, one sequence after another,
+ * starts[sequences] <= count.  first NULL: from row 0.  rows, if not NULL: rows
+ * from rows[b] on come as zeros, as those from max_positions on always do. */
+int swq_q4_read(const swq_q4_cache *cache, int sequences, const int32_t *first, const int32_t *starts,
+                const int32_t *rows, int count, void *k, void *v, int dtype, void *stream);
+
+/* The heaviest rows of each sequence and kv head of src into dst, another
+ * cache (no overlap) of the same heads and at least `budget` rows: of the n =
+ * rows[b] rows the first `sink`, the last `recent` and, of those between, the
+ * budget - sink - recent with the largest weights (ties: the lower row), in
+ * the order that they had; all of them where n <= budget.  weights: f32
+ * [sequences][KVH][src max_positions].  new_weights (or NULL): [sequences][KVH]
+ * [dst max_positions], theirs, and 0 for the rest.  kept: int32 [sequences]
+ * [KVH][budget], their rows in src, -1 past the last.  new_rows [sequences]:
+ * min(n, budget).  A weight that is NaN counts as the lowest.  Two launches. */
+int swq_q4_evict(const swq_q4_cache *src, int sequences, const float *weights, const int32_t *rows,
+                 const swq_q4_cache *dst, int budget, int sink, int recent, float *new_weights,
+                 int32_t *new_rows, int32_t *kept, void *stream);
+
 /* ---- checkpoint and .qpack loading ----------------------------------- */
 
 enum { SWQ_MAX_DIMS = 8 };

@@ -94,6 +94,22 @@ class AttentionLayer(ctypes.Structure):
     ]
 
 
+class Q4CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p), ("bytes", ctypes.c_size_t), ("sequences", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("max_positions", ctypes.c_int32),
+    ]
+
+
+class Q4Batch(ctypes.Structure):
+    _fields_ = [
+        ("sequences", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32), ("starts", ctypes.c_void_p), ("rows", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("rope", ctypes.c_void_p), ("rope_positions", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class MoELayer(ctypes.Structure):
     _fields_ = [
         ("router", QLinear), ("gate", QLinear), ("up", QLinear), ("down", QLinear),
@@ -137,6 +153,14 @@ SIGNATURES = {
     "swq_attention_scratch_floats": (_SZ, [_c.POINTER(AttentionLayer), _c.POINTER(QLinear)]),
     "swq_attention_token": (_I, [_c.POINTER(AttentionLayer), _c.POINTER(QLinear), _c.POINTER(QLinear), _P, _P, _I,
                                  _c.c_float, _P, _SZ, _I64, _P, _SZ, _P, _P, _SZ, _P]),
+    "swq_q4_cache_bytes": (_SZ, [_I, _I, _I, _I]),
+    "swq_q4_rope_table": (_I, [_I, _c.c_float, _I64, _I, _P]),
+    "swq_q4_append": (_I, [_c.POINTER(AttentionLayer), _c.POINTER(Q4CacheDesc), _c.POINTER(Q4Batch), _P, _P, _I, _P]),
+    "swq_attention_q4_workspace_bytes": (_SZ, [_c.POINTER(AttentionLayer), _c.POINTER(Q4CacheDesc), _c.POINTER(Q4Batch), _I]),
+    "swq_attention_q4": (_I, [_c.POINTER(AttentionLayer), _c.POINTER(Q4CacheDesc), _c.POINTER(Q4Batch), _P, _P, _P, _I,
+                              _P, _P, _I, _P, _SZ, _P]),
+    "swq_q4_read": (_I, [_c.POINTER(Q4CacheDesc), _I, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "swq_q4_evict": (_I, [_c.POINTER(Q4CacheDesc), _I, _P, _P, _c.POINTER(Q4CacheDesc), _I, _I, _I, _P, _P, _P, _P]),
     "swq_checkpoint_open": (_I, [_c.c_char_p, _c.POINTER(_P)]),
     "swq_checkpoint_close": (None, [_P]),
     "swq_checkpoint_tensor_count": (_I, [_P]),

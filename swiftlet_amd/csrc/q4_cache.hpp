@@ -1,0 +1,171 @@
+// The KV cache held in 4 bits: where its rows lie, the view that kernels take, and the checks
+// that its entry points share.
+#pragma once
+
+#include <algorithm>
+
+#include "internal.hpp"
+#include "route.hpp"
+
+namespace swq {
+
+constexpr int kQ4Group = 64;      // dims of one scale and bias
+constexpr int kQ4Block = 8;       // rows of one v word
+constexpr int kQ4RowPad = 32;     // rows are allocated in multiples of this: a reader's tile
+constexpr int kQ4MaxHeadGroup = 16;  // query heads per kv head
+
+enum { kQ4KScale = 0, kQ4KBias = 1, kQ4VScale = 2, kQ4VBias = 3 };
+
+// Device view of a swq_q4_cache.  All offsets are 64-bit: a cache passes 4 GiB.
+struct Q4View {
+    uint32_t *k;      // [B][KVH][R][hd / 8]
+    uint32_t *v;      // [B][KVH][R / 8][hd]
+    _Float16 *par;    // [B][KVH][4][hd / 64][R]
+    int32_t B, KVH, hd, maxp, R;
+
+    __host__ __device__ __forceinline__ int64_t head(int b, int h) const { return static_cast<int64_t>(b) * KVH + h; }
+    __device__ __forceinline__ uint32_t *k_head(int b, int h) const { return k + head(b, h) * R * (hd / 8); }
+    __device__ __forceinline__ uint32_t *v_head(int b, int h) const { return v + head(b, h) * (R / 8) * hd; }
+    __device__ __forceinline__ _Float16 *par_head(int b, int h) const { return par + head(b, h) * 4 * (hd / kQ4Group) * R; }
+};
+
+// Device view of a swq_q4_batch.  What comes from device memory is clamped where it is read, so
+// that no value of it leads out of a buffer.
+struct Q4Batch {
+    int32_t B, N, max_tokens, rope_positions, rot;
+    const int32_t *starts, *rows, *positions;
+    const float2 *rope;
+
+    __device__ __forceinline__ int first(int b) const { return starts ? min(max(starts[b], 0), N) : b * max_tokens; }
+    __device__ __forceinline__ int count(int b) const { return starts ? max(min(starts[b + 1], N) - first(b), 0) : max_tokens; }
+    __device__ __forceinline__ int row0(int b, int maxp) const { return min(max(rows[b], 0), maxp); }
+    __device__ __forceinline__ int position(int b, int i) const {
+        const int64_t p = static_cast<int64_t>(positions ? positions[b] : rows[b]) + i;
+        return static_cast<int>(min(max(p, static_cast<int64_t>(0)), static_cast<int64_t>(rope_positions - 1)));
+    }
+};
+
+inline size_t q4_align(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+inline int64_t q4_rows(int maxp) { return (static_cast<int64_t>(maxp) + kQ4RowPad - 1) / kQ4RowPad * kQ4RowPad; }
+
+struct Q4Layout {
+    size_t codes, params, total;  // bytes of either code part and of the parameters, padded
+};
+
+inline Q4Layout q4_layout(int64_t B, int64_t kvh, int64_t hd, int maxp) {
+    const int64_t n = B * kvh * q4_rows(maxp);
+    Q4Layout l{};
+    l.codes = q4_align(static_cast<size_t>(n * hd / 2));
+    l.params = q4_align(static_cast<size_t>(n * 4 * (hd / kQ4Group) * 2));
+    l.total = 2 * l.codes + l.params;
+    return l;
+}
+
+inline bool q4_head_dim(int hd) { return hd == 64 || hd == 128 || hd == 256; }
+
+inline int check_q4_shape(int sequences, int kvh, int hd, int maxp) {
+    if (sequences <= 0 || kvh <= 0 || maxp <= 0 || hd <= 0) return SWQ_ERR_INVALID_ARGUMENT;
+    if (!q4_head_dim(hd) || maxp > (1 << 30) || static_cast<int64_t>(sequences) * kvh > 65535) return SWQ_ERR_LIMIT;
+    return SWQ_OK;
+}
+
+inline int check_q4_cache(const swq_q4_cache *c) {
+    if (!c) return SWQ_ERR_INVALID_ARGUMENT;
+    const int st = check_q4_shape(c->sequences, c->num_kv_heads, c->head_dim, c->max_positions);
+    if (st != SWQ_OK) return st;
+    if (!c->data) return SWQ_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(c->data) % 256 != 0) return SWQ_ERR_MISALIGNED;
+    if (c->bytes < q4_layout(c->sequences, c->num_kv_heads, c->head_dim, c->max_positions).total) return SWQ_ERR_WORKSPACE;
+    return SWQ_OK;
+}
+
+inline Q4View q4_view(const swq_q4_cache *c) {
+    const Q4Layout l = q4_layout(c->sequences, c->num_kv_heads, c->head_dim, c->max_positions);
+    Q4View v{};
+    uint8_t *p = static_cast<uint8_t *>(c->data);
+    v.k = reinterpret_cast<uint32_t *>(p);
+    v.v = reinterpret_cast<uint32_t *>(p + l.codes);
+    v.par = reinterpret_cast<_Float16 *>(p + 2 * l.codes);
+    v.B = c->sequences;
+    v.KVH = c->num_kv_heads;
+    v.hd = c->head_dim;
+    v.maxp = c->max_positions;
+    v.R = static_cast<int32_t>(q4_rows(c->max_positions));
+    return v;
+}
+
+// swq_attention_layer as the 4-bit cache's calls take it (max_positions is the cache's).
+inline int check_q4_layer(const swq_attention_layer *l) {
+    if (!l || l->reserved != 0) return SWQ_ERR_INVALID_ARGUMENT;
+    if (l->num_heads <= 0 || l->num_kv_heads <= 0 || l->num_heads % l->num_kv_heads != 0) return SWQ_ERR_BAD_SHAPE;
+    if (l->num_heads / l->num_kv_heads > kQ4MaxHeadGroup || !q4_head_dim(l->head_dim)) return SWQ_ERR_LIMIT;
+    if (l->rotary_dims < 0 || l->rotary_dims > l->head_dim || l->rotary_dims % 2 != 0) return SWQ_ERR_BAD_SHAPE;
+    if (!(l->norm_eps >= 0.f) || !l->q_norm_weight || !l->k_norm_weight) return SWQ_ERR_INVALID_ARGUMENT;
+    return SWQ_OK;
+}
+
+// The sizes of a batch, without its device arrays.
+inline int check_q4_sizes(const swq_q4_cache *c, const swq_q4_batch *b) {
+    if (!b || b->reserved != 0 || b->sequences <= 0 || b->tokens < 0 || b->max_rows < 0) return SWQ_ERR_INVALID_ARGUMENT;
+    if (b->sequences > c->sequences) return SWQ_ERR_BAD_SHAPE;
+    if (b->starts ? (b->max_tokens <= 0 && b->tokens > 0) : b->tokens % b->sequences != 0) return SWQ_ERR_BAD_SHAPE;
+    return SWQ_OK;
+}
+
+inline int check_q4_batch(const swq_attention_layer *l, const swq_q4_cache *c, const swq_q4_batch *b) {
+    int st = check_q4_layer(l);
+    if (st == SWQ_OK) st = check_q4_cache(c);
+    if (st == SWQ_OK) st = check_q4_sizes(c, b);
+    if (st != SWQ_OK) return st;
+    if (l->num_kv_heads != c->num_kv_heads || l->head_dim != c->head_dim) return SWQ_ERR_BAD_SHAPE;
+    if (!b->rows) return SWQ_ERR_INVALID_ARGUMENT;
+    if (l->rotary_dims > 0 && (!b->rope || b->rope_positions <= 0)) return SWQ_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(b->rope) % 8 != 0) return SWQ_ERR_MISALIGNED;
+    return SWQ_OK;
+}
+
+inline int q4_max_tokens(const swq_q4_batch *b) {
+    return b->starts ? std::min(b->max_tokens, b->tokens) : b->tokens / b->sequences;
+}
+
+inline Q4Batch q4_batch(const swq_attention_layer *l, const swq_q4_batch *b) {
+    Q4Batch d{};
+    d.B = b->sequences;
+    d.N = b->tokens;
+    d.max_tokens = q4_max_tokens(b);
+    d.rope_positions = std::max(b->rope_positions, 1);
+    d.rot = l->rotary_dims;
+    d.starts = b->starts;
+    d.rows = b->rows;
+    d.positions = b->positions;
+    d.rope = reinterpret_cast<const float2 *>(b->rope);
+    return d;
+}
+
+inline int check_q4_dtype(int dt) { return dt == SWQ_F32 || dt == SWQ_BF16 ? SWQ_OK : SWQ_ERR_UNSUPPORTED_DTYPE; }
+
+inline size_t q4_dtype_bytes(int dt) { return dt == SWQ_F32 ? 4 : 2; }
+
+// The append launch (q4_cache.hip), for callers that have checked their arguments.
+void launch_q4_append(const swq_attention_layer *l, const Q4View &c, const Q4Batch &b, const void *k, const void *v,
+                      int dtype, hipStream_t s);
+
+// ---- device ----
+
+template <typename T>
+__device__ __forceinline__ float q4_load(const T *p, int64_t i) {
+    if constexpr (sizeof(T) == 4) return p[i];
+    else return bf16_to_f32(p[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void q4_store(T *p, int64_t i, float v) {
+    if constexpr (sizeof(T) == 4) {
+        p[i] = v;
+    } else {
+        p[i] = v == v ? f32_to_bf16_rne(v) : 0x7FC0;
+    }
+}
+
+}  // namespace swq
