@@ -2,25 +2,12 @@
 // the rows that are there, with the attention that each row gathers if asked for.
 #include <cmath>
 
-#include "q4_cache.hpp"
+#include "attention_q4.hpp"
 
 namespace swq {
 namespace {
 
 constexpr int kRowTile = 256;  // rows of one softmax step, and threads
-
-struct AttnQ4Args {
-    Q4View c;
-    Q4Batch b;
-    const void *q;
-    const float *q_norm_w;
-    void *out;
-    float *weights;
-    float *qn;   // [N][H][hd]: normalised, rotated queries
-    float *lse;  // [N][H]: maximum + log of the sum, natural logarithms
-    int32_t H, group;
-    float eps, scale;
-};
 
 // One wave per (token, query head): q / rms * w, turned by the table.
 template <int HD, typename T>
@@ -182,16 +169,41 @@ void launch(const AttnQ4Args &a, int dtype, int out_dtype, hipStream_t s) {
 
 using namespace swq;
 
+namespace {
+
+struct StepParts {
+    size_t part, ml, scores, total;
+};
+
+StepParts step_parts(const swq_attention_layer *l, const swq_q4_cache *c, int sequences, int splits, bool weights) {
+    const size_t heads = static_cast<size_t>(sequences) * l->num_heads;
+    StepParts p{};
+    p.part = q4_align(heads * splits * l->head_dim * sizeof(float));
+    p.ml = q4_align(heads * splits * sizeof(float2));
+    p.scores = weights ? q4_align(heads * q4_rows(c->max_positions) * sizeof(float)) : 0;
+    p.total = p.part + p.ml + p.scores;
+    return p;
+}
+
+size_t q4_step_workspace(const swq_attention_layer *l, const swq_q4_cache *c, const swq_q4_batch *b, int weights) {
+    return step_parts(l, c, b->sequences, most_q4_splits(c->max_positions, static_cast<int64_t>(b->sequences) * c->num_kv_heads), weights != 0).total;
+}
+
+size_t q4_prompt_workspace(const swq_attention_layer *l, const swq_q4_batch *b) {
+    const size_t rows = static_cast<size_t>(std::max(b->tokens, 1)) * l->num_heads;
+    return q4_align(rows * l->head_dim * sizeof(float)) + q4_align(rows * sizeof(float));
+}
+
+}  // namespace
+
 extern "C" size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const swq_q4_cache *cache,
                                                    const swq_q4_batch *batch, int weights) {
-    (void)weights;
     if (check_q4_layer(layer) != SWQ_OK || !cache ||
         check_q4_shape(cache->sequences, cache->num_kv_heads, cache->head_dim, cache->max_positions) != SWQ_OK ||
         check_q4_sizes(cache, batch) != SWQ_OK || layer->head_dim != cache->head_dim ||
         layer->num_kv_heads != cache->num_kv_heads)
         return 0;
-    const size_t rows = static_cast<size_t>(std::max(batch->tokens, 1)) * layer->num_heads;
-    return q4_align(rows * layer->head_dim * sizeof(float)) + q4_align(rows * sizeof(float));
+    return std::max(q4_step_workspace(layer, cache, batch, weights), q4_prompt_workspace(layer, batch));
 }
 
 extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
@@ -214,17 +226,38 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     a.c = q4_view(cache);
     a.b = q4_batch(layer, batch);
     a.q = q_proj;
+    a.k = k_proj;
+    a.v = v_proj;
+    a.k_norm_w = layer->k_norm_weight;
+    a.in_f32 = dtype == SWQ_F32;
+    a.out_f32 = out_dtype == SWQ_F32;
     a.q_norm_w = layer->q_norm_weight;
     a.out = out;
     a.weights = weights;
     a.H = layer->num_heads;
     a.group = a.H / a.c.KVH;
-    const size_t rows = static_cast<size_t>(batch->tokens) * a.H;
-    a.qn = static_cast<float *>(ws);
-    a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + q4_align(rows * a.c.hd * sizeof(float)));
     a.eps = layer->norm_eps;
     a.scale = 1.0f / std::sqrt(static_cast<float>(a.c.hd));
+    a.scale2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(a.c.hd)));
     hipStream_t s = static_cast<hipStream_t>(stream);
+    uint8_t *p = static_cast<uint8_t *>(ws);
+    if (a.b.max_tokens == 1) {
+        const int64_t rows = batch->max_rows > 0 ? std::min(batch->max_rows, cache->max_positions) : cache->max_positions;
+        const Q4StepPlan plan = plan_q4_step(rows, static_cast<int64_t>(a.b.B) * a.c.KVH);
+        const StepParts parts = step_parts(layer, cache, a.b.B, plan.splits, weights != nullptr);
+        a.per = plan.per;
+        a.splits = plan.splits;
+        if (a.splits > 1 || weights) {
+            a.part = reinterpret_cast<float *>(p);
+            a.ml = reinterpret_cast<float2 *>(p + parts.part);
+            if (weights) a.scores = reinterpret_cast<float *>(p + parts.part + parts.ml);
+        }
+        launch_q4_step(a, s);
+        return launch_status();
+    }
+    const size_t rows = static_cast<size_t>(batch->tokens) * a.H;
+    a.qn = reinterpret_cast<float *>(p);
+    a.lse = reinterpret_cast<float *>(p + q4_align(rows * a.c.hd * sizeof(float)));
     if (k_proj) launch_q4_append(layer, a.c, a.b, k_proj, v_proj, dtype, s);
     switch (a.c.hd) {
         case 64: launch<64>(a, dtype, out_dtype, s); break;

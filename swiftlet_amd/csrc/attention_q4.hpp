@@ -1,0 +1,125 @@
+// What the launches of swq_attention_q4 share: arguments, a query head's norm and rotation, and
+// the way 4-bit codes, scales and f32 numbers meet on the f16 matrix cores without losing bits.
+//
+//   codes   become f16 integers: nibbles 0 and 4 of a word or-ed into the f16 number 1024 and 1024
+//           taken off again, nibbles 1 and 5 likewise but 16 times as large (they need no shift),
+//           nibbles 2, 3, 6 and 7 the same after one shift: 9 operations for 8 codes.  The other
+//           operand has 1/16 at the odd nibbles.  (Left as they lie, codes are f16 numbers below
+//           the normal ones: 5 operations, but the matrix cores add their products with the
+//           leading zeros of the mantissa, and outputs were off by 1.8e-5 where now by 1e-6.)
+//   f32     operands (queries; p times a value scale) are two f16 numbers, high and low part, of
+//           22 bits together; products with codes are exact, sums f32.  A power of two per head
+//           (queries) or per wave (p * scale) keeps them inside f16's range.
+//   scales  of keys multiply a group's sum of products, those of values p; biases meet the sum of
+//           the queries' dims of a group, and p, on the VALU.
+#pragma once
+
+#include "q4_cache.hpp"
+
+namespace swq {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+struct AttnQ4Args {
+    Q4View c;
+    Q4Batch b;
+    const void *q, *k, *v;
+    const float *q_norm_w, *k_norm_w;
+    void *out;
+    float *weights;
+    int32_t H, group;
+    int32_t in_f32, out_f32;  // types of q, k, v and of out: f32, else bf16
+    float eps, scale, scale2;  // 1/sqrt(hd), and times log2(e)
+    // single tokens: rows per split, splits, and their partial results
+    int32_t per, splits;
+    float *part;    // [B][H][splits][hd]
+    float2 *ml;     // [B][H][splits]: reference exponent and sum
+    float *scores;  // [B][H][R] in units of log2, for the gathered weights
+    // prompts
+    float *qn;   // [N][H][hd]: normalised, rotated queries
+    float *lse;  // [N][H]: maximum + log of the sum, natural logarithms
+};
+
+__device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// The 8 codes of a word as operand: elements 0 .. 7 are nibbles 0 4 1 5 2 6 3 7, those of odd
+// nibbles times 16.
+__device__ __forceinline__ h8_t q4_operand(uint32_t w) {
+    constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u, k1024 = 0x64006400u;
+    const uint32_t s = w >> 8;
+    const h2_t off = {static_cast<_Float16>(-1024.f), static_cast<_Float16>(-1024.f)};
+    const h2_t a = __builtin_bit_cast(h2_t, (w & kEven) | k1024) + off, b = __builtin_bit_cast(h2_t, (w & kOdd) | k1024) + off;
+    const h2_t c = __builtin_bit_cast(h2_t, (s & kEven) | k1024) + off, d = __builtin_bit_cast(h2_t, (s & kOdd) | k1024) + off;
+    return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Operand element of a nibble, and the nibble of an element.
+__device__ __forceinline__ constexpr int q4_element(int nibble) { return nibble < 4 ? 2 * nibble : 2 * nibble - 7; }
+__device__ __forceinline__ constexpr int q4_nibble(int element) { return element / 2 + 4 * (element & 1); }
+
+// x = hi + lo with hi, lo f16.
+__device__ __forceinline__ void split_f16(f32x2_t x, h2_t &hi, h2_t &lo) {
+    hi = __builtin_convertvector(x, h2_t);
+    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x2_t), h2_t);
+}
+
+__device__ __forceinline__ float q4_load_any(const void *p, int64_t i, int is_f32) {
+    return is_f32 ? static_cast<const float *>(p)[i] : bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
+}
+
+__device__ __forceinline__ void q4_store_any(void *p, int64_t i, float v, int is_f32) {
+    if (is_f32) q4_store(static_cast<float *>(p), i, v);
+    else q4_store(static_cast<uint16_t *>(p), i, v);
+}
+
+__device__ __forceinline__ float q4_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float sigmoid_exact(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+// A head vector, EPL = HD / 64 consecutive elements per lane: times w / rms, its first 2 * half
+// elements turned by `turn`.  lds: HD floats of this wave.
+template <int EPL>
+__device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const float *w, float eps, const float2 *turn, int half,
+                                             float *lds) {
+    const int lane = threadIdx.x & (kWave - 1);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
+    ss = wave_sum_all(ss);
+    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(EPL * kWave) + eps);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        x[e] *= sc * w[lane * EPL + e];
+        lds[lane * EPL + e] = x[e];
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (half > 0) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int i = lane * EPL + e;
+            if (i < 2 * half) {
+                const float2 cs = turn[i < half ? i : i - half];
+                const float o = lds[i < half ? i + half : i - half];
+                x[e] = i < half ? x[e] * cs.x - o * cs.y : x[e] * cs.x + o * cs.y;
+            }
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Single tokens (attention_q4_step.hip): a split of max_rows rows over workgroups, and its launches.
+struct Q4StepPlan {
+    int per, splits;
+};
+Q4StepPlan plan_q4_step(int64_t rows, int64_t heads);
+int most_q4_splits(int64_t rows, int64_t heads);  // of any number of rows up to this
+void launch_q4_step(const AttnQ4Args &a, hipStream_t s);
+
+}  // namespace swq

@@ -2,7 +2,7 @@
 // smaller cache.  The formats are swq.h's (swq_q4_cache).
 #include <cmath>
 
-#include "q4_cache.hpp"
+#include "q4_row.hpp"
 
 namespace swq {
 namespace {
@@ -18,49 +18,13 @@ struct AppendArgs {
     float eps;
 };
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    return v;
-}
-
-// f16 by way of f32, both roundings as the format has them: the compiler would make one of the two.
-__device__ __forceinline__ _Float16 f16_by_f32(double x) {
-    float f = static_cast<float>(x);
-    asm volatile("" : "+v"(f));
-    return static_cast<_Float16>(f);
-}
-
-// 4-bit codes of one head's row, EPL consecutive dims per lane in 64 bits: the scale and bias of
-// this lane's 64 dims, the codes into q.  Divisions are exact to their last bit, so a value that
-// lies on a border between two codes goes to the even one.
-template <int EPL>
-__device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q)[EPL], _Float16 &scale, _Float16 &bias) {
-    double y[EPL], lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        y[e] = x[e] == x[e] ? fmin(fmax(x[e], -65504.0), 65504.0) : 0.0;
-        lo = fmin(lo, y[e]);
-        hi = fmax(hi, y[e]);
-    }
-    for (int off = kQ4Group / EPL / 2; off > 0; off >>= 1) {
-        lo = fmin(lo, __shfl_xor(lo, off, kWave));
-        hi = fmax(hi, __shfl_xor(hi, off, kWave));
-    }
-    bias = f16_by_f32(lo);
-    scale = f16_by_f32((hi - lo) / 15.0);
-    const double b = static_cast<double>(static_cast<float>(bias)), s = static_cast<double>(static_cast<float>(scale));
-#pragma unroll
-    for (int e = 0; e < EPL; ++e)
-        q[e] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0)) : 0u;
-}
-
 // One workgroup per block of 8 rows, kv head and sequence; a wave takes every fourth row of the
 // block.  k words and all scales and biases belong to one row and are written by its wave; a v
 // word holds 8 rows of one dim, so the codes meet in LDS, and words of which only some rows are
 // new keep the others (the first and last block of a call).
 template <int HD, typename T>
 __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) {
-    constexpr int EPL = HD / kWave, NG = HD / kQ4Group;
+    constexpr int EPL = HD / kWave;
     __shared__ double s_rot[kAppendWaves][HD];
     __shared__ uint8_t s_v[kQ4Block][HD];
     const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH;
@@ -78,58 +42,15 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
             const int64_t at = (static_cast<int64_t>(n0 + row - r0) * a.c.KVH + h) * HD + lane * EPL;
             double x[EPL];
             uint32_t q[EPL];
-            _Float16 scale, bias;
-            double ss = 0.0;
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                x[e] = static_cast<double>(q4_load(kin, at + e));
-                ss += x[e] * x[e];
-            }
-            ss = wave_sum_f64(ss);
-            const double root = sqrt(ss / HD + static_cast<double>(a.eps));
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                x[e] = x[e] / root * static_cast<double>(a.w[lane * EPL + e]);
-                s_rot[wave][lane * EPL + e] = x[e];
-            }
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (half > 0) {
-                const float2 *turn = a.b.rope + static_cast<int64_t>(a.b.position(b, row - r0)) * half;
-#pragma unroll
-                for (int e = 0; e < EPL; ++e) {
-                    const int i = lane * EPL + e;
-                    if (i < 2 * half) {
-                        const float2 cs = turn[i < half ? i : i - half];
-                        const double o = s_rot[wave][i < half ? i + half : i - half];
-                        const double c = static_cast<double>(cs.x), s = static_cast<double>(cs.y);
-                        x[e] = i < half ? x[e] * c - o * s : x[e] * c + o * s;
-                    }
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            q4_quantise<EPL>(x, q, scale, bias);
-            uint32_t word = 0;
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) word |= q[e] << (4 * ((lane * EPL + e) & 7));
-            for (int off = 8 / EPL / 2; off > 0; off >>= 1) word |= __shfl_xor(word, off, kWave);
-            if (lane % (8 / EPL) == 0) kw[static_cast<int64_t>(row) * (HD / 8) + lane * EPL / 8] = word;
-            const int g = lane * EPL / kQ4Group;
-            const bool leads = lane % (kQ4Group / EPL) == 0;
-            if (leads) {
-                par[(static_cast<int64_t>(kQ4KScale) * NG + g) * a.c.R + row] = scale;
-                par[(static_cast<int64_t>(kQ4KBias) * NG + g) * a.c.R + row] = bias;
-            }
+            for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(kin, at + e));
+            const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, row - r0)) * half : nullptr;
+            q4_key_row<HD>(x, a.w, a.eps, turn, half, s_rot[wave], kw, par, a.c.R, row);
 #pragma unroll
             for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(vin, at + e));
-            q4_quantise<EPL>(x, q, scale, bias);
+            q4_value_row<HD>(x, q, par, a.c.R, row);
 #pragma unroll
             for (int e = 0; e < EPL; ++e) s_v[u][lane * EPL + e] = static_cast<uint8_t>(q[e]);
-            if (leads) {
-                par[(static_cast<int64_t>(kQ4VScale) * NG + g) * a.c.R + row] = scale;
-                par[(static_cast<int64_t>(kQ4VBias) * NG + g) * a.c.R + row] = bias;
-            }
         }
         __syncthreads();
         const int u0 = max(r0 - blk * kQ4Block, 0), u1 = min(r1 - blk * kQ4Block, kQ4Block);

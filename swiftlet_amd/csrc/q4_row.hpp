@@ -1,0 +1,108 @@
+// One head's new row into a 4-bit cache, by one wave: EPL = hd / 64 consecutive dims per lane, in 64
+// bits up to the format's own roundings.
+#pragma once
+
+#include "q4_cache.hpp"
+
+namespace swq {
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+    return v;
+}
+
+// f16 by way of f32, both roundings as the format has them: the compiler would make one of the two.
+__device__ __forceinline__ _Float16 f16_by_f32(double x) {
+    float f = static_cast<float>(x);
+    asm volatile("" : "+v"(f));
+    return static_cast<_Float16>(f);
+}
+
+// 4-bit codes of one head's row, EPL consecutive dims per lane in 64 bits: the scale and bias of
+// this lane's 64 dims, the codes into q.  Divisions are exact to their last bit, so a value that
+// lies on a border between two codes goes to the even one.
+template <int EPL>
+__device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q)[EPL], _Float16 &scale, _Float16 &bias) {
+    double y[EPL], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        y[e] = x[e] == x[e] ? fmin(fmax(x[e], -65504.0), 65504.0) : 0.0;
+        lo = fmin(lo, y[e]);
+        hi = fmax(hi, y[e]);
+    }
+    for (int off = kQ4Group / EPL / 2; off > 0; off >>= 1) {
+        lo = fmin(lo, __shfl_xor(lo, off, kWave));
+        hi = fmax(hi, __shfl_xor(hi, off, kWave));
+    }
+    bias = f16_by_f32(lo);
+    scale = f16_by_f32((hi - lo) / 15.0);
+    const double b = static_cast<double>(static_cast<float>(bias)), s = static_cast<double>(static_cast<float>(scale));
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+        q[e] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0)) : 0u;
+}
+
+// Scale and bias of this lane's group to parameters `which` and which + 1 of `row`.
+template <int HD>
+__device__ __forceinline__ void q4_put_params(_Float16 *par, int64_t R, int which, int64_t row, _Float16 scale, _Float16 bias) {
+    constexpr int EPL = HD / kWave, NG = HD / kQ4Group;
+    const int lane = threadIdx.x & (kWave - 1), g = lane * EPL / kQ4Group;
+    if (lane % (kQ4Group / EPL) == 0) {
+        par[(static_cast<int64_t>(which) * NG + g) * R + row] = scale;
+        par[(static_cast<int64_t>(which + 1) * NG + g) * R + row] = bias;
+    }
+}
+
+// A key: x / rms * w, turned, quantised, its words and parameters written.  lds: HD doubles of this
+// wave; turn: the position's cos and sin, `half` of them.
+template <int HD>
+__device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const float *w, float eps, const float2 *turn, int half,
+                                           double *lds, uint32_t *kw, _Float16 *par, int64_t R, int64_t row) {
+    constexpr int EPL = HD / kWave;
+    const int lane = threadIdx.x & (kWave - 1);
+    double ss = 0.0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
+    ss = wave_sum_f64(ss);
+    const double root = sqrt(ss / HD + static_cast<double>(eps));
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        x[e] = x[e] / root * static_cast<double>(w[lane * EPL + e]);
+        lds[lane * EPL + e] = x[e];
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (half > 0) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int i = lane * EPL + e;
+            if (i < 2 * half) {
+                const float2 cs = turn[i < half ? i : i - half];
+                const double o = lds[i < half ? i + half : i - half];
+                const double c = static_cast<double>(cs.x), s = static_cast<double>(cs.y);
+                x[e] = i < half ? x[e] * c - o * s : x[e] * c + o * s;
+            }
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint32_t q[EPL], word = 0;
+    _Float16 scale, bias;
+    q4_quantise<EPL>(x, q, scale, bias);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) word |= q[e] << (4 * ((lane * EPL + e) & 7));
+    for (int off = 8 / EPL / 2; off > 0; off >>= 1) word |= __shfl_xor(word, off, kWave);
+    if (lane % (8 / EPL) == 0) kw[row * (HD / 8) + lane * EPL / 8] = word;
+    q4_put_params<HD>(par, R, kQ4KScale, row, scale, bias);
+}
+
+// A value row quantised, its parameters written; its codes into q, for the words of its block.
+template <int HD>
+__device__ __forceinline__ void q4_value_row(const double (&x)[HD / kWave], uint32_t (&q)[HD / kWave], _Float16 *par, int64_t R,
+                                             int64_t row) {
+    _Float16 scale, bias;
+    q4_quantise<HD / kWave>(x, q, scale, bias);
+    q4_put_params<HD>(par, R, kQ4VScale, row, scale, bias);
+}
+
+}  // namespace swq
