@@ -21,34 +21,13 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     const int i = static_cast<int>(item / a.H), h = static_cast<int>(item % a.H);
     const int64_t n = a.b.first(b) + i;
     const T *q = static_cast<const T *>(a.q) + (n * a.H + h) * 2 * HD + lane * EPL;
-    float x[EPL], ss = 0.f;
+    float x[EPL];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        x[e] = q4_load(q, e);
-        ss += x[e] * x[e];
-    }
-    ss = wave_sum(ss);
-    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        x[e] *= sc * a.q_norm_w[lane * EPL + e];
-        s_rot[wave][lane * EPL + e] = x[e];
-    }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int e = 0; e < EPL; ++e) x[e] = q4_load(q, e);
     const int half = a.b.rot / 2;
-    if (half > 0) {
-        const float2 *turn = a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int d = lane * EPL + e;
-            if (d < 2 * half) {
-                const float2 cs = turn[d < half ? d : d - half];
-                const float o = s_rot[wave][d < half ? d + half : d - half];
-                x[e] = d < half ? x[e] * cs.x - o * cs.y : x[e] * cs.x + o * cs.y;
-            }
-        }
-    }
+    Q4HeadTable<EPL> tab;
+    tab.load(a.q_norm_w, half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half : nullptr, half);
+    q4_norm_rope<EPL>(x, tab, a.eps, half, s_rot[wave]);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) a.qn[(n * a.H + h) * HD + lane * EPL + e] = x[e];
 }

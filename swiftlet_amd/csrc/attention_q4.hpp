@@ -14,7 +14,7 @@
 //           the queries' dims of a group, and p, on the VALU.
 #pragma once
 
-#include "q4_cache.hpp"
+#include "q4_row.hpp"
 
 namespace swq {
 
@@ -48,13 +48,20 @@ __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) {
 }
 
 // The 8 codes of a word as operand: elements 0 .. 7 are nibbles 0 4 1 5 2 6 3 7, those of odd
-// nibbles times 16.
-__device__ __forceinline__ h8_t q4_operand(uint32_t w) {
-    constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u, k1024 = 0x64006400u;
+// nibbles times 16.  magic: two f16 1024, which the caller keeps in a vector register so that
+// masking and or-ing take one operation (kept_1024).
+__device__ __forceinline__ uint32_t kept_1024() {
+    uint32_t m = 0x64006400u;
+    asm volatile("" : "+v"(m));
+    return m;
+}
+
+__device__ __forceinline__ h8_t q4_operand(uint32_t w, uint32_t magic) {
+    constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;
     const uint32_t s = w >> 8;
     const h2_t off = {static_cast<_Float16>(-1024.f), static_cast<_Float16>(-1024.f)};
-    const h2_t a = __builtin_bit_cast(h2_t, (w & kEven) | k1024) + off, b = __builtin_bit_cast(h2_t, (w & kOdd) | k1024) + off;
-    const h2_t c = __builtin_bit_cast(h2_t, (s & kEven) | k1024) + off, d = __builtin_bit_cast(h2_t, (s & kOdd) | k1024) + off;
+    const h2_t a = __builtin_bit_cast(h2_t, (w & kEven) | magic) + off, b = __builtin_bit_cast(h2_t, (w & kOdd) | magic) + off;
+    const h2_t c = __builtin_bit_cast(h2_t, (s & kEven) | magic) + off, d = __builtin_bit_cast(h2_t, (s & kOdd) | magic) + off;
     return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
@@ -65,7 +72,9 @@ __device__ __forceinline__ constexpr int q4_nibble(int element) { return element
 // x = hi + lo with hi, lo f16.
 __device__ __forceinline__ void split_f16(f32x2_t x, h2_t &hi, h2_t &lo) {
     hi = __builtin_convertvector(x, h2_t);
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x2_t), h2_t);
+    // one mixed-precision fma each
+    const f32x2_t rest = {fmaf(static_cast<float>(hi.x), -1.0f, x.x), fmaf(static_cast<float>(hi.y), -1.0f, x.y)};
+    lo = __builtin_convertvector(rest, h2_t);
 }
 
 __device__ __forceinline__ float q4_load_any(const void *p, int64_t i, int is_f32) {
@@ -82,10 +91,9 @@ __device__ __forceinline__ float q4_exp2(float x) { return __builtin_amdgcn_exp2
 __device__ __forceinline__ float sigmoid_exact(float v) { return 1.0f / (1.0f + expf(-v)); }
 
 // A head vector, EPL = HD / 64 consecutive elements per lane: times w / rms, its first 2 * half
-// elements turned by `turn`.  lds: HD floats of this wave.
+// elements turned.  lds: HD floats of this wave.
 template <int EPL>
-__device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const float *w, float eps, const float2 *turn, int half,
-                                             float *lds) {
+__device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const Q4HeadTable<EPL> &tab, float eps, int half, float *lds) {
     const int lane = threadIdx.x & (kWave - 1);
     float ss = 0.f;
 #pragma unroll
@@ -94,7 +102,7 @@ __device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const float *w, fl
     const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(EPL * kWave) + eps);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-        x[e] *= sc * w[lane * EPL + e];
+        x[e] *= sc * tab.w[e];
         lds[lane * EPL + e] = x[e];
     }
     __builtin_amdgcn_wave_barrier();
@@ -104,9 +112,8 @@ __device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const float *w, fl
         for (int e = 0; e < EPL; ++e) {
             const int i = lane * EPL + e;
             if (i < 2 * half) {
-                const float2 cs = turn[i < half ? i : i - half];
                 const float o = lds[i < half ? i + half : i - half];
-                x[e] = i < half ? x[e] * cs.x - o * cs.y : x[e] * cs.x + o * cs.y;
+                x[e] = i < half ? x[e] * tab.cs[e].x - o * tab.cs[e].y : x[e] * tab.cs[e].x + o * tab.cs[e].y;
             }
         }
     }

@@ -3,7 +3,6 @@
 #include <cmath>
 
 #include "attention_q4.hpp"
-#include "q4_row.hpp"
 
 namespace swq {
 namespace {
@@ -22,7 +21,7 @@ struct Q4Tile {
 };
 
 template <int HD, typename T>
-__global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const AttnQ4Args a) {
+__global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void q4_step(const AttnQ4Args a) {
     constexpr int EPL = HD / kWave, NG = HD / kQ4Group, KS = HD / 32;
     constexpr int HP = HD + kHeadPad;
     constexpr int kQBytes = 2 * KS * kWave * 16, kOBytes = kStepWaves * kQ4MaxHeadGroup * HP * 4;
@@ -33,7 +32,10 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
     __shared__ double s_rot[kStepWaves][HD];
     h8_t *s_q = reinterpret_cast<h8_t *>(s_buf);  // [plane][kstep][lane]
     float *s_o = reinterpret_cast<float *>(s_buf);  // [wave][head][HP]
-    const int split = blockIdx.x, kvh = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH;
+    // Workgroups go to the 8 XCDs in turn: with the splits outermost and the heads turned by one from
+    // split to split, no XCD gets the same splits, or the same sequences, of every head.
+    const int split = blockIdx.y, head = (blockIdx.x + blockIdx.y) % gridDim.x;
+    const int kvh = head % a.c.KVH, b = head / a.c.KVH;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int r = lane & 15, q = lane >> 4, G = a.group;
     if (a.b.count(b) <= 0) return;
@@ -42,101 +44,126 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
     const int p0 = split * a.per, p1 = split == a.splits - 1 ? n : min(p0 + a.per, n);
     if (p0 >= n) return;
     const bool last = p1 == n;
-    // the wave that writes the token's row takes the row's tile, and no other, of the last split
+    // In the last split two waves write the token's row before they, or another, load its tile.
     const bool writes = a.k && last && r0 < a.c.maxp;
-    const int tiles = (p1 - p0 + kTile - 1) / kTile;
-    const bool writer = writes && wave == kStepWaves - 1;
-    const int walkers = writes ? kStepWaves - 1 : kStepWaves;
-    const int shared_tiles = writes ? tiles - 1 : tiles;
-    int tile = writer ? tiles - 1 : wave;
-    const int end = writer ? tiles : shared_tiles;
+    const int end = (p1 - p0 + kTile - 1) / kTile;  // tiles
+    int tile = wave;
 
     const uint32_t *kw = a.c.k_head(b, kvh), *vw = a.c.v_head(b, kvh);
     const _Float16 *par = a.c.par_head(b, kvh);
     Q4Tile<NG> cur;
-    auto load = [&](Q4Tile<NG> &d, int t) {
+    auto load_k = [&](int t) {
         const int64_t t0 = p0 + static_cast<int64_t>(t) * kTile;
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                d.k[x][g] = *reinterpret_cast<const uint2 *>(kw + (t0 + 8 * (r >> 2) + 4 * x + (r & 3)) * (HD / 8) + 8 * g + 2 * q);
+                cur.k[x][g] = *reinterpret_cast<const uint2 *>(kw + (t0 + 8 * (r >> 2) + 4 * x + (r & 3)) * (HD / 8) + 8 * g + 2 * q);
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = kQ4KScale; w <= kQ4KBias; ++w)
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                d.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0 + 8 * q);
+                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0 + 8 * q);
+    };
+    auto load_v = [&](int t) {
+        const int64_t t0 = p0 + static_cast<int64_t>(t) * kTile;
+#pragma unroll
+        for (int w = kQ4VScale; w <= kQ4VBias; ++w)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0 + 8 * q);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            d.v[g] = *reinterpret_cast<const uint4 *>(vw + (t0 / 8 + q) * HD + 64 * g + 4 * r);
+            cur.v[g] = *reinterpret_cast<const uint4 *>(vw + (t0 / 8 + q) * HD + 64 * g + 4 * r);
     };
-    if (!writer && tile < end) load(cur, tile);
+    const bool waits = writes && tile == end - 1;  // its first tile is the one with the new row
+    if (tile < end && !waits) {
+        load_k(tile);
+        load_v(tile);
+    }
 
     const int half = a.b.rot / 2;
     const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, 0)) * half : nullptr;
-    if (writer) {
+    const int askers = writes ? kStepWaves - 2 : kStepWaves;  // waves that prepare queries
+    if (wave >= askers) {
         const int64_t at = (static_cast<int64_t>(n0) * a.c.KVH + kvh) * HD + lane * EPL;
-        double x[EPL], y[EPL];
-        uint32_t code[EPL], old[EPL];
-        uint32_t *vp = a.c.v_head(b, kvh) + static_cast<int64_t>(r0 / kQ4Block) * HD + lane * EPL;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            x[e] = static_cast<double>(q4_load(static_cast<const T *>(a.k), at + e));
-            y[e] = static_cast<double>(q4_load(static_cast<const T *>(a.v), at + e));
-            old[e] = vp[e];
-        }
+        double x[EPL];
         _Float16 *pw = a.c.par_head(b, kvh);
-        q4_key_row<HD>(x, a.k_norm_w, a.eps, turn, half, s_rot[wave], a.c.k_head(b, kvh), pw, a.c.R, r0);
-        q4_value_row<HD>(y, code, pw, a.c.R, r0);
-        const int sh = 4 * (r0 & 7);
+        if (wave == askers) {
+            Q4HeadTable<EPL> tab;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) vp[e] = (old[e] & ~(15u << sh)) | (code[e] << sh);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // other lanes' stores, before this wave loads them
-        load(cur, tile);
+            for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(static_cast<const T *>(a.k), at + e));
+            tab.load(a.k_norm_w, turn, half);
+            q4_key_row<HD>(x, tab, a.eps, half, s_rot[wave], a.c.k_head(b, kvh), pw, a.c.R, r0);
+        } else {
+            uint32_t code[EPL], old[EPL];
+            uint32_t *vp = a.c.v_head(b, kvh) + static_cast<int64_t>(r0 / kQ4Block) * HD + lane * EPL;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                x[e] = static_cast<double>(q4_load(static_cast<const T *>(a.v), at + e));
+                old[e] = vp[e];
+            }
+            q4_value_row<HD>(x, code, pw, a.c.R, r0);
+            const int sh = 4 * (r0 & 7);
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) vp[e] = (old[e] & ~(15u << sh)) | (code[e] << sh);
+        }
     } else {
-        for (int u = wave; u < kQ4MaxHeadGroup; u += walkers) {
-            float x[EPL], qs = 0.f;
-            if (u < G) {
+        constexpr int AT_ONCE = 4;  // heads of a wave whose loads are in flight together
+        Q4HeadTable<EPL> tab;
+        tab.load(a.q_norm_w, turn, half);
+        for (int base = 0; base < G; base += AT_ONCE * askers) {
+            float x[AT_ONCE][EPL];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int u = min(base + k * askers + wave, G - 1);
                 const T *src = static_cast<const T *>(a.q) + (static_cast<int64_t>(n0) * a.H + kvh * G + u) * 2 * HD + lane * EPL;
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) x[e] = q4_load(src, e);
-                q4_norm_rope<EPL>(x, a.q_norm_w, a.eps, turn, half, reinterpret_cast<float *>(s_rot[wave]));
-                float top = 0.f;
+                for (int e = 0; e < EPL; ++e) x[k][e] = q4_load(src, e);
+            }
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) top = fmaxf(top, fabsf(x[e]));
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int u = base + k * askers + wave;
+                if (u >= G) break;
+                q4_norm_rope<EPL>(x[k], tab, a.eps, half, reinterpret_cast<float *>(s_rot[wave]));
+                float top = 0.f, qs = 0.f;
+#pragma unroll
+                for (int e = 0; e < EPL; ++e) top = fmaxf(top, fabsf(x[k][e]));
                 top = wave_max_all(top);
                 int ex = 0;
                 if (top > 0.f && top < INFINITY) frexpf(top, &ex);
 #pragma unroll
                 for (int e = 0; e < EPL; ++e) {
-                    x[e] = ldexpf(x[e], 10 - ex);  // below 2^10
-                    qs += x[e];
+                    x[k][e] = ldexpf(x[k][e], 10 - ex);  // below 2^10
+                    qs += x[k][e];
                 }
                 if (lane == 0) s_f[u] = ldexpf(a.scale2, ex - 10);
-            } else {
+                qs = segment_sum(qs, kQ4Group / EPL);
+                if (lane % (kQ4Group / EPL) == 0) s_qs[lane * EPL / kQ4Group][u] = qs;
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) x[e] = 0.f;
-                if (lane == 0) s_f[u] = 0.f;
-            }
-            qs = segment_sum(qs, kQ4Group / EPL);
-            if (lane % (kQ4Group / EPL) == 0) s_qs[lane * EPL / kQ4Group][u] = qs;
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                const int d = lane * EPL + e, j = (d & 63) >> 3, nb = d & 7;  // word of its group, nibble
-                const float v = nb & 1 ? x[e] * 0.0625f : x[e];
-                const _Float16 hi = static_cast<_Float16>(v), lo = static_cast<_Float16>(v - static_cast<float>(hi));
-                _Float16 *dst = reinterpret_cast<_Float16 *>(s_q + (2 * (d >> 6) + (j & 1)) * kWave + (j >> 1) * 16 + u) + q4_element(nb);
-                dst[0] = hi;
-                dst[KS * kWave * 8] = lo;
+                for (int e = 0; e < EPL; ++e) {
+                    const int d = lane * EPL + e, j = (d & 63) >> 3, nb = d & 7;  // word of its group, nibble
+                    const float v = nb & 1 ? x[k][e] * 0.0625f : x[k][e];
+                    const _Float16 hi = static_cast<_Float16>(v), lo = static_cast<_Float16>(v - static_cast<float>(hi));
+                    _Float16 *dst = reinterpret_cast<_Float16 *>(s_q + (2 * (d >> 6) + (j & 1)) * kWave + (j >> 1) * 16 + u) + q4_element(nb);
+                    dst[0] = hi;
+                    dst[KS * kWave * 8] = lo;
+                }
             }
         }
     }
-    lds_barrier();
+    // heads past the group are columns of their own in both products: what they hold reaches nothing
+    if (writes) __syncthreads();  // the row's stores are done
+    else lds_barrier();
+    if (waits) {
+        load_k(tile);
+        load_v(tile);
+    }
 
     float qs[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) qs[g] = s_qs[g][r];
-    const float f = s_f[r];
+    const float f = r < G ? s_f[r] : 0.f;
     float m = -INFINITY, l = 0.f, ref = -INFINITY, cap = 0.f, ce = -24.f;  // 2^ce bounds the value scales so far
     float pb[NG];
     f4_t o[NG][4];
@@ -147,10 +174,13 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
         for (int e = 0; e < 4; ++e) o[g][e] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
     float *sc_out = a.scores && r < G ? a.scores + (static_cast<int64_t>(b) * a.H + kvh * G + r) * a.c.R : nullptr;
-    const int stride = writer ? 1 : walkers;
+    constexpr int stride = kStepWaves;
+    const uint32_t magic = kept_1024();
     for (; tile < end; tile += stride) {
         const int t0 = p0 + tile * kTile;
-        // scores
+        // scores; the queries come from LDS each time, which leaves registers for another wave
+        int ql = lane;
+        asm volatile("" : "+v"(ql));
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = 0.f;
@@ -162,9 +192,9 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
                 f4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const h8_t c = q4_operand(u ? cur.k[x][g].y : cur.k[x][g].x);
-                    d = mfma16(c, s_q[(2 * g + u) * kWave + lane], d);
-                    d = mfma16(c, s_q[(KS + 2 * g + u) * kWave + lane], d);
+                    const h8_t c = q4_operand(u ? cur.k[x][g].y : cur.k[x][g].x, magic);
+                    d = mfma16(c, s_q[(2 * g + u) * kWave + ql], d);
+                    d = mfma16(c, s_q[(KS + 2 * g + u) * kWave + ql], d);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -172,34 +202,43 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
                     p[4 * x + i] = fmaf(static_cast<float>(ks[4 * x + i]), d[i], p[4 * x + i]);
                 }
             }
+            if constexpr (NG > 2) __builtin_amdgcn_sched_barrier(0);
         }
+        const int next = tile + stride < end ? tile + stride : tile;  // the last tile once more: never used
+        load_k(next);
         if (t0 + kTile > p1) {  // rows past the end count nothing, whatever they hold
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = t0 + 8 * q + i < p1 ? p[i] * f : -INFINITY;
+            for (int i = 0; i < 8; ++i) p[i] = t0 + 8 * q + i < p1 ? p[i] : -INFINITY;
+            uint4 keep;
+            const int left = p1 - t0 - 8 * q;  // of this lane's 8 rows
+            keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
+            keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
+            keep.z = (left > 4 ? 0xFFFFu : 0u) | (left > 5 ? 0xFFFF0000u : 0u);
+            keep.w = (left > 6 ? 0xFFFFu : 0u) | (left > 7 ? 0xFFFF0000u : 0u);
 #pragma unroll
             for (int w = kQ4VScale; w <= kQ4VBias; ++w)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    h8_t x = __builtin_bit_cast(h8_t, cur.par[w][g]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = t0 + 8 * q + i < p1 ? x[i] : static_cast<_Float16>(0.f);
-                    cur.par[w][g] = __builtin_bit_cast(uint4, x);
+                    cur.par[w][g].x &= keep.x;
+                    cur.par[w][g].y &= keep.y;
+                    cur.par[w][g].z &= keep.z;
+                    cur.par[w][g].w &= keep.w;
                 }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] *= f;
         }
         if (sc_out) {
-            *reinterpret_cast<float4 *>(sc_out + t0 + 8 * q) = make_float4(p[0], p[1], p[2], p[3]);
-            *reinterpret_cast<float4 *>(sc_out + t0 + 8 * q + 4) = make_float4(p[4], p[5], p[6], p[7]);
+            *reinterpret_cast<float4 *>(sc_out + t0 + 8 * q) = make_float4(p[0] * f, p[1] * f, p[2] * f, p[3] * f);
+            *reinterpret_cast<float4 *>(sc_out + t0 + 8 * q + 4) = make_float4(p[4] * f, p[5] * f, p[6] * f, p[7] * f);
         }
-        float mt = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-        h8_t st = __builtin_bit_cast(h8_t, cur.par[kQ4VScale][0]);
+        float mt = f * fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        h2_t st = {static_cast<_Float16>(0.f), static_cast<_Float16>(0.f)};
 #pragma unroll
-        for (int g = 1; g < NG; ++g) st = __builtin_elementwise_max(st, __builtin_bit_cast(h8_t, cur.par[kQ4VScale][g]));
-        float top = 0.f;
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, static_cast<float>(st[i]));
+            for (int i = 0; i < 4; ++i) {
+                const uint4 u = cur.par[kQ4VScale][g];
+                st = __builtin_elementwise_max(st, __builtin_bit_cast(h2_t, i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w));
+            }
+        float top = fmaxf(static_cast<float>(st.x), static_cast<float>(st.y));
         if (__any(mt > m || top > cap)) {
             mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
             mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
@@ -224,7 +263,7 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            p[i] = q4_exp2(p[i] - ref);
+            p[i] = q4_exp2(fmaf(p[i], f, -ref));
             l += p[i];
         }
         float pe[8];  // in operand order, 1/16 where the codes are 16 times as large
@@ -248,14 +287,15 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 1 : 2) void q4_step(const
             const uint32_t vw4[4] = {cur.v[g].x, cur.v[g].y, cur.v[g].z, cur.v[g].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const h8_t c = q4_operand(vw4[e]);
+                const h8_t c = q4_operand(vw4[e], magic);
                 o[g][e] = mfma16(c, hi, o[g][e]);
                 o[g][e] = mfma16(c, lo, o[g][e]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) pb[g] = fmaf(p[i], static_cast<float>(vb[i]), pb[g]);
+            if constexpr (NG > 2) __builtin_amdgcn_sched_barrier(0);
         }
-        if (tile + stride < end) load(cur, tile + stride);
+        load_v(next);
     }
     // the waves' sums meet
     l += __shfl_xor(l, 16, kWave);
@@ -432,7 +472,7 @@ __global__ __launch_bounds__(kMergeThreads) void q4_step_merge(const AttnQ4Args 
 template <int HD, typename T>
 void launch_typed(const AttnQ4Args &a, hipStream_t s) {
     const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
-    hipLaunchKernelGGL((q4_step<HD, T>), dim3(a.splits, heads), dim3(kStepThreads), 0, s, a);
+    hipLaunchKernelGGL((q4_step<HD, T>), dim3(heads, a.splits), dim3(kStepThreads), 0, s, a);
     if (a.part) {
         const int chunks = a.weights ? (a.c.maxp + kMergeRows - 1) / kMergeRows : 0;
         hipLaunchKernelGGL(q4_step_merge<HD>, dim3(a.group + chunks, heads), dim3(kMergeThreads), 0, s, a);

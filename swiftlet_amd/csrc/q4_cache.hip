@@ -45,7 +45,9 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
 #pragma unroll
             for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(kin, at + e));
             const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, row - r0)) * half : nullptr;
-            q4_key_row<HD>(x, a.w, a.eps, turn, half, s_rot[wave], kw, par, a.c.R, row);
+            Q4HeadTable<EPL> tab;
+            tab.load(a.w, turn, half);
+            q4_key_row<HD>(x, tab, a.eps, half, s_rot[wave], kw, par, a.c.R, row);
 #pragma unroll
             for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(vin, at + e));
             q4_value_row<HD>(x, q, par, a.c.R, row);

@@ -6,10 +6,50 @@
 
 namespace swq {
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = dpp_u32<CTRL>(static_cast<uint32_t>(u)), hi = dpp_u32<CTRL>(static_cast<uint32_t>(u >> 32));
+    return __builtin_bit_cast(double, lo | (hi << 32));
+}
+
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
+    return __builtin_bit_cast(double, lo | (static_cast<uint64_t>(hi) << 32));
+}
+
+// op over LANES consecutive lanes (16, 32 or 64), to each of them: through DPP within 16, then
+// through scalar registers (a ds_bpermute per step and half costs four times as long).
+template <int LANES, typename Op>
+__device__ __forceinline__ double reduce_f64(double v, Op op) {
+    v = op(v, dpp_f64<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = op(v, dpp_f64<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = op(v, dpp_f64<0x141>(v));  // row_half_mirror
+    v = op(v, dpp_f64<0x140>(v));  // row_mirror
+    if constexpr (LANES > 16) {
+        const double a = op(lane_f64(v, 0), lane_f64(v, 16)), b = op(lane_f64(v, 32), lane_f64(v, 48));
+        v = LANES == 64 ? op(a, b) : (threadIdx.x & 32 ? b : a);
+    }
     return v;
 }
+
+// This lane's elements of a norm weight and of the rotation at them: element i < 2 * half turns with
+// its partner i +- half by angle i % half.
+template <int EPL>
+struct Q4HeadTable {
+    float w[EPL];
+    float2 cs[EPL];
+    __device__ __forceinline__ void load(const float *weight, const float2 *turn, int half) {
+        const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int i = lane * EPL + e;
+            w[e] = weight[i];
+            cs[e] = half > 0 ? turn[i < half ? i : i < 2 * half ? i - half : 0] : make_float2(1.f, 0.f);
+        }
+    }
+};
 
 // f16 by way of f32, both roundings as the format has them: the compiler would make one of the two.
 __device__ __forceinline__ _Float16 f16_by_f32(double x) {
@@ -30,10 +70,8 @@ __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q
         lo = fmin(lo, y[e]);
         hi = fmax(hi, y[e]);
     }
-    for (int off = kQ4Group / EPL / 2; off > 0; off >>= 1) {
-        lo = fmin(lo, __shfl_xor(lo, off, kWave));
-        hi = fmax(hi, __shfl_xor(hi, off, kWave));
-    }
+    lo = reduce_f64<kQ4Group / EPL>(lo, [](double a, double b) { return fmin(a, b); });
+    hi = reduce_f64<kQ4Group / EPL>(hi, [](double a, double b) { return fmax(a, b); });
     bias = f16_by_f32(lo);
     scale = f16_by_f32((hi - lo) / 15.0);
     const double b = static_cast<double>(static_cast<float>(bias)), s = static_cast<double>(static_cast<float>(scale));
@@ -54,20 +92,20 @@ __device__ __forceinline__ void q4_put_params(_Float16 *par, int64_t R, int whic
 }
 
 // A key: x / rms * w, turned, quantised, its words and parameters written.  lds: HD doubles of this
-// wave; turn: the position's cos and sin, `half` of them.
+// wave; half: of the rotated dims.
 template <int HD>
-__device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const float *w, float eps, const float2 *turn, int half,
+__device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const Q4HeadTable<HD / kWave> &tab, float eps, int half,
                                            double *lds, uint32_t *kw, _Float16 *par, int64_t R, int64_t row) {
     constexpr int EPL = HD / kWave;
     const int lane = threadIdx.x & (kWave - 1);
     double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
-    ss = wave_sum_f64(ss);
+    ss = reduce_f64<kWave>(ss, [](double a, double b) { return a + b; });
     const double root = sqrt(ss / HD + static_cast<double>(eps));
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-        x[e] = x[e] / root * static_cast<double>(w[lane * EPL + e]);
+        x[e] = x[e] / root * static_cast<double>(tab.w[e]);
         lds[lane * EPL + e] = x[e];
     }
     __builtin_amdgcn_wave_barrier();
@@ -77,9 +115,8 @@ __device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const float 
         for (int e = 0; e < EPL; ++e) {
             const int i = lane * EPL + e;
             if (i < 2 * half) {
-                const float2 cs = turn[i < half ? i : i - half];
                 const double o = lds[i < half ? i + half : i - half];
-                const double c = static_cast<double>(cs.x), s = static_cast<double>(cs.y);
+                const double c = static_cast<double>(tab.cs[e].x), s = static_cast<double>(tab.cs[e].y);
                 x[e] = i < half ? x[e] * c - o * s : x[e] * c + o * s;
             }
         }
@@ -91,7 +128,9 @@ __device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const float 
     q4_quantise<EPL>(x, q, scale, bias);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) word |= q[e] << (4 * ((lane * EPL + e) & 7));
-    for (int off = 8 / EPL / 2; off > 0; off >>= 1) word |= __shfl_xor(word, off, kWave);
+    word |= dpp_u32<0xB1>(word);  // the lanes of one word: 2, 4 or 8
+    if constexpr (EPL <= 2) word |= dpp_u32<0x4E>(word);
+    if constexpr (EPL == 1) word |= dpp_u32<0x141>(word);
     if (lane % (8 / EPL) == 0) kw[row * (HD / 8) + lane * EPL / 8] = word;
     q4_put_params<HD>(par, R, kQ4KScale, row, scale, bias);
 }
