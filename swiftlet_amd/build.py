@@ -40,9 +40,10 @@ def sources() -> list[Path]:
 
 
 # Per-file code generation options.  The MFMA kernels keep their results in
-# VGPRs: the per-group scale is applied by VALU right after each product, and
-# results in AGPRs would each cost a copy back.
-FILE_FLAGS = {"moe_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# VGPRs: scales, softmax and rescaling work on them by VALU right after each
+# product, and results in AGPRs would each cost a copy back.
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+              for name in ("moe_prefill.hip", "attention_q4_step.hip", "attention_q4_prefill.hip")}
 
 
 def _compile(src: Path) -> Path:

@@ -165,7 +165,7 @@ StepParts step_parts(const swq_attention_layer *l, const swq_q4_cache *c, int se
 }
 
 size_t q4_step_workspace(const swq_attention_layer *l, const swq_q4_cache *c, const swq_q4_batch *b, int weights) {
-    return step_parts(l, c, b->sequences, most_q4_splits(c->max_positions, static_cast<int64_t>(b->sequences) * c->num_kv_heads), weights != 0).total;
+    return step_parts(l, c, b->sequences, most_q4_splits(c->max_positions, static_cast<int64_t>(b->sequences) * c->num_kv_heads, c->head_dim), weights != 0).total;
 }
 
 size_t q4_prompt_workspace(const swq_attention_layer *l, const swq_q4_batch *b) {
@@ -195,9 +195,9 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     if (static_cast<int64_t>(batch->sequences) * layer->num_heads > 65535) return SWQ_ERR_LIMIT;
     if (batch->tokens == 0) return SWQ_OK;
     if (!q_proj || !out || !k_proj != !v_proj) return SWQ_ERR_INVALID_ARGUMENT;
-    const size_t in = q4_dtype_bytes(dtype);
-    if (reinterpret_cast<uintptr_t>(q_proj) % in || reinterpret_cast<uintptr_t>(k_proj) % in ||
-        reinterpret_cast<uintptr_t>(v_proj) % in || reinterpret_cast<uintptr_t>(out) % q4_dtype_bytes(out_dtype) ||
+    if (reinterpret_cast<uintptr_t>(q_proj) % 16 || reinterpret_cast<uintptr_t>(k_proj) % 16 ||
+        reinterpret_cast<uintptr_t>(v_proj) % 16 || reinterpret_cast<uintptr_t>(out) % 16 ||
+        reinterpret_cast<uintptr_t>(layer->q_norm_weight) % 16 ||
         reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(ws) % 256)
         return SWQ_ERR_MISALIGNED;
     if (!ws || ws_bytes < swq_attention_q4_workspace_bytes(layer, cache, batch, weights != nullptr)) return SWQ_ERR_WORKSPACE;
@@ -222,7 +222,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     uint8_t *p = static_cast<uint8_t *>(ws);
     if (a.b.max_tokens == 1) {
         const int64_t rows = batch->max_rows > 0 ? std::min(batch->max_rows, cache->max_positions) : cache->max_positions;
-        const Q4StepPlan plan = plan_q4_step(rows, static_cast<int64_t>(a.b.B) * a.c.KVH);
+        const Q4StepPlan plan = plan_q4_step(rows, static_cast<int64_t>(a.b.B) * a.c.KVH, a.c.hd);
         const StepParts parts = step_parts(layer, cache, a.b.B, plan.splits, weights != nullptr);
         a.per = plan.per;
         a.splits = plan.splits;

@@ -125,8 +125,8 @@ __device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const Q4HeadTable<
 struct Q4StepPlan {
     int per, splits;
 };
-Q4StepPlan plan_q4_step(int64_t rows, int64_t heads);
-int most_q4_splits(int64_t rows, int64_t heads);  // of any number of rows up to this
+Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd);
+int most_q4_splits(int64_t rows, int64_t heads, int hd);  // of any number of rows up to this
 void launch_q4_step(const AttnQ4Args &a, hipStream_t s);
 
 }  // namespace swq

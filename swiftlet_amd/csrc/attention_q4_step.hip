@@ -9,77 +9,151 @@ namespace {
 
 constexpr int kStepThreads = 256;
 constexpr int kStepWaves = kStepThreads / kWave;
-constexpr int kTile = 32;    // rows of one step of a wave
+constexpr int kTile = 32;    // rows of one step of a team
 constexpr int kHeadPad = 4;  // floats between heads' sums in LDS
 
-// One tile's words and parameters, as loaded: lane (r = lane % 16, q = lane / 16).
-template <int NG>
+// What one wave reads of a tile: GW * 64 dims of 32 rows; lane (r = lane % 16, q = lane / 16).
+template <int GW>
 struct Q4Tile {
-    uint2 k[2][NG];   // row 8 (r / 4) + 4 t + r % 4, words 2 q and 2 q + 1 of each group
-    uint4 v[NG];      // rows 8 q .. 8 q + 7, dims 4 r .. 4 r + 3 of each group
-    uint4 par[4][NG]; // rows 8 q .. 8 q + 7: k scale, k bias, v scale, v bias
+    uint2 k[GW][2];    // row 8 (r / 4) + 4 t + r % 4, words 2 q and 2 q + 1 of each group
+    uint4 v[GW];       // rows 8 q .. 8 q + 7, dims 4 r .. 4 r + 3 of each group
+    uint4 par[4][GW];  // rows 8 q .. 8 q + 7: k scale, k bias, v scale, v bias
 };
 
+// 8 consecutive numbers, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const T *p) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+}
+
+// Sum and maximum over L consecutive lanes (8, 16 or 32), to each of them.
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += dpp<0xB1, 0xF, true>(v);
+    v += dpp<0x4E, 0xF, true>(v);
+    v += dpp<0x141, 0xF, true>(v);
+    if constexpr (L >= 16) v += dpp<0x140, 0xF, true>(v);
+    if constexpr (L >= 32) v += __shfl_xor(v, 16, kWave);
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, dpp<0xB1, 0xF, true>(v));
+    v = fmaxf(v, dpp<0x4E, 0xF, true>(v));
+    v = fmaxf(v, dpp<0x141, 0xF, true>(v));
+    if constexpr (L >= 16) v = fmaxf(v, dpp<0x140, 0xF, true>(v));
+    if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return v;
+}
+
+// Four dims of head u: to the partial results of `split`, or, of the only one, to the output.
 template <int HD, typename T>
-__global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void q4_step(const AttnQ4Args a) {
-    constexpr int EPL = HD / kWave, NG = HD / kQ4Group, KS = HD / 32;
+__device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n0, int h0, int u, int split, int d, f4_t s, float M, float L) {
+    if (a.part) {
+        *reinterpret_cast<f4_t *>(a.part + ((head0 + u) * a.splits + split) * HD + d) = s;
+        if (d == 0) a.ml[(head0 + u) * a.splits + split] = make_float2(M, L);
+    } else {
+        const int64_t at = static_cast<int64_t>(n0) * a.H + h0 + u;
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            y[e] = s[e] / L * sigmoid_exact(q4_load(static_cast<const T *>(a.q), (2 * at + 1) * HD + d + e));
+        if (a.out_f32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at * HD + d) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q4_store(static_cast<uint16_t *>(a.out), at * HD + d + e, y[e]);
+        }
+    }
+}
+
+// A wave has GW groups of 64 dims of the head (groups as the cache's scales have them): the whole
+// head at hd 64 and 128, half of it at 256.  The waves of a head, a team, walk the same tiles, the
+// teams of a workgroup different ones.  A step of a team:
+//   scores  K's codes are the left operand (rows: 16 of the tile's 32 positions, twice), the queries
+//           of the kv head's group the right one (columns: heads): lane (h, q) gets head h's sums of
+//           positions 8 q .. 8 q + 7, times scale, plus bias * the sum of the query's dims.  Where a
+//           team is two waves their partial scores meet in LDS, a barrier a step (two buffers);
+//   softmax online, on both waves of the team alike.  p is taken against the running maximum and
+//           against the largest value scale so far, so that p * scale fits f16;
+//   values  V's codes are the left operand (rows: dims), p * scale the right one (columns: heads),
+//           straight from the registers that the scores left: no transpose, and the running
+//           maximum's factor is the lane's own.  p * bias is summed on the VALU.
+// Heads past the group are columns that nothing reads.  The next tile's loads are issued as soon as
+// their registers are free.
+template <int HD, typename T>
+__global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const AttnQ4Args a) {
+    constexpr int EPL = HD / kWave, NG = HD / kQ4Group, GW = NG > 1 ? 2 : 1, TW = NG / GW, TEAMS = kStepWaves / TW;
     constexpr int HP = HD + kHeadPad;
-    constexpr int kQBytes = 2 * KS * kWave * 16, kOBytes = kStepWaves * kQ4MaxHeadGroup * HP * 4;
-    // queries in operand order (used up to the last tile), then the waves' sums
-    __shared__ __attribute__((aligned(16))) uint8_t s_buf[kQBytes > kOBytes ? kQBytes : kOBytes];
+    __shared__ h8_t s_q[2][NG][2][kWave];  // queries in operand order: [high, low][group][step][lane]
     __shared__ float s_qs[NG][kQ4MaxHeadGroup], s_f[kQ4MaxHeadGroup];
-    __shared__ float s_rl[kStepWaves][2][kQ4MaxHeadGroup];
-    __shared__ double s_rot[kStepWaves][HD];
-    h8_t *s_q = reinterpret_cast<h8_t *>(s_buf);  // [plane][kstep][lane]
-    float *s_o = reinterpret_cast<float *>(s_buf);  // [wave][head][HP]
+    __shared__ float s_ml[TEAMS][2][kQ4MaxHeadGroup];
+    // one after another, a barrier between them: heads to be rotated, partial scores, teams' sums
+    constexpr int kRotWave = 256;  // doubles of a wave: a key, or all the heads that it takes at once
+    constexpr int kRot = kStepWaves * kRotWave * 8, kPart = TW > 1 ? 2 * kStepWaves * 2 * kWave * 16 : 0;
+    constexpr int kSums = TEAMS * kQ4MaxHeadGroup * HP * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[kRot > kPart ? (kRot > kSums ? kRot : kSums) : (kPart > kSums ? kPart : kSums)];
+    double(*s_rot)[kRotWave] = reinterpret_cast<double(*)[kRotWave]>(s_buf);
+    f4_t(*s_part)[kStepWaves][2][kWave] = reinterpret_cast<f4_t(*)[kStepWaves][2][kWave]>(s_buf);
+    float *s_o = reinterpret_cast<float *>(s_buf);  // [team][head][HP]
     // Workgroups go to the 8 XCDs in turn: with the splits outermost and the heads turned by one from
     // split to split, no XCD gets the same splits, or the same sequences, of every head.
     const int split = blockIdx.y, head = (blockIdx.x + blockIdx.y) % gridDim.x;
     const int kvh = head % a.c.KVH, b = head / a.c.KVH;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int r = lane & 15, q = lane >> 4, G = a.group;
+    const int g0 = wave % TW * GW, team = wave / TW;  // first group
     if (a.b.count(b) <= 0) return;
     const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
     const int n = min(r0 + 1, a.c.maxp);  // rows that the token sees
     const int p0 = split * a.per, p1 = split == a.splits - 1 ? n : min(p0 + a.per, n);
     if (p0 >= n) return;
     const bool last = p1 == n;
-    // In the last split two waves write the token's row before they, or another, load its tile.
+    // In the last split two waves write the token's row before its tile is loaded.
     const bool writes = a.k && last && r0 < a.c.maxp;
     const int end = (p1 - p0 + kTile - 1) / kTile;  // tiles
-    int tile = wave;
 
-    const uint32_t *kw = a.c.k_head(b, kvh), *vw = a.c.v_head(b, kvh);
-    const _Float16 *par = a.c.par_head(b, kvh);
-    Q4Tile<NG> cur;
+    const uint32_t *kw = a.c.k_head(b, kvh) + (8 * (r >> 2) + (r & 3)) * (HD / 8) + 8 * g0 + 2 * q;
+    const uint32_t *vw = a.c.v_head(b, kvh) + q * HD + 64 * g0 + 4 * r;
+    const _Float16 *par = a.c.par_head(b, kvh) + static_cast<int64_t>(g0) * a.c.R + 8 * q;
+    Q4Tile<GW> cur;
     auto load_k = [&](int t) {
         const int64_t t0 = p0 + static_cast<int64_t>(t) * kTile;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int g = 0; g < GW; ++g) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-                cur.k[x][g] = *reinterpret_cast<const uint2 *>(kw + (t0 + 8 * (r >> 2) + 4 * x + (r & 3)) * (HD / 8) + 8 * g + 2 * q);
+            for (int x = 0; x < 2; ++x) cur.k[g][x] = *reinterpret_cast<const uint2 *>(kw + (t0 + 4 * x) * (HD / 8) + 8 * g);
 #pragma unroll
-        for (int w = kQ4KScale; w <= kQ4KBias; ++w)
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0 + 8 * q);
+            for (int w = kQ4KScale; w <= kQ4KBias; ++w)
+                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0);
+        }
     };
     auto load_v = [&](int t) {
         const int64_t t0 = p0 + static_cast<int64_t>(t) * kTile;
 #pragma unroll
-        for (int w = kQ4VScale; w <= kQ4VBias; ++w)
+        for (int g = 0; g < GW; ++g) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0 + 8 * q);
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-            cur.v[g] = *reinterpret_cast<const uint4 *>(vw + (t0 / 8 + q) * HD + 64 * g + 4 * r);
+            for (int w = kQ4VScale; w <= kQ4VBias; ++w)
+                cur.par[w][g] = *reinterpret_cast<const uint4 *>(par + (static_cast<int64_t>(w) * NG + g) * a.c.R + t0);
+            cur.v[g] = *reinterpret_cast<const uint4 *>(vw + t0 / 8 * HD + 64 * g);
+        }
     };
-    const bool waits = writes && tile == end - 1;  // its first tile is the one with the new row
-    if (tile < end && !waits) {
-        load_k(tile);
-        load_v(tile);
+    const bool waits = writes && team >= end - 1;  // its first tile is the one with the new row
+    if (!waits) {
+        load_k(min(team, end - 1));
+        load_v(min(team, end - 1));
     }
 
     const int half = a.b.rot / 2;
@@ -109,108 +183,143 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
             for (int e = 0; e < EPL; ++e) vp[e] = (old[e] & ~(15u << sh)) | (code[e] << sh);
         }
     } else {
-        constexpr int AT_ONCE = 4;  // heads of a wave whose loads are in flight together
-        Q4HeadTable<EPL> tab;
-        tab.load(a.q_norm_w, turn, half);
-        for (int base = 0; base < G; base += AT_ONCE * askers) {
-            float x[AT_ONCE][EPL];
+        // 8 dims per lane, a word's: HD / 8 lanes per head, 512 / HD heads of a wave at once
+        constexpr int LPH = HD / 8, HPW = kWave / LPH;
+        const int j = lane % LPH;
+        float w[8];
+        float2 cs[8];
+        load8<float>(w, a.q_norm_w + 8 * j);
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) {
-                const int u = min(base + k * askers + wave, G - 1);
-                const T *src = static_cast<const T *>(a.q) + (static_cast<int64_t>(n0) * a.H + kvh * G + u) * 2 * HD + lane * EPL;
+        for (int e = 0; e < 8; ++e) {
+            const int i = 8 * j + e;
+            cs[e] = half > 0 ? turn[i < half ? i : i < 2 * half ? i - half : 0] : make_float2(1.f, 0.f);
+        }
+        float *lds = reinterpret_cast<float *>(s_rot[wave]) + lane / LPH * HD;
+        for (int base = 0; base < G; base += askers * HPW) {
+            const int u = base + wave * HPW + lane / LPH;
+            float x[8];
+            load8<T>(x, static_cast<const T *>(a.q) + (static_cast<int64_t>(n0) * a.H + kvh * G + min(u, G - 1)) * 2 * HD + 8 * j);
+            float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) x[k][e] = q4_load(src, e);
+            for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+            ss = lanes_sum<LPH>(ss);
+            const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] *= sc * w[e];
+                lds[8 * j + e] = x[e];
             }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            float top = 0.f;
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) {
-                const int u = base + k * askers + wave;
-                if (u >= G) break;
-                q4_norm_rope<EPL>(x[k], tab, a.eps, half, reinterpret_cast<float *>(s_rot[wave]));
-                float top = 0.f, qs = 0.f;
+            for (int e = 0; e < 8; ++e) {
+                const int i = 8 * j + e;
+                const float o = lds[i < half ? i + half : i < 2 * half ? i - half : i];
+                if (i < 2 * half) x[e] = i < half ? x[e] * cs[e].x - o * cs[e].y : x[e] * cs[e].x + o * cs[e].y;
+                top = fmaxf(top, fabsf(x[e]));
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            top = lanes_max<LPH>(top);
+            int ex = 0;
+            if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+            float qs = 0.f;
+            h8_t hi, lo;
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) top = fmaxf(top, fabsf(x[k][e]));
-                top = wave_max_all(top);
-                int ex = 0;
-                if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-#pragma unroll
-                for (int e = 0; e < EPL; ++e) {
-                    x[k][e] = ldexpf(x[k][e], 10 - ex);  // below 2^10
-                    qs += x[k][e];
-                }
-                if (lane == 0) s_f[u] = ldexpf(a.scale2, ex - 10);
-                qs = segment_sum(qs, kQ4Group / EPL);
-                if (lane % (kQ4Group / EPL) == 0) s_qs[lane * EPL / kQ4Group][u] = qs;
-#pragma unroll
-                for (int e = 0; e < EPL; ++e) {
-                    const int d = lane * EPL + e, j = (d & 63) >> 3, nb = d & 7;  // word of its group, nibble
-                    const float v = nb & 1 ? x[k][e] * 0.0625f : x[k][e];
-                    const _Float16 hi = static_cast<_Float16>(v), lo = static_cast<_Float16>(v - static_cast<float>(hi));
-                    _Float16 *dst = reinterpret_cast<_Float16 *>(s_q + (2 * (d >> 6) + (j & 1)) * kWave + (j >> 1) * 16 + u) + q4_element(nb);
-                    dst[0] = hi;
-                    dst[KS * kWave * 8] = lo;
-                }
+            for (int e = 0; e < 8; ++e) {
+                const float v = ldexpf(x[e], 10 - ex);  // below 2^10
+                qs += v;
+                const float y = e & 1 ? v * 0.0625f : v;
+                hi[q4_element(e)] = static_cast<_Float16>(y);
+                lo[q4_element(e)] = static_cast<_Float16>(y - static_cast<float>(hi[q4_element(e)]));
+            }
+            qs = lanes_sum<8>(qs);
+            if (u < G) {
+                // word j % 8 of group j / 8: lane row (j % 8) / 2 of step j % 2
+                s_q[0][j / 8][j & 1][((j & 7) >> 1) * 16 + u] = hi;
+                s_q[1][j / 8][j & 1][((j & 7) >> 1) * 16 + u] = lo;
+                if ((j & 7) == 0) s_qs[j / 8][u] = qs;
+                if (j == 0) s_f[u] = ldexpf(a.scale2, ex - 10);
             }
         }
     }
-    // heads past the group are columns of their own in both products: what they hold reaches nothing
     if (writes) __syncthreads();  // the row's stores are done
     else lds_barrier();
     if (waits) {
-        load_k(tile);
-        load_v(tile);
+        load_k(min(team, end - 1));
+        load_v(min(team, end - 1));
     }
 
-    float qs[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) qs[g] = s_qs[g][r];
     const float f = r < G ? s_f[r] : 0.f;
-    float m = -INFINITY, l = 0.f, ref = -INFINITY, cap = 0.f, ce = -24.f;  // 2^ce bounds the value scales so far
-    float pb[NG];
-    f4_t o[NG][4];
+    float qs[GW], pb[GW];
+    f4_t o[GW][4];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
+    for (int g = 0; g < GW; ++g) {
+        qs[g] = s_qs[g0 + g][r];
         pb[g] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[g][e] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
-    float *sc_out = a.scores && r < G ? a.scores + (static_cast<int64_t>(b) * a.H + kvh * G + r) * a.c.R : nullptr;
-    constexpr int stride = kStepWaves;
+    float m = -INFINITY, l = 0.f, ref = -INFINITY, cap = 0.f, ce = -24.f;  // 2^ce bounds the value scales so far
+    float *sc_out = a.scores && r < G && g0 == 0 ? a.scores + (static_cast<int64_t>(b) * a.H + kvh * G + r) * a.c.R : nullptr;
     const uint32_t magic = kept_1024();
-    for (; tile < end; tile += stride) {
-        const int t0 = p0 + tile * kTile;
-        // scores; the queries come from LDS each time, which leaves registers for another wave
-        int ql = lane;
-        asm volatile("" : "+v"(ql));
+    const int steps = (end + TEAMS - 1) / TEAMS;
+    for (int step = 0; step < steps; ++step) {
+        const int tile = step * TEAMS + team, t0 = p0 + tile * kTile;
+        const bool have = tile < end;
+        const int next = min(tile + TEAMS, end - 1);  // past the end the last one again: never used
         float p[8];
+        int ql = lane;  // the queries come from LDS each time, which leaves registers for another wave
+        asm volatile("" : "+v"(ql));
+        if (have) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = 0.f;
+            for (int g = 0; g < GW; ++g) {
+                const h8_t ks = __builtin_bit_cast(h8_t, cur.par[kQ4KScale][g]), kb = __builtin_bit_cast(h8_t, cur.par[kQ4KBias][g]);
+                f4_t d[2];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const h8_t ks = __builtin_bit_cast(h8_t, cur.par[kQ4KScale][g]), kb = __builtin_bit_cast(h8_t, cur.par[kQ4KBias][g]);
+                for (int x = 0; x < 2; ++x) d[x] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const h8_t c = q4_operand(u ? cur.k[g][x].y : cur.k[g][x].x, magic);
+                        d[x] = mfma16(c, s_q[0][g0 + g][u][ql], d[x]);
+                        d[x] = mfma16(c, s_q[1][g0 + g][u][ql], d[x]);
+                    }
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float z = static_cast<float>(kb[4 * x + i]);
+                        p[4 * x + i] = g == 0 ? z * qs[g] : fmaf(z, qs[g], p[4 * x + i]);
+                        p[4 * x + i] = fmaf(static_cast<float>(ks[4 * x + i]), d[x][i], p[4 * x + i]);
+                    }
+            }
+            load_k(next);
+            if constexpr (TW > 1) {
+                s_part[step & 1][wave][0][lane] = f4_t{p[0], p[1], p[2], p[3]};
+                s_part[step & 1][wave][1][lane] = f4_t{p[4], p[5], p[6], p[7]};
+            }
+        }
+        if constexpr (TW > 1) lds_barrier();
+        if (!have) continue;
+        if constexpr (TW > 1) {
+            f4_t sum[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                f4_t d = {0.f, 0.f, 0.f, 0.f};
+                sum[x] = s_part[step & 1][team * TW][x][lane];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const h8_t c = q4_operand(u ? cur.k[x][g].y : cur.k[x][g].x, magic);
-                    d = mfma16(c, s_q[(2 * g + u) * kWave + ql], d);
-                    d = mfma16(c, s_q[(KS + 2 * g + u) * kWave + ql], d);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[4 * x + i] = fmaf(static_cast<float>(kb[4 * x + i]), qs[g], p[4 * x + i]);
-                    p[4 * x + i] = fmaf(static_cast<float>(ks[4 * x + i]), d[i], p[4 * x + i]);
-                }
+                for (int w = 1; w < TW; ++w) sum[x] += s_part[step & 1][team * TW + w][x][lane];
             }
-            if constexpr (NG > 2) __builtin_amdgcn_sched_barrier(0);
-        }
-        const int next = tile + stride < end ? tile + stride : tile;  // the last tile once more: never used
-        load_k(next);
-        if (t0 + kTile > p1) {  // rows past the end count nothing, whatever they hold
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = t0 + 8 * q + i < p1 ? p[i] : -INFINITY;
+            for (int i = 0; i < 8; ++i) p[i] = sum[i / 4][i % 4];
+        }
+        if (t0 + kTile > p1) {  // rows past the end count nothing, whatever they hold
             uint4 keep;
             const int left = p1 - t0 - 8 * q;  // of this lane's 8 rows
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = i < left ? p[i] : -INFINITY;
             keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
             keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
             keep.z = (left > 4 ? 0xFFFFu : 0u) | (left > 5 ? 0xFFFF0000u : 0u);
@@ -218,7 +327,7 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
 #pragma unroll
             for (int w = kQ4VScale; w <= kQ4VBias; ++w)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
+                for (int g = 0; g < GW; ++g) {
                     cur.par[w][g].x &= keep.x;
                     cur.par[w][g].y &= keep.y;
                     cur.par[w][g].z &= keep.z;
@@ -232,12 +341,12 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
         float mt = f * fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
         h2_t st = {static_cast<_Float16>(0.f), static_cast<_Float16>(0.f)};
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 u = cur.par[kQ4VScale][g];
-                st = __builtin_elementwise_max(st, __builtin_bit_cast(h2_t, i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w));
-            }
+        for (int g = 0; g < GW; ++g) {
+            const uint4 u = cur.par[kQ4VScale][g];
+            st = __builtin_elementwise_max(st, __builtin_elementwise_max(
+                __builtin_elementwise_max(__builtin_bit_cast(h2_t, u.x), __builtin_bit_cast(h2_t, u.y)),
+                __builtin_elementwise_max(__builtin_bit_cast(h2_t, u.z), __builtin_bit_cast(h2_t, u.w))));
+        }
         float top = fmaxf(static_cast<float>(st.x), static_cast<float>(st.y));
         if (__any(mt > m || top > cap)) {
             mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
@@ -255,7 +364,7 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
             ref = to;
             l *= alpha;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
+            for (int g = 0; g < GW; ++g) {
                 pb[g] *= alpha;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[g][e] *= alpha;
@@ -269,9 +378,8 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
         float pe[8];  // in operand order, 1/16 where the codes are 16 times as large
 #pragma unroll
         for (int j = 0; j < 8; ++j) pe[j] = q4_nibble(j) & 1 ? p[q4_nibble(j)] * 0.0625f : p[q4_nibble(j)];
-        // values
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
+        for (int g = 0; g < GW; ++g) {
             const h8_t vs = __builtin_bit_cast(h8_t, cur.par[kQ4VScale][g]), vb = __builtin_bit_cast(h8_t, cur.par[kQ4VBias][g]);
             h8_t hi, lo;
 #pragma unroll
@@ -293,68 +401,50 @@ __global__ __launch_bounds__(kStepThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) vo
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) pb[g] = fmaf(p[i], static_cast<float>(vb[i]), pb[g]);
-            if constexpr (NG > 2) __builtin_amdgcn_sched_barrier(0);
         }
         load_v(next);
     }
-    // the waves' sums meet
+    // sums over the tile's rows meet, in units of the maximum alone
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
+    for (int g = 0; g < GW; ++g) {
         pb[g] += __shfl_xor(pb[g], 16, kWave);
         pb[g] += __shfl_xor(pb[g], 32, kWave);
     }
-    if (q == 0) {
-        s_rl[wave][0][r] = ref;
-        s_rl[wave][1][r] = l;
-    }
-    lds_barrier();  // and every wave is done with the queries
-    float top = s_rl[0][0][r];
-#pragma unroll
-    for (int w = 1; w < kStepWaves; ++w) top = fmaxf(top, s_rl[w][0][r]);
-    const float mine = q4_exp2(ref - top);
-    float *mo = s_o + (wave * kQ4MaxHeadGroup + r) * HP + 16 * q;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4 v;
-            v.x = mine * (o[g][0][i] + pb[g]);
-            v.y = mine * (o[g][1][i] + pb[g]);
-            v.z = mine * (o[g][2][i] + pb[g]);
-            v.w = mine * (o[g][3][i] + pb[g]);
-            *reinterpret_cast<float4 *>(mo + 64 * g + 4 * i) = v;
-        }
-    lds_barrier();
+    float unit = ref > -INFINITY ? q4_exp2(ce - 15.0f) : 0.f;
+    l *= unit;
     const int64_t head0 = static_cast<int64_t>(b) * a.H + kvh * G;
-    for (int i = tid; i < G * (HD / 4); i += kStepThreads) {
-        const int u = i / (HD / 4), d = i % (HD / 4) * 4;
-        float4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kStepWaves; ++w) {
-            const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * kQ4MaxHeadGroup + u) * HP + d);
-            s.x += v.x;
-            s.y += v.y;
-            s.z += v.z;
-            s.w += v.w;
+    {
+        if (q == 0 && g0 == 0) {
+            s_ml[team][0][r] = m;
+            s_ml[team][1][r] = l;
         }
-        float R = s_rl[0][0][u], L = 0.f;
+        lds_barrier();
+        float M = s_ml[0][0][r], L = 0.f;
 #pragma unroll
-        for (int w = 1; w < kStepWaves; ++w) R = fmaxf(R, s_rl[w][0][u]);
+        for (int w = 1; w < TEAMS; ++w) M = fmaxf(M, s_ml[w][0][r]);
+        unit *= q4_exp2(m - M);
+        float *mo = s_o + (team * kQ4MaxHeadGroup + r) * HP + 64 * g0 + 16 * q;
 #pragma unroll
-        for (int w = 0; w < kStepWaves; ++w) L += q4_exp2(s_rl[w][0][u] - R) * s_rl[w][1][u];
-        if (a.part) {
-            *reinterpret_cast<float4 *>(a.part + ((head0 + u) * a.splits + split) * HD + d) = s;
-            if (d == 0) a.ml[(head0 + u) * a.splits + split] = make_float2(R, L);
-        } else {
-            const int64_t at = static_cast<int64_t>(n0) * a.H + kvh * G + u;
-            const float v[4] = {s.x, s.y, s.z, s.w};
+        for (int g = 0; g < GW; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float gate = q4_load(static_cast<const T *>(a.q), (2 * at + 1) * HD + d + e);
-                q4_store_any(a.out, at * HD + d + e, v[e] / L * sigmoid_exact(gate), a.out_f32);
-            }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(mo + 64 * g + 4 * i) = make_float4(unit * (o[g][0][i] + pb[g]), unit * (o[g][1][i] + pb[g]),
+                                                                              unit * (o[g][2][i] + pb[g]), unit * (o[g][3][i] + pb[g]));
+        lds_barrier();
+        for (int i = tid; i < G * (HD / 4); i += kStepThreads) {
+            const int u = i / (HD / 4), d = i % (HD / 4) * 4;
+            f4_t s = *reinterpret_cast<const f4_t *>(s_o + u * HP + d);
+#pragma unroll
+            for (int w = 1; w < TEAMS; ++w) s += *reinterpret_cast<const f4_t *>(s_o + (w * kQ4MaxHeadGroup + u) * HP + d);
+            M = s_ml[0][0][u];
+            L = 0.f;
+#pragma unroll
+            for (int w = 1; w < TEAMS; ++w) M = fmaxf(M, s_ml[w][0][u]);
+#pragma unroll
+            for (int w = 0; w < TEAMS; ++w) L += q4_exp2(s_ml[w][0][u] - M) * s_ml[w][1][u];
+            finish<HD, T>(a, head0, n0, kvh * G, u, split, d, s, M, L);
         }
     }
 }
@@ -481,18 +571,23 @@ void launch_typed(const AttnQ4Args &a, hipStream_t s) {
 
 }  // namespace
 
-Q4StepPlan plan_q4_step(int64_t rows, int64_t heads) {
+// Rows of one step of a workgroup: a tile of each team.
+static int64_t step_unit(int hd) { return hd == 256 ? 2 * kTile : 4 * kTile; }
+
+Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd) {
+    const int64_t unit = step_unit(hd);
     const int64_t total = rows * heads;
     int64_t per = std::min(total / 512, std::max<int64_t>(512, total / 2048));
-    per = std::max<int64_t>((per + 127) / 128 * 128, 128);
+    per = std::max<int64_t>((per + unit - 1) / unit * unit, unit);
     per = std::max<int64_t>(per, (rows + kMaxSplits - 1) / kMaxSplits);
     per = (per + kTile - 1) / kTile * kTile;
     return {static_cast<int>(per), static_cast<int>((rows + per - 1) / per)};
 }
 
-int most_q4_splits(int64_t rows, int64_t heads) {
-    // rows per split are at least 128, and at least a 2,048th of rows * heads
-    return static_cast<int>(std::min<int64_t>({(rows + 127) / 128, 2048 / heads + 2, kMaxSplits}));
+int most_q4_splits(int64_t rows, int64_t heads, int hd) {
+    const int64_t unit = step_unit(hd);
+    // rows per split are at least a step's, and at least a 2,048th of rows * heads
+    return static_cast<int>(std::min<int64_t>({(rows + unit - 1) / unit, 2048 / heads + 2, kMaxSplits}));
 }
 
 void launch_q4_step(const AttnQ4Args &a, hipStream_t s) {

@@ -315,7 +315,7 @@ extern "C" int swq_q4_append(const swq_attention_layer *layer, const swq_q4_cach
     if (st != SWQ_OK) return st;
     if (batch->tokens == 0) return SWQ_OK;
     if (!k_proj || !v_proj) return SWQ_ERR_INVALID_ARGUMENT;
-    if (reinterpret_cast<uintptr_t>(k_proj) % q4_dtype_bytes(dtype) || reinterpret_cast<uintptr_t>(v_proj) % q4_dtype_bytes(dtype))
+    if (reinterpret_cast<uintptr_t>(k_proj) % 16 || reinterpret_cast<uintptr_t>(v_proj) % 16)
         return SWQ_ERR_MISALIGNED;
     launch_q4_append(layer, q4_view(cache), q4_batch(layer, batch), k_proj, v_proj, dtype, static_cast<hipStream_t>(stream));
     return launch_status();
@@ -328,7 +328,7 @@ extern "C" int swq_q4_read(const swq_q4_cache *cache, int sequences, const int32
     if (st != SWQ_OK) return st;
     if (sequences <= 0 || count < 0 || (!k && !v)) return SWQ_ERR_INVALID_ARGUMENT;
     if (sequences > cache->sequences) return SWQ_ERR_BAD_SHAPE;
-    if (reinterpret_cast<uintptr_t>(k) % q4_dtype_bytes(dtype) || reinterpret_cast<uintptr_t>(v) % q4_dtype_bytes(dtype))
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16)
         return SWQ_ERR_MISALIGNED;
     if (count == 0) return SWQ_OK;
     const ReadArgs a{q4_view(cache), first, starts, rows, count, sequences, k, v};
