@@ -32,15 +32,22 @@ struct AttnQ4Args {
     float *weights;
     int32_t H, group;
     int32_t in_f32, out_f32;  // types of q, k, v and of out: f32, else bf16
-    float eps, scale, scale2;  // 1/sqrt(hd), and times log2(e)
-    // single tokens: rows per split, splits, and their partial results
+    float eps, scale2;        // scale2: 1/sqrt(hd) * log2(e)
+    // the cached rows in splits of `per`, and their partial results, by [row of out][split]: for
+    // single tokens rows are (sequence, query head), for prompts (token, query head)
     int32_t per, splits;
-    float *part;    // [B][H][splits][hd]
-    float2 *ml;     // [B][H][splits]: reference exponent and sum
-    float *scores;  // [B][H][R] in units of log2, for the gathered weights
+    float *part;    // [rows][splits][hd]
+    float2 *ml;     // [rows][splits]: reference exponent and sum
+    float *scores;  // single tokens: [B][H][R] in units of log2, for the gathered weights
     // prompts
-    float *qn;   // [N][H][hd]: normalised, rotated queries
-    float *lse;  // [N][H]: maximum + log of the sum, natural logarithms
+    int32_t planes_q, planes_v;  // f16 parts of queries and keys, and of p and values
+    int32_t tiles, rows_per;     // tiles of (token, head) rows that are started, rows of one
+    int32_t gparts;              // parts of the queries in the gathered weights
+    void *qh, *ql;               // [N][H][hd] f16: queries, high and low part
+    float *qf;                   // [N][H]: what turns a product of them into log2 units
+    uint32_t *vmax;              // [B][KVH][2]: bits of the largest key and value, or NULL
+    float *lse;                  // [N][H]: log2 of the sum of exponentials, or NULL
+    float *gpart;                // [B][KVH][gparts][R]
 };
 
 __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) {
@@ -90,35 +97,63 @@ __device__ __forceinline__ float q4_exp2(float x) { return __builtin_amdgcn_exp2
 
 __device__ __forceinline__ float sigmoid_exact(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-// A head vector, EPL = HD / 64 consecutive elements per lane: times w / rms, its first 2 * half
-// elements turned.  lds: HD floats of this wave.
-template <int EPL>
-__device__ __forceinline__ void q4_norm_rope(float (&x)[EPL], const Q4HeadTable<EPL> &tab, float eps, int half, float *lds) {
-    const int lane = threadIdx.x & (kWave - 1);
-    float ss = 0.f;
+// 8 consecutive numbers, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const T *p) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
-    ss = wave_sum_all(ss);
-    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(EPL * kWave) + eps);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        x[e] *= sc * tab.w[e];
-        lds[lane * EPL + e] = x[e];
-    }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (half > 0) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int i = lane * EPL + e;
-            if (i < 2 * half) {
-                const float o = lds[i < half ? i + half : i - half];
-                x[e] = i < half ? x[e] * tab.cs[e].x - o * tab.cs[e].y : x[e] * tab.cs[e].x + o * tab.cs[e].y;
-            }
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Sum and maximum over L consecutive lanes (8, 16 or 32), to each of them.
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += dpp<0xB1, 0xF, true>(v);
+    v += dpp<0x4E, 0xF, true>(v);
+    v += dpp<0x141, 0xF, true>(v);
+    if constexpr (L >= 16) v += dpp<0x140, 0xF, true>(v);
+    if constexpr (L >= 32) v += __shfl_xor(v, 16, kWave);
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, dpp<0xB1, 0xF, true>(v));
+    v = fmaxf(v, dpp<0x4E, 0xF, true>(v));
+    v = fmaxf(v, dpp<0x141, 0xF, true>(v));
+    if constexpr (L >= 16) v = fmaxf(v, dpp<0x140, 0xF, true>(v));
+    if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return v;
+}
+
+// Four dims, attention * sigmoid(gate), at element `out` of the output; gate: of q_proj.
+__device__ __forceinline__ void store_gated(const AttnQ4Args &a, int64_t out, int64_t gate, f4_t v) {
+    if (a.in_f32) {
+        const float4 g = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + gate);
+        v *= f4_t{sigmoid_exact(g.x), sigmoid_exact(g.y), sigmoid_exact(g.z), sigmoid_exact(g.w)};
+    } else {
+        const uint2 g = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.q) + gate);
+        v *= f4_t{sigmoid_exact(__uint_as_float(g.x << 16)), sigmoid_exact(__uint_as_float(g.x & 0xFFFF0000u)),
+                  sigmoid_exact(__uint_as_float(g.y << 16)), sigmoid_exact(__uint_as_float(g.y & 0xFFFF0000u))};
+    }
+    if (a.out_f32) {
+        *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + out) = v;
+    } else {
+        uint16_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q4_store(u, e, v[e]);
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + out) =
+            make_uint2(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16);
+    }
 }
 
 // Single tokens (attention_q4_step.hip): a split of max_rows rows over workgroups, and its launches.
@@ -128,5 +163,17 @@ struct Q4StepPlan {
 Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd);
 int most_q4_splits(int64_t rows, int64_t heads, int hd);  // of any number of rows up to this
 void launch_q4_step(const AttnQ4Args &a, hipStream_t s);
+
+
+// Several tokens (attention_q4_prefill.hip): how the launches are cut for sequences of up to
+// max_tokens tokens and `rows` rows.
+constexpr int kQ4PrefillMaxSplits = 32;
+constexpr int kQ4GatherMaxParts = 32;
+constexpr int64_t kQ4GatherMost = 4 << 20;  // numbers of all parts' sums
+struct Q4PrefillPlan {
+    int planes_q, planes_v, rows_per, tiles, per, splits, gparts;
+};
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights);
+void launch_q4_prefill(const AttnQ4Args &a, hipStream_t s);
 
 }  // namespace swq

@@ -1,0 +1,594 @@
+// Attention over a 4-bit cache, several tokens per sequence: tiles of (token, query head) rows of one
+// kv head against tiles of cached rows, whose values are unpacked into LDS once for all rows.
+#include <cmath>
+
+#include "attention_q4.hpp"
+
+namespace swq {
+namespace {
+
+constexpr int kPreThreads = 256;
+constexpr int kPreWaves = kPreThreads / kWave;
+constexpr float kLow = -1e30f;  // below every score: exponents against it stay numbers
+
+// ---- queries ----------------------------------------------------------------
+
+// q / rms * w, turned, times a power of two that brings the row's largest below 2^10; as f16 high
+// (and low) parts, the 8 dims of a chunk in the order of a cache word's operand.  8 dims per lane.
+template <int HD, int PQ, typename T>
+__global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
+    constexpr int LPH = HD / 8, HPB = 256 / LPH;
+    __shared__ float s_rot[HPB][HD];
+    const int b = blockIdx.y, tid = threadIdx.x, slot = tid / LPH, j = tid % LPH;
+    if (a.vmax && blockIdx.x == 0)  // for q4_largest
+        for (int u = tid; u < 2 * a.c.KVH; u += 256) a.vmax[a.c.head(b, 0) * 2 + u] = 0;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * HPB + slot;
+    const int cnt = a.b.count(b);
+    const bool here = item < static_cast<int64_t>(cnt) * a.H;
+    const int i = here ? static_cast<int>(item / a.H) : 0, h = here ? static_cast<int>(item % a.H) : 0;
+    const int64_t at = static_cast<int64_t>(a.b.first(b) + i) * a.H + h;
+    if (cnt <= 0) return;
+    float x[8], w[8];
+    load8<T>(x, static_cast<const T *>(a.q) + at * 2 * HD + 8 * j);
+    load8<float>(w, a.q_norm_w + 8 * j);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    ss = lanes_sum<LPH>(ss);
+    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] *= sc * w[e];
+        s_rot[slot][8 * j + e] = x[e];
+    }
+    lds_barrier();
+    const int half = a.b.rot / 2;
+    const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half : nullptr;
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = 8 * j + e;
+        if (d < 2 * half) {
+            const float2 cs = turn[d < half ? d : d - half];
+            const float o = s_rot[slot][d < half ? d + half : d - half];
+            x[e] = d < half ? x[e] * cs.x - o * cs.y : x[e] * cs.x + o * cs.y;
+        }
+        top = fmaxf(top, fabsf(x[e]));
+    }
+    top = lanes_max<LPH>(top);
+    int ex = 0;
+    if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+    h8_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = ldexpf(x[e], 10 - ex);
+        hi[q4_element(e)] = static_cast<_Float16>(v);
+        lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
+    }
+    if (!here) return;
+    reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
+    if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
+    if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 10);
+}
+
+// The largest |bias| + 15 scale of a sequence's keys and of its values, by kv head: what high and low
+// parts are scaled by.  Maxima of non-negative numbers, whose bits order as they do.
+__global__ __launch_bounds__(256) void q4_largest(const AttnQ4Args a) {
+    const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, ng = a.c.hd / kQ4Group;
+    const int cnt = a.b.count(b);
+    if (cnt <= 0) return;
+    const int n = static_cast<int>(min(static_cast<int64_t>(a.b.row0(b, a.c.maxp)) + cnt, static_cast<int64_t>(a.c.maxp)));
+    const _Float16 *par = a.c.par_head(b, h);
+    float top[2] = {0.f, 0.f};
+    for (int row = blockIdx.x * 256 + threadIdx.x; row < n; row += gridDim.x * 256)
+        for (int g = 0; g < ng; ++g)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const float s = static_cast<float>(par[(static_cast<int64_t>(2 * w) * ng + g) * a.c.R + row]);
+                const float z = static_cast<float>(par[(static_cast<int64_t>(2 * w + 1) * ng + g) * a.c.R + row]);
+                top[w] = fmaxf(top[w], fabsf(z) + 15.0f * s);
+            }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const float t = wave_max_all(top[w]);
+        if ((threadIdx.x & (kWave - 1)) == 0 && t > 0.f) atomicMax(a.vmax + 2 * a.c.head(b, h) + w, __float_as_uint(t));
+    }
+}
+
+// The exponent that brings numbers up to `bits` (an f32's) to 2^14 .. 2^15.
+__device__ __forceinline__ int q4_lift(uint32_t bits) {
+    const float t = __uint_as_float(bits);
+    int ex = 0;
+    if (t > 0.f && t < INFINITY) frexpf(t, &ex);
+    return 15 - ex;
+}
+
+// ---- tiles of values in LDS -------------------------------------------------
+
+// Where chunk c (8 numbers) of a line of CH chunks lies, so that the 16 lines that a wave reads at
+// once, and the lines or chunks that it writes, hit different banks.  KEY: lines are cached rows, read
+// in the order 8 (r / 4) + r % 4; else dims, read in order.
+template <int CH, bool KEY>
+__device__ __forceinline__ int q4_place(int line, int c) {
+    int f;
+    if constexpr (KEY) {
+        f = (line & 3) | ((line >> 1) & 12);
+        if constexpr (CH < 16) f >>= 1;
+    } else {
+        f = CH == 4 ? (line >> 2) & 3 : (line >> 1) & 7;
+    }
+    return line * CH + (c ^ f);
+}
+
+// A word's codes times scale plus bias, pairs of nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ void q4_codes(uint32_t w, uint32_t magic, h2_t (&c)[4]) {
+    constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;
+    const uint32_t s = w >> 8;
+    const h2_t off = {static_cast<_Float16>(-1024.f), static_cast<_Float16>(-1024.f)};
+    const h2_t down = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    const h2_t off16 = {static_cast<_Float16>(-64.f), static_cast<_Float16>(-64.f)};
+    c[0] = __builtin_bit_cast(h2_t, (w & kEven) | magic) + off;
+    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(h2_t, (w & kOdd) | magic), down, off16);
+    c[2] = __builtin_bit_cast(h2_t, (s & kEven) | magic) + off;
+    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(h2_t, (s & kOdd) | magic), down, off16);
+}
+
+// One plane: scale * code + bias rounded to f16 once (2^-12 of the value; exact below f16's normal
+// numbers, where all three are multiples of 2^-24).  Two: in f32, times 2^lift, as high and low part.
+template <int PLANES>
+__device__ __forceinline__ void q4_values(uint32_t w, uint32_t magic, const h2_t (&s)[4], const h2_t (&z)[4], float unit, h8_t &hi, h8_t &lo) {
+    h2_t c[4];
+    q4_codes(w, magic, c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (PLANES == 1) {
+            const h2_t v = __builtin_elementwise_fma(c[k], s[k], z[k]);
+            hi[2 * k] = v.x;
+            hi[2 * k + 1] = v.y;
+        } else {
+            const f32x2_t v = {unit * fmaf(static_cast<float>(c[k].x), static_cast<float>(s[k].x), static_cast<float>(z[k].x)),
+                               unit * fmaf(static_cast<float>(c[k].y), static_cast<float>(s[k].y), static_cast<float>(z[k].y))};
+            h2_t h, l;
+            split_f16(v, h, l);
+            hi[2 * k] = h.x;
+            hi[2 * k + 1] = h.y;
+            lo[2 * k] = l.x;
+            lo[2 * k + 1] = l.y;
+        }
+    }
+}
+
+__device__ __forceinline__ h2_t pair_ll(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, (a & 0xFFFFu) | (b << 16)); }
+__device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, (a >> 16) | (b & 0xFFFF0000u)); }
+
+// ---- attention --------------------------------------------------------------
+
+// A workgroup takes M = 64 RT rows (token, query head of the kv head's group; heads of one token next
+// to each other) and the cached rows of one split that the last of them sees, NT at a time.  The tile's
+// words are loaded two tiles ahead into registers, unpacked one tile ahead into the other of two LDS
+// buffers, one barrier per tile.  Each wave has 16 RT rows as columns of both products: scores = K Q
+// (K's rows permuted so that the result's registers are the next operand), out = V^T P, so that
+// maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
+// moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
+template <int HD, int PQ, int PV, int RT, int NT>
+__global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a) {
+    constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * RT * kPreWaves;
+    constexpr int KCH = HD / 8, VCH = NT / 8;
+    constexpr int KW = NT * KCH / kPreThreads, VW = VCH * HD / kPreThreads;  // words per thread
+    __shared__ h8_t s_k[2][PQ][NT * KCH];
+    __shared__ h8_t s_v[2][PV][HD * VCH];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+    const int r = lane & 15, q = lane >> 4, G = a.group;
+    // heads innermost; tiles of rows from the last (most cached rows) down, those of the second half of
+    // the workgroups from the first up, so that the two that share a CU have equal work together
+    const int heads = a.b.B * a.c.KVH;
+    const int head = blockIdx.x % heads, rank = blockIdx.x / heads;
+    const int split = rank % a.splits, order = rank / a.splits;
+    const int up = a.tiles - a.tiles / 2;
+    const int slot = order < up ? a.tiles - 1 - order : order - up;
+    const int kvh = head % a.c.KVH, b = head / a.c.KVH;
+    const int cnt = a.b.count(b);
+    const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
+    const uint32_t all = static_cast<uint32_t>(cnt) * G;  // rows: the host keeps tokens * H below 2^31
+    const uint32_t *kw = a.c.k_head(b, kvh), *vw = a.c.v_head(b, kvh);
+    const _Float16 *par = a.c.par_head(b, kvh);
+    const uint32_t magic = kept_1024();
+    const int seq_rows = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
+    const int klift = PQ == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh)]) : 0, vlift = PV == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh) + 1]) : 0;
+    const float kunit = ldexpf(1.0f, klift), vunit = ldexpf(1.0f, vlift);
+
+    for (uint32_t base = static_cast<uint32_t>(slot) * M; base < all; base += static_cast<uint32_t>(a.tiles) * M) {
+        // rows that the workgroup's last valid one sees, and this split's share of them
+        const uint32_t end_row = min(base + M, all) - 1;
+        const int sees = min(r0 + static_cast<int>(end_row / G) + 1, a.c.maxp);
+        const int kv0 = split * a.per, kv1 = split == a.splits - 1 ? sees : min(kv0 + a.per, sees);
+        if (kv0 >= kv1) continue;
+        // this lane's columns
+        int vis[RT];
+        int64_t at[RT];
+        float f[RT];
+        h8_t qh[RT][KS], ql[PQ == 2 ? RT : 1][PQ == 2 ? KS : 1];
+        int low = 0x7FFFFFFF;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const uint32_t row = min(base + (wave * RT + t) * 16 + r, all - 1), i = row / G;
+            at[t] = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
+            vis[t] = base + (wave * RT + t) * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
+            low = min(low, vis[t]);
+            f[t] = ldexpf(a.qf[at[t]], -klift);
+#pragma unroll
+            for (int u = 0; u < KS; ++u) {
+                qh[t][u] = reinterpret_cast<const h8_t *>(a.qh)[at[t] * KCH + 4 * u + q];
+                if constexpr (PQ == 2) ql[t][u] = reinterpret_cast<const h8_t *>(a.ql)[at[t] * KCH + 4 * u + q];
+            }
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) low = min(low, __shfl_xor(low, off, kWave));
+        low = __builtin_amdgcn_readfirstlane(low);
+        float ref[RT], l[RT];
+        f4_t o[DT][RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            ref[t] = kLow;
+            l[t] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d][t] = f4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
+        uint32_t rk[KW], rv[VW];
+        uint32_t rkp[KW];            // key scale and bias of the word's row
+        uint4 rvs[VW], rvz[VW];      // value scales and biases of the block's rows
+        auto fetch = [&](int t0) {
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const int w = i * kPreThreads + tid, j = w % KCH;
+                const int64_t row = min(t0 + w / KCH, a.c.R - 1);
+                rk[i] = kw[row * KCH + j];
+                const uint16_t *p = reinterpret_cast<const uint16_t *>(par) + static_cast<int64_t>(j / 8) * a.c.R + row;
+                rkp[i] = p[0] | static_cast<uint32_t>(p[static_cast<int64_t>(NG) * a.c.R]) << 16;
+            }
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const int w = __builtin_amdgcn_readfirstlane((i * kPreThreads + tid) / kWave);  // 64 dims of a block
+                const int blk = min(t0 / 8 + w / NG, a.c.R / 8 - 1);
+                rv[i] = vw[static_cast<int64_t>(blk) * HD + w % NG * kWave + lane];
+                const _Float16 *p = par + (static_cast<int64_t>(kQ4VScale) * NG + w % NG) * a.c.R + 8 * static_cast<int64_t>(blk);
+                rvs[i] = *reinterpret_cast<const uint4 *>(p);
+                rvz[i] = *reinterpret_cast<const uint4 *>(p + static_cast<int64_t>(NG) * a.c.R);
+            }
+        };
+        auto unpack = [&](int t0, int buf) {
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const int w = i * kPreThreads + tid, line = w / KCH, j = w % KCH;
+                const h2_t s1 = pair_ll(rkp[i], rkp[i]), z1 = pair_hh(rkp[i], rkp[i]);
+                const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
+                h8_t hi, lo;
+                q4_values<PQ>(rk[i], magic, s, z, kunit, hi, lo);
+                s_k[buf][0][q4_place<KCH, true>(line, j)] = hi;
+                if constexpr (PQ == 2) s_k[buf][1][q4_place<KCH, true>(line, j)] = lo;
+            }
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const int w = i * kPreWaves + wave, blk = w / NG, dim = w % NG * kWave + lane;
+                uint4 us = rvs[i], uz = rvz[i];
+                const int left = seq_rows - (t0 + 8 * blk);
+                if (left < 8) {  // rows past the sequence's: 0, whatever they hold
+                    uint4 keep;
+                    keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
+                    keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
+                    keep.z = (left > 4 ? 0xFFFFu : 0u) | (left > 5 ? 0xFFFF0000u : 0u);
+                    keep.w = (left > 6 ? 0xFFFFu : 0u) | (left > 7 ? 0xFFFF0000u : 0u);
+                    us.x &= keep.x; us.y &= keep.y; us.z &= keep.z; us.w &= keep.w;
+                    uz.x &= keep.x; uz.y &= keep.y; uz.z &= keep.z; uz.w &= keep.w;
+                }
+                const h2_t s[4] = {pair_ll(us.x, us.z), pair_hh(us.x, us.z), pair_ll(us.y, us.w), pair_hh(us.y, us.w)};
+                const h2_t z[4] = {pair_ll(uz.x, uz.z), pair_hh(uz.x, uz.z), pair_ll(uz.y, uz.w), pair_hh(uz.y, uz.w)};
+                h8_t hi, lo;
+                q4_values<PV>(rv[i], magic, s, z, vunit, hi, lo);
+                s_v[buf][0][q4_place<VCH, false>(dim, blk)] = hi;
+                if constexpr (PV == 2) s_v[buf][1][q4_place<VCH, false>(dim, blk)] = lo;
+            }
+        };
+
+        __syncthreads();  // a row tile before this one is done with the buffers
+        fetch(kv0);
+        unpack(kv0, 0);
+        if (kv0 + NT < kv1) fetch(kv0 + NT);
+        int buf = 0;
+        for (int t0 = kv0; t0 < kv1; t0 += NT, buf ^= 1) {
+            lds_barrier();
+            f4_t s[PAIRS][2][RT];
+#pragma unroll
+            for (int pr = 0; pr < PAIRS; ++pr)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) s[pr][x][t] = f4_t{0.f, 0.f, 0.f, 0.f};
+                    const int line = 32 * pr + 8 * (r >> 2) + 4 * x + (r & 3);
+#pragma unroll
+                    for (int u = 0; u < KS; ++u) {
+                        const h8_t kh = s_k[buf][0][q4_place<KCH, true>(line, 4 * u + q)];
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) s[pr][x][t] = mfma16(kh, qh[t][u], s[pr][x][t]);
+                        if constexpr (PQ == 2) {
+                            const h8_t kl = s_k[buf][1][q4_place<KCH, true>(line, 4 * u + q)];
+#pragma unroll
+                            for (int t = 0; t < RT; ++t) {
+                                s[pr][x][t] = mfma16(kh, ql[t][u], s[pr][x][t]);
+                                s[pr][x][t] = mfma16(kl, qh[t][u], s[pr][x][t]);
+                            }
+                        }
+                    }
+                }
+            if (t0 + NT < kv1) {
+                unpack(t0 + NT, buf ^ 1);
+                if (t0 + 2 * NT < kv1) fetch(t0 + 2 * NT);
+            }
+            const bool masked = t0 + NT > low || t0 + NT > kv1;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                float top = -INFINITY;
+                const int lim = min(vis[t], kv1) - t0 - 8 * q;
+#pragma unroll
+                for (int pr = 0; pr < PAIRS; ++pr)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float v = s[pr][x][t][i] * f[t];
+                            if (masked) v = 32 * pr + 4 * x + i < lim ? v : -INFINITY;
+                            s[pr][x][t][i] = v;
+                            top = fmaxf(top, v);
+                        }
+                if (__any(top > ref[t] + 15.0f)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                    const float to = fmaxf(ref[t], top - 7.0f);
+                    const float alpha = q4_exp2(ref[t] - to);
+                    ref[t] = to;
+                    l[t] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[d][t] *= alpha;
+                }
+            }
+            h8_t ph[PAIRS][RT], pl[PV == 2 ? PAIRS : 1][PV == 2 ? RT : 1];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int pr = 0; pr < PAIRS; ++pr) {
+                    float p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        p[i] = q4_exp2(s[pr][i / 4][t][i % 4] - ref[t]);
+                        l[t] += p[i];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const f32x2_t x = {p[q4_nibble(j)], p[q4_nibble(j + 1)]};
+                        h2_t h, w;
+                        if constexpr (PV == 2) {
+                            split_f16(x, h, w);
+                            pl[pr][t][j] = w.x;
+                            pl[pr][t][j + 1] = w.y;
+                        } else {
+                            h = __builtin_convertvector(x, h2_t);
+                        }
+                        ph[pr][t][j] = h.x;
+                        ph[pr][t][j + 1] = h.y;
+                    }
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int pr = 0; pr < PAIRS; ++pr) {
+                    const h8_t vh = s_v[buf][0][q4_place<VCH, false>(16 * d + r, 4 * pr + q)];
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[d][t] = mfma16(vh, ph[pr][t], o[d][t]);
+                    if constexpr (PV == 2) {
+                        const h8_t vl = s_v[buf][1][q4_place<VCH, false>(16 * d + r, 4 * pr + q)];
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) {
+                            o[d][t] = mfma16(vh, pl[pr][t], o[d][t]);
+                            o[d][t] = mfma16(vl, ph[pr][t], o[d][t]);
+                        }
+                    }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            l[t] += __shfl_xor(l[t], 16, kWave);
+            l[t] += __shfl_xor(l[t], 32, kWave);
+            if (base + (wave * RT + t) * 16 + r >= all) continue;
+            const float unit = 1.0f / vunit;
+            if (a.splits > 1) {
+                float *dst = a.part + (at[t] * a.splits + split) * HD + 4 * q;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t *>(dst + 16 * d) = o[d][t] * unit;
+                if (q == 0) a.ml[at[t] * a.splits + split] = make_float2(ref[t], l[t]);
+            } else {
+                const float inv = l[t] > 0.f || l[t] != l[t] ? unit / l[t] : 0.f;
+                const int64_t out = at[t] * HD + 4 * q, gate = (2 * at[t] + 1) * HD + 4 * q;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) store_gated(a, out + 16 * d, gate + 16 * d, o[d][t] * inv);
+                if (q == 0 && a.lse) a.lse[at[t]] = ref[t] + log2f(l[t]);
+            }
+        }
+    }
+}
+
+// The splits of each (token, query head) merged: a wave per row, HD / 64 dims per lane.
+template <int HD>
+__global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
+    constexpr int LPR = HD / 4, RPB = 256 / LPR;  // lanes per row, rows per workgroup
+    const int b = blockIdx.y, cnt = a.b.count(b);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+    if (item >= static_cast<int64_t>(cnt) * a.H) return;
+    const int r0 = a.b.row0(b, a.c.maxp), i = static_cast<int>(item / a.H), d = threadIdx.x % LPR * 4;
+    const int64_t at = static_cast<int64_t>(a.b.first(b) + i) * a.H + item % a.H;
+    // splits that hold rows which this row's tile of rows sees
+    const int64_t row = static_cast<int64_t>(i) * a.group + item % a.H % a.group, all = static_cast<int64_t>(cnt) * a.group;
+    const int64_t end_row = min((row / a.rows_per + 1) * a.rows_per, all) - 1;
+    const int sees = static_cast<int>(min(static_cast<int64_t>(r0) + end_row / a.group + 1, static_cast<int64_t>(a.c.maxp)));
+    const int splits = min((sees + a.per - 1) / a.per, a.splits);
+    const float2 *ml = a.ml + at * a.splits;
+    float top = kLow;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
+    f4_t sum = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const float w = q4_exp2(ml[s].x - top);
+        l += w * ml[s].y;
+        sum += w * *reinterpret_cast<const f4_t *>(a.part + (at * a.splits + s) * HD + d);
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    store_gated(a, at * HD + d, (2 * at + 1) * HD + d, sum * inv);
+    if (d == 0 && a.lse) a.lse[at] = top + log2f(l);
+}
+
+// ---- gathered weights -------------------------------------------------------
+
+// A workgroup has 64 cached rows of a kv head, 16 per wave, as high and low parts in registers, and
+// walks all rows of queries that see any of them, 16 at a time; sums stay with the lane until the end.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
+    constexpr int NG = HD / kQ4Group, KS = HD / 32, KCH = HD / 8;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+    const int r = lane & 15, q = lane >> 4, G = a.group;
+    const int kvh = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH;
+    const int cnt = a.b.count(b);
+    if (cnt <= 0) return;
+    const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
+    const int top = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
+    const uint32_t magic = kept_1024();
+    const int klift = q4_lift(a.vmax[2 * a.c.head(b, kvh)]);
+    const float kunit = ldexpf(1.0f, klift);
+    const uint32_t all = static_cast<uint32_t>(cnt) * G;
+    const int part = blockIdx.z, parts = gridDim.z;  // of the queries
+    for (int t0 = blockIdx.x * 64; t0 < top; t0 += gridDim.x * 64) {
+        const int w0 = t0 + 16 * wave;
+        const int64_t line = min(w0 + r, a.c.R - 1);
+        h8_t kh[KS], kl[KS];
+#pragma unroll
+        for (int u = 0; u < KS; ++u) {
+            const uint32_t w = a.c.k_head(b, kvh)[line * KCH + 4 * u + q];
+            const _Float16 *p = a.c.par_head(b, kvh) + static_cast<int64_t>(u / 2) * a.c.R + line;
+            const h2_t s1 = {p[0], p[0]}, z1 = {p[static_cast<int64_t>(NG) * a.c.R], p[static_cast<int64_t>(NG) * a.c.R]};
+            const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
+            q4_values<2>(w, magic, s, z, kunit, kh[u], kl[u]);
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // the first row of queries that sees row w0, in 16s; this part's share of those from there on
+        const uint32_t from = static_cast<uint32_t>(max(w0 - r0, 0)) * G / 16, blocks = (all + 15) / 16;
+        for (uint32_t blk = from + part; blk < blocks; blk += parts) {
+            const uint32_t row = min(blk * 16 + r, all - 1), i = row / G;
+            const int64_t at = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
+            const int vis = blk * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
+            const float f = ldexpf(a.qf[at], -klift), z = a.lse[at];
+            f4_t s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < KS; ++u) {
+                const h8_t qh = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + q], ql = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + q];
+                s = mfma16(kh[u], qh, s);
+                s2 = mfma16(kh[u], ql, s2);
+                s2 = mfma16(kl[u], qh, s2);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = q4_exp2(fmaf(s[e] + s2[e], f, -z));
+                sum[e] += w0 + 4 * q + e < vis ? p : 0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = lanes_sum<16>(sum[e]);
+        if (r == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = w0 + 4 * q + e;
+                if (t >= top) continue;
+                if (parts > 1) {
+                    a.gpart[(a.c.head(b, kvh) * parts + part) * a.c.R + t] = sum[e];
+                } else {
+                    float *w = a.weights + a.c.head(b, kvh) * a.c.maxp + t;
+                    *w = t < r0 ? *w + sum[e] : sum[e];
+                }
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void q4_gathered_merge(const AttnQ4Args a, int parts) {
+    const int kvh = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, cnt = a.b.count(b);
+    if (cnt <= 0) return;
+    const int r0 = a.b.row0(b, a.c.maxp);
+    const int top = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
+    for (int t = blockIdx.x * 256 + threadIdx.x; t < top; t += gridDim.x * 256) {
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += a.gpart[(a.c.head(b, kvh) * parts + p) * a.c.R + t];
+        float *w = a.weights + a.c.head(b, kvh) * a.c.maxp + t;
+        *w = t < r0 ? *w + s : s;
+    }
+}
+
+// ---- launches ---------------------------------------------------------------
+
+template <int HD, int PQ, typename T>
+void launch_queries(const AttnQ4Args &a, hipStream_t s) {
+    constexpr int HPB = 256 / (HD / 8);
+    const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
+    hipLaunchKernelGGL((q4_queries<HD, PQ, T>), dim3(static_cast<uint32_t>((items + HPB - 1) / HPB), a.b.B), dim3(256), 0, s, a);
+}
+
+template <int HD>
+void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
+    constexpr int NT = HD == 64 ? 64 : 32;
+    const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
+    const int rows = static_cast<int>(std::min<int64_t>(a.c.maxp, 1 << 20));
+    if (a.planes_q == 2) a.in_f32 ? launch_queries<HD, 2, float>(a, s) : launch_queries<HD, 2, uint16_t>(a, s);
+    else a.in_f32 ? launch_queries<HD, 1, float>(a, s) : launch_queries<HD, 1, uint16_t>(a, s);
+    if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows + 1023) / 1024, 64), heads), dim3(256), 0, s, a);
+    const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(kPreThreads);
+    if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, 2, NT>), grid, block, 0, s, a);
+    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, 1, 32>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, 1, 32>), grid, block, 0, s, a);
+    if (a.splits > 1) {
+        constexpr int RPB = 256 / (HD / 4);
+        const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
+        hipLaunchKernelGGL(q4_prefill_merge<HD>, dim3(static_cast<uint32_t>((items + RPB - 1) / RPB), a.b.B), block, 0, s, a);
+    }
+    if (a.weights) {
+        hipLaunchKernelGGL(q4_gathered<HD>, dim3(std::min((rows + 63) / 64, 65535), heads, a.gparts), block, 0, s, a);
+        if (a.gparts > 1) hipLaunchKernelGGL(q4_gathered_merge, dim3(std::min((rows + 255) / 256, 1024), heads), block, 0, s, a, a.gparts);
+    }
+}
+
+}  // namespace
+
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights) {
+    Q4PrefillPlan p{};
+    p.planes_q = f32 || weights ? 2 : 1;
+    p.planes_v = f32 ? 2 : 1;
+    p.rows_per = p.planes_q == 1 ? 128 : 64;
+    p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
+    // two workgroups per CU, if the cached rows can be split that often with 256 rows each
+    const int64_t groups = p.tiles * heads;
+    const int64_t want = std::max<int64_t>(1, 512 / groups), most = std::max<int64_t>(1, rows / 256);
+    const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits});
+    p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
+    p.splits = static_cast<int>((rows + p.per - 1) / p.per);
+    // the gathered weights: as many workgroups, the queries dealt out where the cached rows are few
+    const int64_t cols = (rows + 63) / 64 * heads;
+    p.gparts = weights ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / cols, (max_tokens * group + 127) / 128, kQ4GatherMaxParts,
+                                                                               kQ4GatherMost / (heads * q4_rows(maxp))}))) : 0;
+    return p;
+}
+
+void launch_q4_prefill(const AttnQ4Args &a, hipStream_t s) {
+    switch (a.c.hd) {
+        case 64: launch_head_dim<64>(a, s); break;
+        case 128: launch_head_dim<128>(a, s); break;
+        default: launch_head_dim<256>(a, s); break;
+    }
+}
+
+}  // namespace swq

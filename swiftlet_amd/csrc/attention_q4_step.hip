@@ -20,44 +20,6 @@ struct Q4Tile {
     uint4 par[4][GW];  // rows 8 q .. 8 q + 7: k scale, k bias, v scale, v bias
 };
 
-// 8 consecutive numbers, 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-}
-
-// Sum and maximum over L consecutive lanes (8, 16 or 32), to each of them.
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
-    v += dpp<0xB1, 0xF, true>(v);
-    v += dpp<0x4E, 0xF, true>(v);
-    v += dpp<0x141, 0xF, true>(v);
-    if constexpr (L >= 16) v += dpp<0x140, 0xF, true>(v);
-    if constexpr (L >= 32) v += __shfl_xor(v, 16, kWave);
-    return v;
-}
-template <int L>
-__device__ __forceinline__ float lanes_max(float v) {
-    v = fmaxf(v, dpp<0xB1, 0xF, true>(v));
-    v = fmaxf(v, dpp<0x4E, 0xF, true>(v));
-    v = fmaxf(v, dpp<0x141, 0xF, true>(v));
-    if constexpr (L >= 16) v = fmaxf(v, dpp<0x140, 0xF, true>(v));
-    if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16, kWave));
-    return v;
-}
-
 // Four dims of head u: to the partial results of `split`, or, of the only one, to the output.
 template <int HD, typename T>
 __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n0, int h0, int u, int split, int d, f4_t s, float M, float L) {
@@ -66,16 +28,7 @@ __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n
         if (d == 0) a.ml[(head0 + u) * a.splits + split] = make_float2(M, L);
     } else {
         const int64_t at = static_cast<int64_t>(n0) * a.H + h0 + u;
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            y[e] = s[e] / L * sigmoid_exact(q4_load(static_cast<const T *>(a.q), (2 * at + 1) * HD + d + e));
-        if (a.out_f32) {
-            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at * HD + d) = make_float4(y[0], y[1], y[2], y[3]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q4_store(static_cast<uint16_t *>(a.out), at * HD + d + e, y[e]);
-        }
+        store_gated(a, at * HD + d, (2 * at + 1) * HD + d, s * (1.0f / L));
     }
 }
 
