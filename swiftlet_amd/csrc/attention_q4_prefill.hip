@@ -7,8 +7,6 @@
 namespace swq {
 namespace {
 
-constexpr int kPreThreads = 256;
-constexpr int kPreWaves = kPreThreads / kWave;
 constexpr float kLow = -1e30f;  // below every score: exponents against it stay numbers
 
 // ---- queries ----------------------------------------------------------------
@@ -158,8 +156,8 @@ __device__ __forceinline__ void q4_values(uint32_t w, uint32_t magic, const h2_t
     }
 }
 
-__device__ __forceinline__ h2_t pair_ll(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, (a & 0xFFFFu) | (b << 16)); }
-__device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, (a >> 16) | (b & 0xFFFF0000u)); }
+__device__ __forceinline__ h2_t pair_ll(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(b, a, 0x05040100u)); }
+__device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(b, a, 0x07060302u)); }
 
 // ---- attention --------------------------------------------------------------
 
@@ -170,11 +168,13 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 // (K's rows permuted so that the result's registers are the next operand), out = V^T P, so that
 // maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
-template <int HD, int PQ, int PV, int RT, int NT>
-__global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a) {
-    constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * RT * kPreWaves;
-    constexpr int KCH = HD / 8, VCH = NT / 8;
-    constexpr int KW = NT * KCH / kPreThreads, VW = VCH * HD / kPreThreads;  // words per thread
+template <int HD, int PQ, int PV, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a) {
+    constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, RT = 1, M = 16 * RT * WAVES;
+    constexpr int THREADS = WAVES * kWave, KCH = HD / 8, VCH = NT / 8;
+    // words of a thread: of keys KW, THREADS apart; of values VW of neighbouring dims of one block
+    constexpr int KW = NT * KCH / THREADS, VW = VCH * HD / THREADS;
+    static_assert(VW == 1 || VW == 2 || VW == 4, "one load takes a thread's value words");
     __shared__ h8_t s_k[2][PQ][NT * KCH];
     __shared__ h8_t s_v[2][PV][HD * VCH];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
@@ -236,115 +236,145 @@ __global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a)
         }
 
         uint32_t rk[KW], rv[VW];
-        uint32_t rkp[KW];            // key scale and bias of the word's row
-        uint4 rvs[VW], rvz[VW];      // value scales and biases of the block's rows
+        _Float16 rks[KW], rkz[KW];  // key scale and bias of the word's row
+        uint4 rvs, rvz;             // value scales and biases of the block's rows
+        // The words of a tile lie one after another, keys and values alike.  Of 64 rows the second 32
+        // may lie past the cache's: then they are the first again.
+        const int vblk = tid * VW / HD, vdim = tid * VW % HD;
         auto fetch = [&](int t0) {
+            const bool beyond = NT > 32 && t0 + 32 >= a.c.R;
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const int w = i * kPreThreads + tid, j = w % KCH;
-                const int64_t row = min(t0 + w / KCH, a.c.R - 1);
-                rk[i] = kw[row * KCH + j];
-                const uint16_t *p = reinterpret_cast<const uint16_t *>(par) + static_cast<int64_t>(j / 8) * a.c.R + row;
-                rkp[i] = p[0] | static_cast<uint32_t>(p[static_cast<int64_t>(NG) * a.c.R]) << 16;
+                const int line = i * (THREADS / KCH) + tid / KCH, back = beyond && line >= 32 ? 32 : 0;
+                const int64_t row = t0 + line - back;
+                rk[i] = kw[row * KCH + tid % KCH];
+                const _Float16 *p = par + static_cast<int64_t>(tid % KCH / 8) * a.c.R + row;
+                rks[i] = p[0];
+                rkz[i] = p[static_cast<int64_t>(NG) * a.c.R];
             }
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                const int w = __builtin_amdgcn_readfirstlane((i * kPreThreads + tid) / kWave);  // 64 dims of a block
-                const int blk = min(t0 / 8 + w / NG, a.c.R / 8 - 1);
-                rv[i] = vw[static_cast<int64_t>(blk) * HD + w % NG * kWave + lane];
-                const _Float16 *p = par + (static_cast<int64_t>(kQ4VScale) * NG + w % NG) * a.c.R + 8 * static_cast<int64_t>(blk);
-                rvs[i] = *reinterpret_cast<const uint4 *>(p);
-                rvz[i] = *reinterpret_cast<const uint4 *>(p + static_cast<int64_t>(NG) * a.c.R);
+            const int blk = vblk - (beyond && vblk >= 4 ? 4 : 0);
+            const uint32_t *pv = vw + static_cast<int64_t>(t0 / 8 + blk) * HD + vdim;
+            if constexpr (VW == 4) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(pv);
+                rv[0] = u.x; rv[1] = u.y; rv[2] = u.z; rv[3] = u.w;
+            } else if constexpr (VW == 2) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(pv);
+                rv[0] = u.x; rv[1] = u.y;
+            } else {
+                rv[0] = *pv;
             }
+            const _Float16 *p = par + (static_cast<int64_t>(kQ4VScale) * NG + vdim / kQ4Group) * a.c.R + t0 + 8 * blk;
+            rvs = *reinterpret_cast<const uint4 *>(p);
+            rvz = *reinterpret_cast<const uint4 *>(p + static_cast<int64_t>(NG) * a.c.R);
         };
-        auto unpack = [&](int t0, int buf) {
+        auto unpack_k = [&](int buf) {
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const int w = i * kPreThreads + tid, line = w / KCH, j = w % KCH;
-                const h2_t s1 = pair_ll(rkp[i], rkp[i]), z1 = pair_hh(rkp[i], rkp[i]);
+                const int line = i * (THREADS / KCH) + tid / KCH, j = tid % KCH;
+                const h2_t s1 = {rks[i], rks[i]}, z1 = {rkz[i], rkz[i]};
                 const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
                 h8_t hi, lo;
                 q4_values<PQ>(rk[i], magic, s, z, kunit, hi, lo);
                 s_k[buf][0][q4_place<KCH, true>(line, j)] = hi;
                 if constexpr (PQ == 2) s_k[buf][1][q4_place<KCH, true>(line, j)] = lo;
             }
+        };
+        auto unpack_v = [&](int t0, int buf) {
+            if (t0 + NT > seq_rows) {  // rows past the sequence's: 0, whatever they hold
+                const int left = seq_rows - (t0 + 8 * vblk);
+                uint4 keep;
+                keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
+                keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
+                keep.z = (left > 4 ? 0xFFFFu : 0u) | (left > 5 ? 0xFFFF0000u : 0u);
+                keep.w = (left > 6 ? 0xFFFFu : 0u) | (left > 7 ? 0xFFFF0000u : 0u);
+                rvs.x &= keep.x; rvs.y &= keep.y; rvs.z &= keep.z; rvs.w &= keep.w;
+                rvz.x &= keep.x; rvz.y &= keep.y; rvz.z &= keep.z; rvz.w &= keep.w;
+            }
+            const h2_t s[4] = {pair_ll(rvs.x, rvs.z), pair_hh(rvs.x, rvs.z), pair_ll(rvs.y, rvs.w), pair_hh(rvs.y, rvs.w)};
+            const h2_t z[4] = {pair_ll(rvz.x, rvz.z), pair_hh(rvz.x, rvz.z), pair_ll(rvz.y, rvz.w), pair_hh(rvz.y, rvz.w)};
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                const int w = i * kPreWaves + wave, blk = w / NG, dim = w % NG * kWave + lane;
-                uint4 us = rvs[i], uz = rvz[i];
-                const int left = seq_rows - (t0 + 8 * blk);
-                if (left < 8) {  // rows past the sequence's: 0, whatever they hold
-                    uint4 keep;
-                    keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
-                    keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
-                    keep.z = (left > 4 ? 0xFFFFu : 0u) | (left > 5 ? 0xFFFF0000u : 0u);
-                    keep.w = (left > 6 ? 0xFFFFu : 0u) | (left > 7 ? 0xFFFF0000u : 0u);
-                    us.x &= keep.x; us.y &= keep.y; us.z &= keep.z; us.w &= keep.w;
-                    uz.x &= keep.x; uz.y &= keep.y; uz.z &= keep.z; uz.w &= keep.w;
-                }
-                const h2_t s[4] = {pair_ll(us.x, us.z), pair_hh(us.x, us.z), pair_ll(us.y, us.w), pair_hh(us.y, us.w)};
-                const h2_t z[4] = {pair_ll(uz.x, uz.z), pair_hh(uz.x, uz.z), pair_ll(uz.y, uz.w), pair_hh(uz.y, uz.w)};
                 h8_t hi, lo;
                 q4_values<PV>(rv[i], magic, s, z, vunit, hi, lo);
-                s_v[buf][0][q4_place<VCH, false>(dim, blk)] = hi;
-                if constexpr (PV == 2) s_v[buf][1][q4_place<VCH, false>(dim, blk)] = lo;
+                s_v[buf][0][q4_place<VCH, false>(vdim + i, vblk)] = hi;
+                if constexpr (PV == 2) s_v[buf][1][q4_place<VCH, false>(vdim + i, vblk)] = lo;
             }
         };
 
         __syncthreads();  // a row tile before this one is done with the buffers
+        const int final = kv0 + (kv1 - 1 - kv0) / NT * NT;  // the last tile: past it, it is unpacked again
         fetch(kv0);
-        unpack(kv0, 0);
-        if (kv0 + NT < kv1) fetch(kv0 + NT);
+        unpack_k(0);
+        unpack_v(kv0, 0);
+        fetch(min(kv0 + NT, final));
         int buf = 0;
         for (int t0 = kv0; t0 < kv1; t0 += NT, buf ^= 1) {
             lds_barrier();
             f4_t s[PAIRS][2][RT];
+            // key chunks are read four ahead of the products that take them
+            constexpr int NK = PAIRS * 2 * KS, AHEAD = 4;
+            auto key = [&](int n, int plane) {
+                const int pr = n / (2 * KS), x = n / KS % 2, u = n % KS;
+                return s_k[buf][plane][q4_place<KCH, true>(32 * pr + 8 * (r >> 2) + 4 * x + (r & 3), 4 * u + q)];
+            };
+            h8_t kf[AHEAD][PQ];
 #pragma unroll
-            for (int pr = 0; pr < PAIRS; ++pr)
+            for (int n = 0; n < AHEAD; ++n)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int p = 0; p < PQ; ++p) kf[n][p] = key(n, p);
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) s[pr][x][t] = f4_t{0.f, 0.f, 0.f, 0.f};
-                    const int line = 32 * pr + 8 * (r >> 2) + 4 * x + (r & 3);
+            for (int n = 0; n < NK; ++n) {
+                const int pr = n / (2 * KS), x = n / KS % 2, u = n % KS;
 #pragma unroll
-                    for (int u = 0; u < KS; ++u) {
-                        const h8_t kh = s_k[buf][0][q4_place<KCH, true>(line, 4 * u + q)];
-#pragma unroll
-                        for (int t = 0; t < RT; ++t) s[pr][x][t] = mfma16(kh, qh[t][u], s[pr][x][t]);
-                        if constexpr (PQ == 2) {
-                            const h8_t kl = s_k[buf][1][q4_place<KCH, true>(line, 4 * u + q)];
-#pragma unroll
-                            for (int t = 0; t < RT; ++t) {
-                                s[pr][x][t] = mfma16(kh, ql[t][u], s[pr][x][t]);
-                                s[pr][x][t] = mfma16(kl, qh[t][u], s[pr][x][t]);
-                            }
-                        }
+                for (int t = 0; t < RT; ++t) {
+                    f4_t c = u == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : s[pr][x][t];
+                    c = mfma16(kf[n % AHEAD][0], qh[t][u], c);
+                    if constexpr (PQ == 2) {
+                        c = mfma16(kf[n % AHEAD][0], ql[t][u], c);
+                        c = mfma16(kf[n % AHEAD][1], qh[t][u], c);
                     }
+                    s[pr][x][t] = c;
                 }
-            if (t0 + NT < kv1) {
-                unpack(t0 + NT, buf ^ 1);
-                if (t0 + 2 * NT < kv1) fetch(t0 + 2 * NT);
+                if (n + AHEAD < NK) {
+#pragma unroll
+                    for (int p = 0; p < PQ; ++p) kf[n % AHEAD][p] = key(n + AHEAD, p);
+                }
             }
+            unpack_k(buf ^ 1);
+            unpack_v(min(t0 + NT, final), buf ^ 1);
+            fetch(min(t0 + 2 * NT, final));
             const bool masked = t0 + NT > low || t0 + NT > kv1;
+            if (masked) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const int lim = min(vis[t], kv1) - t0 - 8 * q;
+#pragma unroll
+                    for (int pr = 0; pr < PAIRS; ++pr)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[pr][x][t][i] = 32 * pr + 4 * x + i < lim ? s[pr][x][t][i] : -INFINITY;
+                }
+            }
+            float top[RT];
+            bool over = false;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                float top = -INFINITY;
-                const int lim = min(vis[t], kv1) - t0 - 8 * q;
+                top[t] = -INFINITY;
 #pragma unroll
                 for (int pr = 0; pr < PAIRS; ++pr)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
+                        top[t] = fmaxf(top[t], fmaxf(fmaxf(s[pr][x][t][0], s[pr][x][t][1]), fmaxf(s[pr][x][t][2], s[pr][x][t][3])));
+                top[t] *= f[t];
+                over |= top[t] > ref[t] + 15.0f;
+            }
+            if (__any(over)) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float v = s[pr][x][t][i] * f[t];
-                            if (masked) v = 32 * pr + 4 * x + i < lim ? v : -INFINITY;
-                            s[pr][x][t][i] = v;
-                            top = fmaxf(top, v);
-                        }
-                if (__any(top > ref[t] + 15.0f)) {
-                    top = fmaxf(top, __shfl_xor(top, 16, kWave));
-                    top = fmaxf(top, __shfl_xor(top, 32, kWave));
-                    const float to = fmaxf(ref[t], top - 7.0f);
+                for (int t = 0; t < RT; ++t) {
+                    float m = fmaxf(top[t], __shfl_xor(top[t], 16, kWave));
+                    m = fmaxf(m, __shfl_xor(m, 32, kWave));
+                    const float to = fmaxf(ref[t], m - 7.0f);
                     const float alpha = q4_exp2(ref[t] - to);
                     ref[t] = to;
                     l[t] *= alpha;
@@ -352,6 +382,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a)
                     for (int d = 0; d < DT; ++d) o[d][t] *= alpha;
                 }
             }
+            constexpr int NV = DT * PAIRS;
+            auto value = [&](int n, int plane) { return s_v[buf][plane][q4_place<VCH, false>(16 * (n / PAIRS) + r, 4 * (n % PAIRS) + q)]; };
+            h8_t vf[AHEAD][PV];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n)
+#pragma unroll
+                for (int p = 0; p < PV; ++p) vf[n][p] = value(n, p);
             h8_t ph[PAIRS][RT], pl[PV == 2 ? PAIRS : 1][PV == 2 ? RT : 1];
 #pragma unroll
             for (int t = 0; t < RT; ++t)
@@ -360,7 +397,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a)
                     float p[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        p[i] = q4_exp2(s[pr][i / 4][t][i % 4] - ref[t]);
+                        p[i] = q4_exp2(fmaf(s[pr][i / 4][t][i % 4], f[t], -ref[t]));
                         l[t] += p[i];
                     }
 #pragma unroll
@@ -379,21 +416,21 @@ __global__ __launch_bounds__(kPreThreads, 2) void q4_prefill(const AttnQ4Args a)
                     }
                 }
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int n = 0; n < NV; ++n) {
+                const int d = n / PAIRS, pr = n % PAIRS;
 #pragma unroll
-                for (int pr = 0; pr < PAIRS; ++pr) {
-                    const h8_t vh = s_v[buf][0][q4_place<VCH, false>(16 * d + r, 4 * pr + q)];
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) o[d][t] = mfma16(vh, ph[pr][t], o[d][t]);
+                for (int t = 0; t < RT; ++t) {
+                    o[d][t] = mfma16(vf[n % AHEAD][0], ph[pr][t], o[d][t]);
                     if constexpr (PV == 2) {
-                        const h8_t vl = s_v[buf][1][q4_place<VCH, false>(16 * d + r, 4 * pr + q)];
-#pragma unroll
-                        for (int t = 0; t < RT; ++t) {
-                            o[d][t] = mfma16(vh, pl[pr][t], o[d][t]);
-                            o[d][t] = mfma16(vl, ph[pr][t], o[d][t]);
-                        }
+                        o[d][t] = mfma16(vf[n % AHEAD][0], pl[pr][t], o[d][t]);
+                        o[d][t] = mfma16(vf[n % AHEAD][1], ph[pr][t], o[d][t]);
                     }
                 }
+                if (n + AHEAD < NV) {
+#pragma unroll
+                    for (int p = 0; p < PV; ++p) vf[n % AHEAD][p] = value(n + AHEAD, p);
+                }
+            }
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -541,16 +578,15 @@ void launch_queries(const AttnQ4Args &a, hipStream_t s) {
 
 template <int HD>
 void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
-    constexpr int NT = HD == 64 ? 64 : 32;
     const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
     const int rows = static_cast<int>(std::min<int64_t>(a.c.maxp, 1 << 20));
     if (a.planes_q == 2) a.in_f32 ? launch_queries<HD, 2, float>(a, s) : launch_queries<HD, 2, uint16_t>(a, s);
     else a.in_f32 ? launch_queries<HD, 1, float>(a, s) : launch_queries<HD, 1, uint16_t>(a, s);
     if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows + 1023) / 1024, 64), heads), dim3(256), 0, s, a);
-    const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(kPreThreads);
-    if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, 2, NT>), grid, block, 0, s, a);
-    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, 1, 32>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, 1, 32>), grid, block, 0, s, a);
+    const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
+    if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
+    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, 32, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, 32, 4>), grid, block, 0, s, a);
     if (a.splits > 1) {
         constexpr int RPB = 256 / (HD / 4);
         const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
