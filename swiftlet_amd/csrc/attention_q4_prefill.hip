@@ -105,7 +105,7 @@ __device__ __forceinline__ int q4_lift(uint32_t bits) {
 
 // Where chunk c (8 numbers) of a line of CH chunks lies, so that the 16 lines that a wave reads at
 // once, and the lines or chunks that it writes, hit different banks.  KEY: lines are cached rows, read
-// in the order 8 (r / 4) + r % 4; else dims, read in order.
+// in the order 8 (r / 4) + r % 4; else dims or queries, read in order.
 template <int CH, bool KEY>
 __device__ __forceinline__ int q4_place(int line, int c) {
     int f;
@@ -113,7 +113,7 @@ __device__ __forceinline__ int q4_place(int line, int c) {
         f = (line & 3) | ((line >> 1) & 12);
         if constexpr (CH < 16) f >>= 1;
     } else {
-        f = CH == 4 ? (line >> 2) & 3 : (line >> 1) & 7;
+        f = CH == 4 ? (line >> 2) & 3 : CH == 8 ? (line >> 1) & 7 : line & 15;
     }
     return line * CH + (c ^ f);
 }
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
     constexpr int THREADS = WAVES * kWave, KCH = HD / 8, VCH = NT / 8;
     // words of a thread: of keys KW, THREADS apart; of values VW of neighbouring dims of one block
     constexpr int KW = NT * KCH / THREADS, VW = VCH * HD / THREADS;
-    static_assert(VW == 1 || VW == 2 || VW == 4, "one load takes a thread's value words");
+    static_assert(KW >= 1 && (VW == 1 || VW == 2 || VW == 4), "one load takes a thread's value words");
     __shared__ h8_t s_k[2][PQ][NT * KCH];
     __shared__ h8_t s_v[2][PV][HD * VCH];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             lds_barrier();
             f4_t s[PAIRS][2][RT];
             // key chunks are read four ahead of the products that take them
-            constexpr int NK = PAIRS * 2 * KS, AHEAD = 4;
+            constexpr int NK = PAIRS * 2 * KS, AHEAD = PQ == 2 ? 2 : 4;
             auto key = [&](int n, int plane) {
                 const int pr = n / (2 * KS), x = n / KS % 2, u = n % KS;
                 return s_k[buf][plane][q4_place<KCH, true>(32 * pr + 8 * (r >> 2) + 4 * x + (r & 3), 4 * u + q)];
@@ -382,11 +382,11 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
                     for (int d = 0; d < DT; ++d) o[d][t] *= alpha;
                 }
             }
-            constexpr int NV = DT * PAIRS;
+            constexpr int NV = DT * PAIRS, AHEAD_V = PV == 2 ? 2 : 4;
             auto value = [&](int n, int plane) { return s_v[buf][plane][q4_place<VCH, false>(16 * (n / PAIRS) + r, 4 * (n % PAIRS) + q)]; };
-            h8_t vf[AHEAD][PV];
+            h8_t vf[AHEAD_V][PV];
 #pragma unroll
-            for (int n = 0; n < AHEAD; ++n)
+            for (int n = 0; n < AHEAD_V; ++n)
 #pragma unroll
                 for (int p = 0; p < PV; ++p) vf[n][p] = value(n, p);
             h8_t ph[PAIRS][RT], pl[PV == 2 ? PAIRS : 1][PV == 2 ? RT : 1];
@@ -420,15 +420,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
                 const int d = n / PAIRS, pr = n % PAIRS;
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
-                    o[d][t] = mfma16(vf[n % AHEAD][0], ph[pr][t], o[d][t]);
+                    o[d][t] = mfma16(vf[n % AHEAD_V][0], ph[pr][t], o[d][t]);
                     if constexpr (PV == 2) {
-                        o[d][t] = mfma16(vf[n % AHEAD][0], pl[pr][t], o[d][t]);
-                        o[d][t] = mfma16(vf[n % AHEAD][1], ph[pr][t], o[d][t]);
+                        o[d][t] = mfma16(vf[n % AHEAD_V][0], pl[pr][t], o[d][t]);
+                        o[d][t] = mfma16(vf[n % AHEAD_V][1], ph[pr][t], o[d][t]);
                     }
                 }
-                if (n + AHEAD < NV) {
+                if (n + AHEAD_V < NV) {
 #pragma unroll
-                    for (int p = 0; p < PV; ++p) vf[n % AHEAD][p] = value(n + AHEAD, p);
+                    for (int p = 0; p < PV; ++p) vf[n % AHEAD_V][p] = value(n + AHEAD_V, p);
                 }
             }
         }
@@ -485,11 +485,17 @@ __global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
 
 // ---- gathered weights -------------------------------------------------------
 
-// A workgroup has 64 cached rows of a kv head, 16 per wave, as high and low parts in registers, and
-// walks all rows of queries that see any of them, 16 at a time; sums stay with the lane until the end.
+// A workgroup has kGatherRows cached rows of a kv head, 32 per wave, as high and low parts in
+// registers, and walks the rows of queries that see any of them, 16 at a time: those go through LDS
+// once for all waves, the next 16 on their way meanwhile: 512 tokens of 16 heads after 8,192 rows of 2
+// kv heads of 256 147 us, 720 TFLOP/s in three products (16 cached rows per wave, queries read by each
+// from L1: 911).  Sums stay with the lane until the end.
+constexpr int kGatherRows = 128;
+
 template <int HD>
 __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
-    constexpr int NG = HD / kQ4Group, KS = HD / 32, KCH = HD / 8;
+    constexpr int NG = HD / kQ4Group, KS = HD / 32, KCH = HD / 8, NC = 16 * KCH / 256 > 0 ? 16 * KCH / 256 : 1;
+    __shared__ h8_t s_q[2][2][16 * KCH];  // [buffer][high, low]
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int r = lane & 15, q = lane >> 4, G = a.group;
     const int kvh = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH;
@@ -499,55 +505,110 @@ __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
     const int top = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
     const uint32_t magic = kept_1024();
     const int klift = q4_lift(a.vmax[2 * a.c.head(b, kvh)]);
-    const float kunit = ldexpf(1.0f, klift);
+    const float kunit = ldexpf(1.0f, klift), down = ldexpf(1.0f, -klift);
     const uint32_t all = static_cast<uint32_t>(cnt) * G;
     const int part = blockIdx.z, parts = gridDim.z;  // of the queries
-    for (int t0 = blockIdx.x * 64; t0 < top; t0 += gridDim.x * 64) {
-        const int w0 = t0 + 16 * wave;
-        const int64_t line = min(w0 + r, a.c.R - 1);
-        h8_t kh[KS], kl[KS];
+    for (int t0 = blockIdx.x * kGatherRows; t0 < top; t0 += gridDim.x * kGatherRows) {
+        const int w0 = t0 + 32 * wave;
+        h8_t kh[2][KS], kl[2][KS];
 #pragma unroll
-        for (int u = 0; u < KS; ++u) {
-            const uint32_t w = a.c.k_head(b, kvh)[line * KCH + 4 * u + q];
-            const _Float16 *p = a.c.par_head(b, kvh) + static_cast<int64_t>(u / 2) * a.c.R + line;
-            const h2_t s1 = {p[0], p[0]}, z1 = {p[static_cast<int64_t>(NG) * a.c.R], p[static_cast<int64_t>(NG) * a.c.R]};
-            const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
-            q4_values<2>(w, magic, s, z, kunit, kh[u], kl[u]);
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        // the first row of queries that sees row w0, in 16s; this part's share of those from there on
-        const uint32_t from = static_cast<uint32_t>(max(w0 - r0, 0)) * G / 16, blocks = (all + 15) / 16;
-        for (uint32_t blk = from + part; blk < blocks; blk += parts) {
-            const uint32_t row = min(blk * 16 + r, all - 1), i = row / G;
-            const int64_t at = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
-            const int vis = blk * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
-            const float f = ldexpf(a.qf[at], -klift), z = a.lse[at];
-            f4_t s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int u = 0; u < KS; ++u) {
-                const h8_t qh = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + q], ql = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + q];
-                s = mfma16(kh[u], qh, s);
-                s2 = mfma16(kh[u], ql, s2);
-                s2 = mfma16(kl[u], qh, s2);
+                const int64_t line = min(w0 + 16 * x + r, a.c.R - 1);
+                const uint32_t w = a.c.k_head(b, kvh)[line * KCH + 4 * u + q];
+                const _Float16 *p = a.c.par_head(b, kvh) + static_cast<int64_t>(u / 2) * a.c.R + line;
+                const h2_t s1 = {p[0], p[0]}, z1 = {p[static_cast<int64_t>(NG) * a.c.R], p[static_cast<int64_t>(NG) * a.c.R]};
+                const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
+                q4_values<2>(w, magic, s, z, kunit, kh[x][u], kl[x][u]);
+            }
+        float sum[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[x][e] = 0.f;
+        // the first 16 rows of queries that see row t0; this part's share of those from there on
+        const uint32_t from = static_cast<uint32_t>(max(t0 - r0, 0)) * G / 16 + part, blocks = (all + 15) / 16;
+        uint4 ch[NC], cl[NC];
+        float f, z;
+        int vis;
+        const bool copies = 16 * KCH >= 256 || tid < 16 * KCH;
+        auto fetch = [&](uint32_t blk) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                const uint32_t id = k * 256 + tid, row = min(blk * 16 + id / KCH, all - 1);
+                const int64_t at = (static_cast<int64_t>(n0 + row / G) * a.H + kvh * G + row % G) * KCH + id % KCH;
+                if (copies) {
+                    ch[k] = static_cast<const uint4 *>(a.qh)[at];
+                    cl[k] = static_cast<const uint4 *>(a.ql)[at];
+                }
+            }
+            const uint32_t row = min(blk * 16 + r, all - 1), i = row / G;
+            const int64_t at = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
+            f = a.qf[at];
+            z = a.lse[at];
+            vis = blk * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
+        };
+        auto put = [&](int buf) {
+            if (copies) {
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const int id = k * 256 + tid;
+                    s_q[buf][0][q4_place<KCH, false>(id / KCH, id % KCH)] = __builtin_bit_cast(h8_t, ch[k]);
+                    s_q[buf][1][q4_place<KCH, false>(id / KCH, id % KCH)] = __builtin_bit_cast(h8_t, cl[k]);
+                }
+            }
+        };
+        __syncthreads();  // the rows before these are done with the buffers
+        if (from < blocks) {
+            fetch(from);
+            put(0);
+        }
+        int buf = 0;
+        for (uint32_t blk = from; blk < blocks; blk += parts, buf ^= 1) {
+            const float cf = f * down, cz = z;
+            const int cv = vis;
+            const bool more = blk + parts < blocks;
+            lds_barrier();
+            if (more) fetch(blk + parts);
+            f4_t s[2], s2[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) s[x] = s2[x] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < KS; ++u) {
+                const h8_t qh = s_q[buf][0][q4_place<KCH, false>(r, 4 * u + q)], ql = s_q[buf][1][q4_place<KCH, false>(r, 4 * u + q)];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    s[x] = mfma16(kh[x][u], qh, s[x]);
+                    s2[x] = mfma16(kh[x][u], ql, s2[x]);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) s2[x] = mfma16(kl[x][u], qh, s2[x]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = q4_exp2(fmaf(s[e] + s2[e], f, -z));
-                sum[e] += w0 + 4 * q + e < vis ? p : 0.f;
-            }
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = q4_exp2(fmaf(s[x][e] + s2[x][e], cf, -cz));
+                    sum[x][e] += w0 + 16 * x + 4 * q + e < cv ? p : 0.f;
+                }
+            if (more) put(buf ^ 1);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = lanes_sum<16>(sum[e]);
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[x][e] = lanes_sum<16>(sum[x][e]);
         if (r == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = w0 + 4 * q + e;
+            for (int i = 0; i < 8; ++i) {
+                const int t = w0 + 16 * (i / 4) + 4 * q + i % 4;
+                const float v = sum[i / 4][i % 4];
                 if (t >= top) continue;
                 if (parts > 1) {
-                    a.gpart[(a.c.head(b, kvh) * parts + part) * a.c.R + t] = sum[e];
+                    a.gpart[(a.c.head(b, kvh) * parts + part) * a.c.R + t] = v;
                 } else {
                     float *w = a.weights + a.c.head(b, kvh) * a.c.maxp + t;
-                    *w = t < r0 ? *w + sum[e] : sum[e];
+                    *w = t < r0 ? *w + v : v;
                 }
             }
         }
@@ -585,15 +646,15 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows + 1023) / 1024, 64), heads), dim3(256), 0, s, a);
     const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
     if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
-    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, 32, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, 32, 4>), grid, block, 0, s, a);
+    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
     if (a.splits > 1) {
         constexpr int RPB = 256 / (HD / 4);
         const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
         hipLaunchKernelGGL(q4_prefill_merge<HD>, dim3(static_cast<uint32_t>((items + RPB - 1) / RPB), a.b.B), block, 0, s, a);
     }
     if (a.weights) {
-        hipLaunchKernelGGL(q4_gathered<HD>, dim3(std::min((rows + 63) / 64, 65535), heads, a.gparts), block, 0, s, a);
+        hipLaunchKernelGGL(q4_gathered<HD>, dim3((rows + kGatherRows - 1) / kGatherRows, heads, a.gparts), block, 0, s, a);
         if (a.gparts > 1) hipLaunchKernelGGL(q4_gathered_merge, dim3(std::min((rows + 255) / 256, 1024), heads), block, 0, s, a, a.gparts);
     }
 }
@@ -604,7 +665,7 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, i
     Q4PrefillPlan p{};
     p.planes_q = f32 || weights ? 2 : 1;
     p.planes_v = f32 ? 2 : 1;
-    p.rows_per = p.planes_q == 1 ? 128 : 64;
+    p.rows_per = 128;
     p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
     // two workgroups per CU, if the cached rows can be split that often with 256 rows each
     const int64_t groups = p.tiles * heads;
@@ -613,7 +674,7 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, i
     p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
     p.splits = static_cast<int>((rows + p.per - 1) / p.per);
     // the gathered weights: as many workgroups, the queries dealt out where the cached rows are few
-    const int64_t cols = (rows + 63) / 64 * heads;
+    const int64_t cols = (rows + kGatherRows - 1) / kGatherRows * heads;
     p.gparts = weights ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / cols, (max_tokens * group + 127) / 128, kQ4GatherMaxParts,
                                                                                kQ4GatherMost / (heads * q4_rows(maxp))}))) : 0;
     return p;
