@@ -161,31 +161,30 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 
 // ---- attention --------------------------------------------------------------
 
-// A workgroup takes M = 64 RT rows (token, query head of the kv head's group; heads of one token next
+// A workgroup takes M = 16 WAVES rows (token, query head of the kv head's group; heads of one token next
 // to each other) and the cached rows of one split that the last of them sees, NT at a time.  The tile's
 // words are loaded two tiles ahead into registers, unpacked one tile ahead into the other of two LDS
-// buffers, one barrier per tile.  Each wave has 16 RT rows as columns of both products: scores = K Q
+// buffers, one barrier per tile.  Each wave has 16 rows as columns of both products: scores = K Q
 // (K's rows permuted so that the result's registers are the next operand), out = V^T P, so that
 // maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
 template <int HD, int PQ, int PV, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a) {
-    constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, RT = 1, M = 16 * RT * WAVES;
+    constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * WAVES;
     constexpr int THREADS = WAVES * kWave, KCH = HD / 8, VCH = NT / 8;
     // words of a thread: of keys KW, THREADS apart; of values VW of neighbouring dims of one block
     constexpr int KW = NT * KCH / THREADS, VW = VCH * HD / THREADS;
     static_assert(KW >= 1 && (VW == 1 || VW == 2 || VW == 4), "one load takes a thread's value words");
-    __shared__ h8_t s_k[2][PQ][NT * KCH];
-    __shared__ h8_t s_v[2][PV][HD * VCH];
+    constexpr uint32_t KB = NT * KCH * 16, VB = HD * VCH * 16;  // bytes of one plane of a tile
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * PQ * KB];  // [buffer][plane]
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * PV * VB];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int r = lane & 15, q = lane >> 4, G = a.group;
-    // heads innermost; tiles of rows from the last (most cached rows) down, those of the second half of
-    // the workgroups from the first up, so that the two that share a CU have equal work together
+    // heads innermost; tiles of rows from the last, which sees the most cached rows, to the first: a CU
+    // that is done takes the longest that is left
     const int heads = a.b.B * a.c.KVH;
     const int head = blockIdx.x % heads, rank = blockIdx.x / heads;
-    const int split = rank % a.splits, order = rank / a.splits;
-    const int up = a.tiles - a.tiles / 2;
-    const int slot = order < up ? a.tiles - 1 - order : order - up;
+    const int split = rank % a.splits, slot = a.tiles - 1 - rank / a.splits;
     const int kvh = head % a.c.KVH, b = head / a.c.KVH;
     const int cnt = a.b.count(b);
     const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
@@ -203,57 +202,51 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
         const int sees = min(r0 + static_cast<int>(end_row / G) + 1, a.c.maxp);
         const int kv0 = split * a.per, kv1 = split == a.splits - 1 ? sees : min(kv0 + a.per, sees);
         if (kv0 >= kv1) continue;
-        // this lane's columns
-        int vis[RT];
-        int64_t at[RT];
-        float f[RT];
-        h8_t qh[RT][KS], ql[PQ == 2 ? RT : 1][PQ == 2 ? KS : 1];
-        int low = 0x7FFFFFFF;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const uint32_t row = min(base + (wave * RT + t) * 16 + r, all - 1), i = row / G;
-            at[t] = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
-            vis[t] = base + (wave * RT + t) * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
-            low = min(low, vis[t]);
-            f[t] = ldexpf(a.qf[at[t]], -klift);
+        // this lane's column
+        const uint32_t column = min(base + wave * 16 + r, all - 1);
+        const bool valid = base + wave * 16 + r < all;
+        const int vis = valid ? min(r0 + static_cast<int>(column / G) + 1, a.c.maxp) : 0;
+        int low = vis;
+        float f;
+        h8_t qh[KS], ql[PQ == 2 ? KS : 1];
+        {
+            const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
+            f = ldexpf(a.qf[at], -klift);
 #pragma unroll
             for (int u = 0; u < KS; ++u) {
-                qh[t][u] = reinterpret_cast<const h8_t *>(a.qh)[at[t] * KCH + 4 * u + q];
-                if constexpr (PQ == 2) ql[t][u] = reinterpret_cast<const h8_t *>(a.ql)[at[t] * KCH + 4 * u + q];
+                qh[u] = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + q];
+                if constexpr (PQ == 2) ql[u] = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + q];
             }
         }
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) low = min(low, __shfl_xor(low, off, kWave));
         low = __builtin_amdgcn_readfirstlane(low);
-        float ref[RT], l[RT];
-        f4_t o[DT][RT];
+        float ref = kLow, l = 0.f;
+        f4_t o[DT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            ref[t] = kLow;
-            l[t] = 0.f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][t] = f4_t{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int d = 0; d < DT; ++d) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
 
         uint32_t rk[KW], rv[VW];
         _Float16 rks[KW], rkz[KW];  // key scale and bias of the word's row
         uint4 rvs, rvz;             // value scales and biases of the block's rows
         // The words of a tile lie one after another, keys and values alike.  Of 64 rows the second 32
-        // may lie past the cache's: then they are the first again.
-        const int vblk = tid * VW / HD, vdim = tid * VW % HD;
+        // may lie past the cache's: then they are the first again.  Addresses: the tile's, the same for
+        // all lanes, and the lane's 32-bit offset in it.
+        const uint32_t vblk = tid * VW / HD, vdim = tid * VW % HD;
         auto fetch = [&](int t0) {
             const bool beyond = NT > 32 && t0 + 32 >= a.c.R;
+            const uint32_t *pk = kw + static_cast<int64_t>(t0) * KCH, *pv = vw + static_cast<int64_t>(t0 / 8) * HD;
+            const _Float16 *ps = par + t0, *pz = ps + static_cast<int64_t>(NG) * a.c.R;
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const int line = i * (THREADS / KCH) + tid / KCH, back = beyond && line >= 32 ? 32 : 0;
-                const int64_t row = t0 + line - back;
-                rk[i] = kw[row * KCH + tid % KCH];
-                const _Float16 *p = par + static_cast<int64_t>(tid % KCH / 8) * a.c.R + row;
-                rks[i] = p[0];
-                rkz[i] = p[static_cast<int64_t>(NG) * a.c.R];
+                const uint32_t line = i * (THREADS / KCH) + tid / KCH, back = beyond && line >= 32 ? 32 : 0;
+                rk[i] = pk[(line - back) * KCH + tid % KCH];
+                const uint32_t at = (tid % KCH / 8) * a.c.R + (line - back);
+                rks[i] = ps[at];
+                rkz[i] = pz[at];
             }
-            const int blk = vblk - (beyond && vblk >= 4 ? 4 : 0);
-            const uint32_t *pv = vw + static_cast<int64_t>(t0 / 8 + blk) * HD + vdim;
+            const uint32_t blk = vblk - (beyond && vblk >= 4 ? 4 : 0);
+            pv += blk * HD + vdim;
             if constexpr (VW == 4) {
                 const uint4 u = *reinterpret_cast<const uint4 *>(pv);
                 rv[0] = u.x; rv[1] = u.y; rv[2] = u.z; rv[3] = u.w;
@@ -263,9 +256,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             } else {
                 rv[0] = *pv;
             }
-            const _Float16 *p = par + (static_cast<int64_t>(kQ4VScale) * NG + vdim / kQ4Group) * a.c.R + t0 + 8 * blk;
-            rvs = *reinterpret_cast<const uint4 *>(p);
-            rvz = *reinterpret_cast<const uint4 *>(p + static_cast<int64_t>(NG) * a.c.R);
+            const uint32_t at = vdim / kQ4Group * a.c.R + 8 * blk;
+            rvs = *reinterpret_cast<const uint4 *>(ps + static_cast<int64_t>(kQ4VScale) * NG * a.c.R + at);
+            rvz = *reinterpret_cast<const uint4 *>(ps + static_cast<int64_t>(kQ4VBias) * NG * a.c.R + at);
         };
         auto unpack_k = [&](int buf) {
 #pragma unroll
@@ -275,13 +268,14 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
                 const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
                 h8_t hi, lo;
                 q4_values<PQ>(rk[i], magic, s, z, kunit, hi, lo);
-                s_k[buf][0][q4_place<KCH, true>(line, j)] = hi;
-                if constexpr (PQ == 2) s_k[buf][1][q4_place<KCH, true>(line, j)] = lo;
+                uint8_t *dst = s_k + buf * (PQ * KB) + 16 * q4_place<KCH, true>(line, j);
+                *reinterpret_cast<h8_t *>(dst) = hi;
+                if constexpr (PQ == 2) *reinterpret_cast<h8_t *>(dst + KB) = lo;
             }
         };
         auto unpack_v = [&](int t0, int buf) {
             if (t0 + NT > seq_rows) {  // rows past the sequence's: 0, whatever they hold
-                const int left = seq_rows - (t0 + 8 * vblk);
+                const int left = seq_rows - t0 - 8 * static_cast<int>(vblk);
                 uint4 keep;
                 keep.x = (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
                 keep.y = (left > 2 ? 0xFFFFu : 0u) | (left > 3 ? 0xFFFF0000u : 0u);
@@ -296,8 +290,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             for (int i = 0; i < VW; ++i) {
                 h8_t hi, lo;
                 q4_values<PV>(rv[i], magic, s, z, vunit, hi, lo);
-                s_v[buf][0][q4_place<VCH, false>(vdim + i, vblk)] = hi;
-                if constexpr (PV == 2) s_v[buf][1][q4_place<VCH, false>(vdim + i, vblk)] = lo;
+                uint8_t *dst = s_v + buf * (PV * VB) + 16 * q4_place<VCH, false>(vdim + i, vblk);
+                *reinterpret_cast<h8_t *>(dst) = hi;
+                if constexpr (PV == 2) *reinterpret_cast<h8_t *>(dst + VB) = lo;
             }
         };
 
@@ -310,12 +305,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
         int buf = 0;
         for (int t0 = kv0; t0 < kv1; t0 += NT, buf ^= 1) {
             lds_barrier();
-            f4_t s[PAIRS][2][RT];
-            // key chunks are read four ahead of the products that take them
+            f4_t s[PAIRS][2];
+            // The chains of the tile's products by turns; key chunks are read a few ahead of them.  Step u's chunk lies 64 u
+            // xor-ed into the first one's address, the rows of the second product 4 lines on.
             constexpr int NK = PAIRS * 2 * KS, AHEAD = PQ == 2 ? 2 : 4;
+            uint32_t kat = buf * (PQ * KB) + 16 * q4_place<KCH, true>(8 * (r >> 2) + (r & 3), q);
+            asm volatile("" : "+v"(kat));  // no step's address is kept from tile to tile
             auto key = [&](int n, int plane) {
-                const int pr = n / (2 * KS), x = n / KS % 2, u = n % KS;
-                return s_k[buf][plane][q4_place<KCH, true>(32 * pr + 8 * (r >> 2) + 4 * x + (r & 3), 4 * u + q)];
+                const int pr = n / 2 % PAIRS, x = n % 2, u = n / (2 * PAIRS);
+                return *reinterpret_cast<const h8_t *>(s_k + (kat ^ (64u * u)) + plane * KB + (32 * pr + 4 * x) * KCH * 16);
             };
             h8_t kf[AHEAD][PQ];
 #pragma unroll
@@ -324,17 +322,14 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
                 for (int p = 0; p < PQ; ++p) kf[n][p] = key(n, p);
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
-                const int pr = n / (2 * KS), x = n / KS % 2, u = n % KS;
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    f4_t c = u == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : s[pr][x][t];
-                    c = mfma16(kf[n % AHEAD][0], qh[t][u], c);
-                    if constexpr (PQ == 2) {
-                        c = mfma16(kf[n % AHEAD][0], ql[t][u], c);
-                        c = mfma16(kf[n % AHEAD][1], qh[t][u], c);
-                    }
-                    s[pr][x][t] = c;
+                const int pr = n / 2 % PAIRS, x = n % 2, u = n / (2 * PAIRS);
+                f4_t c = u == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : s[pr][x];
+                c = mfma16(kf[n % AHEAD][0], qh[u], c);
+                if constexpr (PQ == 2) {
+                    c = mfma16(kf[n % AHEAD][0], ql[u], c);
+                    c = mfma16(kf[n % AHEAD][1], qh[u], c);
                 }
+                s[pr][x] = c;
                 if (n + AHEAD < NK) {
 #pragma unroll
                     for (int p = 0; p < PQ; ++p) kf[n % AHEAD][p] = key(n + AHEAD, p);
@@ -343,88 +338,72 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             unpack_k(buf ^ 1);
             unpack_v(min(t0 + NT, final), buf ^ 1);
             fetch(min(t0 + 2 * NT, final));
-            const bool masked = t0 + NT > low || t0 + NT > kv1;
-            if (masked) {
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    const int lim = min(vis[t], kv1) - t0 - 8 * q;
-#pragma unroll
-                    for (int pr = 0; pr < PAIRS; ++pr)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[pr][x][t][i] = 32 * pr + 4 * x + i < lim ? s[pr][x][t][i] : -INFINITY;
-                }
-            }
-            float top[RT];
-            bool over = false;
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                top[t] = -INFINITY;
+            if (t0 + NT > low || t0 + NT > kv1) {
+                const int lim = min(vis, kv1) - t0 - 8 * q;
 #pragma unroll
                 for (int pr = 0; pr < PAIRS; ++pr)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        top[t] = fmaxf(top[t], fmaxf(fmaxf(s[pr][x][t][0], s[pr][x][t][1]), fmaxf(s[pr][x][t][2], s[pr][x][t][3])));
-                top[t] *= f[t];
-                over |= top[t] > ref[t] + 15.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[pr][x][i] = 32 * pr + 4 * x + i < lim ? s[pr][x][i] : -INFINITY;
             }
-            if (__any(over)) {
+            float top = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    float m = fmaxf(top[t], __shfl_xor(top[t], 16, kWave));
-                    m = fmaxf(m, __shfl_xor(m, 32, kWave));
-                    const float to = fmaxf(ref[t], m - 7.0f);
-                    const float alpha = q4_exp2(ref[t] - to);
-                    ref[t] = to;
-                    l[t] *= alpha;
+            for (int pr = 0; pr < PAIRS; ++pr)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) o[d][t] *= alpha;
-                }
+                for (int x = 0; x < 2; ++x) top = fmaxf(top, fmaxf(fmaxf(s[pr][x][0], s[pr][x][1]), fmaxf(s[pr][x][2], s[pr][x][3])));
+            top *= f;
+            if (__any(top > ref + 15.0f)) {
+                top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                const float to = fmaxf(ref, top - 7.0f);
+                const float alpha = q4_exp2(ref - to);
+                ref = to;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= alpha;
             }
             constexpr int NV = DT * PAIRS, AHEAD_V = PV == 2 ? 2 : 4;
-            auto value = [&](int n, int plane) { return s_v[buf][plane][q4_place<VCH, false>(16 * (n / PAIRS) + r, 4 * (n % PAIRS) + q)]; };
+            const uint32_t vat = buf * (PV * VB) + 16 * q4_place<VCH, false>(r, q);
+            auto value = [&](int n, int plane) {
+                return *reinterpret_cast<const h8_t *>(s_v + (vat ^ (64u * (n % PAIRS))) + plane * VB + n / PAIRS * 16 * VCH * 16);
+            };
             h8_t vf[AHEAD_V][PV];
 #pragma unroll
             for (int n = 0; n < AHEAD_V; ++n)
 #pragma unroll
                 for (int p = 0; p < PV; ++p) vf[n][p] = value(n, p);
-            h8_t ph[PAIRS][RT], pl[PV == 2 ? PAIRS : 1][PV == 2 ? RT : 1];
+            h8_t ph[PAIRS], pl[PV == 2 ? PAIRS : 1];
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+            for (int pr = 0; pr < PAIRS; ++pr) {
+                float p[8];
 #pragma unroll
-                for (int pr = 0; pr < PAIRS; ++pr) {
-                    float p[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        p[i] = q4_exp2(fmaf(s[pr][i / 4][t][i % 4], f[t], -ref[t]));
-                        l[t] += p[i];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const f32x2_t x = {p[q4_nibble(j)], p[q4_nibble(j + 1)]};
-                        h2_t h, w;
-                        if constexpr (PV == 2) {
-                            split_f16(x, h, w);
-                            pl[pr][t][j] = w.x;
-                            pl[pr][t][j + 1] = w.y;
-                        } else {
-                            h = __builtin_convertvector(x, h2_t);
-                        }
-                        ph[pr][t][j] = h.x;
-                        ph[pr][t][j + 1] = h.y;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = q4_exp2(fmaf(s[pr][i / 4][i % 4], f, -ref));
+                    l += p[i];
                 }
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const f32x2_t x = {p[q4_nibble(j)], p[q4_nibble(j + 1)]};
+                    h2_t h, w;
+                    if constexpr (PV == 2) {
+                        split_f16(x, h, w);
+                        pl[pr][j] = w.x;
+                        pl[pr][j + 1] = w.y;
+                    } else {
+                        h = __builtin_convertvector(x, h2_t);
+                    }
+                    ph[pr][j] = h.x;
+                    ph[pr][j + 1] = h.y;
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
                 const int d = n / PAIRS, pr = n % PAIRS;
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    o[d][t] = mfma16(vf[n % AHEAD_V][0], ph[pr][t], o[d][t]);
-                    if constexpr (PV == 2) {
-                        o[d][t] = mfma16(vf[n % AHEAD_V][0], pl[pr][t], o[d][t]);
-                        o[d][t] = mfma16(vf[n % AHEAD_V][1], ph[pr][t], o[d][t]);
-                    }
+                o[d] = mfma16(vf[n % AHEAD_V][0], ph[pr], o[d]);
+                if constexpr (PV == 2) {
+                    o[d] = mfma16(vf[n % AHEAD_V][0], pl[pr], o[d]);
+                    o[d] = mfma16(vf[n % AHEAD_V][1], ph[pr], o[d]);
                 }
                 if (n + AHEAD_V < NV) {
 #pragma unroll
@@ -432,23 +411,25 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
                 }
             }
         }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            l[t] += __shfl_xor(l[t], 16, kWave);
-            l[t] += __shfl_xor(l[t], 32, kWave);
-            if (base + (wave * RT + t) * 16 + r >= all) continue;
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
+        if (valid) {
             const float unit = 1.0f / vunit;
+            const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
             if (a.splits > 1) {
-                float *dst = a.part + (at[t] * a.splits + split) * HD + 4 * q;
+                float *dst = a.part + (at * a.splits + split) * HD + 4 * q;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t *>(dst + 16 * d) = o[d][t] * unit;
-                if (q == 0) a.ml[at[t] * a.splits + split] = make_float2(ref[t], l[t]);
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t *>(dst + 16 * d) = o[d] * unit;
+                if (q == 0) a.ml[at * a.splits + split] = make_float2(ref, l);
             } else {
-                const float inv = l[t] > 0.f || l[t] != l[t] ? unit / l[t] : 0.f;
-                const int64_t out = at[t] * HD + 4 * q, gate = (2 * at[t] + 1) * HD + 4 * q;
+                const float inv = l > 0.f || l != l ? unit / l : 0.f;
+                const int64_t out = at * HD + 4 * q, gate = (2 * at + 1) * HD + 4 * q;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) store_gated(a, out + 16 * d, gate + 16 * d, o[d][t] * inv);
-                if (q == 0 && a.lse) a.lse[at[t]] = ref[t] + log2f(l[t]);
+                for (int d = 0; d < DT; ++d) {
+                    store_gated(a, out + 16 * d, gate + 16 * d, o[d] * inv);
+                    if (d % 4 == 3) asm volatile("" ::: "memory");  // else every gate's load comes first, into registers of its own
+                }
+                if (q == 0 && a.lse) a.lse[at] = ref + log2f(l);
             }
         }
     }

@@ -11,6 +11,7 @@ namespace swq {
 
 constexpr int kQ4Group = 64;      // dims of one scale and bias
 constexpr int kQ4Block = 8;       // rows of one v word
+constexpr int kQ4MaxRows = 1 << 27;  // of a sequence: a head's parameters of one kind stay below 4 GiB
 constexpr int kQ4RowPad = 32;     // rows are allocated in multiples of this: a reader's tile
 constexpr int kQ4MaxHeadGroup = 16;  // query heads per kv head
 
@@ -66,7 +67,7 @@ inline bool q4_head_dim(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 
 inline int check_q4_shape(int sequences, int kvh, int hd, int maxp) {
     if (sequences <= 0 || kvh <= 0 || maxp <= 0 || hd <= 0) return SWQ_ERR_INVALID_ARGUMENT;
-    if (!q4_head_dim(hd) || maxp > (1 << 30) || static_cast<int64_t>(sequences) * kvh > 65535) return SWQ_ERR_LIMIT;
+    if (!q4_head_dim(hd) || maxp > kQ4MaxRows || static_cast<int64_t>(sequences) * kvh > 65535) return SWQ_ERR_LIMIT;
     return SWQ_OK;
 }
 
