@@ -103,18 +103,16 @@ __device__ __forceinline__ int q4_lift(uint32_t bits) {
 
 // ---- tiles of values in LDS -------------------------------------------------
 
-// Where chunk c (8 numbers) of a line of CH chunks lies, so that the 16 lines that a wave reads at
-// once, and the lines or chunks that it writes, hit different banks.  KEY: lines are cached rows, read
-// in the order 8 (r / 4) + r % 4; else dims or queries, read in order.
+// Where chunk c (8 numbers, 16 bytes) of a line of CH chunks lies: xor-ed with bits of the line.  LDS
+// serves 16 lanes of 16 bytes at once, lanes 0-3, 12-15, 20-23 and 24-27 together and so on: with chunk
+// q = lane / 16 of line r = lane % 16, these are 16 different places of 256 bytes for the lines below,
+// and for the lines or chunks that a wave writes.  KEY: line r is cached row 8 (r / 4) + r % 4 of the
+// tile (bit 2 of the row is no part of it); else a dim or a query.
 template <int CH, bool KEY>
 __device__ __forceinline__ int q4_place(int line, int c) {
-    int f;
-    if constexpr (KEY) {
-        f = (line & 3) | ((line >> 1) & 12);
-        if constexpr (CH < 16) f >>= 1;
-    } else {
-        f = CH == 4 ? (line >> 2) & 3 : CH == 8 ? (line >> 1) & 7 : line & 15;
-    }
+    const int r = KEY ? (line & 3) | (line >> 1 & 12) : line & 15;
+    const int high = (r >> 3) | ((r >> 2 ^ r >> 3) & 1) << 1;  // 0, 2, 3, 1 for r / 4 = 0 .. 3
+    const int f = CH == 4 ? high : CH == 8 ? (high & 1) | (r & 2) | (high & 2) << 1 : r;
     return line * CH + (c ^ f);
 }
 
@@ -172,9 +170,9 @@ template <int HD, int PQ, int PV, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a) {
     constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * WAVES;
     constexpr int THREADS = WAVES * kWave, KCH = HD / 8, VCH = NT / 8;
-    // words of a thread: of keys KW, THREADS apart; of values VW of neighbouring dims of one block
+    // words of a thread: of keys KW, THREADS apart; of values VW of one block and group, 64 / VW dims apart
     constexpr int KW = NT * KCH / THREADS, VW = VCH * HD / THREADS;
-    static_assert(KW >= 1 && (VW == 1 || VW == 2 || VW == 4), "one load takes a thread's value words");
+    static_assert(KW >= 1 && (VW == 1 || VW == 2 || VW == 4), "a thread's value words share a block and a group");
     constexpr uint32_t KB = NT * KCH * 16, VB = HD * VCH * 16;  // bytes of one plane of a tile
     __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * PQ * KB];  // [buffer][plane]
     __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * PV * VB];
@@ -232,7 +230,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
         // The words of a tile lie one after another, keys and values alike.  Of 64 rows the second 32
         // may lie past the cache's: then they are the first again.  Addresses: the tile's, the same for
         // all lanes, and the lane's 32-bit offset in it.
-        const uint32_t vblk = tid * VW / HD, vdim = tid * VW % HD;
+        constexpr uint32_t VGAP = kQ4Group / VW;
+        const uint32_t vblk = tid / (VGAP * NG), vdim = tid / VGAP % NG * kQ4Group + tid % VGAP;
         auto fetch = [&](int t0) {
             const bool beyond = NT > 32 && t0 + 32 >= a.c.R;
             const uint32_t *pk = kw + static_cast<int64_t>(t0) * KCH, *pv = vw + static_cast<int64_t>(t0 / 8) * HD;
@@ -247,15 +246,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             }
             const uint32_t blk = vblk - (beyond && vblk >= 4 ? 4 : 0);
             pv += blk * HD + vdim;
-            if constexpr (VW == 4) {
-                const uint4 u = *reinterpret_cast<const uint4 *>(pv);
-                rv[0] = u.x; rv[1] = u.y; rv[2] = u.z; rv[3] = u.w;
-            } else if constexpr (VW == 2) {
-                const uint2 u = *reinterpret_cast<const uint2 *>(pv);
-                rv[0] = u.x; rv[1] = u.y;
-            } else {
-                rv[0] = *pv;
-            }
+#pragma unroll
+            for (int i = 0; i < VW; ++i) rv[i] = pv[i * VGAP];
             const uint32_t at = vdim / kQ4Group * a.c.R + 8 * blk;
             rvs = *reinterpret_cast<const uint4 *>(ps + static_cast<int64_t>(kQ4VScale) * NG * a.c.R + at);
             rvz = *reinterpret_cast<const uint4 *>(ps + static_cast<int64_t>(kQ4VBias) * NG * a.c.R + at);
@@ -290,7 +282,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
             for (int i = 0; i < VW; ++i) {
                 h8_t hi, lo;
                 q4_values<PV>(rv[i], magic, s, z, vunit, hi, lo);
-                uint8_t *dst = s_v + buf * (PV * VB) + 16 * q4_place<VCH, false>(vdim + i, vblk);
+                uint8_t *dst = s_v + buf * (PV * VB) + 16 * q4_place<VCH, false>(vdim + i * VGAP, vblk);
                 *reinterpret_cast<h8_t *>(dst) = hi;
                 if constexpr (PV == 2) *reinterpret_cast<h8_t *>(dst + VB) = lo;
             }
