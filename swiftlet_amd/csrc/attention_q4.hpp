@@ -136,6 +136,16 @@ __device__ __forceinline__ float lanes_max(float v) {
     return v;
 }
 
+// Four dims times the sigmoids of four bf16 gates, as bf16: the hardware's exponential and reciprocal,
+// off by 2^-21, and its conversion to the nearest bf16 (a NaN stays one).
+__device__ __forceinline__ uint2 gated_bf16(uint2 g, f4_t v) {
+    typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
+    const f4_t x = {__uint_as_float(g.x << 16), __uint_as_float(g.x & 0xFFFF0000u), __uint_as_float(g.y << 16), __uint_as_float(g.y & 0xFFFF0000u)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= __builtin_amdgcn_rcpf(1.0f + q4_exp2(x[e] * -1.44269504f));
+    return __builtin_bit_cast(uint2, __builtin_convertvector(v, b4_t));
+}
+
 // Four dims, attention * sigmoid(gate), at element `out` of the output; gate: of q_proj.
 __device__ __forceinline__ void store_gated(const AttnQ4Args &a, int64_t out, int64_t gate, f4_t v) {
     if (a.in_f32) {

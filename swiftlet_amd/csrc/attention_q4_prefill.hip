@@ -405,24 +405,66 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void q4_prefill(const AttnQ4Args a
         }
         l += __shfl_xor(l, 16, kWave);
         l += __shfl_xor(l, 32, kWave);
-        if (valid) {
-            const float unit = 1.0f / vunit;
-            const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
-            if (a.splits > 1) {
-                float *dst = a.part + (at * a.splits + split) * HD + 4 * q;
+        const bool last = a.splits == 1;
+        const float unit = last ? (l > 0.f || l != l ? 1.0f / (vunit * l) : 0.f) : 1.0f / vunit;
+        const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
+        if (valid && q == 0) {
+            if (!last) a.ml[at * a.splits + split] = make_float2(ref, l);
+            else if (a.lse) a.lse[at] = ref + log2f(l);
+        }
+        // Up to 128 dims of the wave's 16 rows at a time through its share of the tiles' LDS, so that rows
+        // leave, and gates come, in whole lines.
+        constexpr int PART = HD == 256 ? 128 : 64, CPR = PART / 4, RPI = kWave / CPR;
+        static_assert(sizeof(s_k) >= WAVES / 2 * 16 * PART * 4 && sizeof(s_v) >= WAVES / 2 * 16 * PART * 4, "16 rows for each wave");
+        constexpr int ITS = 16 / RPI, PARTS = HD / PART;
+        // Where one part is used for p and values, inputs and output are bf16.  The gates of a part are all
+        // on their way before any is used, the first part's across the barrier.
+        const int at32 = static_cast<int>(at);
+        uint32_t to[ITS];  // (token, head) of the rows that this lane writes; the host keeps them below 2^31
+        uint2 gates[ITS];
+        const int d0 = lane % CPR * 4;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t *>(dst + 16 * d) = o[d] * unit;
-                if (q == 0) a.ml[at * a.splits + split] = make_float2(ref, l);
-            } else {
-                const float inv = l > 0.f || l != l ? unit / l : 0.f;
-                const int64_t out = at * HD + 4 * q, gate = (2 * at + 1) * HD + 4 * q;
+        for (int it = 0; it < ITS; ++it) to[it] = __shfl(at32, it * RPI + lane / CPR, kWave);
+        const bool any = base + wave * 16 < all;  // of this wave's rows
+        auto load_gates = [&](uint2 (&g)[ITS], int part) {
+            if constexpr (PV == 1) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    store_gated(a, out + 16 * d, gate + 16 * d, o[d] * inv);
-                    if (d % 4 == 3) asm volatile("" ::: "memory");  // else every gate's load comes first, into registers of its own
-                }
-                if (q == 0 && a.lse) a.lse[at] = ref + log2f(l);
+                for (int it = 0; it < ITS; ++it)
+                    g[it] = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.q) + static_cast<uint64_t>(to[it]) * (2 * HD) + HD + part * PART + d0);
             }
+        };
+        if (last && any) load_gates(gates, 0);
+        __syncthreads();
+        if (!any) continue;
+        uint8_t *mine = wave < WAVES / 2 ? s_k + wave * (16 * PART * 4) : s_v + (wave - WAVES / 2) * (16 * PART * 4);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+            for (int d = 0; d < PART / 16; ++d) *reinterpret_cast<f4_t *>(mine + (r * CPR + ((4 * d + q) ^ r)) * 16) = o[part * (PART / 16) + d] * unit;
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            uint2 next[ITS];
+            if (last && part + 1 < PARTS) load_gates(next, part + 1);
+#pragma unroll
+            for (int it = 0; it < ITS; ++it) {
+                const int row = it * RPI + lane / CPR, c = lane % CPR;
+                const f4_t v = *reinterpret_cast<const f4_t *>(mine + (row * CPR + (c ^ row)) * 16);
+                if (base + wave * 16 + row >= all) continue;
+                const int d = part * PART + d0;
+                if (!last) {
+                    *reinterpret_cast<f4_t *>(a.part + (static_cast<uint64_t>(to[it]) * a.splits + split) * HD + d) = v;
+                } else if constexpr (PV == 1) {
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + static_cast<uint64_t>(to[it]) * HD + d) = gated_bf16(gates[it], v);
+                } else {
+                    store_gated(a, static_cast<int64_t>(to[it]) * HD + d, (2 * static_cast<int64_t>(to[it]) + 1) * HD + d, v);
+                }
+            }
+            if constexpr (PV == 1) {
+#pragma unroll
+                for (int it = 0; it < ITS; ++it) gates[it] = next[it];
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
 }
