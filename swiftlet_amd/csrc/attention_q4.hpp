@@ -98,24 +98,6 @@ __device__ __forceinline__ float q4_exp2(float x) { return __builtin_amdgcn_exp2
 // Off by two units in the last place at most: expf, a sum and the hardware's reciprocal.
 __device__ __forceinline__ float sigmoid_exact(float v) { return __builtin_amdgcn_rcpf(1.0f + expf(-v)); }
 
-// 8 consecutive numbers, 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-}
-
 // Sum and maximum over L consecutive lanes (8, 16 or 32), to each of them.
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {

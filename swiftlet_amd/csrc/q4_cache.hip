@@ -8,7 +8,6 @@ namespace swq {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendWaves = kAppendThreads / kWave;
 
 struct AppendArgs {
     Q4View c;
@@ -18,49 +17,108 @@ struct AppendArgs {
     float eps;
 };
 
-// One workgroup per block of 8 rows, kv head and sequence; a wave takes every fourth row of the
-// block.  k words and all scales and biases belong to one row and are written by its wave; a v
-// word holds 8 rows of one dim, so the codes meet in LDS, and words of which only some rows are
-// new keep the others (the first and last block of a call).
+// A workgroup per block of 8 rows, kv head and sequence (two blocks at hd 64).  HD / 8 lanes have a row,
+// 8 dims each, so that a lane's codes are one k word, a wave takes 2 to 8 rows at once and sums cross few
+// lanes.  A v word holds 8 rows of one dim: those codes meet in LDS, and words of which only some rows
+// are new keep the others (the first and last block of a call).  All in 64 bits up to the format's own
+// roundings.  Bound by that arithmetic: 8,192 tokens of 8 heads of 128 (43 MB) 24 us; one row per wave
+// and a division per value took 58.
 template <int HD, typename T>
 __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) {
-    constexpr int EPL = HD / kWave;
-    __shared__ double s_rot[kAppendWaves][HD];
-    __shared__ uint8_t s_v[kQ4Block][HD];
-    const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH;
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+    constexpr int LPR = HD / 8, PER = kQ4Block * LPR;  // lanes of a row, of a block's keys or values
+    constexpr int ROUNDS = 2 * PER > kAppendThreads ? 2 : 1, BLOCKS = ROUNDS == 1 ? kAppendThreads / (2 * PER) : 1, NG = HD / kQ4Group;
+    __shared__ double s_rot[kAppendThreads / LPR][HD];
+    __shared__ uint2 s_v[BLOCKS][kQ4Block][LPR];
+    const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, tid = threadIdx.x, j = tid % LPR;
     const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
-    const int r1 = min(r0 + a.b.count(b), a.c.maxp);  // past the last row written
+    const int r1 = static_cast<int>(min(static_cast<int64_t>(r0) + a.b.count(b), static_cast<int64_t>(a.c.maxp)));  // past the last row written
     const int half = a.b.rot / 2;
     uint32_t *kw = a.c.k_head(b, h), *vw = a.c.v_head(b, h);
     _Float16 *par = a.c.par_head(b, h);
-    const T *kin = static_cast<const T *>(a.k), *vin = static_cast<const T *>(a.v);
-    for (int blk = r0 / kQ4Block + blockIdx.x; blk * kQ4Block < r1; blk += gridDim.x) {
-        for (int u = wave; u < kQ4Block; u += kAppendWaves) {
-            const int row = blk * kQ4Block + u;
-            if (row < r0 || row >= r1) continue;  // the same for the whole wave
-            const int64_t at = (static_cast<int64_t>(n0 + row - r0) * a.c.KVH + h) * HD + lane * EPL;
-            double x[EPL];
-            uint32_t q[EPL];
+    const int r0_block = r0 / kQ4Block;
+    for (int blk0 = r0_block + blockIdx.x * BLOCKS; blk0 * kQ4Block < r1; blk0 += gridDim.x * BLOCKS) {
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(kin, at + e));
-            const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, row - r0)) * half : nullptr;
-            Q4HeadTable<EPL> tab;
-            tab.load(a.w, turn, half);
-            q4_key_row<HD>(x, tab, a.eps, half, s_rot[wave], kw, par, a.c.R, row);
+        for (int round = 0; round < ROUNDS; ++round) {
+            const bool values = ROUNDS == 2 ? round == 1 : tid / PER % 2 == 1;  // the same for a whole wave
+            const int which = ROUNDS == 2 ? 0 : tid / (2 * PER), u = tid % PER / LPR, row = (blk0 + which) * kQ4Block + u;
+            const bool here = row >= r0 && row < r1;
+            const int i = here ? row - r0 : 0;
+            const int64_t at = (static_cast<int64_t>(n0 + i) * a.c.KVH + h) * HD + 8 * j;
+            float in[8];
+            load8<T>(in, static_cast<const T *>(values ? a.v : a.k) + at);
+            double x[8];
+            uint32_t q[8];
+            _Float16 scale, bias;
+            if (!values) {
+                double ss = 0.0;
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) x[e] = static_cast<double>(q4_load(vin, at + e));
-            q4_value_row<HD>(x, q, par, a.c.R, row);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = static_cast<double>(in[e]);
+                    ss += x[e] * x[e];
+                }
+                if constexpr (LPR == 32) {
+                    ss = reduce_f64<16>(ss, [](double p, double r) { return p + r; });
+                    ss += __shfl_xor(ss, 16, kWave);
+                } else {
+                    ss = reduce_f64<LPR>(ss, [](double p, double r) { return p + r; });
+                }
+                const double inv = 1.0 / sqrt(ss / HD + static_cast<double>(a.eps));
+                double *rot = s_rot[tid / LPR];
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) s_v[u][lane * EPL + e] = static_cast<uint8_t>(q[e]);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = x[e] * inv * static_cast<double>(a.w[8 * j + e]);
+                    rot[8 * j + e] = x[e];
+                }
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (8 * j < 2 * half) {
+                    const float2 *turn = a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = 8 * j + e;
+                        if (d < 2 * half) {
+                            const float2 cs = turn[d < half ? d : d - half];
+                            const double o = rot[d < half ? d + half : d - half];
+                            const double c = static_cast<double>(cs.x), s = static_cast<double>(cs.y);
+                            x[e] = d < half ? x[e] * c - o * s : x[e] * c + o * s;
+                        }
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = static_cast<double>(in[e]);
+            }
+            q4_quantise<8>(x, q, scale, bias);
+            if (here && j % 8 == 0) {
+                _Float16 *p = par + (static_cast<int64_t>(values ? kQ4VScale : kQ4KScale) * NG + j / 8) * a.c.R + row;
+                p[0] = scale;
+                p[static_cast<int64_t>(NG) * a.c.R] = bias;
+            }
+            if (values) {
+                s_v[which][u][j] = make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
+            } else if (here) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) word |= q[e] << (4 * e);
+                kw[static_cast<int64_t>(row) * LPR + j] = word;
+            }
         }
         __syncthreads();
-        const int u0 = max(r0 - blk * kQ4Block, 0), u1 = min(r1 - blk * kQ4Block, kQ4Block);
-        for (int d = tid; d < HD; d += kAppendThreads) {
-            uint32_t *p = vw + static_cast<int64_t>(blk) * HD + d;
-            uint32_t word = u1 - u0 < kQ4Block ? *p : 0u;
-            for (int u = u0; u < u1; ++u) word = (word & ~(15u << (4 * u))) | (static_cast<uint32_t>(s_v[u][d]) << (4 * u));
-            *p = word;
+        for (int i = tid; i < BLOCKS * HD; i += kAppendThreads) {
+            const int which = i / HD, d = i % HD, blk = blk0 + which;
+            const int u0 = max(r0 - blk * kQ4Block, 0), u1 = min(r1 - blk * kQ4Block, kQ4Block);
+            if (u0 < u1) {
+                uint32_t *p = vw + static_cast<int64_t>(blk) * HD + d;
+                uint32_t word = 0, mask = 0;
+#pragma unroll
+                for (int u = 0; u < kQ4Block; ++u) {
+                    word |= static_cast<uint32_t>(reinterpret_cast<const uint8_t *>(s_v[which][u])[d]) << (4 * u);
+                    mask |= u >= u0 && u < u1 ? 15u << (4 * u) : 0u;
+                }
+                *p = mask == 0xFFFFFFFFu ? word : (*p & ~mask) | (word & mask);
+            }
         }
         __syncthreads();
     }
@@ -125,17 +183,41 @@ struct EvictArgs {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
+constexpr int kSelectKeep = 48;  // rows of a thread that are in registers at once
+constexpr int kSelectRows = kSelectThreads * kSelectKeep;
+constexpr int kSelectBins = 2048;
+constexpr int kSelectList = 4096;  // rows that are left to decide on, when they are few
+static_assert(kSelectKeep * kSelectWaves <= kSelectThreads && kSelectBins == 2 * kSelectThreads, "a thread per count, two bins per thread");
 
-__device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? orderable(w) : 0u; }
+// What rows are ordered by: the weight (NaN lowest), then the lower row; all different.
+__device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? orderable(w == 0.f ? 0.f : w) : 0u; }
+__device__ __forceinline__ uint64_t rank_key(uint32_t key, int row) { return static_cast<uint64_t>(key) << 32 | ~static_cast<uint32_t>(row); }
 
-// The rows that one (sequence, kv head) keeps.  The smallest key among the kept of the middle is
-// found eight bits at a time from histograms in LDS (their integer counts do not depend on the
-// order of the adds), then the rows are numbered in order: those above it, and of those equal to
-// it the first `need`.
+// Sum over the lanes before this one, and over all of them.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v, uint32_t &all) {
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t s = v;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const uint32_t o = __shfl_up(s, off, kWave);
+        if (lane >= off) s += o;
+    }
+    all = __builtin_amdgcn_readlane(s, kWave - 1);
+    return s - v;
+}
+
+// The rows that one (sequence, kv head) keeps: those of the middle whose rank_key reaches a border, and
+// all before and behind it.  The border is found eleven bits at a time from the top from histograms in
+// LDS, whose integer counts do not depend on the order of the adds, until all rows that share its known
+// bits are kept; once those are few they are listed, and the later passes go over the list alone.  Then
+// the kept rows are counted and numbered in order.  Weights stay in registers, 48 rows of each thread;
+// caches of more than 49,152 rows are gone through in parts, read again by each pass.
 __global__ __launch_bounds__(kSelectThreads) void q4_select(const EvictArgs a) {
-    __shared__ uint32_t s_hist[256];
-    __shared__ uint32_t s_wave[2][kSelectWaves];
-    __shared__ uint32_t s_pick[2];
+    __shared__ uint32_t s_hist[kSelectBins];
+    __shared__ uint64_t s_list[kSelectList];
+    __shared__ uint32_t s_count[kSelectKeep * kSelectWaves];  // by chunk of 1,024 rows and wave
+    __shared__ uint32_t s_wave[kSelectWaves];
+    __shared__ uint32_t s_pick[3], s_listed;
     const int h = blockIdx.x % a.src.KVH, b = blockIdx.x / a.src.KVH;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
     const int n = min(max(a.rows[b], 0), a.src.maxp);
@@ -145,78 +227,136 @@ __global__ __launch_bounds__(kSelectThreads) void q4_select(const EvictArgs a) {
     const bool all = n <= a.budget;
     const int m0 = all ? n : a.sink, m1 = all ? n : n - a.recent;  // the middle
     uint32_t need = all ? 0 : a.budget - a.sink - a.recent;        // of it, still to be found
-    uint32_t key = 0, mask = 0;  // the bits of the border key that are known
-    if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
-            __syncthreads();
-            for (int t = m0 + tid; t < m1; t += kSelectThreads) {
-                const uint32_t k = weight_key(w[t]);
-                if ((k & mask) == key) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+    const int parts = (n + kSelectRows - 1) / kSelectRows;
+    float x[kSelectKeep];
+    // the rows of a part, 1,024 at a time; f(i, row, weight)
+    auto load = [&](int part) {
+#pragma unroll
+        for (int i = 0; i < kSelectKeep; ++i) {
+            const int t = part * kSelectRows + i * kSelectThreads + tid;
+            x[i] = t < n ? w[t] : 0.f;
+        }
+    };
+    if (parts > 0) load(0);
+    uint64_t border = need > 0 ? 0 : ~0ull, mask = 0;  // its known bits
+    bool listed = false;
+    uint32_t left = static_cast<uint32_t>(m1 - m0);  // rows that share them
+    for (int shift = 53; need > 0 && need < left; shift = max(shift - 11, 0)) {
+        s_hist[tid] = s_hist[tid + kSelectThreads] = 0;
+        if (tid == 0) s_listed = 0;
+        __syncthreads();
+        auto count = [&](bool in, uint32_t bin) {
+            const uint64_t who = __ballot(in);
+            if (who == 0) return;
+            const int lead = __builtin_ctzll(who);
+            if (__ballot(in && bin == static_cast<uint32_t>(__builtin_amdgcn_readlane(bin, lead))) == who) {  // one add for all
+                if (lane == lead) atomicAdd(&s_hist[bin], static_cast<uint32_t>(__popcll(who)));
+            } else if (in) {
+                atomicAdd(&s_hist[bin], 1u);
             }
-            __syncthreads();
-            if (wave == 0) {  // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
-                uint32_t c[4], sum = 0;
+        };
+        const uint32_t digit = shift == 0 ? 511u : 2047u;  // 53, 42, 31, 20, 9, 0
+        if (listed) {
+            for (uint32_t i = tid; i < ((left + 63) & ~63u); i += kSelectThreads) {
+                const uint64_t k = i < left ? s_list[i] : 0;
+                count(i < left && (k & mask) == border, static_cast<uint32_t>(k >> shift) & digit);
+            }
+        } else {
+            for (int part = 0; part < parts; ++part) {
+                if (parts > 1) load(part);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c[i] = s_hist[255 - 4 * lane - i];
-                    sum += c[i];
+                for (int i = 0; i < kSelectKeep; ++i) {
+                    if (part * kSelectRows + i * kSelectThreads >= n) break;
+                    const int t = part * kSelectRows + i * kSelectThreads + tid;
+                    const uint64_t k = rank_key(weight_key(x[i]), t);
+                    count(t >= m0 && t < m1 && (k & mask) == border, static_cast<uint32_t>(k >> shift) & digit);
                 }
-                uint32_t upto = sum;
-                for (int off = 1; off < kWave; off <<= 1) {
-                    const uint32_t o = __shfl_up(upto, off, kWave);
-                    if (lane >= off) upto += o;
-                }
-                uint32_t above = upto - sum;
-                if (above < need && upto >= need) {
+            }
+        }
+        __syncthreads();
+        // thread t: bins 2047 - 2 t and the one below, from the top
+        const uint32_t c0 = s_hist[kSelectBins - 1 - 2 * tid], c1 = s_hist[kSelectBins - 2 - 2 * tid];
+        uint32_t total, above = lanes_before(c0 + c1, total);
+        if (lane == 0) s_wave[wave] = total;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) above += s_wave[i];
+        if (above < need && above + c0 + c1 >= need) {
+            const bool second = above + c0 < need;
+            s_pick[0] = kSelectBins - 1 - 2 * tid - second;
+            s_pick[1] = need - above - (second ? c0 : 0u);
+            s_pick[2] = second ? c1 : c0;
+        }
+        __syncthreads();
+        border |= static_cast<uint64_t>(s_pick[0]) << shift;
+        mask |= static_cast<uint64_t>(digit) << shift;
+        need = s_pick[1];
+        const uint32_t share = s_pick[2];
+        if (listed) {
+            __syncthreads();  // all have read the pick; the list stays, `left` is its length
+            if (need == share) left = need;
+        } else {
+            left = share;
+            if (need < left && left <= kSelectList) {
+                for (int part = 0; part < parts; ++part) {
+                    if (parts > 1) load(part);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (above < need && above + c[i] >= need) {
-                            s_pick[0] = 255 - 4 * lane - i;
-                            s_pick[1] = need - above;
-                            break;
-                        }
-                        above += c[i];
+                    for (int i = 0; i < kSelectKeep; ++i) {
+                        if (part * kSelectRows + i * kSelectThreads >= n) break;
+                        const int t = part * kSelectRows + i * kSelectThreads + tid;
+                        const uint64_t k = rank_key(weight_key(x[i]), t);
+                        const bool in = t >= m0 && t < m1 && (k & mask) == border;
+                        const uint64_t who = __ballot(in);
+                        if (who == 0) continue;
+                        uint32_t at = 0;
+                        if (lane == __builtin_ctzll(who)) at = atomicAdd(&s_listed, static_cast<uint32_t>(__popcll(who)));
+                        at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __popcll(who & ((1ull << lane) - 1));
+                        if (in) s_list[at] = k;  // in any order: only counts are taken of it
                     }
                 }
+                listed = true;
             }
             __syncthreads();
-            key |= s_pick[0] << shift;
-            mask |= 255u << shift;
-            need = s_pick[1];
         }
     }
-    uint32_t taken = 0, equal = 0;  // before this tile
-    for (int t0 = 0; t0 < n; t0 += kSelectThreads) {
-        const int t = t0 + tid;
-        const bool here = t < n, mid = here && t >= m0 && t < m1;
-        const uint32_t k = mid ? weight_key(w[t]) : 0u;
-        const bool eq = mid && need > 0 && k == key;
-        const uint64_t eqs = __ballot(eq);
-        if (lane == 0) s_wave[0][wave] = __popcll(eqs);
+    uint32_t taken = 0;  // before this part
+    const uint64_t below = (1ull << lane) - 1;
+    for (int part = 0; part < parts; ++part) {
+        if (parts > 1) load(part);
+        uint64_t takes = 0;  // of this thread's rows, a bit each
+        for (int i = tid; i < kSelectKeep * kSelectWaves; i += kSelectThreads) s_count[i] = 0;
         __syncthreads();
-        uint32_t before = equal, all_eq = 0;
-        for (int i = 0; i < kSelectWaves; ++i) {
-            if (i < wave) before += s_wave[0][i];
-            all_eq += s_wave[0][i];
+#pragma unroll
+        for (int i = 0; i < kSelectKeep; ++i) {
+            if (part * kSelectRows + i * kSelectThreads >= n) break;
+            const int t = part * kSelectRows + i * kSelectThreads + tid;
+            const bool mid = t >= m0 && t < m1;
+            const bool take = t < n && (!mid || rank_key(weight_key(x[i]), t) >= border);
+            takes |= static_cast<uint64_t>(take) << i;
+            const uint32_t c = __popcll(__ballot(take));
+            if (lane == 0) s_count[i * kSelectWaves + wave] = c;
         }
-        const uint64_t below = (1ull << lane) - 1;
-        const bool take = here && (all || !mid || (need > 0 && (k > key || (eq && before + __popcll(eqs & below) < need))));
-        const uint64_t takes = __ballot(take);
-        if (lane == 0) s_wave[1][wave] = __popcll(takes);
         __syncthreads();
-        uint32_t at = taken, all_take = 0;
-        for (int i = 0; i < kSelectWaves; ++i) {
-            if (i < wave) at += s_wave[1][i];
-            all_take += s_wave[1][i];
+        uint32_t total = 0;
+        if (wave < kSelectKeep * kSelectWaves / kWave) {
+            const uint32_t before = lanes_before(s_count[tid], total);
+            s_count[tid] = before;
+            if (lane == 0) s_wave[wave] = total;
         }
-        at += __popcll(takes & below);
-        if (take && at < static_cast<uint32_t>(a.budget)) {
-            kept[at] = t;
-            if (nw) nw[at] = w[t];
+        __syncthreads();
+        uint32_t sum = taken;
+#pragma unroll
+        for (int i = 0; i < kSelectKeep; ++i) {
+            if (part * kSelectRows + i * kSelectThreads >= n) break;
+            if (i > 0 && i * kSelectWaves % kWave == 0) sum += s_wave[i * kSelectWaves / kWave - 1];
+            const bool take = takes >> i & 1;
+            const uint32_t at = sum + s_count[i * kSelectWaves + wave] + __popcll(__ballot(take) & below);
+            if (take && at < static_cast<uint32_t>(a.budget)) {
+                kept[at] = part * kSelectRows + i * kSelectThreads + tid;
+                if (nw) nw[at] = x[i];
+            }
         }
-        taken += all_take;
-        equal += all_eq;
+        for (int i = 0; i < kSelectKeep * kSelectWaves / kWave; ++i) taken += s_wave[i];
+        __syncthreads();
     }
     const int have = min(n, a.budget);
     for (int i = have + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
@@ -225,11 +365,14 @@ __global__ __launch_bounds__(kSelectThreads) void q4_select(const EvictArgs a) {
     if (h == 0 && tid == 0) a.new_rows[b] = have;
 }
 
-// Their codes, scales and biases into the other cache, a workgroup per 8 rows of it and kv head.
+// Their codes, scales and biases into the other cache, a workgroup per 2,048 / HD rows of it and kv head:
+// each thread takes a k word, a v word, which has its codes from 8 rows anywhere, and half of them a
+// parameter; all its loads are in flight together.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_gather(const EvictArgs a) {
-    constexpr int NG = HD / kQ4Group, W = HD / 8;
-    __shared__ int s_row[kQ4Block];
+    constexpr int NG = HD / kQ4Group, W = HD / 8, ROWS = 256 / W;
+    static_assert(4 * NG * ROWS <= 256 && ROWS % kQ4Block == 0, "a thread each");
+    __shared__ int s_row[ROWS];
     const int h = blockIdx.y % a.src.KVH, b = blockIdx.y / a.src.KVH, tid = threadIdx.x;
     const int have = min(min(max(a.rows[b], 0), a.src.maxp), a.budget);
     const int32_t *kept = a.kept + a.src.head(b, h) * a.budget;
@@ -237,24 +380,22 @@ __global__ __launch_bounds__(256) void q4_gather(const EvictArgs a) {
     uint32_t *dk = a.dst.k_head(b, h), *dv = a.dst.v_head(b, h);
     const _Float16 *sp = a.src.par_head(b, h);
     _Float16 *dp = a.dst.par_head(b, h);
-    for (int blk = blockIdx.x; blk * kQ4Block < have; blk += gridDim.x) {
-        const int j0 = blk * kQ4Block, n = min(kQ4Block, have - j0);
-        if (tid < kQ4Block) s_row[tid] = tid < n ? min(max(kept[j0 + tid], 0), a.src.maxp - 1) : 0;
+    for (int j0 = blockIdx.x * ROWS; j0 < have; j0 += gridDim.x * ROWS) {
+        const int n = min(ROWS, have - j0);
+        if (tid < ROWS) s_row[tid] = min(max(kept[j0 + min(tid, n - 1)], 0), a.src.maxp - 1);  // past the last: it again
         __syncthreads();
-        for (int i = tid; i < n * W; i += 256)
-            dk[static_cast<int64_t>(j0) * W + i] = sk[static_cast<int64_t>(s_row[i / W]) * W + i % W];
-        for (int i = tid; i < 4 * NG * n; i += 256) {
-            const int64_t line = static_cast<int64_t>(i / n);
-            dp[line * a.dst.R + j0 + i % n] = sp[line * a.src.R + s_row[i % n]];
-        }
-        for (int d = tid; d < HD; d += 256) {
-            uint32_t word = 0;
-            for (int u = 0; u < n; ++u) {
-                const int r = s_row[u];
-                word |= ((sv[static_cast<int64_t>(r / 8) * HD + d] >> (4 * (r & 7))) & 15u) << (4 * u);
-            }
-            dv[static_cast<int64_t>(blk) * HD + d] = word;
-        }
+        const int blk = tid / HD, d = tid % HD, left = n - blk * kQ4Block;
+        const int64_t line = tid / ROWS % (4 * NG);
+        const uint32_t k = sk[static_cast<int64_t>(s_row[tid / W]) * W + tid % W];
+        const _Float16 p = sp[line * a.src.R + s_row[tid % ROWS]];
+        uint32_t c[kQ4Block], word = 0;
+#pragma unroll
+        for (int u = 0; u < kQ4Block; ++u) c[u] = sv[static_cast<int64_t>(s_row[blk * kQ4Block + u] / 8) * HD + d];
+#pragma unroll
+        for (int u = 0; u < kQ4Block; ++u) word |= u < left ? ((c[u] >> (4 * (s_row[blk * kQ4Block + u] & 7))) & 15u) << (4 * u) : 0u;
+        if (tid / W < n) dk[static_cast<int64_t>(j0) * W + tid] = k;
+        if (tid < 4 * NG * ROWS && tid % ROWS < n) dp[line * a.dst.R + j0 + tid % ROWS] = p;
+        if (left > 0) dv[static_cast<int64_t>(j0 / kQ4Block + blk) * HD + d] = word;
         __syncthreads();
     }
 }
@@ -359,7 +500,8 @@ extern "C" int swq_q4_evict(const swq_q4_cache *src, int sequences, const float 
     hipStream_t s = static_cast<hipStream_t>(stream);
     const uint32_t heads = static_cast<uint32_t>(sequences) * src->num_kv_heads;
     hipLaunchKernelGGL(q4_select, dim3(heads), dim3(kSelectThreads), 0, s, a);
-    const dim3 grid((budget + kQ4Block - 1) / kQ4Block, heads);
+    const int per = 2048 / src->head_dim;
+    const dim3 grid((budget + per - 1) / per, heads);
     switch (src->head_dim) {
         case 64: hipLaunchKernelGGL(q4_gather<64>, grid, dim3(256), 0, s, a); break;
         case 128: hipLaunchKernelGGL(q4_gather<128>, grid, dim3(256), 0, s, a); break;

@@ -19,14 +19,14 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
     return __builtin_bit_cast(double, lo | (static_cast<uint64_t>(hi) << 32));
 }
 
-// op over LANES consecutive lanes (16, 32 or 64), to each of them: through DPP within 16, then
+// op over LANES consecutive lanes (8, 16, 32 or 64), to each of them: through DPP within 16, then
 // through scalar registers (a ds_bpermute per step and half costs four times as long).
 template <int LANES, typename Op>
 __device__ __forceinline__ double reduce_f64(double v, Op op) {
     v = op(v, dpp_f64<0xB1>(v));   // quad_perm [1,0,3,2]
     v = op(v, dpp_f64<0x4E>(v));   // quad_perm [2,3,0,1]
     v = op(v, dpp_f64<0x141>(v));  // row_half_mirror
-    v = op(v, dpp_f64<0x140>(v));  // row_mirror
+    if constexpr (LANES >= 16) v = op(v, dpp_f64<0x140>(v));  // row_mirror
     if constexpr (LANES > 16) {
         const double a = op(lane_f64(v, 0), lane_f64(v, 16)), b = op(lane_f64(v, 32), lane_f64(v, 48));
         v = LANES == 64 ? op(a, b) : (threadIdx.x & 32 ? b : a);
@@ -58,9 +58,10 @@ __device__ __forceinline__ _Float16 f16_by_f32(double x) {
     return static_cast<_Float16>(f);
 }
 
-// 4-bit codes of one head's row, EPL consecutive dims per lane in 64 bits: the scale and bias of
-// this lane's 64 dims, the codes into q.  Divisions are exact to their last bit, so a value that
-// lies on a border between two codes goes to the even one.
+// 4-bit codes of EPL consecutive dims per lane in 64 bits, 64 / EPL lanes to a group: the scale and bias
+// of this lane's group, the codes into q.  (y - b) / s, its difference exact, is first taken with a
+// reciprocal in f32, off by less than 4e-6; where that leaves the nearest integer in doubt, by an exact
+// division, so that a value on a border between two codes goes to the even one.
 template <int EPL>
 __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q)[EPL], _Float16 &scale, _Float16 &bias) {
     double y[EPL], lo = INFINITY, hi = -INFINITY;
@@ -74,10 +75,20 @@ __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q
     hi = reduce_f64<kQ4Group / EPL>(hi, [](double a, double b) { return fmax(a, b); });
     bias = f16_by_f32(lo);
     scale = f16_by_f32((hi - lo) / 15.0);
-    const double b = static_cast<double>(static_cast<float>(bias)), s = static_cast<double>(static_cast<float>(scale));
+    const double b = static_cast<double>(static_cast<float>(bias));
+    const float s = static_cast<float>(scale), inv = s > 0.f ? 1.0f / s : 0.f;
+    bool doubt = false;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e)
-        q[e] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0)) : 0u;
+    for (int e = 0; e < EPL; ++e) {
+        const float t = static_cast<float>(y[e] - b) * inv, n = rintf(t);
+        doubt |= fabsf(t - n) > 0.4999f;
+        q[e] = static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f));
+    }
+    if (__any(doubt)) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            q[e] = s > 0.f ? static_cast<uint32_t>(fmin(fmax(rint((y[e] - b) / static_cast<double>(s)), 0.0), 15.0)) : 0u;
+    }
 }
 
 // Scale and bias of this lane's group to parameters `which` and which + 1 of `row`.
@@ -102,10 +113,10 @@ __device__ __forceinline__ void q4_key_row(double (&x)[HD / kWave], const Q4Head
 #pragma unroll
     for (int e = 0; e < EPL; ++e) ss += x[e] * x[e];
     ss = reduce_f64<kWave>(ss, [](double a, double b) { return a + b; });
-    const double root = sqrt(ss / HD + static_cast<double>(eps));
+    const double inv = 1.0 / sqrt(ss / HD + static_cast<double>(eps));
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-        x[e] = x[e] / root * static_cast<double>(tab.w[e]);
+        x[e] = x[e] * inv * static_cast<double>(tab.w[e]);
         lds[lane * EPL + e] = x[e];
     }
     __builtin_amdgcn_wave_barrier();
