@@ -374,7 +374,8 @@ typedef struct swq_q4_batch {
                                  evicted it is larger than the row); NULL: rows */
     const float *rope;        /* device [rope_positions][rotary_dims / 2][2]:
                                  cos and sin; swq_q4_rope_table gives
-                                 swq_attention_step's.  NULL if rotary_dims 0 */
+                                 swq_attention_step's.  16-byte aligned; NULL if
+                                 rotary_dims 0                                 */
     int32_t rope_positions;   /* positions past the table take its last entry */
     int32_t reserved;         /* must be 0                                    */
 } swq_q4_batch;

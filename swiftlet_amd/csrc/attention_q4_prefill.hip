@@ -12,7 +12,11 @@ constexpr float kLow = -1e30f;  // below every score: exponents against it stay 
 // ---- queries ----------------------------------------------------------------
 
 // q / rms * w, turned, times a power of two that brings the row's largest below 2^10; as f16 high
-// (and low) parts, the 8 dims of a chunk in the order of a cache word's operand.  8 dims per lane.
+// (and low) parts, the 8 dims of a chunk in the order of a cache word's operand.  8 dims per lane, and
+// kQueryRows consecutive (token, head) rows whose loads are in flight together and which read a
+// token's turns once.
+constexpr int kQueryRows = 4;
+
 template <int HD, int PQ, typename T>
 __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     constexpr int LPH = HD / 8, HPB = 256 / LPH;
@@ -20,53 +24,68 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     const int b = blockIdx.y, tid = threadIdx.x, slot = tid / LPH, j = tid % LPH;
     if (a.vmax && blockIdx.x == 0)  // for q4_largest
         for (int u = tid; u < 2 * a.c.KVH; u += 256) a.vmax[a.c.head(b, 0) * 2 + u] = 0;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * HPB + slot;
     const int cnt = a.b.count(b);
-    const bool here = item < static_cast<int64_t>(cnt) * a.H;
-    const int i = here ? static_cast<int>(item / a.H) : 0, h = here ? static_cast<int>(item % a.H) : 0;
-    const int64_t at = static_cast<int64_t>(a.b.first(b) + i) * a.H + h;
     if (cnt <= 0) return;
-    float x[8], w[8];
-    load8<T>(x, static_cast<const T *>(a.q) + at * 2 * HD + 8 * j);
-    load8<float>(w, a.q_norm_w + 8 * j);
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-    ss = lanes_sum<LPH>(ss);
-    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] *= sc * w[e];
-        s_rot[slot][8 * j + e] = x[e];
-    }
-    lds_barrier();
+    const uint32_t all = static_cast<uint32_t>(cnt) * a.H;  // the host keeps it below 2^31
+    const int64_t first = static_cast<int64_t>(a.b.first(b)) * a.H;
     const int half = a.b.rot / 2;
-    const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half : nullptr;
-    float top = 0.f;
+    const uint32_t row = (blockIdx.x * HPB + slot) * kQueryRows;
+    float x[kQueryRows][8], w[8];
+    float2 cs[8];
+    uint32_t turned = ~0u;  // the token whose turns cs holds
+    load8<float>(w, a.q_norm_w + 8 * j);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = 8 * j + e;
-        if (d < 2 * half) {
-            const float2 cs = turn[d < half ? d : d - half];
-            const float o = s_rot[slot][d < half ? d + half : d - half];
-            x[e] = d < half ? x[e] * cs.x - o * cs.y : x[e] * cs.x + o * cs.y;
+    for (int k = 0; k < kQueryRows; ++k) {
+        const uint32_t it = min(row + k, all - 1);
+        load8<T>(x[k], static_cast<const T *>(a.q) + (first + it) * 2 * HD + 8 * j);
+    }
+#pragma unroll
+    for (int k = 0; k < kQueryRows; ++k) {
+        const uint32_t token = min(row + k, all - 1) / a.H;
+        if (8 * j < 2 * half && token != turned) {
+            q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, token)) * half, half, j);
+            turned = token;
         }
-        top = fmaxf(top, fabsf(x[e]));
-    }
-    top = lanes_max<LPH>(top);
-    int ex = 0;
-    if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-    h8_t hi, lo;
+        float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float v = ldexpf(x[e], 10 - ex);
-        hi[q4_element(e)] = static_cast<_Float16>(v);
-        lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
+        for (int e = 0; e < 8; ++e) ss += x[k][e] * x[k][e];
+        ss = lanes_sum<LPH>(ss);
+        const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[k][e] *= sc * w[e];
+            s_rot[slot][8 * j + e] = x[k][e];
+        }
+        __builtin_amdgcn_wave_barrier();  // a head's lanes are of one wave
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = 8 * j + e;
+            if (d < 2 * half) {
+                const float o = s_rot[slot][d < half ? d + half : d - half];
+                x[k][e] = d < half ? x[k][e] * cs[e].x - o * cs[e].y : x[k][e] * cs[e].x + o * cs[e].y;
+            }
+            top = fmaxf(top, fabsf(x[k][e]));
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        top = lanes_max<LPH>(top);
+        int ex = 0;
+        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = ldexpf(x[k][e], 10 - ex);
+            hi[q4_element(e)] = static_cast<_Float16>(v);
+            lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
+        }
+        if (row + k >= all) continue;
+        const int64_t at = first + row + k;
+        reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
+        if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
+        if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 10);
     }
-    if (!here) return;
-    reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
-    if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
-    if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 10);
 }
 
 // The largest |bias| + 15 scale of a sequence's keys and of its values, by kv head: what high and low
@@ -78,14 +97,20 @@ __global__ __launch_bounds__(256) void q4_largest(const AttnQ4Args a) {
     const int n = static_cast<int>(min(static_cast<int64_t>(a.b.row0(b, a.c.maxp)) + cnt, static_cast<int64_t>(a.c.maxp)));
     const _Float16 *par = a.c.par_head(b, h);
     float top[2] = {0.f, 0.f};
-    for (int row = blockIdx.x * 256 + threadIdx.x; row < n; row += gridDim.x * 256)
-        for (int g = 0; g < ng; ++g)
+    // 8 rows of one group and kind per thread
+    const int octs = (n + 7) / 8;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < octs * 2 * ng; i += gridDim.x * 256) {
+        const int oct = i % octs, line = i / octs, w = line / ng, g = line % ng;
+        const _Float16 *p = par + (static_cast<int64_t>(2 * w) * ng + g) * a.c.R + 8 * oct;
+        const h8_t s = __builtin_bit_cast(h8_t, *reinterpret_cast<const uint4 *>(p));
+        const h8_t z = __builtin_bit_cast(h8_t, *reinterpret_cast<const uint4 *>(p + static_cast<int64_t>(ng) * a.c.R));
+        float t = 0.f;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const float s = static_cast<float>(par[(static_cast<int64_t>(2 * w) * ng + g) * a.c.R + row]);
-                const float z = static_cast<float>(par[(static_cast<int64_t>(2 * w + 1) * ng + g) * a.c.R + row]);
-                top[w] = fmaxf(top[w], fabsf(z) + 15.0f * s);
-            }
+        for (int e = 0; e < 8; ++e)
+            if (8 * oct + e < n) t = fmaxf(t, fabsf(static_cast<float>(z[e])) + 15.0f * static_cast<float>(s[e]));
+        top[0] = fmaxf(top[0], w == 0 ? t : 0.f);
+        top[1] = fmaxf(top[1], w == 1 ? t : 0.f);
+    }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         const float t = wave_max_all(top[w]);
@@ -649,7 +674,7 @@ template <int HD, int PQ, typename T>
 void launch_queries(const AttnQ4Args &a, hipStream_t s) {
     constexpr int HPB = 256 / (HD / 8);
     const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
-    hipLaunchKernelGGL((q4_queries<HD, PQ, T>), dim3(static_cast<uint32_t>((items + HPB - 1) / HPB), a.b.B), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((q4_queries<HD, PQ, T>), dim3(static_cast<uint32_t>((items + kQueryRows * HPB - 1) / (kQueryRows * HPB)), a.b.B), dim3(256), 0, s, a);
 }
 
 template <int HD>
@@ -658,7 +683,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     const int rows = static_cast<int>(std::min<int64_t>(a.c.maxp, 1 << 20));
     if (a.planes_q == 2) a.in_f32 ? launch_queries<HD, 2, float>(a, s) : launch_queries<HD, 2, uint16_t>(a, s);
     else a.in_f32 ? launch_queries<HD, 1, float>(a, s) : launch_queries<HD, 1, uint16_t>(a, s);
-    if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows + 1023) / 1024, 64), heads), dim3(256), 0, s, a);
+    if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows / 4 * (HD / kQ4Group) + 255) / 256, 256), heads), dim3(256), 0, s, a);
     const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
     if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
     else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
@@ -684,7 +709,7 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, i
     p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
     // two workgroups per CU, if the cached rows can be split that often with 256 rows each
     const int64_t groups = p.tiles * heads;
-    const int64_t want = std::max<int64_t>(1, 512 / groups), most = std::max<int64_t>(1, rows / 256);
+    const int64_t want = std::max<int64_t>(1, 256 / groups), most = std::max<int64_t>(1, rows / 256);
     const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits});
     p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
     p.splits = static_cast<int>((rows + p.per - 1) / p.per);

@@ -50,6 +50,11 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
             uint32_t q[8];
             _Float16 scale, bias;
             if (!values) {
+                float2 cs[8];
+                float w[8];
+                if (8 * j < 2 * half) q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half, half, j);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = a.w[8 * j + e];
                 double ss = 0.0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -66,20 +71,18 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
                 double *rot = s_rot[tid / LPR];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = x[e] * inv * static_cast<double>(a.w[8 * j + e]);
+                    x[e] = x[e] * inv * static_cast<double>(w[e]);
                     rot[8 * j + e] = x[e];
                 }
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 if (8 * j < 2 * half) {
-                    const float2 *turn = a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int d = 8 * j + e;
                         if (d < 2 * half) {
-                            const float2 cs = turn[d < half ? d : d - half];
                             const double o = rot[d < half ? d + half : d - half];
-                            const double c = static_cast<double>(cs.x), s = static_cast<double>(cs.y);
+                            const double c = static_cast<double>(cs[e].x), s = static_cast<double>(cs[e].y);
                             x[e] = d < half ? x[e] * c - o * s : x[e] * c + o * s;
                         }
                     }
