@@ -13,11 +13,10 @@ constexpr float kLow = -1e30f;  // below every score: exponents against it stay 
 
 // q / rms * w, turned, times a power of two that brings the row's largest below 2^10; as f16 high
 // (and low) parts, the 8 dims of a chunk in the order of a cache word's operand.  8 dims per lane, and
-// kQueryRows consecutive (token, head) rows whose loads are in flight together and which read a
-// token's turns once.
-constexpr int kQueryRows = 4;
-
-template <int HD, int PQ, typename T>
+// ROWS consecutive (token, head) rows whose loads are in flight together and which read a token's turns
+// once: four where that gives each compute unit two workgroups, else one (77 tokens of 16 heads of 256: 5
+// us, with four 8; 4,096 tokens of 32 heads of 128: 21, with one 28).
+template <int HD, int PQ, int ROWS, typename T>
 __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     constexpr int LPH = HD / 8, HPB = 256 / LPH;
     __shared__ float s_rot[HPB][HD];
@@ -29,18 +28,18 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     const uint32_t all = static_cast<uint32_t>(cnt) * a.H;  // the host keeps it below 2^31
     const int64_t first = static_cast<int64_t>(a.b.first(b)) * a.H;
     const int half = a.b.rot / 2;
-    const uint32_t row = (blockIdx.x * HPB + slot) * kQueryRows;
-    float x[kQueryRows][8], w[8];
+    const uint32_t row = (blockIdx.x * HPB + slot) * ROWS;
+    float x[ROWS][8], w[8];
     float2 cs[8];
     uint32_t turned = ~0u;  // the token whose turns cs holds
     load8<float>(w, a.q_norm_w + 8 * j);
 #pragma unroll
-    for (int k = 0; k < kQueryRows; ++k) {
+    for (int k = 0; k < ROWS; ++k) {
         const uint32_t it = min(row + k, all - 1);
         load8<T>(x[k], static_cast<const T *>(a.q) + (first + it) * 2 * HD + 8 * j);
     }
 #pragma unroll
-    for (int k = 0; k < kQueryRows; ++k) {
+    for (int k = 0; k < ROWS; ++k) {
         const uint32_t token = min(row + k, all - 1) / a.H;
         if (8 * j < 2 * half && token != turned) {
             q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, token)) * half, half, j);
@@ -674,7 +673,10 @@ template <int HD, int PQ, typename T>
 void launch_queries(const AttnQ4Args &a, hipStream_t s) {
     constexpr int HPB = 256 / (HD / 8);
     const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
-    hipLaunchKernelGGL((q4_queries<HD, PQ, T>), dim3(static_cast<uint32_t>((items + kQueryRows * HPB - 1) / (kQueryRows * HPB)), a.b.B), dim3(256), 0, s, a);
+    if (items * a.b.B >= 4 * HPB * 512)
+        hipLaunchKernelGGL((q4_queries<HD, PQ, 4, T>), dim3(static_cast<uint32_t>((items + 4 * HPB - 1) / (4 * HPB)), a.b.B), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((q4_queries<HD, PQ, 1, T>), dim3(static_cast<uint32_t>((items + HPB - 1) / HPB), a.b.B), dim3(256), 0, s, a);
 }
 
 template <int HD>

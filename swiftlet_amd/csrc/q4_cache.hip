@@ -46,10 +46,10 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
             const int64_t at = (static_cast<int64_t>(n0 + i) * a.c.KVH + h) * HD + 8 * j;
             float in[8];
             load8<T>(in, static_cast<const T *>(values ? a.v : a.k) + at);
-            double x[8];
             uint32_t q[8];
             _Float16 scale, bias;
             if (!values) {
+                double x[8];
                 float2 cs[8];
                 float w[8];
                 if (8 * j < 2 * half) q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half, half, j);
@@ -89,11 +89,10 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
                 }
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                q4_quantise<8>(x, q, scale, bias);
             } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = static_cast<double>(in[e]);
+                q4_quantise(in, q, scale, bias);
             }
-            q4_quantise<8>(x, q, scale, bias);
             if (here && j % 8 == 0) {
                 _Float16 *p = par + (static_cast<int64_t>(values ? kQ4VScale : kQ4KScale) * NG + j / 8) * a.c.R + row;
                 p[0] = scale;

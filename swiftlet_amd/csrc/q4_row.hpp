@@ -13,6 +13,11 @@ __device__ __forceinline__ double dpp_f64(double v) {
     return __builtin_bit_cast(double, lo | (hi << 32));
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+    return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(v)));
+}
+
 __device__ __forceinline__ double lane_f64(double v, int lane) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
@@ -58,10 +63,31 @@ __device__ __forceinline__ _Float16 f16_by_f32(double x) {
     return static_cast<_Float16>(f);
 }
 
-// 4-bit codes of EPL consecutive dims per lane in 64 bits, 64 / EPL lanes to a group: the scale and bias
-// of this lane's group, the codes into q.  (y - b) / s, its difference exact, is first taken with a
-// reciprocal in f32, off by less than 4e-6; where that leaves the nearest integer in doubt, by an exact
-// division, so that a value on a border between two codes goes to the even one.
+// The codes of values whose group has scale and bias.  (y - b) / s is first taken in f32 with a
+// reciprocal: codes are at most 15 and a bit and the difference, the reciprocal and the product each
+// round once, so it is off by less than 16 * 4 * 2^-24 = 4e-6.  Where that leaves the nearest integer in
+// doubt an exact division decides, so that a value on a border between two codes goes to the even one.
+template <int EPL, typename X>
+__device__ __forceinline__ void q4_codes(const X (&y)[EPL], uint32_t (&q)[EPL], _Float16 scale, _Float16 bias) {
+    const X b = static_cast<X>(static_cast<float>(bias));
+    const float s = static_cast<float>(scale), inv = s > 0.f ? 1.0f / s : 0.f;
+    bool doubt = false;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        const float t = static_cast<float>(y[e] - b) * inv, n = rintf(t);
+        doubt |= fabsf(t - n) > 0.49999f;
+        q[e] = static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f));
+    }
+    if (__any(doubt)) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            q[e] = s > 0.f ? static_cast<uint32_t>(fmin(fmax(rint((static_cast<double>(y[e]) - static_cast<double>(b)) / static_cast<double>(s)), 0.0), 15.0))
+                           : 0u;
+    }
+}
+
+// 4-bit codes of EPL consecutive dims per lane, 64 / EPL lanes to a group: the scale and bias of this
+// lane's group, the codes into q.
 template <int EPL>
 __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q)[EPL], _Float16 &scale, _Float16 &bias) {
     double y[EPL], lo = INFINITY, hi = -INFINITY;
@@ -75,20 +101,27 @@ __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q
     hi = reduce_f64<kQ4Group / EPL>(hi, [](double a, double b) { return fmax(a, b); });
     bias = f16_by_f32(lo);
     scale = f16_by_f32((hi - lo) / 15.0);
-    const double b = static_cast<double>(static_cast<float>(bias));
-    const float s = static_cast<float>(scale), inv = s > 0.f ? 1.0f / s : 0.f;
-    bool doubt = false;
+    q4_codes<EPL>(y, q, scale, bias);
+}
+
+// The same of numbers that come in 32 bits, 8 per lane: only their difference needs more.
+__device__ __forceinline__ void q4_quantise(const float (&x)[8], uint32_t (&q)[8], _Float16 &scale, _Float16 &bias) {
+    float y[8], lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        const float t = static_cast<float>(y[e] - b) * inv, n = rintf(t);
-        doubt |= fabsf(t - n) > 0.4999f;
-        q[e] = static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f));
+    for (int e = 0; e < 8; ++e) {
+        y[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -65504.f), 65504.f) : 0.f;
+        lo = fminf(lo, y[e]);
+        hi = fmaxf(hi, y[e]);
     }
-    if (__any(doubt)) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-            q[e] = s > 0.f ? static_cast<uint32_t>(fmin(fmax(rint((y[e] - b) / static_cast<double>(s)), 0.0), 15.0)) : 0u;
-    }
+    lo = fminf(lo, dpp_f32<0xB1>(lo));
+    hi = fmaxf(hi, dpp_f32<0xB1>(hi));
+    lo = fminf(lo, dpp_f32<0x4E>(lo));
+    hi = fmaxf(hi, dpp_f32<0x4E>(hi));
+    lo = fminf(lo, dpp_f32<0x141>(lo));
+    hi = fmaxf(hi, dpp_f32<0x141>(hi));
+    bias = static_cast<_Float16>(lo);
+    scale = f16_by_f32((static_cast<double>(hi) - static_cast<double>(lo)) / 15.0);
+    q4_codes<8>(y, q, scale, bias);
 }
 
 // Scale and bias of this lane's group to parameters `which` and which + 1 of `row`.
