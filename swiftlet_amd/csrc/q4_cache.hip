@@ -21,8 +21,8 @@ struct AppendArgs {
 // 8 dims each, so that a lane's codes are one k word, a wave takes 2 to 8 rows at once and sums cross few
 // lanes.  A v word holds 8 rows of one dim: those codes meet in LDS, and words of which only some rows
 // are new keep the others (the first and last block of a call).  All in 64 bits up to the format's own
-// roundings.  Bound by that arithmetic: 8,192 tokens of 8 heads of 128 (43 MB) 24 us; one row per wave
-// and a division per value took 58.
+// roundings.  Bound by that arithmetic (24 of the time in VALU instructions at 8,192 tokens of 8 heads
+// of 128, 43 MB: 36 us); one row per wave and a division per value took 58.
 template <int HD, typename T>
 __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) {
     constexpr int LPR = HD / 8, PER = kQ4Block * LPR;  // lanes of a row, of a block's keys or values
@@ -133,43 +133,70 @@ struct ReadArgs {
     void *k, *v;
 };
 
-// A thread per (row, kv head, 8 dims): one k word, and 8 v words of which it takes its row's codes.
+// A thread per (kReadRows rows, kv head, 8 dims): their k words, and the block's 8 v words, of which it
+// takes its rows' codes.  Bound by the bytes it writes: 8,192 rows of 8 heads of 128 to f32 (77 MB) 18 us,
+// 4.3 TB/s; a row or a block of 8 per thread take as long there, but 8 rows 8 us where two take 5 (2,048
+// rows of 2 heads of 256, too few waves).
+constexpr int kReadRows = 2;
+
 template <typename T>
 __global__ __launch_bounds__(256) void q4_read(const ReadArgs a) {
     const int b = blockIdx.y;
-    const int oct = a.c.hd / 8, per_row = a.c.KVH * oct;
+    const uint32_t oct = a.c.hd / 8, per_row = a.c.KVH * oct;
     const int s0 = a.starts ? min(max(a.starts[b], 0), a.count) : 0;
     const int n = a.starts ? max(min(a.starts[b + 1], a.count) - s0, 0) : a.count;
+    if (n <= 0) return;
     const int64_t out0 = a.starts ? s0 : static_cast<int64_t>(b) * a.count;
+    const int64_t first = a.first ? a.first[b] : 0;
     const int top = a.rows ? min(a.rows[b], a.c.maxp) : a.c.maxp;
-    const int first = a.first ? a.first[b] : 0;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < static_cast<int64_t>(n) * per_row;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int t = static_cast<int>(i / per_row), h = static_cast<int>(i % per_row) / oct, j = static_cast<int>(i % oct);
-        const int64_t row = static_cast<int64_t>(first) + t;
-        const bool there = row >= 0 && row < top;
-        const int64_t at = ((out0 + t) * a.c.KVH + h) * a.c.hd + 8 * j;
-        const int ng = a.c.hd / kQ4Group, g = 8 * j / kQ4Group;
-        const _Float16 *par = a.c.par_head(b, h) + row;
+    const int64_t base = first & ~static_cast<int64_t>(kReadRows - 1);  // an even row: a pair is of one block
+    const int64_t pairs = (first + n - base + kReadRows - 1) / kReadRows;
+    const int ng = a.c.hd / kQ4Group;
+    const uint32_t each = per_row < 256 ? 256 / per_row : 1;  // pairs of a workgroup, which follow one another
+    for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * each; c0 < pairs; c0 += static_cast<int64_t>(gridDim.x) * each) {
+        for (uint32_t i = threadIdx.x; i < each * per_row; i += 256) {
+            const uint32_t u = i / per_row, v = i - u * per_row, h = v / oct, j = v - h * oct;
+            const int64_t row0 = base + (c0 + u) * kReadRows, t0 = row0 - first;
+            if (c0 + u >= pairs) continue;
+            const bool inside = row0 >= 0 && row0 < top;
+            const _Float16 *par = a.c.par_head(b, h) + row0 + static_cast<int64_t>(j / 8) * a.c.R;
+            const uint32_t *kp = a.c.k_head(b, h) + row0 * oct + j, *vp = a.c.v_head(b, h) + (row0 / 8) * a.c.hd + 8 * j;
+            const int lift = 4 * static_cast<int>(row0 & 7);
+            uint32_t kw[kReadRows] = {}, sz[4] = {};
+            uint4 v0{}, v1{};
+            if (inside) {
+                if (a.k) {
+                    kw[0] = kp[0];
+                    kw[1] = kp[oct];
+                }
+                if (a.v) {
+                    v0 = reinterpret_cast<const uint4 *>(vp)[0];
+                    v1 = reinterpret_cast<const uint4 *>(vp)[1];
+                }
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            T *out = static_cast<T *>(which ? a.v : a.k);
-            if (!out) continue;
-            float s = 0.f, z = 0.f;
-            uint32_t word = 0;
-            if (there) {
-                s = static_cast<float>(par[(static_cast<int64_t>(2 * which) * ng + g) * a.c.R]);
-                z = static_cast<float>(par[(static_cast<int64_t>(2 * which + 1) * ng + g) * a.c.R]);
-                if (which) {
-                    const uint32_t *p = a.c.v_head(b, h) + (row / 8) * a.c.hd + 8 * j;
+                for (int w = 0; w < 4; ++w) sz[w] = *reinterpret_cast<const uint32_t *>(par + static_cast<int64_t>(w) * ng * a.c.R);
+            }
+            const uint32_t vw[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) word |= ((p[e] >> (4 * (row & 7))) & 15u) << (4 * e);
-                } else {
-                    word = a.c.k_head(b, h)[row * oct + j];
+            for (int r = 0; r < kReadRows; ++r) {
+                if (t0 + r < 0 || t0 + r >= n) continue;
+                const bool there = inside && row0 + r < top;
+                const int64_t at = ((out0 + t0 + r) * a.c.KVH + h) * a.c.hd + 8 * j;
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    T *out = static_cast<T *>(which ? a.v : a.k);
+                    if (!out) continue;
+                    const float s = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[2 * which] >> (16 * r))));
+                    const float z = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[2 * which + 1] >> (16 * r))));
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t q = which ? vw[e] >> (lift + 4 * r) : kw[r] >> (4 * e);
+                        x[e] = there ? fmaf(s, static_cast<float>(q & 15u), z) : 0.f;
+                    }
+                    store8(out + at, x);
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q4_store(out, at + e, there ? fmaf(s, static_cast<float>((word >> (4 * e)) & 15u), z) : 0.f);
         }
     }
 }
@@ -475,8 +502,9 @@ extern "C" int swq_q4_read(const swq_q4_cache *cache, int sequences, const int32
         return SWQ_ERR_MISALIGNED;
     if (count == 0) return SWQ_OK;
     const ReadArgs a{q4_view(cache), first, starts, rows, count, sequences, k, v};
-    const int64_t items = static_cast<int64_t>(count) * cache->num_kv_heads * (cache->head_dim / 8);
-    const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((items + 255) / 256, 4096)), sequences);
+    // count rows may begin and end inside a pair
+    const int64_t pairs = static_cast<int64_t>(count) / kReadRows + 1, each = std::max(1, 256 / (cache->num_kv_heads * (cache->head_dim / 8)));
+    const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((pairs + each - 1) / each, 4096)), sequences);
     if (dtype == SWQ_F32) hipLaunchKernelGGL(q4_read<float>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
     else hipLaunchKernelGGL(q4_read<uint16_t>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
     return launch_status();

@@ -187,6 +187,24 @@ __device__ __forceinline__ void load8(float (&x)[8], const T *p) {
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            T lo, hi;
+            q4_store(&lo, 0, x[2 * i]);
+            q4_store(&hi, 0, x[2 * i + 1]);
+            w[i] = lo | static_cast<uint32_t>(hi) << 16;
+        }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 // cos and sin of dims 8 j .. 8 j + 7 of a row's turns (those below 2 half: the others' are not used).
 // 64 bytes in a row where half allows: as 8 pairs the loads took more time than the rest of a query's
 // work (4,096 tokens of 32 heads of 128: 28 us, now 21).
