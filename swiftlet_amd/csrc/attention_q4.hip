@@ -113,6 +113,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
         if (ws_bytes < parts.total) return SWQ_ERR_WORKSPACE;
         a.per = plan.per;
         a.splits = plan.splits;
+        a.planes_q = a.in_f32 || a.out_f32 || weights ? 2 : 1;
         if (a.splits > 1 || weights) {
             a.part = reinterpret_cast<float *>(p);
             a.ml = reinterpret_cast<float2 *>(p + parts.part);

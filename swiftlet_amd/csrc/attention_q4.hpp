@@ -72,6 +72,14 @@ __device__ __forceinline__ h8_t q4_operand(uint32_t w, uint32_t magic) {
     return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// The same with 1024 added to each element.
+__device__ __forceinline__ h8_t q4_operand_1024(uint32_t w, uint32_t magic) {
+    constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;
+    const uint32_t s = w >> 8;
+    const uint4 u = make_uint4((w & kEven) | magic, (w & kOdd) | magic, (s & kEven) | magic, (s & kOdd) | magic);
+    return __builtin_bit_cast(h8_t, u);
+}
+
 // Operand element of a nibble, and the nibble of an element.
 __device__ __forceinline__ constexpr int q4_element(int nibble) { return nibble < 4 ? 2 * nibble : 2 * nibble - 7; }
 __device__ __forceinline__ constexpr int q4_nibble(int element) { return element / 2 + 4 * (element & 1); }

@@ -46,21 +46,23 @@ __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n
 //           maximum's factor is the lane's own.  p * bias is summed on the VALU.
 // Heads past the group are columns that nothing reads.  The next tile's loads are issued as soon as
 // their registers are free.
-template <int HD, typename T>
+template <int HD, int P, typename T>
 __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const AttnQ4Args a) {
     constexpr int EPL = HD / kWave, NG = HD / kQ4Group, GW = NG > 1 ? 2 : 1, TW = NG / GW, TEAMS = kStepWaves / TW;
     constexpr int HP = HD + kHeadPad;
-    __shared__ h8_t s_q[2][NG][2][kWave];  // queries in operand order: [high, low][group][step][lane]
+    __shared__ h8_t s_q[P][NG][2][kWave];  // queries in operand order: [high, low][group][step][lane]
+    __shared__ float s_off[P == 1 ? NG : 1][kQ4MaxHeadGroup];
     __shared__ float s_qs[NG][kQ4MaxHeadGroup], s_f[kQ4MaxHeadGroup];
     __shared__ float s_ml[TEAMS][2][kQ4MaxHeadGroup];
     // one after another, a barrier between them: heads to be rotated, partial scores, teams' sums
     constexpr int kRotWave = 256;  // doubles of a wave: a key, or all the heads that it takes at once
     constexpr int kRot = kStepWaves * kRotWave * 8, kPart = TW > 1 ? 2 * kStepWaves * 2 * kWave * 16 : 0;
-    constexpr int kSums = TEAMS * kQ4MaxHeadGroup * HP * 4;
+    constexpr int SETS = TEAMS > 2 ? 2 : TEAMS;  // two teams' sums at a time
+    constexpr int kSums = SETS * kQ4MaxHeadGroup * HP * 4;
     __shared__ __attribute__((aligned(16))) uint8_t s_buf[kRot > kPart ? (kRot > kSums ? kRot : kSums) : (kPart > kSums ? kPart : kSums)];
     double(*s_rot)[kRotWave] = reinterpret_cast<double(*)[kRotWave]>(s_buf);
     f4_t(*s_part)[kStepWaves][2][kWave] = reinterpret_cast<f4_t(*)[kStepWaves][2][kWave]>(s_buf);
-    float *s_o = reinterpret_cast<float *>(s_buf);  // [team][head][HP]
+    float *s_o = reinterpret_cast<float *>(s_buf);  // [team % SETS][head][HP]
     // Workgroups go to the 8 XCDs in turn: with the splits outermost and the heads turned by one from
     // split to split, no XCD gets the same splits, or the same sequences, of every head.
     const int split = blockIdx.y, head = (blockIdx.x + blockIdx.y) % gridDim.x;
@@ -187,12 +189,24 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
                 hi[q4_element(e)] = static_cast<_Float16>(y);
                 lo[q4_element(e)] = static_cast<_Float16>(y - static_cast<float>(hi[q4_element(e)]));
             }
+            float off = 0.f;
+            if constexpr (P == 1) {  // the sum of what the products will take
+                float even = 0.f, odd = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    even += static_cast<float>(hi[q4_element(e)]);
+                    odd += static_cast<float>(hi[q4_element(e + 1)]);
+                }
+                qs = fmaf(odd, 16.0f, even);
+                off = lanes_sum<8>(even + odd) * -1024.0f;
+            }
             qs = lanes_sum<8>(qs);
             if (u < G) {
                 // word j % 8 of group j / 8: lane row (j % 8) / 2 of step j % 2
                 s_q[0][j / 8][j & 1][((j & 7) >> 1) * 16 + u] = hi;
-                s_q[1][j / 8][j & 1][((j & 7) >> 1) * 16 + u] = lo;
+                if constexpr (P == 2) s_q[P - 1][j / 8][j & 1][((j & 7) >> 1) * 16 + u] = lo;
                 if ((j & 7) == 0) s_qs[j / 8][u] = qs;
+                if (P == 1 && (j & 7) == 0) s_off[j / 8][u] = off;
                 if (j == 0) s_f[u] = ldexpf(a.scale2, ex - 10);
             }
         }
@@ -205,11 +219,12 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
     }
 
     const float f = r < G ? s_f[r] : 0.f;
-    float qs[GW], pb[GW];
+    float qs[GW], pb[GW], off[GW];
     f4_t o[GW][4];
 #pragma unroll
     for (int g = 0; g < GW; ++g) {
         qs[g] = s_qs[g0 + g][r];
+        off[g] = P == 1 ? s_off[P == 1 ? g0 + g : 0][r] : 0.f;
         pb[g] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[g][e] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -231,14 +246,15 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
                 const h8_t ks = __builtin_bit_cast(h8_t, cur.par[kQ4KScale][g]), kb = __builtin_bit_cast(h8_t, cur.par[kQ4KBias][g]);
                 f4_t d[2];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) d[x] = f4_t{0.f, 0.f, 0.f, 0.f};
+                for (int x = 0; x < 2; ++x) d[x] = f4_t{off[g], off[g], off[g], off[g]};
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const h8_t c = q4_operand(u ? cur.k[g][x].y : cur.k[g][x].x, magic);
+                        const uint32_t word = u ? cur.k[g][x].y : cur.k[g][x].x;
+                        const h8_t c = P == 1 ? q4_operand_1024(word, magic) : q4_operand(word, magic);
                         d[x] = mfma16(c, s_q[0][g0 + g][u][ql], d[x]);
-                        d[x] = mfma16(c, s_q[1][g0 + g][u][ql], d[x]);
+                        if constexpr (P == 2) d[x] = mfma16(c, s_q[P - 1][g0 + g][u][ql], d[x]);
                     }
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
@@ -335,22 +351,27 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
         for (int g = 0; g < GW; ++g) {
             const h8_t vs = __builtin_bit_cast(h8_t, cur.par[kQ4VScale][g]), vb = __builtin_bit_cast(h8_t, cur.par[kQ4VBias][g]);
             h8_t hi, lo;
+            if constexpr (P == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const f32x2_t x = {pe[j] * static_cast<float>(vs[q4_nibble(j)]), pe[j + 1] * static_cast<float>(vs[q4_nibble(j + 1)])};
-                h2_t h, w;
-                split_f16(x, h, w);
-                hi[j] = h.x;
-                hi[j + 1] = h.y;
-                lo[j] = w.x;
-                lo[j + 1] = w.y;
+                for (int j = 0; j < 8; ++j) hi[j] = static_cast<_Float16>(fmaf(pe[j], static_cast<float>(vs[q4_nibble(j)]), 0.f));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const f32x2_t x = {pe[j] * static_cast<float>(vs[q4_nibble(j)]), pe[j + 1] * static_cast<float>(vs[q4_nibble(j + 1)])};
+                    h2_t h, w;
+                    split_f16(x, h, w);
+                    hi[j] = h.x;
+                    hi[j + 1] = h.y;
+                    lo[j] = w.x;
+                    lo[j + 1] = w.y;
+                }
             }
             const uint32_t vw4[4] = {cur.v[g].x, cur.v[g].y, cur.v[g].z, cur.v[g].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const h8_t c = q4_operand(vw4[e], magic);
                 o[g][e] = mfma16(c, hi, o[g][e]);
-                o[g][e] = mfma16(c, lo, o[g][e]);
+                if constexpr (P == 2) o[g][e] = mfma16(c, lo, o[g][e]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) pb[g] = fmaf(p[i], static_cast<float>(vb[i]), pb[g]);
@@ -378,19 +399,28 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
 #pragma unroll
         for (int w = 1; w < TEAMS; ++w) M = fmaxf(M, s_ml[w][0][r]);
         unit *= q4_exp2(m - M);
-        float *mo = s_o + (team * kQ4MaxHeadGroup + r) * HP + 64 * g0 + 16 * q;
+        float *mo = s_o + (team % SETS * kQ4MaxHeadGroup + r) * HP + 64 * g0 + 16 * q;
 #pragma unroll
-        for (int g = 0; g < GW; ++g)
+        for (int set = TEAMS / SETS - 1; set >= 0; --set) {
+            if (team / SETS == set) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4 *>(mo + 64 * g + 4 * i) = make_float4(unit * (o[g][0][i] + pb[g]), unit * (o[g][1][i] + pb[g]),
-                                                                              unit * (o[g][2][i] + pb[g]), unit * (o[g][3][i] + pb[g]));
+                for (int g = 0; g < GW; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f4_t x = {unit * (o[g][0][i] + pb[g]), unit * (o[g][1][i] + pb[g]), unit * (o[g][2][i] + pb[g]), unit * (o[g][3][i] + pb[g])};
+                        f4_t *to = reinterpret_cast<f4_t *>(mo + 64 * g + 4 * i);
+                        if (set < TEAMS / SETS - 1) x += *to;
+                        *to = x;
+                    }
+            }
+            if (set > 0) lds_barrier();
+        }
         lds_barrier();
         for (int i = tid; i < G * (HD / 4); i += kStepThreads) {
             const int u = i / (HD / 4), d = i % (HD / 4) * 4;
             f4_t s = *reinterpret_cast<const f4_t *>(s_o + u * HP + d);
 #pragma unroll
-            for (int w = 1; w < TEAMS; ++w) s += *reinterpret_cast<const f4_t *>(s_o + (w * kQ4MaxHeadGroup + u) * HP + d);
+            for (int w = 1; w < SETS; ++w) s += *reinterpret_cast<const f4_t *>(s_o + (w * kQ4MaxHeadGroup + u) * HP + d);
             M = s_ml[0][0][u];
             L = 0.f;
 #pragma unroll
@@ -515,7 +545,9 @@ __global__ __launch_bounds__(kMergeThreads) void q4_step_merge(const AttnQ4Args 
 template <int HD, typename T>
 void launch_typed(const AttnQ4Args &a, hipStream_t s) {
     const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
-    hipLaunchKernelGGL((q4_step<HD, T>), dim3(heads, a.splits), dim3(kStepThreads), 0, s, a);
+    const dim3 grid(heads, a.splits), block(kStepThreads);
+    if (sizeof(T) == 2 && a.planes_q == 1) hipLaunchKernelGGL((q4_step<HD, sizeof(T) == 2 ? 1 : 2, T>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((q4_step<HD, 2, T>), grid, block, 0, s, a);
     if (a.part) {
         const int chunks = a.weights ? (a.c.maxp + kMergeRows - 1) / kMergeRows : 0;
         hipLaunchKernelGGL(q4_step_merge<HD>, dim3(a.group + chunks, heads), dim3(kMergeThreads), 0, s, a);
