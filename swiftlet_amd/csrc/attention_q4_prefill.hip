@@ -685,6 +685,15 @@ void launch_queries(const AttnQ4Args &a, hipStream_t s) {
         hipLaunchKernelGGL((q4_queries<HD, PQ, 1, T>), dim3(static_cast<uint32_t>((items + HPB - 1) / HPB), a.b.B), dim3(256), 0, s, a);
 }
 
+template <int HD, int WAVES>
+void launch_tiles(const AttnQ4Args &a, dim3 grid, hipStream_t s) {
+    constexpr int NT = HD == 64 ? 64 : 32;
+    const dim3 block(WAVES * kWave);
+    if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, NT, WAVES>), grid, block, 0, s, a);
+    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, NT, WAVES>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, NT, WAVES>), grid, block, 0, s, a);
+}
+
 template <int HD>
 void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
@@ -693,9 +702,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     else a.in_f32 ? launch_queries<HD, 1, float>(a, s) : launch_queries<HD, 1, uint16_t>(a, s);
     if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows / 4 * (HD / kQ4Group) + 255) / 256, 256), heads), dim3(256), 0, s, a);
     const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
-    if (a.planes_q == 1) hipLaunchKernelGGL((q4_prefill<HD, 1, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
-    else if (a.planes_v == 1) hipLaunchKernelGGL((q4_prefill<HD, 2, 1, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((q4_prefill<HD, 2, 2, HD == 64 ? 64 : 32, 8>), grid, dim3(512), 0, s, a);
+    a.rows_per == 64 ? launch_tiles<HD, 4>(a, grid, s) : launch_tiles<HD, 8>(a, grid, s);
     if (a.splits > 1) {
         constexpr int RPB = 256 / (HD / 4);
         const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
@@ -713,9 +720,12 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, i
     Q4PrefillPlan p{};
     p.planes_q = f32 || weights ? 2 : 1;
     p.planes_v = f32 ? 2 : 1;
-    p.rows_per = 128;
+    // 128 rows share a tile's values; where that leaves half of the compute units without work however
+    // the cached rows are split, 64, whose steps are shorter (77 tokens of 16 heads of 256 in f32: 26 us,
+    // with 64 rows 21.6)
+    p.rows_per = (max_tokens * group + 127) / 128 * heads * std::max<int64_t>(1, rows / 256) <= 128 ? 64 : 128;
     p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
-    // two workgroups per CU, if the cached rows can be split that often with 256 rows each
+    // a workgroup per CU, if the cached rows can be split that often with 256 rows each
     const int64_t groups = p.tiles * heads;
     const int64_t want = std::max<int64_t>(1, 256 / groups), most = std::max<int64_t>(1, rows / 256);
     const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits});
