@@ -24,11 +24,12 @@ def _code(t, what):
     raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, what)
 
 
-def _ptr(t, count, what, dtype=None):
-    """The address of a contiguous tensor of `count` elements (at least, for int32 arrays)."""
-    torch = _torch()
+def _ptr(t, count, what, device, dtype=None):
+    """The address of a contiguous tensor of `count` elements (at least, for int32 arrays) on the cache's device."""
     if t is None:
         return None
+    if t.get_device() != device:
+        raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": not on the cache's device")
     if not t.is_contiguous() or t.numel() < count or (dtype is not None and t.dtype != dtype):
         raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
     return t.data_ptr()
@@ -55,6 +56,13 @@ class Q4Cache:
         self.desc = Q4CacheDesc(data=data.data_ptr(), bytes=data.numel(), sequences=sequences, num_kv_heads=num_kv_heads,
                                 head_dim=head_dim, max_positions=max_positions)
         self.ref = ctypes.byref(self.desc)
+        self.device_index = data.get_device()
+
+    def here(self, what):
+        """The cache's device, if it is the current one, to which streams and launches belong."""
+        if self.device_index < 0 or self.device_index != _torch().cuda.current_device():
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": the cache is not on the current device")
+        return self.device_index
 
     def views(self):
         """(k words int32 [B, KVH, R, hd/8], v words int32 [B, KVH, R/8, hd], params f16 [B, KVH, 4, hd/64, R])
@@ -77,13 +85,14 @@ class Q4Cache:
         if stream is not None and _elsewhere(stream):
             with torch.cuda.stream(stream):
                 return self.read(first, count, dtype, starts, tokens, rows, sequences)
-        B = sequences or self.sequences
+        B, at = sequences or self.sequences, self.here("q4_read")
         shape = (B, count, self.KVH, self.hd) if starts is None else (tokens, self.KVH, self.hd)
         if starts is not None and tokens is None:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "q4_read: starts without tokens")
         k, v = torch.empty((2, *shape), dtype=dtype or torch.float32, device=self.data.device).unbind(0)
-        check(self.lib.swq_q4_read(self.ref, B, _ptr(first, B, "q4_read: first", torch.int32),
-                                   _ptr(starts, B + 1, "q4_read: starts", torch.int32), _ptr(rows, B, "q4_read: rows", torch.int32),
+        check(self.lib.swq_q4_read(self.ref, B, _ptr(first, B, "q4_read: first", at, torch.int32),
+                                   _ptr(starts, B + 1, "q4_read: starts", at, torch.int32),
+                                   _ptr(rows, B, "q4_read: rows", at, torch.int32),
                                    shape[0] if starts is not None else count, k.data_ptr(), v.data_ptr(),
                                    _code(k, "q4_read"), _stream_handle(stream)), "q4_read")
         return k, v
@@ -92,8 +101,9 @@ class Q4Cache:
 class AttentionQ4GPU:
     """One self_attn block over a 4-bit cache: AttentionGPU's shapes, q/k norm
     weights (f32, device) and, optionally, projections and o_proj.  rope_table:
-    f32 device [positions, rotary_dims / 2, 2], cos and sin, which layers may
-    share; made for `max_positions` positions by the first workspace or call if not given."""
+    f32 device [positions, rotary_dims / 2, 2], cos and sin, 16-byte aligned, which
+    layers may share; made for `max_positions` positions by the first workspace or
+    call if not given (before a graph is captured, then)."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dims: int, rope_theta: float,
                  eps: float, max_positions: int, q_norm_weight, k_norm_weight, projections=(),
@@ -113,6 +123,8 @@ class AttentionQ4GPU:
                 rope_table.dtype != torch.float32 or not rope_table.is_contiguous()
                 or tuple(rope_table.shape[1:]) != (rotary_dims // 2, 2) or not len(rope_table)):
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "AttentionQ4GPU: rope_table")
+        if rope_table is not None and rotary_dims and rope_table.get_device() != self.q_norm.get_device():
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "AttentionQ4GPU: rope_table on another device than the norm weights")
         self._table = rope_table
         self._rope = None if rotary_dims else (None, 0)
         self._c = AttentionLayer(num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
@@ -161,9 +173,11 @@ class AttentionQ4GPU:
 
     def _batch(self, cache, rows, tokens, starts, max_tokens, max_rows, positions, what):
         torch = _torch()
-        B = rows.numel()
-        return Q4Batch(B, tokens, max_tokens, max_rows, _ptr(starts, B + 1, what + ": starts", torch.int32),
-                       _ptr(rows, 1, what + ": rows", torch.int32), _ptr(positions, B, what + ": positions", torch.int32),
+        B, at = rows.numel(), cache.here(what)
+        if self.q_norm.get_device() != at:
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": the cache is not on the block's device")
+        return Q4Batch(B, tokens, max_tokens, max_rows, _ptr(starts, B + 1, what + ": starts", at, torch.int32),
+                       _ptr(rows, 1, what + ": rows", at, torch.int32), _ptr(positions, B, what + ": positions", at, torch.int32),
                        *self._rope_args(), 0)
 
     def append(self, k, v, cache: Q4Cache, rows, starts=None, max_tokens: int | None = None, positions=None, stream=None):
@@ -172,10 +186,11 @@ class AttentionQ4GPU:
         bring different numbers of tokens, then max_tokens, at most that many of one (default: N)."""
         N = k.numel() // (self.KVH * self.hd)
         b = self._batch(cache, rows, N, starts, max_tokens or N, 0, positions, "q4_append")
-        n = N * self.KVH * self.hd
+        n, at = N * self.KVH * self.hd, cache.device_index
         if k.dtype != v.dtype:
             raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, "q4_append")
-        check(self.lib.swq_q4_append(self._ref, cache.ref, ctypes.byref(b), _ptr(k, n, "q4_append: k"), _ptr(v, n, "q4_append: v"),
+        check(self.lib.swq_q4_append(self._ref, cache.ref, ctypes.byref(b), _ptr(k, n, "q4_append: k", at),
+                                     _ptr(v, n, "q4_append: v", at),
                                      _code(k, "q4_append"), _stream_handle(stream)), "q4_append")
 
     def prefill(self, q, k, v, cache: Q4Cache, rows, ws, starts=None, max_tokens: int | None = None, out=None, weights=None,
@@ -198,13 +213,13 @@ class AttentionQ4GPU:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "attention_q4: k and v")
         if k is not None and (k.dtype != q.dtype or v.dtype != q.dtype):
             raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, "attention_q4: k and v")
-        n, val = N * self.KVH * self.hd, N * self.H * self.hd
+        n, val, at = N * self.KVH * self.hd, N * self.H * self.hd, cache.device_index
         check(self.lib.swq_attention_q4(
-            self._ref, cache.ref, ctypes.byref(b), _ptr(q, 2 * val, "attention_q4: q"), _ptr(k, n, "attention_q4: k"),
-            _ptr(v, n, "attention_q4: v"), _code(q, "attention_q4"),
-            _ptr(weights, rows.numel() * self.KVH * cache.max_positions, "attention_q4: weights", torch.float32),
-            _ptr(out, val, "attention_q4: out"), _code(out, "attention_q4"), ws.data_ptr(), ws.numel(),
-            _stream_handle(stream)), "attention_q4")
+            self._ref, cache.ref, ctypes.byref(b), _ptr(q, 2 * val, "attention_q4: q", at), _ptr(k, n, "attention_q4: k", at),
+            _ptr(v, n, "attention_q4: v", at), _code(q, "attention_q4"),
+            _ptr(weights, rows.numel() * self.KVH * cache.max_positions, "attention_q4: weights", at, torch.float32),
+            _ptr(out, val, "attention_q4: out", at), _code(out, "attention_q4"), _ptr(ws, 1, "attention_q4: ws", at, torch.uint8),
+            ws.numel(), _stream_handle(stream)), "attention_q4")
         return out
 
     def step(self, q, k, v, cache: Q4Cache, rows, ws, out=None, weights=None, positions=None, max_rows: int = 0, stream=None):
@@ -222,15 +237,17 @@ class AttentionQ4GPU:
         if stream is not None and _elsewhere(stream):
             with torch.cuda.stream(stream):
                 return self.evict(cache, weights, rows, into, budget, sink, recent, new_weights)
-        B = rows.numel()
+        B, at = rows.numel(), cache.here("q4_evict")
+        if into.device_index != at:
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "q4_evict: caches on two devices")
         if budget <= 0:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "q4_evict: budget")
         kept = torch.empty((B, self.KVH, budget), dtype=torch.int32, device=rows.device)
         new_rows = torch.empty(B, dtype=torch.int32, device=rows.device)
         check(self.lib.swq_q4_evict(
-            cache.ref, B, _ptr(weights, B * self.KVH * cache.max_positions, "q4_evict: weights", torch.float32),
-            _ptr(rows, B, "q4_evict: rows", torch.int32), into.ref, budget, sink, recent,
-            _ptr(new_weights, B * self.KVH * into.max_positions, "q4_evict: new_weights", torch.float32),
+            cache.ref, B, _ptr(weights, B * self.KVH * cache.max_positions, "q4_evict: weights", at, torch.float32),
+            _ptr(rows, B, "q4_evict: rows", at, torch.int32), into.ref, budget, sink, recent,
+            _ptr(new_weights, B * self.KVH * into.max_positions, "q4_evict: new_weights", at, torch.float32),
             new_rows.data_ptr(), kept.data_ptr(), _stream_handle(stream)), "q4_evict")
         return kept, new_rows
 

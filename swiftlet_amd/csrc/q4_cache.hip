@@ -496,7 +496,7 @@ extern "C" int swq_q4_read(const swq_q4_cache *cache, int sequences, const int32
     int st = check_q4_cache(cache);
     if (st == SWQ_OK) st = check_q4_dtype(dtype);
     if (st != SWQ_OK) return st;
-    if (sequences <= 0 || count < 0 || (!k && !v)) return SWQ_ERR_INVALID_ARGUMENT;
+    if (sequences <= 0 || count < 0 || (count > 0 && !k && !v)) return SWQ_ERR_INVALID_ARGUMENT;
     if (sequences > cache->sequences) return SWQ_ERR_BAD_SHAPE;
     if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16)
         return SWQ_ERR_MISALIGNED;
