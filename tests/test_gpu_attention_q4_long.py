@@ -312,3 +312,41 @@ def test_tensors_of_the_host_are_refused():
             call()
         assert e.value.code == _lib.SWQ_ERR_INVALID_ARGUMENT
     assert cache.read(None, 0)[0].shape == (2, 0, KVH, hd)  # no rows: nothing to do
+
+
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_not_finite_stays_with_its_head(T, dtype, bad):
+    """A query that is not finite makes its head's output NaN and no other's, nor the weights of another
+    kv head; such a gate its dim's (a sigmoid of infinity is 0 or 1); rows behind the last token stay."""
+    torch = _torch()
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    H, KVH, hd = 8, 2, 128
+    blk, _, _ = _block(H, KVH, hd, 64, 400, 6)
+    cache = blk.new_cache(1)
+    k0, v0, q, k, v = _random(7, (300, KVH * hd), (300, KVH * hd), (T, 2 * H * hd), (T, KVH * hd), (T, KVH * hd), dtype=dt)
+    rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    blk.append(k0, v0, cache, rows)
+    rows += 300
+    ws = blk.new_workspace(cache, tokens=T, max_tokens=T, weights=True)
+    r = q.clone().view(T, H, 2, hd)
+    r[T - 1, 2, 0, 77] = bad
+    r[0, 5, 1, 3] = bad
+    for weights in (False, True):
+        outs, gathered = [], []
+        for x in (q, r.view(T, -1)):
+            w = blk.new_weights(cache) if weights else None
+            out = torch.full((T + 1, H * hd), 7.0, dtype=dt, device="cuda")
+            blk.prefill(x, k, v, cache, rows, ws, out=out[:T], weights=w)
+            assert bool((out[T] == 7).all())
+            outs.append(out[:T].float().view(T, H, hd))
+            gathered.append(w)
+        good, got = outs
+        assert bool(got[T - 1, 2].isnan().all())
+        at = got[0, 5, 3].item()
+        assert math.isnan(at) if math.isnan(bad) else bool((at == 0) if bad < 0 else abs(at) >= abs(good[0, 5, 3].item()))
+        got[T - 1, 2], got[0, 5, 3] = good[T - 1, 2], good[0, 5, 3]
+        assert torch.equal(good, got)
+        if weights:
+            assert torch.equal(gathered[0][:, 1], gathered[1][:, 1])
