@@ -71,7 +71,18 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
     const int r = lane & 15, q = lane >> 4, G = a.group;
     const int g0 = wave % TW * GW, team = wave / TW;  // first group
     if (a.b.count(b) <= 0) return;
-    const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
+    const int n0 = a.b.first(b);
+    // 8 dims of a query per lane, a word's: HD / 8 lanes per head, 512 / HD heads of a wave at once.  Its
+    // loads go first: they need no row count, and nothing that they would queue behind.
+    constexpr int LPH = HD / 8, HPW = kWave / LPH;
+    float x[8], w[8];
+    auto load_query = [&](int base) {
+        const int u = base + wave * HPW + lane / LPH;
+        load8<T>(x, static_cast<const T *>(a.q) + (static_cast<int64_t>(n0) * a.H + kvh * G + min(u, G - 1)) * 2 * HD + 8 * (lane % LPH));
+    };
+    load_query(0);
+    load8<float>(w, a.q_norm_w + 8 * (lane % LPH));
+    const int r0 = a.b.row0(b, a.c.maxp);
     const int n = min(r0 + 1, a.c.maxp);  // rows that the token sees
     const int p0 = split * a.per, p1 = split == a.splits - 1 ? n : min(p0 + a.per, n);
     if (p0 >= n) return;
@@ -79,6 +90,11 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
     // In the last split two waves write the token's row before its tile is loaded.
     const bool writes = a.k && last && r0 < a.c.maxp;
     const int end = (p1 - p0 + kTile - 1) / kTile;  // tiles
+
+    const int half = a.b.rot / 2;
+    const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, 0)) * half : nullptr;
+    float2 cs[8];
+    if (8 * (lane % LPH) < 2 * half) q4_turns(cs, turn, half, lane % LPH);
 
     const uint32_t *kw = a.c.k_head(b, kvh) + (8 * (r >> 2) + (r & 3)) * (HD / 8) + 8 * g0 + 2 * q;
     const uint32_t *vw = a.c.v_head(b, kvh) + q * HD + 64 * g0 + 4 * r;
@@ -111,8 +127,6 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
         load_v(min(team, end - 1));
     }
 
-    const int half = a.b.rot / 2;
-    const float2 *turn = half > 0 ? a.b.rope + static_cast<int64_t>(a.b.position(b, 0)) * half : nullptr;
     const int askers = writes ? kStepWaves - 2 : kStepWaves;  // waves that prepare queries
     if (wave >= askers) {
         const int64_t at = (static_cast<int64_t>(n0) * a.c.KVH + kvh) * HD + lane * EPL;
@@ -138,22 +152,11 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
             for (int e = 0; e < EPL; ++e) vp[e] = (old[e] & ~(15u << sh)) | (code[e] << sh);
         }
     } else {
-        // 8 dims per lane, a word's: HD / 8 lanes per head, 512 / HD heads of a wave at once
-        constexpr int LPH = HD / 8, HPW = kWave / LPH;
         const int j = lane % LPH;
-        float w[8];
-        float2 cs[8];
-        load8<float>(w, a.q_norm_w + 8 * j);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = 8 * j + e;
-            cs[e] = half > 0 ? turn[i < half ? i : i < 2 * half ? i - half : 0] : make_float2(1.f, 0.f);
-        }
         float *lds = reinterpret_cast<float *>(s_rot[wave]) + lane / LPH * HD;
         for (int base = 0; base < G; base += askers * HPW) {
             const int u = base + wave * HPW + lane / LPH;
-            float x[8];
-            load8<T>(x, static_cast<const T *>(a.q) + (static_cast<int64_t>(n0) * a.H + kvh * G + min(u, G - 1)) * 2 * HD + 8 * j);
+            if (base > 0) load_query(base);
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
