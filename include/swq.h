@@ -396,9 +396,10 @@ int swq_q4_rope_table(int rotary_dims, float rope_theta, int64_t first, int coun
 int swq_q4_append(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
                   const void *k_proj, const void *v_proj, int dtype, void *stream);
 
-/* Workspace bytes of swq_attention_q4 for calls of up to batch->tokens tokens,
- * batch->max_tokens per sequence and any rows; weights: whether they are asked
- * for.  Only the sizes of batch are read.  0 on bad input. */
+/* Workspace bytes of swq_attention_q4 for calls of up to batch->sequences
+ * sequences and batch->tokens tokens, batch->max_tokens per sequence and any
+ * rows; weights: whether they are asked for.  Of starts only whether it is NULL
+ * is read, of rows and positions nothing.  0 on bad input. */
 size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const swq_q4_cache *cache,
                                         const swq_q4_batch *batch, int weights);
 
@@ -413,9 +414,11 @@ size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const 
  * each row has gathered, summed over tokens and the kv head's query heads:
  * added to for rows below rows[b], set for the call's rows; others are left as
  * they are.  Scores, softmax and sums in 32 bits; f32 outputs and weights are
- * exact to about 1e-6, bf16 ones to their rounding.  Repeatable bit for bit.
- * One token per sequence: split over the rows, two launches; more: tiles of
- * queries on the matrix cores.  The workspace needs no preparation. */
+ * exact to about 1e-6 of the largest, bf16 ones (of bf16 inputs: queries and
+ * softmax numerators then have 11 bits) to their rounding.  Repeatable bit for
+ * bit with the same max_rows.  One token per sequence: split over the rows, two
+ * launches; more: tiles of queries on the matrix cores.  The workspace, 256-byte
+ * aligned, needs no preparation; out, weights and workspace overlap nothing. */
 int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
                      const void *q_proj, const void *k_proj, const void *v_proj, int dtype, float *weights,
                      void *out, int out_dtype, void *ws, size_t ws_bytes, void *stream);

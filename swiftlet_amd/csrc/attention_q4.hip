@@ -12,11 +12,12 @@ struct StepParts {
     size_t part, ml, scores, total;
 };
 
-StepParts step_parts(const swq_attention_layer *l, const swq_q4_cache *c, int sequences, int splits, bool weights) {
-    const size_t heads = static_cast<size_t>(sequences) * l->num_heads;
+// head_splits: splits of all kv heads of all sequences.
+StepParts step_parts(const swq_attention_layer *l, const swq_q4_cache *c, int sequences, int64_t head_splits, bool weights) {
+    const size_t heads = static_cast<size_t>(sequences) * l->num_heads, triples = static_cast<size_t>(head_splits) * (l->num_heads / c->num_kv_heads);
     StepParts p{};
-    p.part = q4_align(heads * splits * l->head_dim * sizeof(float));
-    p.ml = q4_align(heads * splits * sizeof(float2));
+    p.part = q4_align(triples * l->head_dim * sizeof(float));
+    p.ml = q4_align(triples * sizeof(float2));
     p.scores = weights ? q4_align(heads * q4_rows(c->max_positions) * sizeof(float)) : 0;
     p.total = p.part + p.ml + p.scores;
     return p;
@@ -41,18 +42,17 @@ PrefillParts prefill_parts(const swq_attention_layer *l, const swq_q4_cache *c, 
     return p;
 }
 
-// What any call of up to these tokens can take.  Splits are made where tiles of 64 or 128 rows are
-// fewer than 512, so that rows * splits stays below 512 * 128 + rows.
+// What any call of up to these tokens can take.
 size_t prefill_workspace(const swq_attention_layer *l, const swq_q4_cache *c, const swq_q4_batch *b, int weights) {
     const int64_t tokens = std::max(b->tokens, 1), rows = tokens * l->num_heads;
     const int64_t heads = static_cast<int64_t>(b->sequences) * c->num_kv_heads;
-    const int64_t part_rows = std::min<int64_t>(rows * kQ4PrefillMaxSplits, 512 * 128 + rows);
+    const int64_t part_rows = std::min<int64_t>(rows * kQ4PrefillMaxSplits, kQ4PartRows + rows);
     const int64_t gathered = weights ? std::min<int64_t>(heads * q4_rows(c->max_positions) * kQ4GatherMaxParts, kQ4GatherMost) : 0;
     return prefill_parts(l, c, b->sequences, tokens, part_rows, gathered).total;
 }
 
 size_t step_workspace(const swq_attention_layer *l, const swq_q4_cache *c, const swq_q4_batch *b, int weights) {
-    const int splits = most_q4_splits(c->max_positions, static_cast<int64_t>(b->sequences) * c->num_kv_heads, c->head_dim);
+    const int64_t splits = most_q4_head_splits(c->max_positions, static_cast<int64_t>(b->sequences) * c->num_kv_heads, c->head_dim);
     return step_parts(l, c, b->sequences, splits, weights != 0).total;
 }
 
@@ -109,7 +109,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     uint8_t *p = static_cast<uint8_t *>(ws);
     if (a.b.max_tokens == 1) {
         const Q4StepPlan plan = plan_q4_step(rows, heads, a.c.hd);
-        const StepParts parts = step_parts(layer, cache, a.b.B, plan.splits, weights != nullptr);
+        const StepParts parts = step_parts(layer, cache, a.b.B, heads * plan.splits, weights != nullptr);
         if (ws_bytes < parts.total) return SWQ_ERR_WORKSPACE;
         a.per = plan.per;
         a.splits = plan.splits;
@@ -122,7 +122,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
         launch_q4_step(a, s);
         return launch_status();
     }
-    const Q4PrefillPlan plan = plan_q4_prefill(a.b.max_tokens, rows, heads, a.group, cache->max_positions, a.in_f32 || a.out_f32, weights != nullptr);
+    const Q4PrefillPlan plan = plan_q4_prefill(a.b.max_tokens, static_cast<int64_t>(batch->tokens) * a.H, rows, heads, a.group, cache->max_positions, a.in_f32 || a.out_f32, weights != nullptr);
     const PrefillParts parts = prefill_parts(layer, cache, a.b.B, batch->tokens,
                                              plan.splits > 1 ? static_cast<int64_t>(batch->tokens) * a.H * plan.splits : 0,
                                              plan.gparts > 1 ? heads * a.c.R * plan.gparts : 0);

@@ -162,19 +162,21 @@ struct Q4StepPlan {
     int per, splits;
 };
 Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd);
-int most_q4_splits(int64_t rows, int64_t heads, int hd);  // of any number of rows up to this
+int64_t most_q4_head_splits(int64_t rows, int64_t heads, int hd);  // heads * splits, of any number of rows and heads up to these
 void launch_q4_step(const AttnQ4Args &a, hipStream_t s);
 
-
 // Several tokens (attention_q4_prefill.hip): how the launches are cut for sequences of up to
-// max_tokens tokens and `rows` rows.
+// max_tokens tokens and `rows` rows, `all` (token, query head) rows of the batch.  Splits are made where
+// tiles of 64 or 128 rows are fewer than 256: all * splits stays below 256 * 128 + all, and the workspace
+// has room for twice that; a batch that is padded a lot has fewer splits.
 constexpr int kQ4PrefillMaxSplits = 32;
+constexpr int64_t kQ4PartRows = 512 * 128;
 constexpr int kQ4GatherMaxParts = 32;
 constexpr int64_t kQ4GatherMost = 4 << 20;  // numbers of all parts' sums
 struct Q4PrefillPlan {
     int planes_q, planes_v, rows_per, tiles, per, splits, gparts;
 };
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights);
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights);
 void launch_q4_prefill(const AttnQ4Args &a, hipStream_t s);
 
 }  // namespace swq

@@ -88,7 +88,8 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
 }
 
 // The largest |bias| + 15 scale of a sequence's keys and of its values, by kv head: what high and low
-// parts are scaled by.  Maxima of non-negative numbers, whose bits order as they do.
+// parts are scaled by.  Maxima of non-negative numbers, whose bits order as they do.  8,704 rows of 2
+// heads of 256: 5 us.
 __global__ __launch_bounds__(256) void q4_largest(const AttnQ4Args a) {
     const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, ng = a.c.hd / kQ4Group;
     const int cnt = a.b.count(b);
@@ -191,9 +192,10 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 // maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
 // Bound by LDS at hd 256: each wave reads the whole tile's operands for its 16 rows (32 KB), eight waves
-// 2,048 of the 2,560 clocks of a step.  4,096 tokens of 16 heads of 256: 207 us, 664 TFLOP/s; 512 after
-// 8,192 rows, queries in two parts: 174.  32 rows per wave halve the bytes but leave one wave per SIMD
-// (slower); scores of the next tile beside the softmax (237 us), too.  Heads of 64 in bf16: two
+// 2,048 of the 2,560 clocks of a step.  4,096 tokens of 16 heads of 256: 207 to 228 us, 600 to 664
+// TFLOP/s (the card's clock decides); 512 after 8,192 rows, queries in two parts: 174.  32 rows per wave
+// halve the bytes but leave one wave per SIMD (slower); scores of the next tile beside the softmax (237
+// us), too.  Heads of 64 in bf16: two
 // workgroups per CU, their registers bounded to 128 (4,096 tokens of 32 heads 159 us with its other
 // kernels, else 182); at 128 that is 8% less time for one long sequence and 7% more for four of 1,000.
 template <int HD, int PQ, int PV, int NT, int WAVES>
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
 // A workgroup has kGatherRows cached rows of a kv head, 32 per wave, as high and low parts in
 // registers, and walks the rows of queries that see any of them, 16 at a time: those go through LDS
 // once for all waves, the next 16 on their way meanwhile: 512 tokens of 16 heads after 8,192 rows of 2
-// kv heads of 256 147 us, 720 TFLOP/s in three products (16 cached rows per wave, queries read by each
+// kv heads of 256 143 us, 744 TFLOP/s in three products (16 cached rows per wave, queries read by each
 // from L1: 911).  Sums stay with the lane until the end.
 constexpr int kGatherRows = 128;
 
@@ -720,7 +722,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
 
 }  // namespace
 
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights) {
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights) {
     Q4PrefillPlan p{};
     p.planes_q = f32 || weights ? 2 : 1;
     p.planes_v = f32 ? 2 : 1;
@@ -732,7 +734,8 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t rows, int64_t heads, i
     // a workgroup per CU, if the cached rows can be split that often with 256 rows each
     const int64_t groups = p.tiles * heads;
     const int64_t want = std::max<int64_t>(1, 256 / groups), most = std::max<int64_t>(1, rows / 256);
-    const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits});
+    // a padded batch has more rows than its longest sequence accounts for
+    const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits, (kQ4PartRows + all) / all});
     p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
     p.splits = static_cast<int>((rows + p.per - 1) / p.per);
     // the gathered weights: as many workgroups, the queries dealt out where the cached rows are few

@@ -46,6 +46,14 @@ __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n
 //           maximum's factor is the lane's own.  p * bias is summed on the VALU.
 // Heads past the group are columns that nothing reads.  The next tile's loads are issued as soon as
 // their registers are free.
+//   P = 1   (bf16 in and out, no gathered weights): queries and p * scale as one f16 number instead of
+//           two, and K's codes with the 1024 left on, whose share of a score is the same for all rows
+//           and starts the sum.  32 sequences of up to 16,384 rows of 8 heads of 128: 80 us, with two 88.
+//           (Not for V's: there the 1024 would swallow the bits of an average that is near zero.)
+// Wide batches are bound by instruction issue beside the loads: those 80 us are 3.8 TB/s of cache, with
+// VALU and matrix instructions for some 45 of them on every SIMD; three waves are all that 160 registers
+// leave (bounded to 128 they spill: 163 us).  Small ones are a chain: of 7.8 us at 500 rows of 2 heads of
+// 256 a workgroup's life is 6.2, rows and addresses 0.9, queries 1.9, one step 1.6, the teams' sums 1.2.
 template <int HD, int P, typename T>
 __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const AttnQ4Args a) {
     constexpr int EPL = HD / kWave, NG = HD / kQ4Group, GW = NG > 1 ? 2 : 1, TW = NG / GW, TEAMS = kStepWaves / TW;
@@ -436,7 +444,8 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
 }
 
 // The splits merged: a workgroup per (sequence, query head) for the output, then workgroups per 1,024
-// rows of a kv head for the gathered weights.
+// rows of a kv head for the gathered weights.  A chain of loads and two exchanges: 4 us, with the weights
+// of 33,000 rows of 2 heads (4.2 MB of scores) 7.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeRows = 1024;
 constexpr int kMaxSplits = 1024;
@@ -562,6 +571,10 @@ void launch_typed(const AttnQ4Args &a, hipStream_t s) {
 // Rows of one step of a workgroup: a tile of each team.
 static int64_t step_unit(int hd) { return hd == 256 ? 2 * kTile : 4 * kTile; }
 
+// Rows of a split: 512 workgroups (two per CU) where rows are few, 512 rows where that leaves more, and
+// no more than 2,048 workgroups.  16 sequences of up to 8,192 rows of 2 heads of 256: 512 rows 25.3 us,
+// 256 28.8; one of 33,000: 192 rows 16.6 + 7.1 for the merge, 128 17.4 + 9.1, 64 21.0 + 15.1; 32 of up to
+// 16,384 of 8 heads of 128, where all have 512 rows at least: 2,048 rows 80 us, 1,024 81, 512 96.
 Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd) {
     const int64_t unit = step_unit(hd);
     const int64_t total = rows * heads;
@@ -572,10 +585,11 @@ Q4StepPlan plan_q4_step(int64_t rows, int64_t heads, int hd) {
     return {static_cast<int>(per), static_cast<int>((rows + per - 1) / per)};
 }
 
-int most_q4_splits(int64_t rows, int64_t heads, int hd) {
+int64_t most_q4_head_splits(int64_t rows, int64_t heads, int hd) {
     const int64_t unit = step_unit(hd);
-    // rows per split are at least a step's, and at least a 2,048th of rows * heads
-    return static_cast<int>(std::min<int64_t>({(rows + unit - 1) / unit, 2048 / heads + 2, kMaxSplits}));
+    // rows per split are at least a step's, and at least a 2,048th of rows * heads, rounded down from 512
+    // or more (which can make 4 splits more)
+    return std::min<int64_t>({heads * ((rows + unit - 1) / unit), 2052 + 2 * heads, heads * kMaxSplits});
 }
 
 void launch_q4_step(const AttnQ4Args &a, hipStream_t s) {

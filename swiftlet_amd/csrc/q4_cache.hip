@@ -21,8 +21,8 @@ struct AppendArgs {
 // 8 dims each, so that a lane's codes are one k word, a wave takes 2 to 8 rows at once and sums cross few
 // lanes.  A v word holds 8 rows of one dim: those codes meet in LDS, and words of which only some rows
 // are new keep the others (the first and last block of a call).  All in 64 bits up to the format's own
-// roundings.  Bound by that arithmetic (24 of the time in VALU instructions at 8,192 tokens of 8 heads
-// of 128, 43 MB: 36 us); one row per wave and a division per value took 58.
+// roundings.  Bound by that arithmetic (8,192 tokens of 8 heads of 128, 43 MB: 36 us, VALU
+// instructions for 24 of them); one row per wave and a division per value took 58.
 template <int HD, typename T>
 __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) {
     constexpr int LPR = HD / 8, PER = kQ4Block * LPR;  // lanes of a row, of a block's keys or values
@@ -240,7 +240,10 @@ __device__ __forceinline__ uint32_t lanes_before(uint32_t v, uint32_t &all) {
 // LDS, whose integer counts do not depend on the order of the adds, until all rows that share its known
 // bits are kept; once those are few they are listed, and the later passes go over the list alone.  Then
 // the kept rows are counted and numbered in order.  Weights stay in registers, 48 rows of each thread;
-// caches of more than 49,152 rows are gone through in parts, read again by each pass.
+// caches of more than 49,152 rows are gone through in parts, read again by each pass.  One workgroup per
+// head, because all its rows decide together: 33,000 rows to 4,096 34 us on two CUs, bound by their VALU
+// (every row is looked at by the first one or two passes, the count and the writing); 8,193 rows of 64
+// heads to 2,047 16 us.
 __global__ __launch_bounds__(kSelectThreads) void q4_select(const EvictArgs a) {
     __shared__ uint32_t s_hist[kSelectBins];
     __shared__ uint64_t s_list[kSelectList];
@@ -396,7 +399,8 @@ __global__ __launch_bounds__(kSelectThreads) void q4_select(const EvictArgs a) {
 
 // Their codes, scales and biases into the other cache, a workgroup per 2,048 / HD rows of it and kv head:
 // each thread takes a k word, a v word, which has its codes from 8 rows anywhere, and half of them a
-// parameter; all its loads are in flight together.
+// parameter; all its loads are in flight together.  8 x 2,047 rows of 8 heads of 128 (38 MB read and
+// written) 14 us, 4,096 of 2 heads of 256 5.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_gather(const EvictArgs a) {
     constexpr int NG = HD / kQ4Group, W = HD / 8, ROWS = 256 / W;

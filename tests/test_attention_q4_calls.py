@@ -153,3 +153,15 @@ def test_refused_evictions(lib):
                      (dict(dst=cache(lib, data=far, head_dim=128)), E.SWQ_ERR_BAD_SHAPE),
                      (dict(dst=cache(lib, data=far, sequences=2)), E.SWQ_ERR_BAD_SHAPE)):
         assert evict(**kw) == want, kw
+
+
+@pytest.mark.parametrize("weights", [0, 1])
+@pytest.mark.parametrize("tokens_each", [1, 40])
+def test_a_workspace_does_for_calls_of_fewer_sequences(lib, weights, tokens_each):
+    l, c = layer(num_heads=4, num_kv_heads=1, head_dim=64), cache(lib, sequences=2100, num_kv_heads=1, head_dim=64, max_positions=200_000)
+    before = 0
+    for b in range(1, 2101):
+        x = batch(sequences=b, tokens=b * tokens_each, max_tokens=tokens_each, starts=FAKE)
+        n = lib.swq_attention_q4_workspace_bytes(ctypes.byref(l), ctypes.byref(c), ctypes.byref(x), weights)
+        assert n >= before, b
+        before = n

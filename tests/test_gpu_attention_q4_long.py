@@ -350,3 +350,31 @@ def test_what_is_not_finite_stays_with_its_head(T, dtype, bad):
         assert torch.equal(good, got)
         if weights:
             assert torch.equal(gathered[0][:, 1], gathered[1][:, 1])
+
+
+@pytest.mark.parametrize("T", [1, 2, 9])
+def test_a_padded_batch(T):
+    """Room for many more tokens than the sequences bring: the queried workspace does, the rows behind
+    the last sequence's stay as they are, in and out, and the results are those of the tight call."""
+    torch = _torch()
+    H, KVH, hd, room = 16, 2, 128, 3000
+    blk, _, _ = _block(H, KVH, hd, 64, 20000, 8)
+    results = []
+    for N in (2 * T, room):
+        cache = blk.new_cache(2)
+        q, k, v = _random(9, (room, 2 * H * hd), (room, KVH * hd), (room, KVH * hd))
+        rows = torch.zeros(2, dtype=torch.int32, device="cuda")
+        k0, v0 = _random(10, (4000, KVH * hd), (4000, KVH * hd))
+        blk.append(k0, v0, cache, rows)
+        rows += 2000
+        starts = torch.tensor([0, T, 2 * T], dtype=torch.int32, device="cuda")
+        ws, w = blk.new_workspace(cache, tokens=N, max_tokens=T, weights=True), blk.new_weights(cache)
+        out = torch.full((N, H * hd), 7.0, device="cuda")
+        blk.prefill(q[:N], k[:N], v[:N], cache, rows, ws, starts=starts, max_tokens=T, out=out, weights=w)
+        assert bool((out[2 * T:] == 7).all())
+        results.append((out[:2 * T], w, cache.data))
+    for i, (a, b) in enumerate(zip(*results)):
+        if i == 2:
+            assert torch.equal(a, b)
+        else:  # the padded call may be split in another way
+            assert bool(((a - b).abs() <= 2e-5 * a.abs().max()).all())
