@@ -191,11 +191,11 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 // (K's rows permuted so that the result's registers are the next operand), out = V^T P, so that
 // maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
-// Bound by LDS at hd 256: each wave reads the whole tile's operands for its 16 rows (32 KB), eight waves
-// 2,048 of the 2,560 clocks of a step.  4,096 tokens of 16 heads of 256: 207 to 228 us, 600 to 664
-// TFLOP/s (the card's clock decides); 512 after 8,192 rows, queries in two parts: 174.  32 rows per wave
-// halve the bytes but leave one wave per SIMD (slower); scores of the next tile beside the softmax (237
-// us), too.  Heads of 64 in bf16: two
+// Bound, at hd 256, by what two waves per SIMD and a barrier a tile let overlap: of 2,560 clocks a step
+// VALU takes 42%, LDS (each wave reads the whole tile's operands for its 16 rows) as much, the matrix units
+// 30%.  4,096 tokens of 16 heads of 256: 207 to 228 us, 600 to 664 TFLOP/s (the card's clock decides); 512
+// after 8,192 rows, queries in two parts: 173.  32 rows per wave halve the LDS bytes but leave one wave
+// per SIMD (slower); scores of the next tile beside the softmax (237 us) cost more registers.  Heads of 64 in bf16: two
 // workgroups per CU, their registers bounded to 128 (4,096 tokens of 32 heads 159 us with its other
 // kernels, else 182); at 128 that is 8% less time for one long sequence and 7% more for four of 1,000.
 template <int HD, int PQ, int PV, int NT, int WAVES>
