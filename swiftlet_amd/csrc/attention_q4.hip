@@ -24,7 +24,7 @@ StepParts step_parts(const swq_attention_layer *l, const swq_q4_cache *c, int se
 }
 
 struct PrefillParts {
-    size_t q, qf, vmax, lse, part, ml, gpart, total;
+    size_t q, qf, qs, vmax, lse, part, ml, gpart, total;
 };
 
 // part_rows: (token, query head, split) triples; 0 where nothing is split.
@@ -33,12 +33,13 @@ PrefillParts prefill_parts(const swq_attention_layer *l, const swq_q4_cache *c, 
     PrefillParts p{};
     p.q = q4_align(rows * l->head_dim * 2);  // each of two
     p.qf = q4_align(rows * sizeof(float));
+    p.qs = q4_align(rows * 16 * 2);
     p.vmax = q4_align(static_cast<size_t>(sequences) * c->num_kv_heads * 2 * sizeof(uint32_t));
     p.lse = q4_align(rows * sizeof(float));
     p.part = q4_align(static_cast<size_t>(part_rows) * l->head_dim * sizeof(float));
     p.ml = q4_align(static_cast<size_t>(part_rows) * sizeof(float2));
     p.gpart = q4_align(static_cast<size_t>(gathered) * sizeof(float));
-    p.total = 2 * p.q + p.qf + p.vmax + p.lse + p.part + p.ml + p.gpart;
+    p.total = 2 * p.q + p.qf + p.qs + p.vmax + p.lse + p.part + p.ml + p.gpart;
     return p;
 }
 
@@ -139,6 +140,8 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     p += 2 * parts.q;
     a.qf = reinterpret_cast<float *>(p);
     p += parts.qf;
+    if (weights) a.qs = p;
+    p += parts.qs;
     if (a.planes_q == 2) a.vmax = reinterpret_cast<uint32_t *>(p);
     p += parts.vmax;
     if (weights) a.lse = reinterpret_cast<float *>(p);

@@ -45,6 +45,7 @@ struct AttnQ4Args {
     int32_t gparts;              // parts of the queries in the gathered weights
     void *qh, *ql;               // [N][H][hd] f16: queries, high and low part
     float *qf;                   // [N][H]: what turns a product of them into log2 units
+    void *qs;                    // [N][H][16] f16: sums of their groups as three parts, or NULL
     uint32_t *vmax;              // [B][KVH][2]: bits of the largest key and value, or NULL
     float *lse;                  // [N][H]: log2 of the sum of exponentials, or NULL
     float *gpart;                // [B][KVH][gparts][R]

@@ -11,8 +11,9 @@ constexpr float kLow = -1e30f;  // below every score: exponents against it stay 
 
 // ---- queries ----------------------------------------------------------------
 
-// q / rms * w, turned, times a power of two that brings the row's largest below 2^10; as f16 high
-// (and low) parts, the 8 dims of a chunk in the order of a cache word's operand.  8 dims per lane, and
+// q / rms * w, turned, times a power of two that brings the row's largest below 2^8 (the sum of a group
+// fits f16); as f16 high (and low) parts, the 8 dims of a chunk in the order of a cache word's operand,
+// and, for the gathered weights, the groups' sums: three parts, 32 bits.  8 dims per lane, and
 // ROWS consecutive (token, head) rows whose loads are in flight together and which read a token's turns
 // once: four where that gives each compute unit two workgroups, else one (77 tokens of 16 heads of 256: 5
 // us, with four 8; 4,096 tokens of 32 heads of 128: 21, with one 28).
@@ -75,15 +76,36 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
         h8_t hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = ldexpf(x[k][e], 10 - ex);
+            const float v = ldexpf(x[k][e], 8 - ex);
             hi[q4_element(e)] = static_cast<_Float16>(v);
             lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
         }
+        float qs = 0.f;
+        if constexpr (PQ == 2) {
+            if (a.qs) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qs += static_cast<float>(hi[e]) + static_cast<float>(lo[e]);
+                qs = lanes_sum<8>(qs);
+            }
+        }
         if (row + k >= all) continue;
         const int64_t at = first + row + k;
+        if (PQ == 2 && a.qs && j % 8 == 0) {
+            _Float16 *to = static_cast<_Float16 *>(a.qs) + at * 16;
+#pragma unroll
+            for (int g = 0; g < 4; g += HD / kQ4Group) {  // zeros for groups that heads of less than 256 lack
+                float rest = g == 0 ? qs : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const _Float16 h = i < 3 ? static_cast<_Float16>(rest) : static_cast<_Float16>(0.f);
+                    rest -= static_cast<float>(h);
+                    to[4 * i + g + j / 8] = h;
+                }
+            }
+        }
         reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
         if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
-        if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 10);
+        if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 8);
     }
 }
 
@@ -536,11 +558,11 @@ __global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
 
 // ---- gathered weights -------------------------------------------------------
 
-// A workgroup has kGatherRows cached rows of a kv head, 32 per wave, as high and low parts in
+// A workgroup has kGatherRows cached rows of a kv head, 32 per wave, their codes as f16 integers in
 // registers, and walks the rows of queries that see any of them, 16 at a time: those go through LDS
-// once for all waves, the next 16 on their way meanwhile: 512 tokens of 16 heads after 8,192 rows of 2
-// kv heads of 256 143 us, 744 TFLOP/s in three products (16 cached rows per wave, queries read by each
-// from L1: 911).  Sums stay with the lane until the end.
+// once for all waves, the next 16 on their way meanwhile.  A group's products with the queries' two parts
+// are exact and take the rows' scales on the VALU; the biases meet the groups' sums, which are in three
+// parts, in one more matrix product.  Sums of p stay with the lane until the end.
 constexpr int kGatherRows = 128;
 
 template <int HD>
@@ -555,24 +577,32 @@ __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
     const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
     const int top = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
     const uint32_t magic = kept_1024();
-    const int klift = q4_lift(a.vmax[2 * a.c.head(b, kvh)]);
-    const float kunit = ldexpf(1.0f, klift), down = ldexpf(1.0f, -klift);
     const uint32_t all = static_cast<uint32_t>(cnt) * G;
     const int part = blockIdx.z, parts = gridDim.z;  // of the queries
     for (int t0 = blockIdx.x * kGatherRows; t0 < top; t0 += gridDim.x * kGatherRows) {
         const int w0 = t0 + 32 * wave;
-        h8_t kh[2][KS], kl[2][KS];
+        typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+        h8_t kc[2][KS], kb[2];  // biases of a row: twice in lanes q = 0, once in 1, as the sums' parts lie
+        h4_t ks[2][NG];         // scales of the four rows whose scores the lane gets
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) {
+            const int64_t line = min(w0 + 16 * x + r, a.c.R - 1);
+            const _Float16 *par = a.c.par_head(b, kvh);
+            kb[x] = h8_t{};
 #pragma unroll
             for (int u = 0; u < KS; ++u) {
-                const int64_t line = min(w0 + 16 * x + r, a.c.R - 1);
-                const uint32_t w = a.c.k_head(b, kvh)[line * KCH + 4 * u + q];
-                const _Float16 *p = a.c.par_head(b, kvh) + static_cast<int64_t>(u / 2) * a.c.R + line;
-                const h2_t s1 = {p[0], p[0]}, z1 = {p[static_cast<int64_t>(NG) * a.c.R], p[static_cast<int64_t>(NG) * a.c.R]};
-                const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
-                q4_values<2>(w, magic, s, z, kunit, kh[x][u], kl[x][u]);
+                h2_t c[4];
+                q4_codes(a.c.k_head(b, kvh)[line * KCH + 4 * u + q], magic, c);
+                kc[x][u] = h8_t{c[0].x, c[0].y, c[1].x, c[1].y, c[2].x, c[2].y, c[3].x, c[3].y};
             }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                ks[x][g] = *reinterpret_cast<const h4_t *>(par + static_cast<int64_t>(g) * a.c.R + min(w0 + 16 * x + 4 * q, a.c.R - 4));
+                const _Float16 z = par[static_cast<int64_t>(kQ4KBias * NG + g) * a.c.R + line];
+                if (q < 2) kb[x][g] = z;
+                if (q == 0) kb[x][4 + g] = z;
+            }
+        }
         float sum[2][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -581,6 +611,7 @@ __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
         // the first 16 rows of queries that see row t0; this part's share of those from there on
         const uint32_t from = static_cast<uint32_t>(max(t0 - r0, 0)) * G / 16 + part, blocks = (all + 15) / 16;
         uint4 ch[NC], cl[NC];
+        h8_t qs;
         float f, z;
         int vis;
         const bool copies = 16 * KCH >= 256 || tid < 16 * KCH;
@@ -598,6 +629,7 @@ __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
             const int64_t at = static_cast<int64_t>(n0 + i) * a.H + kvh * G + row % G;
             f = a.qf[at];
             z = a.lse[at];
+            qs = static_cast<const h8_t *>(a.qs)[2 * at + (q & 1)];
             vis = blk * 16 + r < all ? min(r0 + static_cast<int>(i) + 1, a.c.maxp) : 0;
         };
         auto put = [&](int buf) {
@@ -617,30 +649,36 @@ __global__ __launch_bounds__(256, 2) void q4_gathered(const AttnQ4Args a) {
         }
         int buf = 0;
         for (uint32_t blk = from; blk < blocks; blk += parts, buf ^= 1) {
-            const float cf = f * down, cz = z;
+            const float cf = f, cz = z;
             const int cv = vis;
             const bool more = blk + parts < blocks;
+            f4_t s[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) s[x] = mfma16(kb[x], qs, f4_t{0.f, 0.f, 0.f, 0.f});
             lds_barrier();
             if (more) fetch(blk + parts);
-            f4_t s[2], s2[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) s[x] = s2[x] = f4_t{0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < NG; ++g) {
+                f4_t d[2];
 #pragma unroll
-            for (int u = 0; u < KS; ++u) {
-                const h8_t qh = s_q[buf][0][q4_place<KCH, false>(r, 4 * u + q)], ql = s_q[buf][1][q4_place<KCH, false>(r, 4 * u + q)];
+                for (int v = 0; v < 2; ++v) {
+                    const int u = 2 * g + v;
+                    const h8_t qh = s_q[buf][0][q4_place<KCH, false>(r, 4 * u + q)], ql = s_q[buf][1][q4_place<KCH, false>(r, 4 * u + q)];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    s[x] = mfma16(kh[x][u], qh, s[x]);
-                    s2[x] = mfma16(kh[x][u], ql, s2[x]);
+                    for (int x = 0; x < 2; ++x) d[x] = mfma16(kc[x][u], qh, v == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : d[x]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) d[x] = mfma16(kc[x][u], ql, d[x]);
                 }
 #pragma unroll
-                for (int x = 0; x < 2; ++x) s2[x] = mfma16(kl[x][u], qh, s2[x]);
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[x][e] = fmaf(static_cast<float>(ks[x][g][e]), d[x][e], s[x][e]);
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = q4_exp2(fmaf(s[x][e] + s2[x][e], cf, -cz));
+                    const float p = q4_exp2(fmaf(s[x][e], cf, -cz));
                     sum[x][e] += w0 + 16 * x + 4 * q + e < cv ? p : 0.f;
                 }
             if (more) put(buf ^ 1);
