@@ -140,9 +140,9 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     p += 2 * parts.q;
     a.qf = reinterpret_cast<float *>(p);
     p += parts.qf;
-    if (weights) a.qs = p;
+    if (a.planes_q == 2) a.qs = p;
     p += parts.qs;
-    if (a.planes_q == 2) a.vmax = reinterpret_cast<uint32_t *>(p);
+    if (a.planes_v == 2) a.vmax = reinterpret_cast<uint32_t *>(p);
     p += parts.vmax;
     if (weights) a.lse = reinterpret_cast<float *>(p);
     p += parts.lse;

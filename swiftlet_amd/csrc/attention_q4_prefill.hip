@@ -13,7 +13,7 @@ constexpr float kLow = -1e30f;  // below every score: exponents against it stay 
 
 // q / rms * w, turned, times a power of two that brings the row's largest below 2^8 (the sum of a group
 // fits f16); as f16 high (and low) parts, the 8 dims of a chunk in the order of a cache word's operand,
-// and, for the gathered weights, the groups' sums: three parts, 32 bits.  8 dims per lane, and
+// and, with two parts, the groups' sums: three parts, 32 bits.  8 dims per lane, and
 // ROWS consecutive (token, head) rows whose loads are in flight together and which read a token's turns
 // once: four where that gives each compute unit two workgroups, else one (77 tokens of 16 heads of 256: 5
 // us, with four 8; 4,096 tokens of 32 heads of 128: 21, with one 28).
@@ -82,15 +82,13 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
         }
         float qs = 0.f;
         if constexpr (PQ == 2) {
-            if (a.qs) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) qs += static_cast<float>(hi[e]) + static_cast<float>(lo[e]);
-                qs = lanes_sum<8>(qs);
-            }
+            for (int e = 0; e < 8; ++e) qs += static_cast<float>(hi[e]) + static_cast<float>(lo[e]);
+            qs = lanes_sum<8>(qs);
         }
         if (row + k >= all) continue;
         const int64_t at = first + row + k;
-        if (PQ == 2 && a.qs && j % 8 == 0) {
+        if (PQ == 2 && j % 8 == 0) {
             _Float16 *to = static_cast<_Float16 *>(a.qs) + at * 16;
 #pragma unroll
             for (int g = 0; g < 4; g += HD / kQ4Group) {  // zeros for groups that heads of less than 256 lack
@@ -110,8 +108,7 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
 }
 
 // The largest |bias| + 15 scale of a sequence's keys and of its values, by kv head: what high and low
-// parts are scaled by.  Maxima of non-negative numbers, whose bits order as they do.  8,704 rows of 2
-// heads of 256: 5 us.
+// parts are scaled by.  Maxima of non-negative numbers, whose bits order as they do.
 __global__ __launch_bounds__(256) void q4_largest(const AttnQ4Args a) {
     const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, ng = a.c.hd / kQ4Group;
     const int cnt = a.b.count(b);
@@ -228,7 +225,16 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
     constexpr int KW = NT * KCH / THREADS, VW = VCH * HD / THREADS;
     static_assert(KW >= 1 && (VW == 1 || VW == 2 || VW == 4), "a thread's value words share a block and a group");
     constexpr uint32_t KB = NT * KCH * 16, VB = HD * VCH * 16;  // bytes of one plane of a tile
-    __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * PQ * KB];  // [buffer][plane]
+    // Keys: [buffer][plane] of values.  Or, with two parts of the queries and one of p and values, codes: their
+    // products are exact, a product and a plane less for a scale and score on the VALU (bf16 with gathered
+    // weights, 512 tokens after 8,192 rows: 157 us, with planes 173; but in f32 2,048 tokens of 32 heads of 128
+    // 175 against 169: there the VALU has enough to do with values and p).  Beside the codes lie, by buffer,
+    // scales by group and row, and the biases of a row's groups twice, as the sums' parts lie.
+    constexpr bool CODES = PQ == 2 && PV == 1;
+    constexpr int KP = CODES ? 1 : PQ;
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * KP * KB];
+    __shared__ __attribute__((aligned(16))) _Float16 s_ks[CODES ? 2 : 1][CODES ? NG : 1][CODES ? NT : 8];
+    __shared__ __attribute__((aligned(16))) _Float16 s_kz[CODES ? 2 : 1][CODES ? NT : 1][8];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * PV * VB];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int r = lane & 15, q = lane >> 4, G = a.group;
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
     const _Float16 *par = a.c.par_head(b, kvh);
     const uint32_t magic = kept_1024();
     const int seq_rows = static_cast<int>(min(static_cast<int64_t>(r0) + cnt, static_cast<int64_t>(a.c.maxp)));
-    const int klift = PQ == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh)]) : 0, vlift = PV == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh) + 1]) : 0;
+    const int klift = KP == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh)]) : 0, vlift = PV == 2 ? q4_lift(a.vmax[2 * a.c.head(b, kvh) + 1]) : 0;
     const float kunit = ldexpf(1.0f, klift), vunit = ldexpf(1.0f, vlift);
 
     for (uint32_t base = static_cast<uint32_t>(slot) * M; base < all; base += static_cast<uint32_t>(a.tiles) * M) {
@@ -264,14 +270,17 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
         const int vis = valid ? min(r0 + static_cast<int>(column / G) + 1, a.c.maxp) : 0;
         int low = vis;
         float f;
-        h8_t qh[KS], ql[PQ == 2 ? KS : 1];
+        h8_t qh[KS], ql[PQ == 2 ? KS : 1], qs = h8_t{};
         {
             const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
+            int lq = q;  // as below: addresses kept from row tile to row tile were spilled
+            asm volatile("" : "+v"(lq));
             f = ldexpf(a.qf[at], -klift);
+            if (CODES && q < 2) qs = static_cast<const h8_t *>(a.qs)[2 * at + q];
 #pragma unroll
             for (int u = 0; u < KS; ++u) {
-                qh[u] = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + q];
-                if constexpr (PQ == 2) ql[u] = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + q];
+                qh[u] = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + lq];
+                if constexpr (PQ == 2) ql[u] = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + lq];
             }
         }
 #pragma unroll
@@ -291,14 +300,17 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
         constexpr uint32_t VGAP = kQ4Group / VW;
         const uint32_t vblk = tid / (VGAP * NG), vdim = tid / VGAP % NG * kQ4Group + tid % VGAP;
         auto fetch = [&](int t0) {
+            int tf = tid;
+            if constexpr (CODES && HD == 256) asm volatile("" : "+v"(tf));
+            const uint32_t vblk = tf / (VGAP * NG), vdim = tf / VGAP % NG * kQ4Group + tf % VGAP;
             const bool beyond = NT > 32 && t0 + 32 >= a.c.R;
             const uint32_t *pk = kw + static_cast<int64_t>(t0) * KCH, *pv = vw + static_cast<int64_t>(t0 / 8) * HD;
             const _Float16 *ps = par + t0, *pz = ps + static_cast<int64_t>(NG) * a.c.R;
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const uint32_t line = i * (THREADS / KCH) + tid / KCH, back = beyond && line >= 32 ? 32 : 0;
-                rk[i] = pk[(line - back) * KCH + tid % KCH];
-                const uint32_t at = (tid % KCH / 8) * a.c.R + (line - back);
+                const uint32_t line = i * (THREADS / KCH) + tf / KCH, back = beyond && line >= 32 ? 32 : 0;
+                rk[i] = pk[(line - back) * KCH + tf % KCH];
+                const uint32_t at = (tf % KCH / 8) * a.c.R + (line - back);
                 rks[i] = ps[at];
                 rkz[i] = pz[at];
             }
@@ -311,16 +323,33 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
             rvz = *reinterpret_cast<const uint4 *>(ps + static_cast<int64_t>(kQ4VBias) * NG * a.c.R + at);
         };
         auto unpack_k = [&](int buf) {
+            int tk = tid;
+            if constexpr (CODES && HD == 256) asm volatile("" : "+v"(tk));
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const int line = i * (THREADS / KCH) + tid / KCH, j = tid % KCH;
+                const int line = i * (THREADS / KCH) + tk / KCH, j = tk % KCH;
                 const h2_t s1 = {rks[i], rks[i]}, z1 = {rkz[i], rkz[i]};
                 const h2_t s[4] = {s1, s1, s1, s1}, z[4] = {z1, z1, z1, z1};
                 h8_t hi, lo;
-                q4_values<PQ>(rk[i], magic, s, z, kunit, hi, lo);
-                uint8_t *dst = s_k + buf * (PQ * KB) + 16 * q4_place<KCH, true>(line, j);
+                if constexpr (!CODES) {
+                    q4_values<KP>(rk[i], magic, s, z, kunit, hi, lo);
+                } else {
+                    h2_t c[4];
+                    q4_codes(rk[i], magic, c);
+                    hi = h8_t{c[0].x, c[0].y, c[1].x, c[1].y, c[2].x, c[2].y, c[3].x, c[3].y};
+                    if (j % 8 == 0) {
+                        s_ks[buf][j / 8][line] = rks[i];
+#pragma unroll
+                        for (int g = 0; g < 4; g += NG) {  // zeros for groups that heads of less than 256 lack
+                            const _Float16 b0 = g == 0 ? rkz[i] : static_cast<_Float16>(0.f);
+                            s_kz[buf][line][g + j / 8] = b0;
+                            s_kz[buf][line][4 + g + j / 8] = b0;
+                        }
+                    }
+                }
+                uint8_t *dst = s_k + buf * (KP * KB) + 16 * q4_place<KCH, true>(line, j);
                 *reinterpret_cast<h8_t *>(dst) = hi;
-                if constexpr (PQ == 2) *reinterpret_cast<h8_t *>(dst + KB) = lo;
+                if constexpr (KP == 2) *reinterpret_cast<h8_t *>(dst + KB) = lo;
             }
         };
         auto unpack_v = [&](int t0, int buf) {
@@ -359,30 +388,51 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
             // The chains of the tile's products by turns; key chunks are read a few ahead of them.  Step u's chunk lies 64 u
             // xor-ed into the first one's address, the rows of the second product 4 lines on.
             constexpr int NK = PAIRS * 2 * KS, AHEAD = PQ == 2 ? 2 : 4;
-            uint32_t kat = buf * (PQ * KB) + 16 * q4_place<KCH, true>(8 * (r >> 2) + (r & 3), q);
+            uint32_t kat = buf * (KP * KB) + 16 * q4_place<KCH, true>(8 * (r >> 2) + (r & 3), q);
             asm volatile("" : "+v"(kat));  // no step's address is kept from tile to tile
             auto key = [&](int n, int plane) {
                 const int pr = n / 2 % PAIRS, x = n % 2, u = n / (2 * PAIRS);
                 return *reinterpret_cast<const h8_t *>(s_k + (kat ^ (64u * u)) + plane * KB + (32 * pr + 4 * x) * KCH * 16);
             };
-            h8_t kf[AHEAD][PQ];
+            h8_t kf[AHEAD][KP];
 #pragma unroll
             for (int n = 0; n < AHEAD; ++n)
 #pragma unroll
-                for (int p = 0; p < PQ; ++p) kf[n][p] = key(n, p);
+                for (int p = 0; p < KP; ++p) kf[n][p] = key(n, p);
+            if constexpr (CODES) {
+                // sums of codes by group, times the rows' scales; the biases and the sums of the queries are one
+                // more product
+#pragma unroll
+                for (int n = 0; n < 2 * PAIRS; ++n)
+                    s[n / 2][n % 2] = mfma16(*reinterpret_cast<const h8_t *>(s_kz[buf][32 * (n / 2) + 8 * (r >> 2) + 4 * (n % 2) + (r & 3)]), qs, f4_t{0.f, 0.f, 0.f, 0.f});
+            }
+            f4_t d[PAIRS][2];
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
                 const int pr = n / 2 % PAIRS, x = n % 2, u = n / (2 * PAIRS);
-                f4_t c = u == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : s[pr][x];
-                c = mfma16(kf[n % AHEAD][0], qh[u], c);
-                if constexpr (PQ == 2) {
-                    c = mfma16(kf[n % AHEAD][0], ql[u], c);
-                    c = mfma16(kf[n % AHEAD][1], qh[u], c);
+                if constexpr (CODES) {
+                    d[pr][x] = mfma16(kf[n % AHEAD][0], qh[u], u % 2 == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : d[pr][x]);
+                    d[pr][x] = mfma16(kf[n % AHEAD][0], ql[u], d[pr][x]);
+                } else {
+                    f4_t c = u == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : s[pr][x];
+                    c = mfma16(kf[n % AHEAD][0], qh[u], c);
+                    if constexpr (PQ == 2) {
+                        c = mfma16(kf[n % AHEAD][0], ql[u], c);
+                        c = mfma16(kf[n % AHEAD][1], qh[u], c);
+                    }
+                    s[pr][x] = c;
                 }
-                s[pr][x] = c;
                 if (n + AHEAD < NK) {
 #pragma unroll
-                    for (int p = 0; p < PQ; ++p) kf[n % AHEAD][p] = key(n + AHEAD, p);
+                    for (int p = 0; p < KP; ++p) kf[n % AHEAD][p] = key(n + AHEAD, p);
+                }
+                if (CODES && u % 2 == 1 && n % (2 * PAIRS) == 2 * PAIRS - 1) {  // a group is complete
+#pragma unroll
+                    for (int p = 0; p < PAIRS; ++p) {
+                        const h8_t ks = *reinterpret_cast<const h8_t *>(&s_ks[CODES ? buf : 0][CODES ? u / 2 : 0][CODES ? 32 * p + 8 * q : 0]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s[p][i / 4][i % 4] = fmaf(static_cast<float>(ks[i]), d[p][i / 4][i % 4], s[p][i / 4][i % 4]);
+                    }
                 }
             }
             unpack_k(buf ^ 1);
@@ -478,11 +528,13 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
         // Where one part is used for p and values, inputs and output are bf16.  The gates of a part are all
         // on their way before any is used, the first part's across the barrier.
         const int at32 = static_cast<int>(at);
+        int el = lane;  // no address of what follows is kept across the tiles
+        asm volatile("" : "+v"(el));
         uint32_t to[ITS];  // (token, head) of the rows that this lane writes; the host keeps them below 2^31
         uint2 gates[ITS];
-        const int d0 = lane % CPR * 4;
+        const int d0 = el % CPR * 4;
 #pragma unroll
-        for (int it = 0; it < ITS; ++it) to[it] = __shfl(at32, it * RPI + lane / CPR, kWave);
+        for (int it = 0; it < ITS; ++it) to[it] = __shfl(at32, it * RPI + el / CPR, kWave);
         const bool any = base + wave * 16 < all;  // of this wave's rows
         auto load_gates = [&](uint2 (&g)[ITS], int part) {
             if constexpr (PV == 1) {
@@ -498,14 +550,14 @@ __global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
-            for (int d = 0; d < PART / 16; ++d) *reinterpret_cast<f4_t *>(mine + (r * CPR + ((4 * d + q) ^ r)) * 16) = o[part * (PART / 16) + d] * unit;
+            for (int d = 0; d < PART / 16; ++d) *reinterpret_cast<f4_t *>(mine + ((el & 15) * CPR + ((4 * d + (el >> 4)) ^ (el & 15))) * 16) = o[part * (PART / 16) + d] * unit;
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             uint2 next[ITS];
             if (last && part + 1 < PARTS) load_gates(next, part + 1);
 #pragma unroll
             for (int it = 0; it < ITS; ++it) {
-                const int row = it * RPI + lane / CPR, c = lane % CPR;
+                const int row = it * RPI + el / CPR, c = el % CPR;
                 const f4_t v = *reinterpret_cast<const f4_t *>(mine + (row * CPR + (c ^ row)) * 16);
                 if (base + wave * 16 + row >= all) continue;
                 const int d = part * PART + d0;
@@ -776,9 +828,10 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int
     const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits, (kQ4PartRows + all) / all});
     p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
     p.splits = static_cast<int>((rows + p.per - 1) / p.per);
-    // the gathered weights: as many workgroups, the queries dealt out where the cached rows are few
+    // the gathered weights: three rounds of two workgroups per CU, the queries dealt out where the cached
+    // rows are few (512 tokens after 8,192 rows: 118 us, in one round of 408 workgroups 127, in four 121)
     const int64_t cols = (rows + kGatherRows - 1) / kGatherRows * heads;
-    p.gparts = weights ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / cols, (max_tokens * group + 127) / 128, kQ4GatherMaxParts,
+    p.gparts = weights ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1536 / cols, (max_tokens * group + 127) / 128, kQ4GatherMaxParts,
                                                                                kQ4GatherMost / (heads * q4_rows(maxp))}))) : 0;
     return p;
 }
