@@ -168,8 +168,8 @@ void launch_q4_step(const AttnQ4Args &a, hipStream_t s);
 
 // Several tokens (attention_q4_prefill.hip): how the launches are cut for sequences of up to
 // max_tokens tokens and `rows` rows, `all` (token, query head) rows of the batch.  Splits are made where
-// tiles of 64 or 128 rows are fewer than 256: all * splits stays below 256 * 128 + all, and the workspace
-// has room for twice that; a batch that is padded a lot has fewer splits.
+// tiles of 64 or 128 rows are fewer than 512: all * splits stays below 512 * 128 + all, which the
+// workspace has room for; a batch that is padded a lot has fewer splits.
 constexpr int kQ4PrefillMaxSplits = 32;
 constexpr int64_t kQ4PartRows = 512 * 128;
 constexpr int kQ4GatherMaxParts = 32;
@@ -177,7 +177,7 @@ constexpr int64_t kQ4GatherMost = 4 << 20;  // numbers of all parts' sums
 struct Q4PrefillPlan {
     int planes_q, planes_v, rows_per, tiles, per, splits, gparts;
 };
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights);
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int maxp, bool f32, bool weights);
 void launch_q4_prefill(const AttnQ4Args &a, hipStream_t s);
 
 }  // namespace swq

@@ -214,11 +214,11 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 // VALU takes 42%, LDS (each wave reads the whole tile's operands for its 16 rows) as much, the matrix units
 // 30%.  4,096 tokens of 16 heads of 256: 207 to 228 us, 600 to 664 TFLOP/s (the card's clock decides); 512
 // after 8,192 rows, queries in two parts: 173.  32 rows per wave halve the LDS bytes but leave one wave
-// per SIMD (slower); scores of the next tile beside the softmax (237 us) cost more registers.  Heads of 64 in bf16: two
-// workgroups per CU, their registers bounded to 128 (4,096 tokens of 32 heads 159 us with its other
-// kernels, else 182); at 128 that is 8% less time for one long sequence and 7% more for four of 1,000.
+// per SIMD (slower); scores of the next tile beside the softmax (237 us) cost more registers.  Heads of up to 128 in bf16: two
+// workgroups per CU, their registers bounded to 128 (4,096 tokens of 32 heads of 128 250 us with the
+// other launches, else 284; of 64 154, else 182).
 template <int HD, int PQ, int PV, int NT, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave, HD == 64 && PQ == 1 ? 4 : 2) void q4_prefill(const AttnQ4Args a) {
+__global__ __launch_bounds__(WAVES *kWave, HD <= 128 && PQ == 1 ? 4 : 2) void q4_prefill(const AttnQ4Args a) {
     constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * WAVES;
     constexpr int THREADS = WAVES * kWave, KCH = HD / 8, VCH = NT / 8;
     // words of a thread: of keys KW, THREADS apart; of values VW of one block and group, 64 / VW dims apart
@@ -812,7 +812,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
 
 }  // namespace
 
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int maxp, bool f32, bool weights) {
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int maxp, bool f32, bool weights) {
     Q4PrefillPlan p{};
     p.planes_q = f32 || weights ? 2 : 1;
     p.planes_v = f32 ? 2 : 1;
@@ -821,9 +821,11 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int
     // with 64 rows 21.6)
     p.rows_per = (max_tokens * group + 127) / 128 * heads * std::max<int64_t>(1, rows / 256) <= 128 ? 64 : 128;
     p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
-    // a workgroup per CU, if the cached rows can be split that often with 256 rows each
+    // as many workgroups as the CUs hold, if the cached rows can be split that often with 256 rows each:
+    // two per CU where registers are bounded for that (512 tokens after 16,384 rows, 32 heads of 128: 193
+    // us, with one 220), else one (16 heads of 256: 196, with two 212)
     const int64_t groups = p.tiles * heads;
-    const int64_t want = std::max<int64_t>(1, 256 / groups), most = std::max<int64_t>(1, rows / 256);
+    const int64_t want = std::max<int64_t>(1, (hd <= 128 && p.planes_q == 1 ? 512 : 256) / groups), most = std::max<int64_t>(1, rows / 256);
     // a padded batch has more rows than its longest sequence accounts for
     const int64_t splits = std::min<int64_t>({want, most, kQ4PrefillMaxSplits, (kQ4PartRows + all) / all});
     p.per = static_cast<int>(((rows + splits - 1) / splits + 63) / 64 * 64);
