@@ -123,7 +123,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
         launch_q4_step(a, s);
         return launch_status();
     }
-    const Q4PrefillPlan plan = plan_q4_prefill(a.b.max_tokens, static_cast<int64_t>(batch->tokens) * a.H, rows, heads, a.group, a.c.hd, cache->max_positions, a.in_f32 || a.out_f32, weights != nullptr);
+    const Q4PrefillPlan plan = plan_q4_prefill(a.b.max_tokens, static_cast<int64_t>(batch->tokens) * a.H, rows, heads, a.group, a.c.hd, layer->rotary_dims, cache->max_positions, a.in_f32 || a.out_f32, weights != nullptr);
     const PrefillParts parts = prefill_parts(layer, cache, a.b.B, batch->tokens,
                                              plan.splits > 1 ? static_cast<int64_t>(batch->tokens) * a.H * plan.splits : 0,
                                              plan.gparts > 1 ? heads * a.c.R * plan.gparts : 0);
@@ -135,7 +135,7 @@ extern "C" int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_c
     a.per = plan.per;
     a.splits = plan.splits;
     a.gparts = plan.gparts;
-    a.qh = p;
+    if (!plan.prepares) a.qh = p;
     a.ql = p + parts.q;
     p += 2 * parts.q;
     a.qf = reinterpret_cast<float *>(p);

@@ -43,7 +43,7 @@ struct AttnQ4Args {
     int32_t planes_q, planes_v;  // f16 parts of queries and keys, and of p and values
     int32_t tiles, rows_per;     // tiles of (token, head) rows that are started, rows of one
     int32_t gparts;              // parts of the queries in the gathered weights
-    void *qh, *ql;               // [N][H][hd] f16: queries, high and low part
+    void *qh, *ql;               // [N][H][hd] f16: queries, high and low part; qh NULL: not made
     float *qf;                   // [N][H]: what turns a product of them into log2 units
     void *qs;                    // [N][H][16] f16: sums of their groups as three parts, or NULL
     uint32_t *vmax;              // [B][KVH][2]: bits of the largest key and value, or NULL
@@ -176,8 +176,9 @@ constexpr int kQ4GatherMaxParts = 32;
 constexpr int64_t kQ4GatherMost = 4 << 20;  // numbers of all parts' sums
 struct Q4PrefillPlan {
     int planes_q, planes_v, rows_per, tiles, per, splits, gparts;
+    bool prepares;  // queries in the attention's own launch
 };
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int maxp, bool f32, bool weights);
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int rot, int maxp, bool f32, bool weights);
 void launch_q4_prefill(const AttnQ4Args &a, hipStream_t s);
 
 }  // namespace swq

@@ -203,6 +203,70 @@ __device__ __forceinline__ h2_t pair_hh(uint32_t a, uint32_t b) { return __built
 
 // ---- attention --------------------------------------------------------------
 
+// Whether a bf16 call's queries are prepared where they are used: pairs of dims that turn together, `half`
+// apart, are then the same lane's, chunks 4 u + q and 4 (u + half / 32) + q.  A launch less and the queries
+// read once: 4,096 tokens of 16 heads of 256 240 us, now 224 (all launches), 4 x 1,000 of 32 heads of 128
+// 131, now 112; 512 after 16,384 rows in two splits, which prepare them twice, 193 and 194.
+bool prepares_queries(int rot) { return rot == 0 || rot == 64 || rot == 128 || rot == 256; }
+
+template <int HU, int KS>
+__device__ __forceinline__ void turn_chunks(float (&x)[KS][8], const float2 *turn, int half, int q) {
+    if constexpr (2 * HU <= KS) {
+#pragma unroll
+        for (int u = 0; u < HU; ++u) {
+            float2 cs[8];
+            q4_turns(cs, turn, half, 4 * u + q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float m = x[u][e], n = x[u + HU][e];
+                x[u][e] = m * cs[e].x - n * cs[e].y;
+                x[u + HU][e] = n * cs[e].x + m * cs[e].y;
+            }
+        }
+    }
+}
+
+// What q4_queries makes of one row, by the four lanes that have it as operand: chunks 4 u + q as f16, and
+// what turns a product of them into log2 units.
+template <int HD>
+__device__ __forceinline__ float prepare_queries(const AttnQ4Args &a, const uint16_t *src, const float2 *turn, int q, h8_t (&out)[HD / 32]) {
+    constexpr int KS = HD / 32;
+    const int half = a.b.rot / 2;
+    float x[KS][8], ss = 0.f, top = 0.f;
+#pragma unroll
+    for (int u = 0; u < KS; ++u) load8<uint16_t>(x[u], src + 8 * (4 * u + q));
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x[u][e] * x[u][e];
+    ss += __shfl_xor(ss, 16, kWave);
+    ss += __shfl_xor(ss, 32, kWave);
+    const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+        float w[8];
+        load8<float>(w, a.q_norm_w + 8 * (4 * u + q));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] *= sc * w[e];
+    }
+    if (half == 32) turn_chunks<1>(x, turn, half, q);
+    else if (half == 64) turn_chunks<2>(x, turn, half, q);
+    else if (half == 128) turn_chunks<4>(x, turn, half, q);
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[u][e]));
+    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+    int ex = 0;
+    if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[u][q4_element(e)] = static_cast<_Float16>(ldexpf(x[u][e], 8 - ex));
+    return ldexpf(a.scale2, ex - 8);
+}
+
 // A workgroup takes M = 16 WAVES rows (token, query head of the kv head's group; heads of one token next
 // to each other) and the cached rows of one split that the last of them sees, NT at a time.  The tile's
 // words are loaded two tiles ahead into registers, unpacked one tile ahead into the other of two LDS
@@ -275,12 +339,17 @@ __global__ __launch_bounds__(WAVES *kWave, HD <= 128 && PQ == 1 ? 4 : 2) void q4
             const int64_t at = static_cast<int64_t>(n0 + column / G) * a.H + kvh * G + column % G;
             int lq = q;  // as below: addresses kept from row tile to row tile were spilled
             asm volatile("" : "+v"(lq));
-            f = ldexpf(a.qf[at], -klift);
-            if (CODES && q < 2) qs = static_cast<const h8_t *>(a.qs)[2 * at + q];
+            if (PQ == 1 && !a.qh) {
+                const float2 *turn = a.b.rope + static_cast<int64_t>(a.b.position(b, column / G)) * (a.b.rot / 2);
+                f = prepare_queries<HD>(a, static_cast<const uint16_t *>(a.q) + at * 2 * HD, turn, lq, qh);
+            } else {
+                f = ldexpf(a.qf[at], -klift);
+                if (CODES && q < 2) qs = static_cast<const h8_t *>(a.qs)[2 * at + q];
 #pragma unroll
-            for (int u = 0; u < KS; ++u) {
-                qh[u] = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + lq];
-                if constexpr (PQ == 2) ql[u] = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + lq];
+                for (int u = 0; u < KS; ++u) {
+                    qh[u] = reinterpret_cast<const h8_t *>(a.qh)[at * KCH + 4 * u + lq];
+                    if constexpr (PQ == 2) ql[u] = reinterpret_cast<const h8_t *>(a.ql)[at * KCH + 4 * u + lq];
+                }
             }
         }
 #pragma unroll
@@ -795,7 +864,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     const uint32_t heads = static_cast<uint32_t>(a.b.B) * a.c.KVH;
     const int rows = static_cast<int>(std::min<int64_t>(a.c.maxp, 1 << 20));
     if (a.planes_q == 2) a.in_f32 ? launch_queries<HD, 2, float>(a, s) : launch_queries<HD, 2, uint16_t>(a, s);
-    else a.in_f32 ? launch_queries<HD, 1, float>(a, s) : launch_queries<HD, 1, uint16_t>(a, s);
+    else if (a.qh) launch_queries<HD, 1, uint16_t>(a, s);  // one part: bf16 in and out
     if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows / 4 * (HD / kQ4Group) + 255) / 256, 256), heads), dim3(256), 0, s, a);
     const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
     a.rows_per == 64 ? launch_tiles<HD, 4>(a, grid, s) : launch_tiles<HD, 8>(a, grid, s);
@@ -812,10 +881,11 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
 
 }  // namespace
 
-Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int maxp, bool f32, bool weights) {
+Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int64_t heads, int group, int hd, int rot, int maxp, bool f32, bool weights) {
     Q4PrefillPlan p{};
     p.planes_q = f32 || weights ? 2 : 1;
     p.planes_v = f32 ? 2 : 1;
+    p.prepares = p.planes_q == 1 && prepares_queries(rot);
     // 128 rows share a tile's values; where that leaves half of the compute units without work however
     // the cached rows are split, 64, whose steps are shorter (77 tokens of 16 heads of 256 in f32: 26 us,
     // with 64 rows 21.6)

@@ -378,3 +378,22 @@ def test_a_padded_batch(T):
             assert torch.equal(a, b)
         else:  # the padded call may be split in another way
             assert bool(((a - b).abs() <= 2e-5 * a.abs().max()).all())
+
+
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 62), (128, 64), (128, 32), (256, 128), (256, 256), (256, 254)])
+@pytest.mark.parametrize("n,T", [(0, 150), (900, 33)])
+def test_every_kind_of_rotation_in_bf16(hd, rot, n, T):
+    """bf16 prompts prepare their queries where they are used if the dims that turn together allow it."""
+    torch = _torch()
+    H, KVH = 6, 2
+    blk, qw, _ = _block(H, KVH, hd, rot, n + T, rot + n)
+    cache = blk.new_cache(1)
+    k0, v0, k, v, q = _random(n + T, (n, KVH * hd), (n, KVH * hd), (T, KVH * hd), (T, KVH * hd), (T, 2 * H * hd), dtype=torch.bfloat16)
+    rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    if n:
+        blk.append(k0, v0, cache, rows)
+    rows += n
+    out = blk.prefill(q, k, v, cache, rows, blk.new_workspace(cache, tokens=T, max_tokens=T))
+    kk, vv = cache.read(None, n + T)
+    want, _ = _attend(*_queries(q, H, hd, qw, blk.rope_table.cpu().numpy()[n:n + T]), kk[0].double(), vv[0].double(), n)
+    _close(out, want, True, f"{hd} {rot}")
