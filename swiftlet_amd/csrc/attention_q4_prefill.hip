@@ -276,11 +276,11 @@ __device__ __forceinline__ float prepare_queries(const AttnQ4Args &a, const uint
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
 // Bound, at hd 256, by what two waves per SIMD and a barrier a tile let overlap: of 2,560 clocks a step
 // VALU takes 42%, LDS (each wave reads the whole tile's operands for its 16 rows) as much, the matrix units
-// 30%.  4,096 tokens of 16 heads of 256: 207 to 228 us, 600 to 664 TFLOP/s (the card's clock decides); 512
-// after 8,192 rows, queries in two parts: 173.  32 rows per wave halve the LDS bytes but leave one wave
-// per SIMD (slower); scores of the next tile beside the softmax (237 us) cost more registers.  Heads of up to 128 in bf16: two
-// workgroups per CU, their registers bounded to 128 (4,096 tokens of 32 heads of 128 250 us with the
-// other launches, else 284; of 64 154, else 182).
+// 30%.  4,096 tokens of 16 heads of 256: 209 us traced, 660 TFLOP/s, some 180 in a row of calls; 512 after
+// 8,192 rows, queries in two parts: 157.  32 rows per wave halve the LDS bytes but leave one wave per
+// SIMD (slower); scores of the next tile beside the softmax (237 us, then 217) cost more registers.
+// Heads of up to 128 in bf16: two workgroups per CU, their registers bounded to 128 (4,096 tokens of 32
+// heads of 128 250 us with the other launches, else 284; of 64 154, else 182).
 template <int HD, int PQ, int PV, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, HD <= 128 && PQ == 1 ? 4 : 2) void q4_prefill(const AttnQ4Args a) {
     constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * WAVES;
@@ -683,7 +683,9 @@ __global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
 // registers, and walks the rows of queries that see any of them, 16 at a time: those go through LDS
 // once for all waves, the next 16 on their way meanwhile.  A group's products with the queries' two parts
 // are exact and take the rows' scales on the VALU; the biases meet the groups' sums, which are in three
-// parts, in one more matrix product.  Sums of p stay with the lane until the end.
+// parts, in one more matrix product.  Sums of p stay with the lane until the end.  512 tokens of 16 heads
+// after 8,192 rows of 2 kv heads of 256: 115 us, 616 TFLOP/s in the two products, with values as two parts
+// and so three products 143 (16 cached rows per wave and queries read by each from L1: 911).
 constexpr int kGatherRows = 128;
 
 template <int HD>
