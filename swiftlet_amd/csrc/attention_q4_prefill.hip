@@ -160,7 +160,7 @@ __device__ __forceinline__ int q4_place(int line, int c) {
     return line * CH + (c ^ f);
 }
 
-// A word's codes times scale plus bias, pairs of nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+// A word's codes as f16 integers, pairs of nibbles (0, 4), (1, 5), (2, 6), (3, 7).
 __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t magic, h2_t (&c)[4]) {
     constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;
     const uint32_t s = w >> 8;
@@ -173,8 +173,8 @@ __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t magic, h2_t (&c)[4
     c[3] = __builtin_elementwise_fma(__builtin_bit_cast(h2_t, (s & kOdd) | magic), down, off16);
 }
 
-// One plane: scale * code + bias rounded to f16 once (2^-12 of the value; exact below f16's normal
-// numbers, where all three are multiples of 2^-24).  Two: in f32, times 2^lift, as high and low part.
+// One plane: scale * code + bias rounded to f16 once (2^-12 of the value, none past f16's largest; exact
+// below f16's normal numbers, where all three are multiples of 2^-24).  Two: in f32, times 2^lift, as high and low part.
 template <int PLANES>
 __device__ __forceinline__ void q4_values(uint32_t w, uint32_t magic, const h2_t (&s)[4], const h2_t (&z)[4], float unit, h8_t &hi, h8_t &lo) {
     h2_t c[4];

@@ -63,6 +63,13 @@ __device__ __forceinline__ _Float16 f16_by_f32(double x) {
     return static_cast<_Float16>(f);
 }
 
+// A group's scale: x to f16, or the number below where its largest value, bias + 15 scale, would pass f16's.
+__device__ __forceinline__ _Float16 q4_scale(double x, _Float16 bias) {
+    const _Float16 s = f16_by_f32(x);
+    const bool over = fmaf(15.0f, static_cast<float>(s), static_cast<float>(bias)) > 65504.0f;  // exact: 24 bits hold it
+    return __builtin_bit_cast(_Float16, static_cast<uint16_t>(__builtin_bit_cast(uint16_t, s) - (over ? 1 : 0)));
+}
+
 // The codes of values whose group has scale and bias.  (y - b) / s is first taken in f32 with a
 // reciprocal: codes are at most 15 and a bit and the difference, the reciprocal and the product each
 // round once, so it is off by less than 16 * 4 * 2^-24 = 4e-6.  Where that leaves the nearest integer in
@@ -100,7 +107,7 @@ __device__ __forceinline__ void q4_quantise(const double (&x)[EPL], uint32_t (&q
     lo = reduce_f64<kQ4Group / EPL>(lo, [](double a, double b) { return fmin(a, b); });
     hi = reduce_f64<kQ4Group / EPL>(hi, [](double a, double b) { return fmax(a, b); });
     bias = f16_by_f32(lo);
-    scale = f16_by_f32((hi - lo) / 15.0);
+    scale = q4_scale((hi - lo) / 15.0, bias);
     q4_codes<EPL>(y, q, scale, bias);
 }
 
@@ -120,7 +127,7 @@ __device__ __forceinline__ void q4_quantise(const float (&x)[8], uint32_t (&q)[8
     lo = fminf(lo, dpp_f32<0x141>(lo));
     hi = fmaxf(hi, dpp_f32<0x141>(hi));
     bias = static_cast<_Float16>(lo);
-    scale = f16_by_f32((static_cast<double>(hi) - static_cast<double>(lo)) / 15.0);
+    scale = q4_scale((static_cast<double>(hi) - static_cast<double>(lo)) / 15.0, bias);
     q4_codes<8>(y, q, scale, bias);
 }
 

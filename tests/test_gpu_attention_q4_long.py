@@ -397,3 +397,29 @@ def test_every_kind_of_rotation_in_bf16(hd, rot, n, T):
     kk, vv = cache.read(None, n + T)
     want, _ = _attend(*_queries(q, H, hd, qw, blk.rope_table.cpu().numpy()[n:n + T]), kk[0].double(), vv[0].double(), n)
     _close(out, want, True, f"{hd} {rot}")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_largest_values(hd, T, dtype):
+    """Values at both ends of what the cache takes: 15 steps of a rounded scale do not pass f16's
+    largest number, and attention over them is finite."""
+    torch = _torch()
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    H, KVH, n = 4, 2, 70
+    blk, qw, _ = _block(H, KVH, hd, 0, n + T, hd + T)
+    cache = blk.new_cache(1)
+    k, q, v = _random(hd, (n + T, KVH * hd), (T, 2 * H * hd), (n + T, KVH * hd))
+    k, q, v = k.to(dt), q.to(dt), (v.sign() * 7e4).to(dt)
+    rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    blk.append(k[:n], v[:n], cache, rows)
+    rows += n
+    ws, w = blk.new_workspace(cache, tokens=T, max_tokens=T, weights=True), blk.new_weights(cache)
+    out = blk.prefill(q, k[n:], v[n:], cache, rows, ws)
+    beside = blk.prefill(q, None, None, cache, rows, ws, weights=w)
+    kk, vv = cache.read(None, n + T)
+    assert 65300 < vv.max().item() <= 65504 and vv.min().item() == -65504
+    want, _ = _attend(*_queries(q, H, hd, qw, np.zeros((T, 0, 2), f32)), kk[0].double(), vv[0].double(), n)
+    _close(out, want, dtype == "bf16", "out")
+    _close(beside, want, dtype == "bf16", "out beside weights")

@@ -73,3 +73,16 @@ def test_keep_ties_and_short_sequences():
     assert R.keep(w, 3, 4, 1, 1).tolist() == [0, 1, 2]
     w[1] = np.nan
     assert R.keep(w, 8, 3, 1, 1).tolist() == [0, 5, 7]
+
+
+def test_no_value_passes_the_largest_f16():
+    rng = np.random.default_rng(9)
+    lo = -65504 + 400 * rng.random((300, 1, 1))
+    hi = 65504 - 400 * rng.random((300, 1, 1))
+    x = np.concatenate([lo, hi, lo + (hi - lo) * rng.random((300, 1, 62))], -1)
+    part = R.quantise(x)
+    v = R.values(part)
+    assert (v <= 65504).all() and (np.abs(v - x) <= (hi - lo) / 30 + 140).all()  # half a step, the scale's and the bias' rounding
+    plain = ((hi - lo) / 15).astype(np.float32).astype(np.float16)
+    up = part[2].astype(np.float64) + 15 * plain.astype(np.float64)
+    assert (up > 65504).any() and ((up > 65504) == (part[1] < plain)).all()
