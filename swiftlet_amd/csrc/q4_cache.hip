@@ -30,20 +30,18 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
     __shared__ double s_rot[kAppendThreads / LPR][HD];
     __shared__ uint2 s_v[BLOCKS][kQ4Block][LPR];
     const int h = blockIdx.y % a.c.KVH, b = blockIdx.y / a.c.KVH, tid = threadIdx.x, j = tid % LPR;
-    const int n0 = a.b.first(b), r0 = a.b.row0(b, a.c.maxp);
-    const int r1 = static_cast<int>(min(static_cast<int64_t>(r0) + a.b.count(b), static_cast<int64_t>(a.c.maxp)));  // past the last row written
-    const int half = a.b.rot / 2;
+    const Q4Rows rows = a.b.written(b, a.c.maxp);
+    const int half = a.b.rot / 2, block_end = rows.block_end();
     uint32_t *kw = a.c.k_head(b, h), *vw = a.c.v_head(b, h);
     _Float16 *par = a.c.par_head(b, h);
-    const int r0_block = r0 / kQ4Block;
-    for (int blk0 = r0_block + blockIdx.x * BLOCKS; blk0 * kQ4Block < r1; blk0 += gridDim.x * BLOCKS) {
+    for (int blk0 = rows.block0() + blockIdx.x * BLOCKS; blk0 < block_end; blk0 += gridDim.x * BLOCKS) {
 #pragma unroll
         for (int round = 0; round < ROUNDS; ++round) {
             const bool values = ROUNDS == 2 ? round == 1 : tid / PER % 2 == 1;  // the same for a whole wave
             const int which = ROUNDS == 2 ? 0 : tid / (2 * PER), u = tid % PER / LPR, row = (blk0 + which) * kQ4Block + u;
-            const bool here = row >= r0 && row < r1;
-            const int i = here ? row - r0 : 0;
-            const int64_t at = (static_cast<int64_t>(n0 + i) * a.c.KVH + h) * HD + 8 * j;
+            const bool here = rows.has(row);
+            const int n = rows.token(row);
+            const int64_t at = (static_cast<int64_t>(n) * a.c.KVH + h) * HD + 8 * j;
             float in[8];
             load8<T>(in, static_cast<const T *>(values ? a.v : a.k) + at);
             uint32_t q[8];
@@ -52,7 +50,7 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
                 double x[8];
                 float2 cs[8];
                 float w[8];
-                if (8 * j < 2 * half) q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, i)) * half, half, j);
+                if (8 * j < 2 * half) q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, n - rows.n0)) * half, half, j);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = a.w[8 * j + e];
                 double ss = 0.0;
@@ -110,7 +108,7 @@ __global__ __launch_bounds__(kAppendThreads) void q4_append(const AppendArgs a) 
         __syncthreads();
         for (int i = tid; i < BLOCKS * HD; i += kAppendThreads) {
             const int which = i / HD, d = i % HD, blk = blk0 + which;
-            const int u0 = max(r0 - blk * kQ4Block, 0), u1 = min(r1 - blk * kQ4Block, kQ4Block);
+            const int u0 = max(rows.r0 - blk * kQ4Block, 0), u1 = min(rows.r1 - blk * kQ4Block, kQ4Block);
             if (u0 < u1) {
                 uint32_t *p = vw + static_cast<int64_t>(blk) * HD + d;
                 uint32_t word = 0, mask = 0;

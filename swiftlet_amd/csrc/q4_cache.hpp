@@ -30,6 +30,18 @@ struct Q4View {
     __device__ __forceinline__ _Float16 *par_head(int b, int h) const { return par + head(b, h) * 4 * (hd / kQ4Group) * R; }
 };
 
+// Rows r0 .. r1 - 1 of the cache, which a sequence's tokens n0, n0 + 1, .. go into.
+struct Q4Rows {
+    int32_t n0, r0, r1;
+
+    // Blocks with such rows.  None where there are no rows: then n0 may be no token of the call, and nothing is loaded.
+    __host__ __device__ __forceinline__ int block0() const { return r0 / kQ4Block; }
+    __host__ __device__ __forceinline__ int block_end() const { return r0 < r1 ? (r1 - 1) / kQ4Block + 1 : block0(); }
+    __host__ __device__ __forceinline__ bool has(int row) const { return row >= r0 && row < r1; }
+    // The token whose k and v a lane loads for a row of these blocks (the first for rows that are not its sequence's new ones).
+    __host__ __device__ __forceinline__ int token(int row) const { return n0 + (has(row) ? row - r0 : 0); }
+};
+
 // Device view of a swq_q4_batch.  What comes from device memory is clamped where it is read, so
 // that no value of it leads out of a buffer.
 struct Q4Batch {
@@ -37,9 +49,13 @@ struct Q4Batch {
     const int32_t *starts, *rows, *positions;
     const float2 *rope;
 
-    __device__ __forceinline__ int first(int b) const { return starts ? min(max(starts[b], 0), N) : b * max_tokens; }
-    __device__ __forceinline__ int count(int b) const { return starts ? max(min(starts[b + 1], N) - first(b), 0) : max_tokens; }
-    __device__ __forceinline__ int row0(int b, int maxp) const { return min(max(rows[b], 0), maxp); }
+    __host__ __device__ __forceinline__ int first(int b) const { return starts ? min(max(starts[b], 0), N) : b * max_tokens; }
+    __host__ __device__ __forceinline__ int count(int b) const { return starts ? max(min(starts[b + 1], N) - first(b), 0) : max_tokens; }
+    __host__ __device__ __forceinline__ int row0(int b, int maxp) const { return min(max(rows[b], 0), maxp); }
+    __host__ __device__ __forceinline__ Q4Rows written(int b, int maxp) const {
+        const int r0 = row0(b, maxp);
+        return {first(b), r0, static_cast<int32_t>(min(static_cast<int64_t>(r0) + count(b), static_cast<int64_t>(maxp)))};
+    }
     __device__ __forceinline__ int position(int b, int i) const {
         const int64_t p = static_cast<int64_t>(positions ? positions[b] : rows[b]) + i;
         return static_cast<int>(min(max(p, static_cast<int64_t>(0)), static_cast<int64_t>(rope_positions - 1)));
