@@ -867,7 +867,7 @@ void launch_head_dim(const AttnQ4Args &a, hipStream_t s) {
     const int rows = static_cast<int>(std::min<int64_t>(a.c.maxp, 1 << 20));
     if (a.planes_q == 2) a.in_f32 ? launch_queries<HD, 2, float>(a, s) : launch_queries<HD, 2, uint16_t>(a, s);
     else if (a.qh) launch_queries<HD, 1, uint16_t>(a, s);  // one part: bf16 in and out
-    if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min((rows / 4 * (HD / kQ4Group) + 255) / 256, 256), heads), dim3(256), 0, s, a);
+    if (a.vmax) hipLaunchKernelGGL(q4_largest, dim3(std::min(((rows + 7) / 8 * 2 * (HD / kQ4Group) + 255) / 256, 256), heads), dim3(256), 0, s, a);
     const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.tiles) * a.splits * heads)), block(256);
     a.rows_per == 64 ? launch_tiles<HD, 4>(a, grid, s) : launch_tiles<HD, 8>(a, grid, s);
     if (a.splits > 1) {

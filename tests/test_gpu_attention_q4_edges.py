@@ -33,3 +33,30 @@ def test_sequences_that_bring_nothing(hd, KVH, before, counts, dtype):
     out = s.blk.prefill(q, k, v, s.cache, s.rows(), ws, starts=s.starts(counts), max_tokens=max(counts))
     _close(out, want, dtype)
     s.check_cache()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("before,T,most", [(0, 2, 1), (0, 2, 2), (1, 2, 2), (0, 2, 3), (2, 5, 3), (1, 2, 3), (0, 4, 4), (3, 20, 4), (5, 3, 7)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("weights", [False, True])
+def test_prompts_over_the_smallest_caches(hd, before, T, most, dtype, weights):
+    """Caches of a few rows, with room for the tokens or not: those past the last row see all of them."""
+    torch = _torch()
+    H, KVH = 4, 2
+    s = Setup(hd + most + T, H, KVH, hd, 16, [before], most)
+    q, k, v = s.tokens([T], _types()[dtype])
+    ws = s.blk.new_workspace(s.cache, tokens=T, max_tokens=T, weights=weights)
+    ws.fill_(255)
+    w = torch.full((1, KVH, most), 0.25, device="cuda") if weights else None
+    print(f"{before} + {T} of {most} rows, hd {hd}", flush=True)
+    out = s.blk.prefill(q, k, v, s.cache, s.rows(), ws, weights=w)
+    new = min(T, most - before)
+    turns = s.table[np.minimum(np.arange(before, before + new), most - 1)]
+    s.seqs[0] = R.append(s.seqs[0], *(x[:new].reshape(new, KVH, hd) for x in (s.k, s.v)), s.kw, 1e-6, turns)
+    want, got = s.expect([T], appended=False)
+    _close(out, want, dtype)
+    s.check_cache()
+    if weights:
+        got[0][:, :before] += 0.25
+        w, n = w[0].cpu().numpy(), before + new
+        assert np.abs(w[:, :n] - got[0]).max() <= 1e-5 * max(1.0, got[0].max()) and (w[:, n:] == 0.25).all()
