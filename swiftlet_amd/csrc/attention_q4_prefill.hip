@@ -29,81 +29,84 @@ __global__ __launch_bounds__(256) void q4_queries(const AttnQ4Args a) {
     const uint32_t all = static_cast<uint32_t>(cnt) * a.H;  // the host keeps it below 2^31
     const int64_t first = static_cast<int64_t>(a.b.first(b)) * a.H;
     const int half = a.b.rot / 2;
-    const uint32_t row = (blockIdx.x * HPB + slot) * ROWS;
-    float x[ROWS][8], w[8];
-    float2 cs[8];
-    uint32_t turned = ~0u;  // the token whose turns cs holds
+    float w[8];
     load8<float>(w, a.q_norm_w + 8 * j);
+    for (uint32_t base = blockIdx.x * (HPB * ROWS); base < all; base += gridDim.x * (HPB * ROWS)) {
+        const uint32_t row = base + slot * ROWS;
+        float x[ROWS][8];
+        float2 cs[8];
+        uint32_t turned = ~0u;  // the token whose turns cs holds
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const uint32_t it = min(row + k, all - 1);
-        load8<T>(x[k], static_cast<const T *>(a.q) + (first + it) * 2 * HD + 8 * j);
-    }
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const uint32_t token = min(row + k, all - 1) / a.H;
-        if (8 * j < 2 * half && token != turned) {
-            q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, token)) * half, half, j);
-            turned = token;
+        for (int k = 0; k < ROWS; ++k) {
+            const uint32_t it = min(row + k, all - 1);
+            load8<T>(x[k], static_cast<const T *>(a.q) + (first + it) * 2 * HD + 8 * j);
         }
-        float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[k][e] * x[k][e];
-        ss = lanes_sum<LPH>(ss);
-        const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[k][e] *= sc * w[e];
-            s_rot[slot][8 * j + e] = x[k][e];
-        }
-        __builtin_amdgcn_wave_barrier();  // a head's lanes are of one wave
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        float top = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = 8 * j + e;
-            if (d < 2 * half) {
-                const float o = s_rot[slot][d < half ? d + half : d - half];
-                x[k][e] = d < half ? x[k][e] * cs[e].x - o * cs[e].y : x[k][e] * cs[e].x + o * cs[e].y;
+        for (int k = 0; k < ROWS; ++k) {
+            const uint32_t token = min(row + k, all - 1) / a.H;
+            if (8 * j < 2 * half && token != turned) {
+                q4_turns(cs, a.b.rope + static_cast<int64_t>(a.b.position(b, token)) * half, half, j);
+                turned = token;
             }
-            top = fmaxf(top, fabsf(x[k][e]));
-        }
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        top = lanes_max<LPH>(top);
-        int ex = 0;
-        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-        h8_t hi, lo;
+            float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float v = ldexpf(x[k][e], 8 - ex);
-            hi[q4_element(e)] = static_cast<_Float16>(v);
-            lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
-        }
-        float qs = 0.f;
-        if constexpr (PQ == 2) {
+            for (int e = 0; e < 8; ++e) ss += x[k][e] * x[k][e];
+            ss = lanes_sum<LPH>(ss);
+            const float sc = 1.0f / __fsqrt_rn(ss / static_cast<float>(HD) + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qs += static_cast<float>(hi[e]) + static_cast<float>(lo[e]);
-            qs = lanes_sum<8>(qs);
-        }
-        if (row + k >= all) continue;
-        const int64_t at = first + row + k;
-        if (PQ == 2 && j % 8 == 0) {
-            _Float16 *to = static_cast<_Float16 *>(a.qs) + at * 16;
+            for (int e = 0; e < 8; ++e) {
+                x[k][e] *= sc * w[e];
+                s_rot[slot][8 * j + e] = x[k][e];
+            }
+            __builtin_amdgcn_wave_barrier();  // a head's lanes are of one wave
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            float top = 0.f;
 #pragma unroll
-            for (int g = 0; g < 4; g += HD / kQ4Group) {  // zeros for groups that heads of less than 256 lack
-                float rest = g == 0 ? qs : 0.f;
+            for (int e = 0; e < 8; ++e) {
+                const int d = 8 * j + e;
+                if (d < 2 * half) {
+                    const float o = s_rot[slot][d < half ? d + half : d - half];
+                    x[k][e] = d < half ? x[k][e] * cs[e].x - o * cs[e].y : x[k][e] * cs[e].x + o * cs[e].y;
+                }
+                top = fmaxf(top, fabsf(x[k][e]));
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            top = lanes_max<LPH>(top);
+            int ex = 0;
+            if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+            h8_t hi, lo;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const _Float16 h = i < 3 ? static_cast<_Float16>(rest) : static_cast<_Float16>(0.f);
-                    rest -= static_cast<float>(h);
-                    to[4 * i + g + j / 8] = h;
+            for (int e = 0; e < 8; ++e) {
+                const float v = ldexpf(x[k][e], 8 - ex);
+                hi[q4_element(e)] = static_cast<_Float16>(v);
+                lo[q4_element(e)] = static_cast<_Float16>(v - static_cast<float>(hi[q4_element(e)]));
+            }
+            float qs = 0.f;
+            if constexpr (PQ == 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qs += static_cast<float>(hi[e]) + static_cast<float>(lo[e]);
+                qs = lanes_sum<8>(qs);
+            }
+            if (row + k >= all) continue;
+            const int64_t at = first + row + k;
+            if (PQ == 2 && j % 8 == 0) {
+                _Float16 *to = static_cast<_Float16 *>(a.qs) + at * 16;
+#pragma unroll
+                for (int g = 0; g < 4; g += HD / kQ4Group) {  // zeros for groups that heads of less than 256 lack
+                    float rest = g == 0 ? qs : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const _Float16 h = i < 3 ? static_cast<_Float16>(rest) : static_cast<_Float16>(0.f);
+                        rest -= static_cast<float>(h);
+                        to[4 * i + g + j / 8] = h;
+                    }
                 }
             }
+            reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
+            if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
+            if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 8);
         }
-        reinterpret_cast<h8_t *>(a.qh)[at * LPH + j] = hi;
-        if constexpr (PQ == 2) reinterpret_cast<h8_t *>(a.ql)[at * LPH + j] = lo;
-        if (j == 0) a.qf[at] = ldexpf(a.scale2, ex - 8);
     }
 }
 
@@ -845,11 +848,12 @@ __global__ __launch_bounds__(256) void q4_gathered_merge(const AttnQ4Args a, int
 template <int HD, int PQ, typename T>
 void launch_queries(const AttnQ4Args &a, hipStream_t s) {
     constexpr int HPB = 256 / (HD / 8);
-    const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H;
-    if (items * a.b.B >= 4 * HPB * 512)
-        hipLaunchKernelGGL((q4_queries<HD, PQ, 4, T>), dim3(static_cast<uint32_t>((items + 4 * HPB - 1) / (4 * HPB)), a.b.B), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((q4_queries<HD, PQ, 1, T>), dim3(static_cast<uint32_t>((items + HPB - 1) / HPB), a.b.B), dim3(256), 0, s, a);
+    const int64_t items = static_cast<int64_t>(a.b.max_tokens) * a.H, all = static_cast<int64_t>(a.b.N) * a.H;
+    const bool four = items * a.b.B >= 4 * HPB * 512;
+    const int64_t per = four ? 4 * HPB : HPB;
+    const dim3 grid(static_cast<uint32_t>(q4_workgroups((items + per - 1) / per, a.b.B, all / per + a.b.B)), a.b.B);
+    if (four) hipLaunchKernelGGL((q4_queries<HD, PQ, 4, T>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((q4_queries<HD, PQ, 1, T>), grid, dim3(256), 0, s, a);
 }
 
 template <int HD, int WAVES>
@@ -892,7 +896,7 @@ Q4PrefillPlan plan_q4_prefill(int64_t max_tokens, int64_t all, int64_t rows, int
     // the cached rows are split, 64, whose steps are shorter (77 tokens of 16 heads of 256 in f32: 26 us,
     // with 64 rows 21.6)
     p.rows_per = (max_tokens * group + 127) / 128 * heads * std::max<int64_t>(1, rows / 256) <= 128 ? 64 : 128;
-    p.tiles = static_cast<int>(std::min<int64_t>((max_tokens * group + p.rows_per - 1) / p.rows_per, (1 << 30) / heads));
+    p.tiles = static_cast<int>(q4_workgroups((max_tokens * group + p.rows_per - 1) / p.rows_per, heads, all / p.rows_per + heads));
     // as many workgroups as the CUs hold, if the cached rows can be split that often with 256 rows each:
     // two per CU where registers are bounded for that (512 tokens after 16,384 rows, 32 heads of 128: 193
     // us, with one 220), else one (16 heads of 256: 196, with two 212)

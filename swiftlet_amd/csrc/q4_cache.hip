@@ -448,7 +448,9 @@ void launch_q4_append(const swq_attention_layer *l, const Q4View &c, const Q4Bat
     const AppendArgs a{c, b, k, v, l->k_norm_weight, l->norm_eps};
     // blocks that a sequence's tokens can touch: one more than they fill where the first row is
     // inside a block; a sequence that brings more goes round
-    const dim3 grid((b.max_tokens + kQ4Block - 1) / kQ4Block + (b.max_tokens > 1), static_cast<uint32_t>(b.B) * c.KVH);
+    const int64_t heads = static_cast<int64_t>(b.B) * c.KVH;
+    const int64_t blocks = q4_workgroups((b.max_tokens + kQ4Block - 1) / kQ4Block + (b.max_tokens > 1), heads, b.N / kQ4Block * static_cast<int64_t>(c.KVH) + 2 * heads);
+    const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(heads));
     if (dtype == SWQ_F32) append_typed<float>(a, grid, s);
     else append_typed<uint16_t>(a, grid, s);
 }

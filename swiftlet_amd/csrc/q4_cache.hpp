@@ -160,6 +160,16 @@ inline Q4Batch q4_batch(const swq_attention_layer *l, const swq_q4_batch *b) {
     return d;
 }
 
+// Workgroups along one sequence's tokens of a launch whose kernel goes round: `most` for one that brings
+// max_tokens, at `heads` (sequence, head) pairs whose work fills `work` workgroups.  max_tokens is a bound, and a caller
+// that does not know better gives the tokens of the whole call: then nearly all of `most` would find nothing
+// (256 sequences of 512 tokens ask for 8 M workgroups of 512, 2^32 work-items, which no launch takes).  A batch
+// of like lengths stays below 4 * work; the longest of a mixed one goes round.  128 sequences of 512 tokens of
+// 32 heads of 64 in bf16: 714 us, without the longest given 785, with all of `most` 7,140.
+inline int64_t q4_workgroups(int64_t most, int64_t heads, int64_t work) {
+    return std::max<int64_t>(1, std::min(most, std::max<int64_t>(1 << 16, 4 * work) / heads));
+}
+
 inline int check_q4_dtype(int dt) { return dt == SWQ_F32 || dt == SWQ_BF16 ? SWQ_OK : SWQ_ERR_UNSUPPORTED_DTYPE; }
 
 inline size_t q4_dtype_bytes(int dt) { return dt == SWQ_F32 ? 4 : 2; }

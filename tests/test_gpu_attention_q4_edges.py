@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from oracle import attention_q4_ref as R
+from swiftlet_amd.attention_q4 import AttentionQ4GPU
 from tests.test_gpu_attention_q4 import Setup, _close, _torch, _types
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +61,28 @@ def test_prompts_over_the_smallest_caches(hd, before, T, most, dtype, weights):
         got[0][:, :before] += 0.25
         w, n = w[0].cpu().numpy(), before + new
         assert np.abs(w[:, :n] - got[0]).max() <= 1e-5 * max(1.0, got[0].max()) and (w[:, n:] == 0.25).all()
+
+
+@pytest.mark.parametrize("dtype,weights", [("bf16", False), ("bf16", True), ("f32", False)])
+def test_many_sequences_without_their_longest(dtype, weights):
+    """max_tokens left out is that of all tokens, as much as 8 M workgroups for a tile each; lengths mixed or alike,
+    the same bits as with the longest given."""
+    torch = _torch()
+    H, KVH, hd, B, most = 32, 8, 64, 1024, 64
+    blk = AttentionQ4GPU(H, KVH, hd, 64, 1e6, 1e-6, 2 * most, np.ones(hd, f32), np.ones(hd, f32))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for counts in ([32] * B, [most if b % 3 == 0 else b % 7 for b in range(B)]):
+        N = sum(counts)
+        q, k, v = (torch.randn((N, n), generator=g, device="cuda").to(_types()[dtype]) for n in (2 * H * hd, KVH * hd, KVH * hd))
+        rows = torch.arange(B, dtype=torch.int32, device="cuda") % most
+        starts = torch.tensor(np.cumsum([0, *counts]), dtype=torch.int32, device="cuda")
+        got = []
+        for longest in (max(counts), None):
+            print(f"{N} tokens, longest {longest}", flush=True)
+            cache = blk.new_cache(B, 2 * most)
+            w = blk.new_weights(cache) if weights else None
+            ws = blk.new_workspace(cache, tokens=N, max_tokens=longest or N, weights=weights)
+            out = blk.prefill(q, k, v, cache, rows, ws, starts=starts, max_tokens=longest, weights=w)
+            got.append((out, cache.data, w))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and (not weights or torch.equal(got[0][2], got[1][2]))
+        assert bool(got[1][0].isfinite().all()) and bool(got[1][0].any())
