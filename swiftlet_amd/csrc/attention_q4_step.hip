@@ -43,7 +43,8 @@ __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n
 //           against the largest value scale so far, so that p * scale fits f16;
 //   values  V's codes are the left operand (rows: dims), p * scale the right one (columns: heads),
 //           straight from the registers that the scores left: no transpose, and the running
-//           maximum's factor is the lane's own.  p * bias is summed on the VALU.
+//           maximum's factor is the lane's own.  Codes are taken about zero (q4_operand_signed), and p *
+//           (bias + 8 or 7 scale) is summed on the VALU.
 // Heads past the group are columns that nothing reads.  The next tile's loads are issued as soon as
 // their registers are free.
 //   P = 1   (bf16 in and out, no gathered weights): queries and p * scale as one f16 number instead of
@@ -380,12 +381,12 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
             const uint32_t vw4[4] = {cur.v[g].x, cur.v[g].y, cur.v[g].z, cur.v[g].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const h8_t c = q4_operand(vw4[e], magic);
+                const h8_t c = q4_operand_signed(vw4[e], magic);
                 o[g][e] = mfma16(c, hi, o[g][e]);
                 if constexpr (P == 2) o[g][e] = mfma16(c, lo, o[g][e]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) pb[g] = fmaf(p[i], static_cast<float>(vb[i]), pb[g]);
+            for (int i = 0; i < 8; ++i) pb[g] = fmaf(p[i], fmaf(i & 1 ? kQ4Odd : kQ4Even, static_cast<float>(vs[i]), static_cast<float>(vb[i])), pb[g]);
         }
         load_v(next);
     }

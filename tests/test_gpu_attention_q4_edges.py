@@ -7,6 +7,7 @@ import pytest
 from oracle import attention_q4_ref as R
 from swiftlet_amd.attention_q4 import AttentionQ4GPU
 from tests.test_gpu_attention_q4 import Setup, _close, _torch, _types
+from tests.test_gpu_attention_q4_long import _attend, _block, _queries, _random
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,55 @@ def test_many_sequences_without_their_longest(dtype, weights):
             got.append((out, cache.data, w))
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and (not weights or torch.equal(got[0][2], got[1][2]))
         assert bool(got[1][0].isfinite().all()) and bool(got[1][0].any())
+
+
+# Single tokens in f32 whose splits are long.  A sum over a split adds 32 rows at a time, twice (p * scale is two
+# numbers), on two or four accumulators: 33,000 rows are 2 * 33,000 / 32 / 2 = 1,031 additions, each off by half a unit
+# in the last place at most, 2^-25 of the running sum, of either sign: 32 * 2^-25 = 1e-6 of it for all, as one standard
+# deviation at most; the largest of a few hundred outputs is off by three times that at most.  A running sum of signed terms
+# is about the size of the outputs.  Scores, off by some 3e-7 of either sign each, add a part of that: 64 * 2^-24 = 3.8e-6.
+LONG = 64 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("H,KVH,hd,n", [(8, 2, 64, 33000), (4, 2, 128, 20011), (16, 2, 256, 33000)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_long_splits_keep_their_precision(H, KVH, hd, n, weights):
+    """A hint of few rows leaves a long sequence to one split."""
+    torch = _torch()
+    blk, qw, _ = _block(H, KVH, hd, 0, n + 1, n)
+    cache = blk.new_cache(1)
+    k0, v0, k, v, q = _random(n, (n, KVH * hd), (n, KVH * hd), (1, KVH * hd), (1, KVH * hd), (1, 2 * H * hd))
+    rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    blk.append(k0, v0, cache, rows)
+    rows += n
+    w = blk.new_weights(cache) if weights else None
+    out = blk.step(q, k, v, cache, rows, blk.new_workspace(cache, weights=weights), weights=w, max_rows=64)
+    kk, vv = cache.read(None, n + 1)
+    want, got = _attend(*_queries(q, H, hd, qw, np.zeros((1, 0, 2), f32)), kk[0].double(), vv[0].double(), n)
+    off = ((out.double() - want).abs().max() / want.abs().max()).item()
+    print(f"{n} rows of {hd}: off by {off:.1e}", flush=True)
+    assert off <= LONG
+    if weights:
+        assert (w[0].double() - got).abs().max() <= 1e-5 * got.max()
+
+
+def test_a_wide_batch_in_f32_keeps_its_precision():
+    """32 sequences of up to 16,383 rows of 8 heads: splits of 2,048 rows."""
+    torch = _torch()
+    B, H, KVH, hd, n = 32, 16, 8, 64, 16383
+    blk, qw, _ = _block(H, KVH, hd, 0, n + 1, 7)
+    cache = blk.new_cache(B)
+    k0, v0 = _random(8, (B * n, KVH * hd), (B * n, KVH * hd))
+    blk.append(k0, v0, cache, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    del k0, v0
+    k, v, q = _random(9, (B, KVH * hd), (B, KVH * hd), (B, 2 * H * hd))
+    rows = torch.tensor([n - 400 * b for b in range(B)], dtype=torch.int32, device="cuda")
+    out = blk.step(q, k, v, cache, rows, blk.new_workspace(cache))
+    for b in (0, 1, 17, B - 1):
+        m = n - 400 * b
+        first = torch.zeros(B, dtype=torch.int32, device="cuda")
+        kk, vv = (x[b, :m + 1].double() for x in cache.read(first, m + 1))
+        want, _ = _attend(*_queries(q[b:b + 1], H, hd, qw, np.zeros((1, 0, 2), f32)), kk, vv, m)
+        off = ((out[b:b + 1].double() - want).abs().max() / want.abs().max()).item()
+        print(f"sequence {b}, {m} rows: off by {off:.1e}", flush=True)
+        assert off <= LONG, b
