@@ -389,10 +389,11 @@ int swq_q4_rope_table(int rotary_dims, float rope_theta, int64_t first, int coun
  * swq_attention_step, v as it is, both clamped to +-65504 with NaN as 0 (the
  * cache holds finite values only).  Per 64 dims bias = f16(min) and scale =
  * f16((max - min) / 15), each rounded to f32 first; where bias + 15 scale would
- * pass 65504, the scale is the f16 number below (every value of the cache is in
- * f16's range); code = (x - bias) / scale rounded to nearest even, 0 .. 15.  All in 64 bits up to these roundings, so
- * that a value next to a border falls to the same side everywhere.  Rows from
- * max_positions on are not written.  layer->max_positions is not read.  Here
+ * pass 65504, the scale is the largest f16 number with which it does not (every
+ * value of the cache is in f16's range); code = (x - bias) / scale rounded to
+ * nearest even, 0 .. 15.  All in 64 bits up to these roundings, so that a value
+ * next to a border falls to the same side everywhere.  Rows from max_positions
+ * on are not written.  layer->max_positions is not read.  Here
  * and below k, v, q, out and the norm weights are 16-byte aligned. */
 int swq_q4_append(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
                   const void *k_proj, const void *v_proj, int dtype, void *stream);

@@ -41,8 +41,10 @@ def quantise(x):
     y = np.where(np.isnan(x), 0.0, np.clip(x, -65504.0, 65504.0)).reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP)
     lo, hi = y.min(-1), y.max(-1)
     bias, scale = lo.astype(np.float32).astype(np.float16), ((hi - lo) / 15.0).astype(np.float32).astype(np.float16)
-    below = np.nextafter(scale, np.float16(0))
-    scale = np.where(bias.astype(f64) + 15 * scale.astype(f64) > 65504, below, scale)
+    # the largest scale with which no value passes 65504, where the rounded one is larger
+    passes = lambda s: bias.astype(f64) + 15 * s.astype(f64) > 65504  # noqa: E731
+    most = ((65504 - bias.astype(f64)) / 15).astype(np.float16)
+    scale = np.where(passes(scale), np.where(passes(most), np.nextafter(most, np.float16(0)), most), scale)
     s, b = scale.astype(f64)[..., None], bias.astype(f64)[..., None]
     with np.errstate(divide="ignore", invalid="ignore"):
         codes = np.where(s > 0, np.clip(np.rint((y - b) / s), 0, 15), 0).astype(np.uint8)

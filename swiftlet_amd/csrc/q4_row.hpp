@@ -63,11 +63,19 @@ __device__ __forceinline__ _Float16 f16_by_f32(double x) {
     return static_cast<_Float16>(f);
 }
 
-// A group's scale: x to f16, or the number below where its largest value, bias + 15 scale, would pass f16's.
+// A group's scale: x to f16, or the largest number with which no value, bias + 15 scale at most, passes f16's
+// largest.  One below x's is not always enough: a bias of that size may have been rounded up by 16.
 __device__ __forceinline__ _Float16 q4_scale(double x, _Float16 bias) {
-    const _Float16 s = f16_by_f32(x);
-    const bool over = fmaf(15.0f, static_cast<float>(s), static_cast<float>(bias)) > 65504.0f;  // exact: 24 bits hold it
-    return __builtin_bit_cast(_Float16, static_cast<uint16_t>(__builtin_bit_cast(uint16_t, s) - (over ? 1 : 0)));
+    _Float16 s = f16_by_f32(x);
+    if (fmaf(15.0f, static_cast<float>(s), static_cast<float>(bias)) >= 65504.0f) {
+        const double b = static_cast<double>(static_cast<float>(bias));
+        auto over = [&](_Float16 v) { return fma(15.0, static_cast<double>(static_cast<float>(v)), b) > 65504.0; };  // exact
+        if (over(s)) {
+            s = f16_by_f32((65504.0 - b) / 15.0);  // to one of the two numbers about it
+            if (over(s)) s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(__builtin_bit_cast(uint16_t, s) - 1));
+        }
+    }
+    return s;
 }
 
 // The codes of values whose group has scale and bias.  (y - b) / s is first taken in f32 with a

@@ -8,6 +8,7 @@ from oracle import attention_q4_ref as R
 from swiftlet_amd.attention_q4 import AttentionQ4GPU
 from tests.test_gpu_attention_q4 import Setup, _close, _torch, _types
 from tests.test_gpu_attention_q4_long import _attend, _block, _queries, _random
+from tests.test_oracle_attention_q4_range import near_the_top
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +140,31 @@ def test_a_wide_batch_in_f32_keeps_its_precision():
         off = ((out[b:b + 1].double() - want).abs().max() / want.abs().max()).item()
         print(f"sequence {b}, {m} rows: off by {off:.1e}", flush=True)
         assert off <= LONG, b
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 40])
+def test_values_up_to_the_largest_number(hd, T):
+    """Groups whose bias rounds up next to f16's largest number: rows as the oracle's, bit for bit, none of their values
+    past it, and finite attention; by the call for rows alone and by that of a single token."""
+    torch = _torch()
+    H, KVH, n = 2, 1, 41
+    s = Setup(hd + T, H, KVH, hd, 0, [0, 0], n)
+    x = near_the_top(2 * n * (hd // 64), hd).reshape(2, n, hd).astype(f32)
+    x[1] = -x[1]  # the bias is -65504 there
+    x[0, 3, :64] = np.linspace(65462.25, 65504, 64)
+    rows = s.rows()
+    ws = s.blk.new_workspace(s.cache, tokens=2 * T, max_tokens=T)
+    for t in range(0, n - T + 1, T):
+        q, k, _ = s.tokens([T, T], torch.float32)
+        s.v = x[:, t:t + T].reshape(2 * T, hd)
+        v = torch.from_numpy(s.v).cuda()
+        out = s.blk.prefill(q, k, v, s.cache, rows, ws)
+        assert bool(out.isfinite().all()) and out.abs().max() <= 65504
+        assert bool(s.blk.prefill(q.bfloat16(), None, None, s.cache, rows, ws).isfinite().all())
+        s.expect([T, T], attend=False)
+        s.before = [b + T for b in s.before]
+        rows = s.rows()
+    s.check_cache()
+    _, vv = s.cache.read(None, n, rows=rows)
+    assert vv.max() <= 65504 and vv.min() >= -65504
