@@ -442,7 +442,8 @@ int swq_q4_read(const swq_q4_cache *cache, int sequences, const int32_t *first, 
  * [sequences][KVH][src max_positions].  new_weights (or NULL): [sequences][KVH]
  * [dst max_positions], theirs, and 0 for the rest.  kept: int32 [sequences]
  * [KVH][budget], their rows in src, -1 past the last.  new_rows [sequences]:
- * min(n, budget).  A weight that is NaN counts as the lowest.  Two launches. */
+ * min(n, budget).  A weight that is NaN counts as the lowest.  No output
+ * overlaps weights or rows.  Two launches. */
 int swq_q4_evict(const swq_q4_cache *src, int sequences, const float *weights, const int32_t *rows,
                  const swq_q4_cache *dst, int budget, int sink, int recent, float *new_weights,
                  int32_t *new_rows, int32_t *kept, void *stream);

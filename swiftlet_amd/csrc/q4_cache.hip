@@ -526,16 +526,28 @@ extern "C" int swq_q4_evict(const swq_q4_cache *src, int sequences, const float 
         src->head_dim != dst->head_dim || static_cast<int64_t>(sink) + recent > budget)
         return SWQ_ERR_BAD_SHAPE;
     if (budget > dst->max_positions) return SWQ_ERR_LIMIT;
-    const uint8_t *s0 = static_cast<const uint8_t *>(src->data), *d0 = static_cast<const uint8_t *>(dst->data);
-    const size_t sn = q4_layout(src->sequences, src->num_kv_heads, src->head_dim, src->max_positions).total;
-    const size_t dn = q4_layout(dst->sequences, dst->num_kv_heads, dst->head_dim, dst->max_positions).total;
-    if ((s0 < d0 + dn && d0 < s0 + sn) || weights == new_weights || rows == new_rows) return SWQ_ERR_INVALID_ARGUMENT;
+    const size_t heads = static_cast<size_t>(sequences) * src->num_kv_heads;
+    struct Span {
+        const void *at;
+        size_t bytes;
+        bool over(const Span &o) const {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+            return at && a < b + o.bytes && b < a + bytes;
+        }
+    };
+    const Span in[] = {{weights, heads * src->max_positions * sizeof(float)}, {rows, sequences * sizeof(int32_t)}};
+    const Span out[] = {{new_weights, heads * dst->max_positions * sizeof(float)}, {new_rows, sequences * sizeof(int32_t)}, {kept, heads * budget * sizeof(int32_t)}};
+    for (const Span &o : out)
+        for (const Span &i : in)
+            if (o.over(i)) return SWQ_ERR_INVALID_ARGUMENT;
+    const Span from{src->data, q4_layout(src->sequences, src->num_kv_heads, src->head_dim, src->max_positions).total};
+    const Span to{dst->data, q4_layout(dst->sequences, dst->num_kv_heads, dst->head_dim, dst->max_positions).total};
+    if (from.over(to)) return SWQ_ERR_INVALID_ARGUMENT;
     const EvictArgs a{q4_view(src), q4_view(dst), weights, rows, new_weights, new_rows, kept, budget, sink, recent};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t heads = static_cast<uint32_t>(sequences) * src->num_kv_heads;
-    hipLaunchKernelGGL(q4_select, dim3(heads), dim3(kSelectThreads), 0, s, a);
+    hipLaunchKernelGGL(q4_select, dim3(static_cast<uint32_t>(heads)), dim3(kSelectThreads), 0, s, a);
     const int per = 2048 / src->head_dim;
-    const dim3 grid((budget + per - 1) / per, heads);
+    const dim3 grid((budget + per - 1) / per, static_cast<uint32_t>(heads));
     switch (src->head_dim) {
         case 64: hipLaunchKernelGGL(q4_gather<64>, grid, dim3(256), 0, s, a); break;
         case 128: hipLaunchKernelGGL(q4_gather<128>, grid, dim3(256), 0, s, a); break;
