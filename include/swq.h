@@ -362,7 +362,8 @@ size_t swq_q4_cache_bytes(int sequences, int num_kv_heads, int head_dim, int max
 typedef struct swq_q4_batch {
     int32_t sequences;        /* at most the cache's                          */
     int32_t tokens;           /* of all sequences together                    */
-    int32_t max_tokens;       /* no sequence brings more; starts NULL: not read */
+    int32_t max_tokens;       /* no sequence brings more (far too much: empty
+                                 workgroups); starts NULL: not read           */
     int32_t max_rows;         /* rows that a sequence has after the call, about:
                                  sets how the work is split, not what is read;
                                  0: the cache's max_positions                 */
@@ -417,10 +418,12 @@ size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const 
  * added to for rows below rows[b], set for the call's rows; others are left as
  * they are.  Scores, softmax and sums in 32 bits; f32 outputs and weights are
  * exact to about 1e-6 of the largest, bf16 ones (of bf16 inputs: queries and
- * softmax numerators then have 11 bits) to their rounding.  Repeatable bit for
- * bit with the same max_rows.  One token per sequence: split over the rows, two
- * launches; more: tiles of queries on the matrix cores.  The workspace, 256-byte
- * aligned, needs no preparation; out, weights and workspace overlap nothing. */
+ * softmax numerators then have 11 bits; in prompts keys and values too) to their
+ * rounding.  The same call gives the same bits again; sequences, max_tokens and
+ * max_rows set the order of sums.  One token per sequence: split over the rows,
+ * two launches; more: tiles of queries on the matrix cores.  The workspace,
+ * 256-byte aligned, needs no preparation; out, weights and workspace overlap
+ * nothing. */
 int swq_attention_q4(const swq_attention_layer *layer, const swq_q4_cache *cache, const swq_q4_batch *batch,
                      const void *q_proj, const void *k_proj, const void *v_proj, int dtype, float *weights,
                      void *out, int out_dtype, void *ws, size_t ws_bytes, void *stream);

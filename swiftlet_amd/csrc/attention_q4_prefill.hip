@@ -277,13 +277,15 @@ __device__ __forceinline__ float prepare_queries(const AttnQ4Args &a, const uint
 // (K's rows permuted so that the result's registers are the next operand), out = V^T P, so that
 // maxima, sums and rescaling belong to the lane's own column.  p is taken against a reference that only
 // moves when a score passes it by 2^15: most tiles need no maximum across lanes and no rescaling.
-// Bound, at hd 256, by what two waves per SIMD and a barrier a tile let overlap: of 2,560 clocks a step
-// VALU takes 42%, LDS (each wave reads the whole tile's operands for its 16 rows) as much, the matrix units
-// 30%.  4,096 tokens of 16 heads of 256: 209 us traced, 660 TFLOP/s, some 180 in a row of calls; 512 after
-// 8,192 rows, queries in two parts: 157.  32 rows per wave halve the LDS bytes but leave one wave per
-// SIMD (slower); scores of the next tile beside the softmax (237 us, then 217) cost more registers.
+// Bound, at hd 256, by what two waves per SIMD and a barrier a tile let overlap: 4,096 tokens of 16 heads of
+// 256 in bf16 take 220 us traced, 625 TFLOP/s, their queries prepared here; of those clocks VALU has 46%, LDS (each
+// wave reads the whole tile's operands for its 16 rows) 44%, the matrix units 31%.  512 after 8,192 rows, queries
+// in two parts: 158.  32 rows per wave halve the LDS bytes but leave one wave per SIMD (slower); scores of the
+// next tile beside the softmax (237 us, when this took 217) cost more registers.
 // Heads of up to 128 in bf16: two workgroups per CU, their registers bounded to 128 (4,096 tokens of 32
-// heads of 128 250 us with the other launches, else 284; of 64 154, else 182).
+// heads of 128 250 us with the other launches, else 284; of 64 154, else 182).  Registers are spilled once a row
+// tile, none in the loop over cached rows: 23 (<128, 1, 1, 32, 8>), 51 (4 waves), 4 and 18 at hd 64, and at
+// hd 256, which has 256, 29 (<256, 2, 1, 32, 8>), 55 (4 waves) and 18 (<256, 1, 1, 32, 4>).
 template <int HD, int PQ, int PV, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, HD <= 128 && PQ == 1 ? 4 : 2) void q4_prefill(const AttnQ4Args a) {
     constexpr int NG = HD / kQ4Group, KS = HD / 32, DT = HD / 16, PAIRS = NT / 32, M = 16 * WAVES;
@@ -651,7 +653,7 @@ __global__ __launch_bounds__(WAVES *kWave, HD <= 128 && PQ == 1 ? 4 : 2) void q4
     }
 }
 
-// The splits of each (token, query head) merged: a wave per row, HD / 64 dims per lane.
+// The splits of each (token, query head) merged: HD / 4 lanes per row, 4 dims each.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_prefill_merge(const AttnQ4Args a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;  // lanes per row, rows per workgroup

@@ -21,7 +21,7 @@ struct Q4Tile {
 };
 
 // Four dims of head u: to the partial results of `split`, or, of the only one, to the output.
-template <int HD, typename T>
+template <int HD>
 __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n0, int h0, int u, int split, int d, f4_t s, float M, float L) {
     if (a.part) {
         *reinterpret_cast<f4_t *>(a.part + ((head0 + u) * a.splits + split) * HD + d) = s;
@@ -49,12 +49,12 @@ __device__ __forceinline__ void finish(const AttnQ4Args &a, int64_t head0, int n
 // their registers are free.
 //   P = 1   (bf16 in and out, no gathered weights): queries and p * scale as one f16 number instead of
 //           two, and K's codes with the 1024 left on, whose share of a score is the same for all rows
-//           and starts the sum.  32 sequences of up to 16,384 rows of 8 heads of 128: 80 us, with two 88.
+//           and starts the sum.  32 sequences of up to 16,384 rows of 8 heads of 128: 81 us, with two 9 more.
 //           (Not for V's: there the 1024 would swallow the bits of an average that is near zero.)
-// Wide batches are bound by instruction issue beside the loads: those 80 us are 3.8 TB/s of cache, with
-// VALU and matrix instructions for some 45 of them on every SIMD; three waves are all that 160 registers
-// leave (bounded to 128 they spill: 163 us).  Small ones are a chain: of 7.8 us at 500 rows of 2 heads of
-// 256 a workgroup's life is 6.2, rows and addresses 0.9, queries 1.9, one step 1.6, the teams' sums 1.2.
+// Wide batches are bound by instruction issue beside the loads: those 81 us are 3.8 TB/s of cache, with
+// VALU and matrix instructions for some 50 of them on every SIMD; three waves are all that 160 registers
+// leave (bounded to 128 they spill: 163 us).  Small ones are a chain, 9 us at 500 rows of 2 heads of 256 in
+// f32: by a workgroup's own clock rows and addresses 0.9, queries 1.9, one step 1.6, the teams' sums 1.2.
 template <int HD, int P, typename T>
 __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const AttnQ4Args a) {
     constexpr int EPL = HD / kWave, NG = HD / kQ4Group, GW = NG > 1 ? 2 : 1, TW = NG / GW, TEAMS = kStepWaves / TW;
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(kStepThreads, HD == 64 ? 4 : 3) void q4_step(const 
             for (int w = 1; w < TEAMS; ++w) M = fmaxf(M, s_ml[w][0][u]);
 #pragma unroll
             for (int w = 0; w < TEAMS; ++w) L += q4_exp2(s_ml[w][0][u] - M) * s_ml[w][1][u];
-            finish<HD, T>(a, head0, n0, kvh * G, u, split, d, s, M, L);
+            finish<HD>(a, head0, n0, kvh * G, u, split, d, s, M, L);
         }
     }
 }
