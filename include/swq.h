@@ -417,7 +417,8 @@ size_t swq_attention_q4_workspace_bytes(const swq_attention_layer *layer, const 
  * each row has gathered, summed over tokens and the kv head's query heads:
  * added to for rows below rows[b], set for the call's rows; others are left as
  * they are.  Scores, softmax and sums in 32 bits; f32 outputs and weights are
- * exact to about 1e-6 of the largest, bf16 ones (of bf16 inputs: queries and
+ * exact to about 1e-6 of the largest (5e-6 where a prompt's workgroup sums 33,000
+ * rows, and more where scores are far larger than usual), bf16 ones (of bf16 inputs: queries and
  * softmax numerators then have 11 bits; in prompts keys and values too) to their
  * rounding.  The same call gives the same bits again; sequences, max_tokens and
  * max_rows set the order of sums.  One token per sequence: split over the rows,

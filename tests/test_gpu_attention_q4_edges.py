@@ -120,6 +120,30 @@ def test_long_splits_keep_their_precision(H, KVH, hd, n, weights):
         assert (w[0].double() - got).abs().max() <= 1e-5 * got.max()
 
 
+@pytest.mark.parametrize("H,KVH,hd", [(8, 2, 64), (16, 2, 256)])
+@pytest.mark.parametrize("T", [3, 130])
+@pytest.mark.parametrize("sharp", [1, 6])
+def test_prompts_of_one_long_split(H, KVH, hd, T, sharp):
+    """As above for several tokens: three products a tile of 32 rows are 3,093 additions to one accumulator, each off by
+    2^-24 of it at most, evenly spread: one standard deviation is sqrt(3093 / 3) * 2^-24 = 1.9e-6, the largest of
+    some thousand outputs four of them, 7.7e-6, and 2e-6 of sums of weights and scores make 1e-5."""
+    torch = _torch()
+    n = 33000
+    blk, qw, _ = _block(H, KVH, hd, 0, n + T, n)
+    blk.q_norm.mul_(sharp)
+    cache = blk.new_cache(1)
+    k0, v0, k, v, q = _random(n + T, (n, KVH * hd), (n, KVH * hd), (T, KVH * hd), (T, KVH * hd), (T, 2 * H * hd))
+    rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    blk.append(k0, v0, cache, rows)
+    rows += n
+    out = blk.prefill(q, k, v, cache, rows, blk.new_workspace(cache, tokens=T, max_tokens=T), max_rows=64)
+    kk, vv = cache.read(None, n + T)
+    want, _ = _attend(*_queries(q, H, hd, qw * f32(sharp), np.zeros((T, 0, 2), f32)), kk[0].double(), vv[0].double(), n)
+    off = ((out.double() - want).abs().max() / want.abs().max()).item()
+    print(f"{T} tokens of {hd}: off by {off:.1e}", flush=True)
+    assert off <= 1e-5
+
+
 def test_a_wide_batch_in_f32_keeps_its_precision():
     """32 sequences of up to 16,383 rows of 8 heads: splits of 2,048 rows."""
     torch = _torch()
