@@ -277,6 +277,55 @@ int swq_deltanet_token(const swq_deltanet_layer *layer, const swq_qlinear *proje
                        float norm_eps, void *state, size_t state_bytes, int64_t position, float *scratch,
                        size_t scratch_floats, float *out, void *stream);
 
+/* ---- gated DeltaNet block over many tokens ------------------------------- */
+
+/* Bytes of one slot of a buffer of many sequences' states:
+ * swq_deltanet_state_bytes rounded up to 256 (0 on bad input).  Each slot is
+ * a state as swq_deltanet_step takes it. */
+size_t swq_deltanet_slot_bytes(const swq_deltanet_layer *layer);
+
+/* The tokens of one call, sequence after sequence: sequence b brings T_b of
+ * them.  A sequence may bring none; its state is then left as it is.  Arrays
+ * on the device are read by the kernels, so the same call may be captured and
+ * replayed as they change. */
+typedef struct swq_deltanet_batch {
+    int32_t sequences;
+    int32_t tokens;           /* of all sequences together                    */
+    int32_t max_tokens;       /* of one sequence: of one that brings more, only
+                                 the first max_tokens are taken; starts NULL:
+                                 not read                                     */
+    int32_t slots;            /* states in the buffer                         */
+    const int32_t *starts;    /* device [sequences + 1], rising: T_b = starts[b +
+                                 1] - starts[b]; NULL: tokens / sequences each */
+    const int32_t *positions; /* device [sequences]: tokens already in each
+                                 sequence's state                             */
+    const int32_t *slot;      /* device [sequences]: the state of each, no two
+                                 the same; a sequence whose slot is none of the
+                                 buffer's (-1, say) is left out, its rows of out
+                                 and all states as they are; NULL: b          */
+    int64_t qkvz_stride;      /* elements from one token's row to the next; 0:
+                                 rows lie end to end                          */
+    int64_t ba_stride;        /* likewise                                     */
+    int32_t reserved;         /* must be 0                                    */
+} swq_deltanet_batch;
+
+/* Workspace bytes of swq_deltanet_tokens for calls of up to batch->sequences
+ * sequences, batch->tokens tokens and batch->max_tokens of one sequence.  Of
+ * starts and slot only whether they are NULL is read, of positions nothing.  0
+ * on bad input. */
+size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch);
+
+/* swq_deltanet_step for the tokens of many sequences, prompts or one token
+ * each: qkvz [tokens] rows of 2*nk*dk + 2*nv*dv, ba [tokens] rows of 2*nv, of
+ * dtype (SWQ_F32 / SWQ_BF16), in the layer's layout; out [tokens][nv*dv] of
+ * out_dtype.  Each sequence goes on from its state, which is updated in place
+ * (f32): the results of as many swq_deltanet_step calls, up to the order of f32
+ * sums.  The same call gives the same bits again.  No output overlaps an input or the workspace.  states and workspace:
+ * 256-byte aligned; the workspace needs no preparation. */
+int swq_deltanet_tokens(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch, const void *qkvz,
+                        const void *ba, int dtype, void *states, size_t states_bytes, void *out, int out_dtype,
+                        void *ws, size_t ws_bytes, void *stream);
+
 /* ---- gated GQA attention decode step ------------------------------------ */
 
 /* One full-attention block (self_attn) between q/k/v_proj and o_proj. */
@@ -327,6 +376,70 @@ int swq_attention_token(const swq_attention_layer *layer, const swq_qlinear *pro
                         const swq_qlinear *o_proj, const float *x, const void *norm_weight, int norm_dtype,
                         float norm_eps, void *cache, size_t cache_bytes, int64_t position, float *scratch,
                         size_t scratch_floats, float *out, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- rotary positions ---------------------------------------------------- */
+
+/* How a model reads contexts longer than it was trained on; the angle of
+ * position p and pair j is p * f_j, f_j = theta^(-2 j / rotary_dims) if PLAIN. */
+enum {
+    SWQ_ROPE_PLAIN = 0,
+    SWQ_ROPE_LINEAR = 1, /* f_j / factor                                      */
+    SWQ_ROPE_NTK = 2,    /* theta * factor^(d / (d - 2)) for theta, d =
+                            rotary_dims > 2                                   */
+    SWQ_ROPE_YARN = 3    /* f_j where pair j turns beta_fast times or more
+                            over original_positions, f_j / factor where it
+                            turns beta_slow times or fewer, and a ramp over
+                            j between: from floor(j of beta_fast) to ceil(j of
+                            beta_slow), j of t = d ln(original_positions / (2
+                            pi t)) / (2 ln theta)                             */
+};
+typedef struct swq_rope_scaling {
+    int32_t kind;
+    int32_t original_positions;  /* YARN only, as are the next three          */
+    double beta_fast, beta_slow; /* usually 32 and 1                          */
+    double magnitude;            /* cos and sin are multiplied by it; 0: 1 +
+                                    0.1 ln(factor), 1 for factor <= 1         */
+    double factor;               /* > 0; not read if PLAIN                    */
+    int64_t reserved;            /* must be 0                                 */
+} swq_rope_scaling;
+
+/* cos and sin (device) of angles in 64 bits into table [count][rotary_dims / 2]
+ * [2] f32: row i for position positions[i] (device), or first + i where
+ * positions is NULL.  scaling NULL: PLAIN.  rotary_dims <= 512.  The table is
+ * what swq_rope and swq_attention_q4 take.  (swq_q4_rope_table rounds
+ * frequencies and angles to f32, as swq_attention_step does: from some 10,000
+ * positions on the two differ by more than 1e-3.) */
+int swq_rope_table(int rotary_dims, double rope_theta, const swq_rope_scaling *scaling, const int32_t *positions,
+                   int64_t first, int count, float *table, void *stream);
+
+/* Layouts of a turned pair j: elements j and j + rotary_dims / 2, or 2 j and
+ * 2 j + 1. */
+enum { SWQ_ROPE_HALF = 0, SWQ_ROPE_INTERLEAVED = 1 };
+
+/* Heads of one tensor, queries or keys: element e of head h of token t at
+ * x[t * token_stride + h * head_stride + e].  out may be x with the same
+ * strides; other than that nothing overlaps. */
+typedef struct swq_rope_heads {
+    const void *x;
+    void *out;
+    int64_t token_stride, head_stride;         /* elements                    */
+    int64_t out_token_stride, out_head_stride;
+    const float *norm_weight;                  /* [head_dim] f32 device: heads
+                                                  are RMS-normalised first, x *
+                                                  (scale * w); NULL: not      */
+    int32_t heads;
+    int32_t reserved;                          /* must be 0                   */
+} swq_rope_heads;
+
+/* The first rotary_dims elements of the heads of up to four tensors turned, one
+ * launch: (a, b) of pair j to (a c - b s, b c + a s) with c, s = table[row][j];
+ * the others are copied (normalised too).  row of token t: rows[t] (device; those
+ * outside 0 .. table_rows - 1 take the nearest), or t where rows is NULL.
+ * inverse (0 or 1): -s for s, which turns back and is the gradient.  dtype:
+ * SWQ_F32 or SWQ_BF16 of x and out; sums and products in f32, rounded once.
+ * head_dim <= 512, any strides. */
+int swq_rope(const swq_rope_heads *parts, int n, int tokens, int head_dim, int rotary_dims, int layout, int inverse,
+             float norm_eps, const float *table, int table_rows, const int32_t *rows, int dtype, void *stream);
 
 /* ---- attention over a KV cache held in 4 bits ---------------------------- */
 

@@ -1,0 +1,51 @@
+"""The gated DeltaNet block over the tokens of many sequences, in 64 bits — TEST INFRASTRUCTURE ONLY, the checker of
+swq_deltanet_tokens: QwenCPUModel.deltaNetForward's formulas (QwenCPUModel.swift:371-496) token after token, as
+deltanet_ref.deltanet_core has them in 32 bits.  torch, on any device."""
+
+from __future__ import annotations
+
+import torch
+
+
+def split_rows(qkvz, ba, nk, nv, dk, dv, split):
+    """The parts of projection rows in either layout, f64: mixed [N, q|k|v], z [N, nv, dv], b and a [N, nv]."""
+    x, ba = qkvz.double(), ba.double()
+    N, rep = x.shape[0], nv // nk
+    if split:
+        conv = 2 * nk * dk + nv * dv
+        return x[:, :conv], x[:, conv:conv + nv * dv].reshape(N, nv, dv), ba[:, :nv], ba[:, nv:2 * nv]
+    per = x[:, :2 * nk * dk + 2 * nv * dv].reshape(N, nk, -1)
+    q, k, v, z = per.split([dk, dk, rep * dv, rep * dv], -1)
+    gates = ba[:, :2 * nv].reshape(N, nk, 2, rep)
+    mixed = torch.cat([t.reshape(N, -1) for t in (q, k, v)], 1)
+    return mixed, z.reshape(N, nv, dv), gates[:, :, 0].reshape(N, nv), gates[:, :, 1].reshape(N, nv)
+
+
+def tokens(qkvz, ba, ring, state, position, conv_w, a_log, dt_bias, norm_w, nk, nv, dk, dv, eps, split):
+    """T tokens of one sequence whose conv ring [K, convD] and matrices [nv, dv, dk] hold `position` tokens already.
+    Returns (y [T, nv * dv], ring, state), f64."""
+    mixed, z, b, a = split_rows(qkvz, ba, nk, nv, dk, dv, split)
+    T, conv, rep = mixed.shape[0], mixed.shape[1], nv // nk
+    w = conv_w.double().reshape(conv, -1)
+    K = w.shape[1]
+    ring, S = ring.double().clone(), state.double().clone()
+    back = [ring[(position - K + 1 + j) % K] for j in range(K - 1)]
+    rows = torch.cat([torch.stack(back), mixed]) if back else mixed
+    x = sum(w[:, j] * rows[j:j + T] for j in range(K))
+    x = x / (1 + torch.exp(-x))
+    for i in range(max(0, T - K), T):
+        ring[(position + i) % K] = mixed[i]
+    q, k = (t.reshape(T, nk, dk) for t in x[:, :2 * nk * dk].chunk(2, 1))
+    q, k = (t / torch.sqrt((t * t).mean(-1, keepdim=True) + 1e-6) for t in (q, k))
+    q, k = (q / dk).repeat_interleave(rep, 1), (k / dk ** 0.5).repeat_interleave(rep, 1)
+    v = x[:, 2 * nk * dk:].reshape(T, nv, dv)
+    g = torch.exp(-torch.exp(a_log.double()) * torch.nn.functional.softplus(a + dt_bias.double(), threshold=40.0))
+    beta = 1 / (1 + torch.exp(-b))
+    out = torch.empty((T, nv, dv), dtype=torch.float64, device=S.device)
+    for t in range(T):
+        S = S * g[t][:, None, None]
+        d = beta[t][:, None] * (v[t] - (S * k[t][:, None]).sum(-1))
+        S = S + d[:, :, None] * k[t][:, None]
+        out[t] = (S * q[t][:, None]).sum(-1)
+    y = out / torch.sqrt((out * out).mean(-1, keepdim=True) + eps) * norm_w.double()
+    return (y * z / (1 + torch.exp(-z))).reshape(T, nv * dv), ring, S

@@ -85,6 +85,14 @@ class DeltaNetLayer(ctypes.Structure):
     ]
 
 
+class DeltaNetBatch(ctypes.Structure):
+    _fields_ = [
+        ("sequences", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_tokens", ctypes.c_int32), ("slots", ctypes.c_int32),
+        ("starts", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("slot", ctypes.c_void_p),
+        ("qkvz_stride", ctypes.c_int64), ("ba_stride", ctypes.c_int64), ("reserved", ctypes.c_int32),
+    ]
+
+
 class AttentionLayer(ctypes.Structure):
     _fields_ = [
         ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
@@ -107,6 +115,25 @@ class Q4Batch(ctypes.Structure):
         ("max_rows", ctypes.c_int32), ("starts", ctypes.c_void_p), ("rows", ctypes.c_void_p),
         ("positions", ctypes.c_void_p), ("rope", ctypes.c_void_p), ("rope_positions", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+    ]
+
+
+SWQ_ROPE_HALF, SWQ_ROPE_INTERLEAVED = 0, 1
+SWQ_ROPE_PLAIN, SWQ_ROPE_LINEAR, SWQ_ROPE_NTK, SWQ_ROPE_YARN = 0, 1, 2, 3
+
+
+class RopeScalingDesc(ctypes.Structure):
+    _fields_ = [
+        ("kind", ctypes.c_int32), ("original_positions", ctypes.c_int32), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double),
+        ("magnitude", ctypes.c_double), ("factor", ctypes.c_double), ("reserved", ctypes.c_int64),
+    ]
+
+
+class RopeHeads(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64), ("norm_weight", ctypes.c_void_p),
+        ("heads", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -144,6 +171,9 @@ SIGNATURES = {
     "swq_sample": (_I, [_P, _I, _c.POINTER(SampleOptions), _P, _P, _I, _P, _I, _c.c_float, _P, _P, _SZ, _P]),
     "swq_deltanet_state_bytes": (_SZ, [_c.POINTER(DeltaNetLayer)]),
     "swq_deltanet_step": (_I, [_c.POINTER(DeltaNetLayer), _P, _P, _P, _SZ, _I64, _P, _P]),
+    "swq_deltanet_slot_bytes": (_SZ, [_c.POINTER(DeltaNetLayer)]),
+    "swq_deltanet_tokens_workspace_bytes": (_SZ, [_c.POINTER(DeltaNetLayer), _c.POINTER(DeltaNetBatch)]),
+    "swq_deltanet_tokens": (_I, [_c.POINTER(DeltaNetLayer), _c.POINTER(DeltaNetBatch), _P, _P, _I, _P, _SZ, _P, _I, _P, _SZ, _P]),
     "swq_attention_cache_bytes": (_SZ, [_c.POINTER(AttentionLayer)]),
     "swq_attention_workspace_bytes": (_SZ, [_c.POINTER(AttentionLayer)]),
     "swq_attention_step": (_I, [_c.POINTER(AttentionLayer), _P, _P, _P, _P, _SZ, _I64, _P, _P, _SZ, _P]),
@@ -153,6 +183,8 @@ SIGNATURES = {
     "swq_attention_scratch_floats": (_SZ, [_c.POINTER(AttentionLayer), _c.POINTER(QLinear)]),
     "swq_attention_token": (_I, [_c.POINTER(AttentionLayer), _c.POINTER(QLinear), _c.POINTER(QLinear), _P, _P, _I,
                                  _c.c_float, _P, _SZ, _I64, _P, _SZ, _P, _P, _SZ, _P]),
+    "swq_rope_table": (_I, [_I, _c.c_double, _c.POINTER(RopeScalingDesc), _P, _I64, _I, _P, _P]),
+    "swq_rope": (_I, [_c.POINTER(RopeHeads), _I, _I, _I, _I, _I, _I, _c.c_float, _P, _I, _P, _I, _P]),
     "swq_q4_cache_bytes": (_SZ, [_I, _I, _I, _I]),
     "swq_q4_rope_table": (_I, [_I, _c.c_float, _I64, _I, _P]),
     "swq_q4_append": (_I, [_c.POINTER(AttentionLayer), _c.POINTER(Q4CacheDesc), _c.POINTER(Q4Batch), _P, _P, _I, _P]),

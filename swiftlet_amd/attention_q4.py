@@ -11,28 +11,8 @@ from __future__ import annotations
 import ctypes
 
 from . import _lib
-from ._lib import SWQ_BF16, SWQ_F32, AttentionLayer, Q4Batch, Q4CacheDesc, SwqError, check
-from .engine import GPULinear, HipEngine, _elsewhere, _stream_handle, _torch
-
-
-def _code(t, what):
-    torch = _torch()
-    if t.dtype == torch.float32:
-        return SWQ_F32
-    if t.dtype == torch.bfloat16:
-        return SWQ_BF16
-    raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, what)
-
-
-def _ptr(t, count, what, device, dtype=None):
-    """The address of a contiguous tensor of `count` elements (at least, for int32 arrays) on the cache's device."""
-    if t is None:
-        return None
-    if t.get_device() != device:
-        raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": not on the cache's device")
-    if not t.is_contiguous() or t.numel() < count or (dtype is not None and t.dtype != dtype):
-        raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
-    return t.data_ptr()
+from ._lib import AttentionLayer, Q4Batch, Q4CacheDesc, SwqError, check
+from .engine import GPULinear, HipEngine, _code, _elsewhere, _ptr, _stream_handle, _torch
 
 
 class Q4Cache:

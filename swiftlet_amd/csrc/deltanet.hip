@@ -27,7 +27,7 @@
 // Bound: a chain of round trips (the conv rows, then LDS hand-offs) over 141 KB per workgroup.
 // Step of 16 / 32 heads of 128: 6.2 us, 5.3 with the conv rows loaded at once, LDS-only
 // barriers and the norms' sums formed by every wave for itself.
-#include "internal.hpp"
+#include "deltanet.hpp"
 #include "route.hpp"
 
 namespace swq {
@@ -35,8 +35,6 @@ namespace {
 
 constexpr int kDnThreads = 512;
 constexpr int kDnWaves = kDnThreads / kWave;
-constexpr int kDnMaxDv = 1024;
-constexpr int kDnMaxConv = 8;
 
 struct DnArgs {
     const float *qkvz, *ba;
@@ -47,34 +45,6 @@ struct DnArgs {
     int32_t nk, nv, dk, dv, K, layout, rep, keyD, valD, convD, slot_new;
     float eps;
 };
-
-__device__ __forceinline__ float sigmoid_acc(float v) { return 1.0f / (1.0f + expf(-v)); }
-__device__ __forceinline__ float silu_acc(float v) { return v * sigmoid_acc(v); }
-
-// Mixed channel c ([q | k | v] order) of the token's projections.
-__device__ __forceinline__ float mixed_in(const DnArgs &a, int c) {
-    if (a.layout == SWQ_DELTA_SPLIT) return a.qkvz[c];
-    const int chunk = 2 * a.dk + 2 * a.rep * a.dv;
-    if (c < a.keyD) return a.qkvz[(c / a.dk) * chunk + c % a.dk];
-    if (c < 2 * a.keyD) {
-        const int t = c - a.keyD;
-        return a.qkvz[(t / a.dk) * chunk + a.dk + t % a.dk];
-    }
-    const int t = c - 2 * a.keyD, hv = t / a.dv, i = t % a.dv;
-    return a.qkvz[(hv / a.rep) * chunk + 2 * a.dk + (hv % a.rep) * a.dv + i];
-}
-
-__device__ __forceinline__ float z_in(const DnArgs &a, int hv, int i) {
-    if (a.layout == SWQ_DELTA_SPLIT) return a.qkvz[a.convD + hv * a.dv + i];
-    const int chunk = 2 * a.dk + 2 * a.rep * a.dv;
-    return a.qkvz[(hv / a.rep) * chunk + 2 * a.dk + a.rep * a.dv + (hv % a.rep) * a.dv + i];
-}
-
-// b (which = 0) or a (which = 1) of value head hv.
-__device__ __forceinline__ float ba_in(const DnArgs &a, int hv, int which) {
-    if (a.layout == SWQ_DELTA_SPLIT) return a.ba[which * a.nv + hv];
-    return a.ba[(hv / a.rep) * 2 * a.rep + which * a.rep + hv % a.rep];
-}
 
 // Sum of squares of n floats in LDS, by every wave for itself: no barrier, and the lanes meet by
 // DPP.
@@ -112,7 +82,7 @@ __global__ __launch_bounds__(kDnThreads) void deltanet_step_kernel(const DnArgs 
     // norm weight), which would otherwise cost a round trip at the end
     float z0 = 0.f, nw0 = 0.f;
     if (tid < a.dv) {
-        z0 = z_in(a, hv, tid);
+        z0 = a.qkvz[z_at(a, hv, tid)];
         nw0 = a.norm_w[tid];
     }
     asm volatile("" ::: "memory");
@@ -137,7 +107,7 @@ __global__ __launch_bounds__(kDnThreads) void deltanet_step_kernel(const DnArgs 
             dst = &s_v[t - 2 * DK];
             own = true;
         }
-        const float xn = mixed_in(a, c);
+        const float xn = a.qkvz[mixed_at(a, c)];
         const float *w = a.conv_w + static_cast<int64_t>(c) * a.K;
         float acc = 0.f;
         if (a.K == 4) {
@@ -160,12 +130,11 @@ __global__ __launch_bounds__(kDnThreads) void deltanet_step_kernel(const DnArgs 
         *dst = silu_acc(acc);
         if (own) a.ring[static_cast<int64_t>(a.slot_new) * a.convD + c] = xn;
     }
-    // 2. gates (delta_pre, softplus as log1p(exp(.)) below 20)
+    // 2. gates (delta_pre)
     if (tid == 0) {
-        const float av = ba_in(a, hv, 1) + a.dt_bias[hv];
-        const float sp = av > 20.f ? av : log1pf(expf(av));
+        const float sp = softplus_acc(a.ba[ba_at(a, hv, 1)] + a.dt_bias[hv]);
         s_gb[0] = expf(-expf(a.a_log[hv]) * sp);
-        s_gb[1] = sigmoid_acc(ba_in(a, hv, 0));
+        s_gb[1] = sigmoid_acc(a.ba[ba_at(a, hv, 0)]);
     }
     // only LDS is handed over, here and below: a full barrier would also wait for the ring's and
     // the state's stores
@@ -222,13 +191,13 @@ __global__ __launch_bounds__(kDnThreads) void deltanet_step_kernel(const DnArgs 
     const float sc = 1.0f / __fsqrt_rn(sso / static_cast<float>(a.dv) + a.eps);
     for (int i = tid; i < a.dv; i += kDnThreads) {
         const float y = s_o[i] * (sc * (i == tid ? nw0 : a.norm_w[i]));
-        a.out[hv * a.dv + i] = y * silu_acc(i == tid ? z0 : z_in(a, hv, i));
+        a.out[hv * a.dv + i] = y * silu_acc(i == tid ? z0 : a.qkvz[z_at(a, hv, i)]);
     }
 }
 
-inline size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+}  // namespace
 
-int check_layer(const swq_deltanet_layer *l) {
+int check_deltanet_layer(const swq_deltanet_layer *l) {
     if (!l) return SWQ_ERR_INVALID_ARGUMENT;
     if (l->reserved != 0) return SWQ_ERR_INVALID_ARGUMENT;
     if (l->num_key_heads <= 0 || l->num_value_heads <= 0 || l->num_value_heads % l->num_key_heads != 0)
@@ -243,25 +212,24 @@ int check_layer(const swq_deltanet_layer *l) {
     return SWQ_OK;
 }
 
-size_t ring_bytes(const swq_deltanet_layer *l) {
+size_t deltanet_ring_bytes(const swq_deltanet_layer *l) {
     const int64_t convD = 2LL * l->num_key_heads * l->key_head_dim + 1LL * l->num_value_heads * l->value_head_dim;
-    return align256(static_cast<size_t>(l->conv_kernel) * convD * 4);
+    return dn_align(static_cast<size_t>(l->conv_kernel) * convD * 4);
 }
 
-}  // namespace
 }  // namespace swq
 
 using namespace swq;
 
 extern "C" size_t swq_deltanet_state_bytes(const swq_deltanet_layer *l) {
-    if (check_layer(l) != SWQ_OK) return 0;
-    return ring_bytes(l) +
+    if (check_deltanet_layer(l) != SWQ_OK) return 0;
+    return deltanet_ring_bytes(l) +
            static_cast<size_t>(l->num_value_heads) * l->value_head_dim * l->key_head_dim * sizeof(float);
 }
 
 static int check_step(const swq_deltanet_layer *l, const float *qkvz, const float *ba, const void *state,
                       size_t state_bytes, int64_t position, const float *out) {
-    const int st = check_layer(l);
+    const int st = check_deltanet_layer(l);
     if (st != SWQ_OK) return st;
     if (!qkvz || !ba || !state || !out || position < 0) return SWQ_ERR_INVALID_ARGUMENT;
     if (state_bytes < swq_deltanet_state_bytes(l)) return SWQ_ERR_WORKSPACE;
@@ -283,7 +251,7 @@ extern "C" int swq_deltanet_step(const swq_deltanet_layer *l, const float *qkvz,
     a.dt_bias = l->dt_bias;
     a.norm_w = l->norm_weight;
     a.ring = static_cast<float *>(state);
-    a.state = reinterpret_cast<float *>(static_cast<uint8_t *>(state) + ring_bytes(l));
+    a.state = reinterpret_cast<float *>(static_cast<uint8_t *>(state) + deltanet_ring_bytes(l));
     a.out = out;
     a.nk = l->num_key_heads;
     a.nv = l->num_value_heads;
@@ -314,7 +282,7 @@ extern "C" int swq_deltanet_step(const swq_deltanet_layer *l, const float *qkvz,
 // instead of three (with the descriptors rebuilt for each, a token's block took ~40 us of host
 // time through ctypes, twice the device's 21 us).
 extern "C" size_t swq_deltanet_scratch_floats(const swq_deltanet_layer *l) {
-    if (check_layer(l) != SWQ_OK) return 0;
+    if (check_deltanet_layer(l) != SWQ_OK) return 0;
     const int64_t val = 1LL * l->num_value_heads * l->value_head_dim;
     const int64_t qkvz = 2LL * l->num_key_heads * l->key_head_dim + 2 * val;
     return static_cast<size_t>(pad_floats(qkvz) + pad_floats(2LL * l->num_value_heads) + val);
@@ -324,7 +292,7 @@ extern "C" int swq_deltanet_token(const swq_deltanet_layer *l, const swq_qlinear
                                   const swq_qlinear *out_proj, const float *x, const void *norm_weight,
                                   int norm_dtype, float norm_eps, void *state, size_t state_bytes, int64_t position,
                                   float *scratch, size_t scratch_floats, float *out, void *stream) {
-    int st = check_layer(l);
+    int st = check_deltanet_layer(l);
     if (st != SWQ_OK) return st;
     if (!projections || !out_proj || !scratch || !out) return SWQ_ERR_INVALID_ARGUMENT;
     const int64_t nv = l->num_value_heads, val = nv * l->value_head_dim;

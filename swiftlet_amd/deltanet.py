@@ -2,15 +2,26 @@
 projections (swq_encode_gemv), the decode step (swq_deltanet_step) and
 out_proj — QwenMetalModel.encDeltaLayer (QwenMetalModel.swift:989-1084) for
 one token, numerics of QwenCPUModel.deltaNetForward (QwenCPUModel.swift:
-371-496).  torch supplies device memory and streams only."""
+371-496); and the block between its projections for the tokens of many
+sequences (swq_deltanet_tokens), prompts (`prefill`) or one token each
+(`step_batch`).  torch supplies device memory and streams only."""
 
 from __future__ import annotations
 
 import ctypes
 
 from . import _lib
-from ._lib import SWQ_DELTA_INTERLEAVED, SWQ_DELTA_SPLIT, DeltaNetLayer, check
-from .engine import DescArray, GPULinear, HipEngine, _elsewhere, _norm_arg, _stream_handle, _torch, own_launches
+from ._lib import SWQ_DELTA_INTERLEAVED, SWQ_DELTA_SPLIT, DeltaNetBatch, DeltaNetLayer, SwqError, check
+from .engine import DescArray, GPULinear, HipEngine, _code, _elsewhere, _norm_arg, _ptr, _stream_handle, _torch, own_launches
+
+
+def _row_stride(t, rows, width, what, device):
+    """Elements between the rows of a tensor [rows, width] (or wider) whose rows are contiguous."""
+    if t.get_device() != device:
+        raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": not on the block's device")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.stride(1) != 1 or (rows > 1 and t.stride(0) < width):
+        raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
+    return t.stride(0) if rows > 1 else 0
 
 
 class DeltaNetGPU:
@@ -63,6 +74,74 @@ class DeltaNetGPU:
         ring = state[:self.K * self.conv_dim * 4].view(torch.float32).reshape(self.K, self.conv_dim)
         rec = state[ring_bytes:ring_bytes + self.nv * self.dv * self.dk * 4].view(torch.float32)
         return ring, rec.reshape(self.nv, self.dv, self.dk)
+
+    @property
+    def slot_bytes(self) -> int:
+        return self.lib.swq_deltanet_slot_bytes(ctypes.byref(self._c))
+
+    def new_states(self, slots: int):
+        """Fresh states (zeros) of `slots` sequences, as a flat uint8 device tensor."""
+        torch = _torch()
+        return torch.zeros(slots * self.slot_bytes, dtype=torch.uint8, device=self.conv_weight.device)
+
+    def states_views(self, states):
+        """(conv rings [slots, K, convD], recurrent states [slots, nv, dv, dk]) views of a buffer of many states."""
+        torch = _torch()
+        n, at = self.slot_bytes, (self.K * self.conv_dim * 4 + 255) // 256 * 256
+        slots = states.numel() // n
+        whole = states[:slots * n].view(slots, n)
+        return (whole[:, :self.K * self.conv_dim * 4].view(torch.float32).view(slots, self.K, self.conv_dim),
+                whole[:, at:at + self.nv * self.dv * self.dk * 4].view(torch.float32).view(slots, self.nv, self.dv, self.dk))
+
+    def new_batch_workspace(self, sequences: int, tokens: int | None = None, max_tokens: int | None = None):
+        """For calls of up to `sequences` sequences, `tokens` tokens (one each if not given) and
+        `max_tokens` of one sequence (any number of the call's if not given)."""
+        torch = _torch()
+        tokens = sequences if tokens is None else tokens
+        b = DeltaNetBatch(sequences=sequences, tokens=tokens, max_tokens=max_tokens or max(tokens, 1), slots=sequences, starts=1)
+        n = self.lib.swq_deltanet_tokens_workspace_bytes(ctypes.byref(self._c), ctypes.byref(b))
+        if n == 0:
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "deltanet_tokens_workspace_bytes")
+        return torch.empty(n, dtype=torch.uint8, device=self.conv_weight.device)
+
+    def prefill(self, qkvz, ba, states, positions, ws, starts=None, slots=None, max_tokens: int | None = None, out=None,
+                stream=None):
+        """The tokens of many sequences from their projection outputs (swq_deltanet_tokens): qkvz [N, convD +
+        nv*dv], ba [N, 2*nv], f32 or bf16, rows as far apart as they may be; returns out [N, nv*dv] of qkvz's
+        type and updates `states` (new_states).  positions (int32 device [B]): tokens in each state already.
+        starts (int32 device [B + 1]) where sequences bring different numbers of tokens, then max_tokens, the most
+        that one brings (default: N).  slots (int32 device [B]): each sequence's state, none twice; one that is out
+        of range leaves its sequence out (default: the b-th)."""
+        torch = _torch()
+        if out is None:
+            if stream is not None and _elsewhere(stream):
+                with torch.cuda.stream(stream):
+                    return self.prefill(qkvz, ba, states, positions, ws, starts, slots, max_tokens)
+            out = torch.empty((qkvz.shape[0], self.value_dim), dtype=qkvz.dtype, device=qkvz.device)
+        what, at, B, N = "deltanet_tokens", self.conv_weight.get_device(), positions.numel(), qkvz.shape[0]
+        if at < 0 or at != torch.cuda.current_device():
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": the block is not on the current device")
+        if ba.dtype != qkvz.dtype:
+            raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, what + ": ba")
+        if out.numel() != N * self.value_dim:
+            raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what + ": out")
+        b = DeltaNetBatch(B, N, max_tokens or max(N, 1), states.numel() // self.slot_bytes,
+                          _ptr(starts, B + 1, what + ": starts", at, torch.int32),
+                          _ptr(positions, 1, what + ": positions", at, torch.int32),
+                          _ptr(slots, B, what + ": slots", at, torch.int32),
+                          _row_stride(qkvz, N, self.conv_dim + self.value_dim, what + ": qkvz", at),
+                          _row_stride(ba, N, 2 * self.nv, what + ": ba", at), 0)
+        check(self.lib.swq_deltanet_tokens(
+            ctypes.byref(self._c), ctypes.byref(b), qkvz.data_ptr(), ba.data_ptr(), _code(qkvz, what),
+            _ptr(states, 1, what + ": states", at, torch.uint8), states.numel(), _ptr(out, 0, what + ": out", at), _code(out, what),
+            _ptr(ws, 1, what + ": ws", at, torch.uint8), ws.numel(), _stream_handle(stream)), what)
+        return out
+
+    def step_batch(self, qkvz, ba, states, positions, ws, slots=None, out=None, stream=None):
+        """One token of each of positions.numel() sequences, as `prefill`."""
+        if qkvz.shape[0] != positions.numel():
+            raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "deltanet_tokens: qkvz")
+        return self.prefill(qkvz, ba, states, positions, ws, None, slots, 1, out, stream)
 
     def step(self, qkvz, ba, state, position: int, out=None, stream=None):
         """One token from its projection outputs; returns the gated-normed

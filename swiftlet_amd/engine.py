@@ -52,6 +52,26 @@ def _norm_arg(weight):
     return {torch.float32: SWQ_F32, torch.float16: SWQ_F16, torch.bfloat16: SWQ_BF16}[weight.dtype], weight.data_ptr()
 
 
+def _code(t, what):
+    torch = _torch()
+    if t.dtype == torch.float32:
+        return SWQ_F32
+    if t.dtype == torch.bfloat16:
+        return SWQ_BF16
+    raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, what)
+
+
+def _ptr(t, count, what, device, dtype=None):
+    """The address of a contiguous tensor of `count` elements (at least, for int32 arrays) on `device`."""
+    if t is None:
+        return None
+    if t.get_device() != device:
+        raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": not on the device of the call")
+    if not t.is_contiguous() or t.numel() < count or (dtype is not None and t.dtype != dtype):
+        raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
+    return t.data_ptr()
+
+
 class DescArray:
     """The descriptors of several linears as one C array, rebuilt when one of them changed."""
 
