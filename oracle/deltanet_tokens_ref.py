@@ -23,7 +23,9 @@ def split_rows(qkvz, ba, nk, nv, dk, dv, split):
 
 def tokens(qkvz, ba, ring, state, position, conv_w, a_log, dt_bias, norm_w, nk, nv, dk, dv, eps, split):
     """T tokens of one sequence whose conv ring [K, convD] and matrices [nv, dv, dk] hold `position` tokens already.
-    Returns (y [T, nv * dv], ring, state), f64."""
+    Returns (y [T, nv * dv], ring, state), f64, and terms [T, nv * dv]: the size of what an output is the sum of where
+    tokens are taken 64 at a time, so with what multiplies the sum.  That is q S over dk for the state before the 64 (as it
+    has faded), and (q.k_j) d_j over the tokens since, each q.k_j itself a sum over dk; roots of the sums of squares."""
     mixed, z, b, a = split_rows(qkvz, ba, nk, nv, dk, dv, split)
     T, conv, rep = mixed.shape[0], mixed.shape[1], nv // nk
     w = conv_w.double().reshape(conv, -1)
@@ -41,11 +43,17 @@ def tokens(qkvz, ba, ring, state, position, conv_w, a_log, dt_bias, norm_w, nk, 
     v = x[:, 2 * nk * dk:].reshape(T, nv, dv)
     g = torch.exp(-torch.exp(a_log.double()) * torch.nn.functional.softplus(a + dt_bias.double(), threshold=40.0))
     beta = 1 / (1 + torch.exp(-b))
-    out = torch.empty((T, nv, dv), dtype=torch.float64, device=S.device)
+    out, terms = torch.empty((2, T, nv, dv), dtype=torch.float64, device=S.device)
     for t in range(T):
-        S = S * g[t][:, None, None]
+        if t % 64 == 0:
+            start, ks, ds = S, [], []
+        S, start, ks = S * g[t][:, None, None], start * g[t][:, None, None], [x * g[t][:, None] for x in ks]
         d = beta[t][:, None] * (v[t] - (S * k[t][:, None]).sum(-1))
         S = S + d[:, :, None] * k[t][:, None]
         out[t] = (S * q[t][:, None]).sum(-1)
-    y = out / torch.sqrt((out * out).mean(-1, keepdim=True) + eps) * norm_w.double()
-    return (y * z / (1 + torch.exp(-z))).reshape(T, nv * dv), ring, S
+        ks, ds = ks + [k[t]], ds + [d]
+        p = torch.stack(ks) * q[t]  # [tokens since, nv, dk]
+        size = (p.sum(-1).square() + p.square().sum(-1))[..., None] * torch.stack(ds).square()
+        terms[t] = ((start * q[t][:, None]).square().sum(-1) + size.sum(0)).sqrt()
+    lift = norm_w.double() * z / (1 + torch.exp(-z)) / torch.sqrt((out * out).mean(-1, keepdim=True) + eps)
+    return (out * lift).reshape(T, nv * dv), ring, S, (terms * lift.abs()).reshape(T, nv * dv)

@@ -83,6 +83,14 @@ struct DnTokens {
 
 inline size_t dn_align(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
+// Prompts, a chunk of tokens at a time (deltanet_chunks.hip): which heads are taken, the workspace of a call, its
+// launches.
+constexpr int kDnChunk = 64;
+bool deltanet_chunks_take(const swq_deltanet_layer *l);
+bool deltanet_chunks_fit(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens);  // launches of fewer than 2^32 work-items
+size_t deltanet_chunks_bytes(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens);
+void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_t s);
+
 int check_deltanet_layer(const swq_deltanet_layer *l);
 size_t deltanet_ring_bytes(const swq_deltanet_layer *l);
 

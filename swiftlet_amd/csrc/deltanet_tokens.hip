@@ -245,10 +245,16 @@ int check_sizes(const swq_deltanet_layer *l, const swq_deltanet_batch *b) {
     if (!b->slot && b->slots < b->sequences) return SWQ_ERR_BAD_SHAPE;
     // rows that 32 bits address, and launches of fewer than 2^32 work-items
     if (conv + val > INT32_MAX || (1LL << 32) / kTokThreads <= 1LL * b->sequences * l->num_value_heads ||
-        (1LL << 32) <= b->sequences * (conv + kRingThreads))
+        (1LL << 32) <= b->sequences * (conv + kRingThreads) || (deltanet_chunks_take(l) && !deltanet_chunks_fit(l, b->sequences, b->tokens)))
         return SWQ_ERR_LIMIT;
     return SWQ_OK;
 }
+
+// Most tokens of one sequence.
+int most_tokens(const swq_deltanet_batch *b) { return b->starts ? std::min(b->max_tokens, b->tokens) : b->tokens / b->sequences; }
+
+// From so many tokens of a sequence on it goes a chunk at a time.
+constexpr int kChunksFrom = 24;
 
 bool misaligned(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 
@@ -260,7 +266,8 @@ using namespace swq;
 extern "C" size_t swq_deltanet_slot_bytes(const swq_deltanet_layer *l) { return dn_align(swq_deltanet_state_bytes(l)); }
 
 extern "C" size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *l, const swq_deltanet_batch *b) {
-    return check_sizes(l, b) == SWQ_OK ? 256 : 0;
+    if (check_sizes(l, b) != SWQ_OK) return 0;
+    return most_tokens(b) >= kChunksFrom && deltanet_chunks_take(l) ? deltanet_chunks_bytes(l, b->sequences, b->tokens) : 256;
 }
 
 extern "C" int swq_deltanet_tokens(const swq_deltanet_layer *l, const swq_deltanet_batch *b, const void *qkvz, const void *ba, int dtype,
@@ -292,7 +299,7 @@ extern "C" int swq_deltanet_tokens(const swq_deltanet_layer *l, const swq_deltan
     a.slot = b->slot;
     a.B = b->sequences;
     a.N = b->tokens;
-    a.max_tokens = b->starts ? std::min(b->max_tokens, b->tokens) : b->tokens / b->sequences;
+    a.max_tokens = most_tokens(b);
     a.slots = b->slots;
     a.nk = l->num_key_heads;
     a.nv = l->num_value_heads;
@@ -308,7 +315,10 @@ extern "C" int swq_deltanet_tokens(const swq_deltanet_layer *l, const swq_deltan
     a.out_f32 = out_dtype == SWQ_F32;
     a.eps = l->norm_eps;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == SWQ_F32) launch_tokens_dk<float>(a, s);
+    // chunks are loaded and stored four elements at a time
+    const bool four = !misaligned(qkvz, 4 * in) && a.qkvz_stride % 4 == 0 && !misaligned(out, a.out_f32 ? 16 : 8);
+    if (a.max_tokens >= kChunksFrom && four && deltanet_chunks_take(l)) launch_deltanet_chunks(a, dtype == SWQ_F32, ws, s);
+    else if (dtype == SWQ_F32) launch_tokens_dk<float>(a, s);
     else launch_tokens_dk<uint16_t>(a, s);
     return launch_status();
 }
