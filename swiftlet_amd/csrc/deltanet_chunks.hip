@@ -123,50 +123,73 @@ __device__ __forceinline__ f4_t load4(const uint16_t *p) {
     return f4_t{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u)};
 }
 
-// A lane's token of one sequence: its place there, and where its and the earlier rows lie.
+// silu by the hardware's exponential and reciprocal: off by less than 2^-22 of the larger of 1 and the value.
+__device__ __forceinline__ float silu_hw(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504f)); }
+
+// Four bf16 or f32 numbers as they are loaded.
 template <typename T>
-struct Rows {
-    const T *x;         // the sequence's first row
-    const float *ring;
-    uint32_t pos;
-    int32_t tau, tokens;  // the token, and how many the sequence brings
+struct Four;
+template <>
+struct Four<float> {
+    f4_t v;
+    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const f4_t *>(p); }
+    __device__ __forceinline__ f4_t get() const { return v; }
+};
+template <>
+struct Four<uint16_t> {
+    uint2 u;
+    __device__ __forceinline__ void load(const uint16_t *p) { u = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ f4_t get() const {
+        return f4_t{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u)};
+    }
 };
 
-// Convolution and silu of 4 consecutive mixed channels from ch on, whose elements lie at `at`; zeros for a token that
-// the sequence does not have.
-template <bool K4, typename T>
-__device__ __forceinline__ f4_t conv4(const DnTokens &a, const Rows<T> &r, int at, int ch) {
-    const int K = K4 ? 4 : a.K;
-    f4_t acc = {0.f, 0.f, 0.f, 0.f};
-    auto row = [&](int j) { return min(max(r.tau - (K - 1) + j, 0), r.tokens - 1); };
-    auto earlier = [&](int j) { return load4(r.ring + static_cast<int64_t>((r.pos + static_cast<uint32_t>(r.tau + 1 + j)) % K) * a.convD + ch); };
-    auto add = [&](int e, float w, float v) { acc[e] = __fadd_rn(acc[e], __fmul_rn(w, v)); };
-    if constexpr (K4) {
-        f4_t v[4], w[4];
+// Convolution and silu of a tile of 16 tokens, N of them per lane from `tau` on (places in the sequence) and 4 mixed channels
+// from ch on, whose elements lie at `at`: a row's channels side by side over the lanes, a token's earlier rows in
+// registers.  Zeros for tokens that the sequence does not have.  KM: rows of the kernel that are held, 4 or 8; shorter
+// kernels have zero weights in front.
+template <int KM, int N, typename T>
+__device__ __forceinline__ void conv_tile(const DnTokens &a, const T *x, const float *ring, uint32_t pos, int tokens, int tau, int at, int ch, f4_t (&y)[N]) {
+    Four<T> rows[N + KM - 1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = load4(r.x + row(j) * a.qkvz_stride + at);
+    for (int i = 0; i < N + KM - 1; ++i) rows[i].load(x + min(max(tau + i - (KM - 1), 0), tokens - 1) * a.qkvz_stride + at);
+    f4_t w[KM];
+    if (KM == 4 && a.K == 4) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = load4(a.conv_w + 4 * (ch + e));
-        if (r.tau < 3) {
+        for (int e = 0; e < 4; ++e) {
+            const f4_t k = load4(a.conv_w + 4 * (ch + e));
 #pragma unroll
-            for (int j = 0; j < 3; ++j)
-                if (r.tau + j < 3) v[j] = earlier(j);
+            for (int j = 0; j < 4; ++j) w[j][e] = k[j];
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) add(e, w[e][j], v[j][e]);
     } else {
-        for (int j = 0; j < K; ++j) {
-            f4_t v = load4(r.x + row(j) * a.qkvz_stride + at);
-            if (r.tau + j < K - 1) v = earlier(j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) add(e, a.conv_w[static_cast<int64_t>(ch + e) * K + j], v[e]);
-        }
+        for (int j = 0; j < KM; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[j][e] = j >= KM - a.K ? a.conv_w[static_cast<int64_t>(ch + e) * a.K + j - (KM - a.K)] : 0.f;
+    }
+    f4_t win[KM];
+#pragma unroll
+    for (int j = 0; j < KM - 1; ++j) win[j + 1] = rows[j].get();
+    if (tau < KM - 1) {
+        // rows before the sequence's first, from its ring; those of zero weights are any
+#pragma unroll
+        for (int j = 0; j < KM - 1; ++j)
+            if (tau + j < KM - 1)
+                win[j + 1] = j >= KM - a.K ? load4(ring + static_cast<int64_t>((pos + static_cast<uint32_t>(tau + 1 + j - (KM - a.K))) % a.K) * a.convD + ch) : f4_t{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = r.tau < r.tokens ? silu_acc(acc[e]) : 0.f;
-    return acc;
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int j = 0; j < KM - 1; ++j) win[j] = win[j + 1];
+        win[KM - 1] = rows[i + KM - 1].get();
+        f4_t acc = w[0] * win[0];
+#pragma unroll
+        for (int j = 1; j < KM; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(w[j][e], win[j][e], acc[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[i][e] = tau + i < tokens ? silu_hw(acc[e]) : 0.f;
+    }
 }
 
 // Block (row tile, column tile) of a lower triangular matrix of 4 x 4 blocks of 16 x 16, rows 20 apart.
@@ -214,11 +237,11 @@ __device__ __forceinline__ void tri_invert(float *blk, int lane) {
 
 // One workgroup per (chunk, value head).  Waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query
 // tile, then P and the values while the others make T.
-template <int DK, bool HQ, bool K4, typename T>
-__global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const DnTokens a, const DnChunks w) {
+template <int DK, bool HQ, int KM, typename T>
+__global__ __launch_bounds__(kPrepThreads, 4) void deltanet_prepare_kernel(const DnTokens a, const DnChunks w) {
     constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1;
     __shared__ uint4 s_kv[kRowTiles * (kVBlock / 32) * 2 * kWave];  // keys by tokens; then values, transposed
-    __shared__ uint4 s_kt[DT * 2 * 2 * kWave];                      // keys, transposed
+    __shared__ uint4 s_kt[DT * 2 * 2 * kWave];                      // queries by tokens; then keys, transposed
     __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
     __shared__ double s_c[kC];
     __shared__ float s_beta[kC], s_grown[kC], s_max[8];
@@ -229,16 +252,20 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, g = lane >> 4;
     const int tokens = a.count(b), n0 = a.first(b), tile = wave & 3;
     const bool keys = wave < 4;
-    Rows<T> r{static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(a.state(b)), a.position(b), m * kC + tile * 16 + col, tokens};
+    const T *x0 = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride;
+    const float *ring = reinterpret_cast<const float *>(a.state(b));
+    const uint32_t pos = a.position(b);
+    const int v_base = 2 * a.keyD + hv * a.dv;
+    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 
-    // gates, and their logarithms' sums
+    // gates, and their logarithms' sums, in units of log 2
     if (wave == 0) {
         const int t = min(m * kC + lane, tokens - 1);
         const T *ba = static_cast<const T *>(a.ba) + (n0 + static_cast<int64_t>(t)) * a.ba_stride;
         const bool is = m * kC + lane < tokens;
         const float log_g = -expf(a.a_log[hv]) * softplus_acc(dn_load(ba, ba_at(a, hv, 1)) + a.dt_bias[hv]);
         // below 2^-149 a decay is 0 like any other, and sums stay exact beside it
-        double c = is ? static_cast<double>(fmaxf(log_g, -110.f)) : 0.0;
+        double c = is ? 1.4426950408889634 * static_cast<double>(fmaxf(log_g, -110.f)) : 0.0;
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
             const double up = __shfl_up(c, d, kWave);
@@ -246,60 +273,61 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
         }
         s_c[lane] = c;
         s_beta[lane] = is ? sigmoid_acc(dn_load(ba, ba_at(a, hv, 0))) : 0.f;
-        s_grown[lane] = expf(static_cast<float>(c));
+        const float grown = __builtin_amdgcn_exp2f(static_cast<float>(c));
+        s_grown[lane] = grown;
         const double last = __shfl(c, kWave - 1, kWave);
         float *decay = w.decay + (chunk * a.nv + hv) * 2 * kC;
-        decay[lane] = expf(static_cast<float>(c));
-        decay[kC + lane] = expf(static_cast<float>(last - c));
+        decay[lane] = grown;
+        decay[kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(last - c));
     }
 
-    // keys and queries, normalised
-    Op x[KS];
-    {
-        f4_t y[KS][2];
-        float ss = 0.f;
-        const int ch = (keys ? a.keyD : 0) + hk * DK + 4 * g, at = mixed_at(a, ch);
+    auto kv_at = [&](int t, int ks, int plane) { return ((t * KS + ks) * 2 + plane) * kWave; };
+    auto kt_at = [&](int dt, int ks, int plane) { return ((dt * 2 + ks) * 2 + plane) * kWave; };
+    // four tokens of four channels of a tile, transposed: `token` of the tile, `ch` of the operand's rows
+    auto put_transposed = [&](uint4 *to, int token, int ch, const f4_t *v) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int e = 32 * ks + 16 * half;
-                const f4_t v = conv4<K4>(a, r, at + e, ch + e);
-                ss += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
-                y[ks][half] = v;
-            }
-        ss += __shfl_xor(ss, 16, kWave);
-        ss += __shfl_xor(ss, 32, kWave);
-        const float inv = 1.0f / __fsqrt_rn(static_cast<float>(DK));
-        const float sc = inv / __fsqrt_rn(ss / static_cast<float>(DK) + 1e-6f);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x[ks] = op_of(y[ks][0] * sc, y[ks][1] * sc);
-    }
-    auto kv_at = [&](int t, int ks, int plane) { return ((t * KS + ks) * 2 + plane) * kWave + lane; };
-    auto kt_at = [&](int dt, int ks, int plane) { return ((dt * 2 + ks) * 2 + plane) * kWave + lane; };
-    // a tile's transpose: products with the columns of the identity, exact
-    h8_t one[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) one[half][j] = static_cast<_Float16>(j / 4 == half && 4 * g + j % 4 == col ? 1.f : 0.f);
-    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
-    auto transpose = [&](uint4 *to, int ks, const Op &v) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int plane = 0; plane < 2; ++plane) {
-                const f4_t d = mfma16(plane ? v.lo : v.hi, one[half], zero);
-                reinterpret_cast<uint2 *>(to + kt_at(2 * ks + half, tile >> 1, plane))[tile & 1] = as_u2(__builtin_convertvector(d, h4_t));
-            }
+        for (int e = 0; e < 4; ++e) {
+            h4_t hi, lo;
+            split4(f4_t{v[0][e], v[1][e], v[2][e], v[3][e]}, hi, lo);
+            uint2 *at = reinterpret_cast<uint2 *>(to + kt_at(ch / 16, tile >> 1, 0) + 16 * (token / 4) + ch % 16 + e) + (tile & 1);
+            at[0] = as_u2(hi);
+            at[2 * kWave] = as_u2(lo);
+        }
     };
+
+    // keys and queries, normalised: N tokens and 4 channels per lane
+    constexpr int N = DK / 16;
+    const int ch = 4 * (lane % (DK / 4)), t0 = N * (lane / (DK / 4));
+    f4_t y[N];
+    {
+        const int c = (keys ? a.keyD : 0) + hk * DK + ch;
+        conv_tile<KM, N>(a, x0, ring, pos, tokens, m * kC + 16 * tile + t0, mixed_at(a, c), c, y);
+        uint4 *to = keys ? s_kv : s_kt;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float ss = y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3];
+            ss = segment_sum(ss, DK / 4);
+            y[i] *= 1.0f / __fsqrt_rn(ss + DK * 1e-6f);
+            h4_t hi, lo;
+            split4(y[i], hi, lo);
+            uint2 *at = reinterpret_cast<uint2 *>(to + kv_at(tile, ch / 32, 0) + t0 + i + 16 * (ch % 16 / 4)) + ch / 16 % 2;
+            at[0] = as_u2(hi);
+            at[2 * kWave] = as_u2(lo);
+        }
+    }
+    // a wave reads its own tile back as operands, the queries' before keys take their place
+    asm volatile("" ::: "memory");
+    Op x[KS];
+    auto read_back = [&](const uint4 *from) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x[ks] = {as_h8(from[kv_at(tile, ks, 0) + lane]), as_h8(from[kv_at(tile, ks, 1) + lane])};
+    };
+    if (!keys) read_back(s_kt);
+    lds_barrier();
     if (keys) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            s_kv[kv_at(tile, ks, 0)] = as_u4(x[ks].hi);
-            s_kv[kv_at(tile, ks, 1)] = as_u4(x[ks].lo);
-            transpose(s_kt, ks, x[ks]);
-        }
+        for (int i = 0; i < N; i += 4) put_transposed(s_kt, t0 + i, ch, y + i);
+        read_back(s_kv);
     } else if (ri == 0) {
         uint4 *q = w.q + (chunk * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave + lane;
 #pragma unroll
@@ -308,16 +336,15 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
             if (HQ) q[(ks * PL + 1) * kWave] = as_u4(x[ks].lo);
         }
     }
-    lds_barrier();
 
     // k_i.k_j and k_j.q_i of the lower triangle's tiles
-    auto fade = [&](int i, int j) { return expf(static_cast<float>(s_c[i] - s_c[j])); };
+    auto fade = [&](int i, int j) { return __builtin_amdgcn_exp2f(static_cast<float>(s_c[i] - s_c[j])); };
     if (keys) {
         for (int jt = 0; jt <= tile; ++jt) {
             Acc acc;
             acc.clear();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) acc.add(x[ks].hi, x[ks].lo, as_h8(s_kv[kv_at(jt, ks, 0)]), as_h8(s_kv[kv_at(jt, ks, 1)]));
+            for (int ks = 0; ks < KS; ++ks) acc.add(x[ks].hi, x[ks].lo, as_h8(s_kv[kv_at(jt, ks, 0) + lane]), as_h8(s_kv[kv_at(jt, ks, 1) + lane]));
             f4_t d = acc.sum();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -342,8 +369,8 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
                 acc.clear();
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const h8_t kh = as_h8(s_kv[kv_at(jt, ks, 0)]);
-                    if constexpr (HQ) acc.add(kh, as_h8(s_kv[kv_at(jt, ks, 1)]), x[ks].hi, x[ks].lo);
+                    const h8_t kh = as_h8(s_kv[kv_at(jt, ks, 0) + lane]);
+                    if constexpr (HQ) acc.add(kh, as_h8(s_kv[kv_at(jt, ks, 1) + lane]), x[ks].hi, x[ks].lo);
                     else acc.main = mfma16(kh, x[ks].hi, acc.main);
                 }
                 d[half] = HQ ? acc.sum() : acc.main;
@@ -353,35 +380,33 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
                     d[half][e] = i >= j ? d[half][e] * fade(i, j) : 0.f;
                 }
             }
-            const Op v = op_of(d[0], d[1]);
-            p[ks2 * PL * kWave] = as_u4(v.hi);
-            if (HQ) p[(ks2 * PL + 1) * kWave] = as_u4(v.lo);
+            const Op o = op_of(d[0], d[1]);
+            p[ks2 * PL * kWave] = as_u4(o.hi);
+            if (HQ) p[(ks2 * PL + 1) * kWave] = as_u4(o.lo);
         }
     }
     lds_barrier();
 
     // T below the diagonal blocks, while waves 4 to 7 have the values
-    const int v_base = 2 * a.keyD + hv * a.dv;
-    f4_t y[kVBlock / 16];
+    constexpr int VN = kVBlock / 16;
+    const int vch = 4 * (lane % (kVBlock / 4)), vt0 = VN * (lane / (kVBlock / 4));
+    f4_t v[VN];
     auto values = [&](int c0) {  // columns c0 .. of this wave's tile, and their largest
         float most = 0.f;
+        const int c = v_base + min(c0 + vch, a.dv - 4);
+        conv_tile<KM, VN>(a, x0, ring, pos, tokens, m * kC + 16 * tile + vt0, mixed_at(a, c), c, v);
 #pragma unroll
-        for (int i = 0; i < kVBlock / 16; ++i) {
-            y[i] = zero;
-            if (c0 + 16 * i >= a.dv) continue;
-            const int ch = v_base + c0 + 16 * i + 4 * g;
-            y[i] = conv4<K4>(a, r, mixed_at(a, ch), ch);
+        for (int i = 0; i < VN; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(y[i][e]));
-        }
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[i][e]));
         most = wave_max_all(most);
         if (lane == 0) s_max[wave] = most;
     };
     if (keys) {
         if (wave < 2) {
             const int i = 2 * wave + 1, j = 2 * wave;
-            const f4_t v = tri_mul(s_t + tri(i, j), s_t + tri(j, j), lane, zero);
-            tri_put(s_t + tri(i, j), -tri_mul(s_t + tri(i, i), v, lane, zero), lane);
+            const f4_t t = tri_mul(s_t + tri(i, j), s_t + tri(j, j), lane, zero);
+            tri_put(s_t + tri(i, j), -tri_mul(s_t + tri(i, i), t, lane, zero), lane);
         }
     } else {
         values(0);
@@ -392,7 +417,9 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
     float v_scale = scale_of(vmax, v_inv);
     auto put_values = [&]() {
 #pragma unroll
-        for (int i = 0; i < kVBlock / 32; ++i) transpose(s_kv, i, op_of(y[2 * i] * v_scale, y[2 * i + 1] * v_scale));
+        for (int i = 0; i < VN; ++i) v[i] *= v_scale;
+#pragma unroll
+        for (int i = 0; i < VN; i += 4) put_transposed(s_kv, vt0 + i, vch, v + i);
     };
     if (wave < 2) {
         // columns of the lower left 32 x 32 part
@@ -418,7 +445,7 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
     Op tu[2], tw[2];
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
-        f4_t u[2], v[2];
+        f4_t u[2], e_u[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int jt = 2 * ks2 + half, j = 16 * jt + 4 * g;
@@ -426,11 +453,11 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 u[half][e] *= s_beta[j + e];
-                v[half][e] = u[half][e] * s_grown[j + e];
+                e_u[half][e] = u[half][e] * s_grown[j + e];
             }
         }
         tu[ks2] = op_of(u[0], u[1]);
-        tw[ks2] = op_of(v[0], v[1]);
+        tw[ks2] = op_of(e_u[0], e_u[1]);
     }
     const int half_of = wave >> 2, last = tile / 2;  // contraction steps past `last` are zeros
     {
@@ -446,7 +473,7 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
                 Acc acc;
                 acc.clear();
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
-                    const uint4 kh = s_kt[kt_at(dt, ks2, 0)], kl = s_kt[kt_at(dt, ks2, 1)];
+                    const uint4 kh = s_kt[kt_at(dt, ks2, 0) + lane], kl = s_kt[kt_at(dt, ks2, 1) + lane];
                     if (ks2 <= last) acc.add(as_h8(kh), as_h8(kl), tw[ks2].hi, tw[ks2].lo);
                     if (ri == 0 && (dt & 3) == tile) {
                         k_to[(dt * 2 + ks2) * 2 * kWave] = kh;
@@ -455,9 +482,9 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
                 }
                 d[half] = acc.sum();
             }
-            const Op v = op_of(d[0], d[1]);
-            to[ks * 2 * kWave] = as_u4(v.hi);
-            to[(ks * 2 + 1) * kWave] = as_u4(v.lo);
+            const Op o = op_of(d[0], d[1]);
+            to[ks * 2 * kWave] = as_u4(o.hi);
+            to[(ks * 2 + 1) * kWave] = as_u4(o.lo);
         }
     }
     f4_t *u_to = w.u + (chunk * a.nv + hv) * (a.dv / 16 * kRowTiles * kWave) + lane;
@@ -466,7 +493,7 @@ __global__ __launch_bounds__(kPrepThreads) void deltanet_prepare_kernel(const Dn
             Acc acc;
             acc.clear();
             for (int ks2 = 0; ks2 <= last; ++ks2)
-                acc.add(tu[ks2].hi, tu[ks2].lo, as_h8(s_kv[kt_at(i, ks2, 0)]), as_h8(s_kv[kt_at(i, ks2, 1)]));
+                acc.add(tu[ks2].hi, tu[ks2].lo, as_h8(s_kv[kt_at(i, ks2, 0) + lane]), as_h8(s_kv[kt_at(i, ks2, 1) + lane]));
             u_to[((c0 / 16 + i) * kRowTiles + tile) * kWave] = acc.sum() * v_inv;
         }
         c0 += kVBlock;
@@ -770,8 +797,8 @@ int64_t cap_of(int64_t sequences, int64_t tokens) { return tokens / kC + sequenc
 template <int DK, bool HQ, typename T>
 void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const dim3 grid(static_cast<uint32_t>(w.cap * a.nv)), block(kPrepThreads);
-    if (a.K == 4 && reinterpret_cast<uintptr_t>(a.conv_w) % 16 == 0) hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, true, T>), grid, block, 0, s, a, w);
-    else hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, false, T>), grid, block, 0, s, a, w);
+    if (a.K <= 4) hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, 4, T>), grid, block, 0, s, a, w);
+    else hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, 8, T>), grid, block, 0, s, a, w);
 }
 
 template <int DK, bool HQ>
