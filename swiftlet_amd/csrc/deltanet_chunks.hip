@@ -5,16 +5,18 @@
 //                            A_ij = b_i e^(c_i - c_j) k_i.k_j for i > j
 //   o = e^c (q S) + P d      P_ij = e^(c_i - c_j) q_i.k_j for i >= j
 //   S = e^c_last S + k^T (e^(c_last - c) d)
-// which is the token after token recurrence written out.  Three launches:
-//   prepare  per (chunk, value head), all chunks at once: convolution, norms, gates, A, T, W, U, P;
+// which is the token after token recurrence written out.  Four launches:
+//   keys     per (chunk, key head), all chunks at once: convolution and norms of k and q, k.k and k.q, gates;
+//   solve    per (chunk, value head), all chunks at once: convolution of v, A, T, W, U, P;
 //   chain    per (sequence, value head, 16 to 64 columns of S), chunk after chunk: d, o, S;
 //   finish   the gated norm, and the ring's rows.
 //
-// Numbers.  f32 numbers meet on the f16 matrix cores as two f16 numbers each, x = hi + lo / 2048 with lo = (x - hi) *
-// 2048, and three products (hi hi, and hi lo + lo hi in sums of their own): 22 bits.  k, q, W and T stay inside
-// f16's range by themselves: |k|, |q| <= 1, and b, g <= 1, so that a step of the rule lengthens nothing.  v, d and S do
-// not: a power of two per (sequence, head, column group), from the largest v and S, brings them to about 1; S
-// grows by sqrt(tokens) at most from there.  Sums are f32, c is summed and subtracted in 64 bits, and T is made by f32
+// Numbers.  f32 numbers meet on the f16 matrix cores as two f16 numbers each, x = hi + lo, and three products (hi hi, hi
+// lo, lo hi): 22 bits of what is large enough for lo to be a normal f16 number, 2^-25 of 1 below.  Powers of two keep
+// them there.  k, q, P and T are bounded by 1 and W by 8 (|k|, |q| <= 1 and b, g <= 1: a step of the rule lengthens
+// nothing) and take fixed ones.  v, d and S have no bound: one per (sequence, head, columns), from the largest v and
+// S, brings them to 32 .. 64, from where S grows by sqrt(tokens) at most, so past f16's largest only after 2^20
+// tokens that all agree.  Sums are f32, c is summed and subtracted in 64 bits, and T is made by f32
 // substitution and f32 matrix instructions.  Where projections and out are bf16, q S and P d take the high parts alone:
 // their terms are off by 2^-12, an eighth of what the projections' own rounding makes them.
 //
@@ -40,14 +42,18 @@ constexpr int kPrepThreads = 512;
 constexpr int kChainThreads = 512;
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
-constexpr float kLo = 2048.f, kLoInv = 1.f / 2048.f;
+// What operands are multiplied by; of d times e^(c_last - c), so that its product with k has S's own.
+constexpr float kScaleK = 256.f, kScaleT = 16.f, kScaleP = 256.f, kScaleE = 1.f / kScaleK;
 
 // The workspace: operands of every (chunk, key head) and (chunk, value head).
 struct DnChunks {
     uint4 *k, *q, *w, *p;  // f16 operands; k, w two planes, q, p `planes`
     f4_t *u;               // [chunk][nv][dv / 16][4][64]
-    float *decay;          // [chunk][nv][2][64]: e^c_i and e^(c_last - c_i)
+    float *decay;          // [chunk][nv][2][64]: e^c_i and kScaleE e^(c_last - c_i)
+    double *sums;          // [chunk][nv][64]: c, in units of log 2
+    float *beta;           // [chunk][nv][64]
     float *vmax;           // [chunk][nv]
+    f4_t *dots;            // [chunk][nk][2][10][64]: k_i.k_j and k_j.q_i, tiles of the lower triangle
     float *o;              // [N][nv * dv]: the outputs before their norm
     int32_t cap;           // chunks that there is room for
     int32_t planes;
@@ -64,7 +70,8 @@ __device__ __forceinline__ void here(f4_t &v) { asm volatile("" : "+v"(v)); }
 
 __device__ __forceinline__ void split4(f4_t x, h4_t &hi, h4_t &lo) {
     hi = __builtin_convertvector(x, h4_t);
-    lo = __builtin_convertvector((x - __builtin_convertvector(hi, f4_t)) * kLo, h4_t);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lo[e] = static_cast<_Float16>(fmaf(static_cast<float>(hi[e]), -1.0f, x[e]));
 }
 __device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ h8_t as_h8(uint4 u) { return __builtin_bit_cast(h8_t, u); }
@@ -81,23 +88,14 @@ __device__ __forceinline__ Op op_of(f4_t a, f4_t b) {
     split4(b, bh, bl);
     return {join(ah, bh), join(al, bl)};
 }
-// Products of 22-bit numbers: the high parts' sum and that of the mixed ones, 2048 times as large.
-struct Acc {
-    f4_t main, cross;
-    __device__ __forceinline__ void clear() { main = cross = f4_t{0.f, 0.f, 0.f, 0.f}; }
-    __device__ __forceinline__ void add(h8_t ah, h8_t al, h8_t bh, h8_t bl) {
-        main = mfma16(ah, bh, main);
-        cross = mfma16(ah, bl, cross);
-        cross = mfma16(al, bh, cross);
-    }
-    __device__ __forceinline__ f4_t sum() const { return main + cross * kLoInv; }
-};
+// c + a b in 22 bits.
+__device__ __forceinline__ f4_t mfma22(h8_t ah, h8_t al, h8_t bh, h8_t bl, f4_t c) { return mfma16(ah, bh, mfma16(ah, bl, mfma16(al, bh, c))); }
 
-// A power of two that brings m to 1 .. 2, and its inverse; 1 where m is 0 or no number.
+// A power of two that brings m to 32 .. 64, and its inverse; 32 where m is 0 or no number.
 __device__ __forceinline__ float scale_of(float m, float &inverse) {
-    int e = static_cast<int>((__float_as_uint(m) >> 23) & 255u);
-    if (e == 255 || !(m > 0.f)) e = 127;
-    e = min(max(e, 2), 252);
+    int e = static_cast<int>((__float_as_uint(m) >> 23) & 255u) - 5;
+    if (e >= 250 || !(m > 0.f)) e = 122;
+    e = max(e, 2);
     inverse = __uint_as_float(static_cast<uint32_t>(e) << 23);
     return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
@@ -144,15 +142,39 @@ struct Four<uint16_t> {
     }
 };
 
+// Sum over 16 or 32 consecutive lanes, to each of them.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += dpp<0xB1, 0xF, true>(v);   // quad_perm [1,0,3,2]
+    v += dpp<0x4E, 0xF, true>(v);   // quad_perm [2,3,0,1]
+    v += dpp<0x141, 0xF, true>(v);  // row_half_mirror
+    v += dpp<0x140, 0xF, true>(v);  // row_mirror
+    if constexpr (LANES == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 // Convolution and silu of a tile of 16 tokens, N of them per lane from `tau` on (places in the sequence) and 4 mixed channels
 // from ch on, whose elements lie at `at`: a row's channels side by side over the lanes, a token's earlier rows in
-// registers.  Zeros for tokens that the sequence does not have.  KM: rows of the kernel that are held, 4 or 8; shorter
-// kernels have zero weights in front.
+// registers.  Zeros for tokens that the sequence does not have.  tau0: the wave's first token.  KM: rows of the kernel that
+// are held, 4 or 8; shorter kernels have zero weights in front.
 template <int KM, int N, typename T>
-__device__ __forceinline__ void conv_tile(const DnTokens &a, const T *x, const float *ring, uint32_t pos, int tokens, int tau, int at, int ch, f4_t (&y)[N]) {
+__device__ __forceinline__ void conv_tile(const DnTokens &a, const T *x, const float *ring, uint32_t pos, int tokens, int tau0, int t0, int at, int ch,
+                                          f4_t (&y)[N]) {
     Four<T> rows[N + KM - 1];
+    const int tau = tau0 + t0;
+    if (tau0 >= KM - 1 && tau0 + 16 <= tokens) {
+        // the usual tile: a scalar address per row
+        const uint32_t off = static_cast<uint32_t>(t0) * static_cast<uint32_t>(a.qkvz_stride) + at;
+        const T *p = x + (tau0 - (KM - 1)) * a.qkvz_stride;
 #pragma unroll
-    for (int i = 0; i < N + KM - 1; ++i) rows[i].load(x + min(max(tau + i - (KM - 1), 0), tokens - 1) * a.qkvz_stride + at);
+        for (int i = 0; i < N + KM - 1; ++i, p += a.qkvz_stride) rows[i].load(p + off);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N + KM - 1; ++i) rows[i].load(x + min(max(tau + i - (KM - 1), 0), tokens - 1) * a.qkvz_stride + at);
+    }
     f4_t w[KM];
     if (KM == 4 && a.K == 4) {
 #pragma unroll
@@ -235,32 +257,97 @@ __device__ __forceinline__ void tri_invert(float *blk, int lane) {
     }
 }
 
-// One workgroup per (chunk, value head).  Waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query
-// tile, then P and the values while the others make T.
+// Where a lane puts or finds operands of a tile by tokens, [tile][contraction step][plane], and transposed.
+template <int DK>
+__device__ __forceinline__ constexpr int by_tokens(int tile, int ks, int plane) { return ((tile * (DK / 32) + ks) * 2 + plane) * kWave; }
+__device__ __forceinline__ constexpr int transposed(int dt, int ks2, int plane) { return ((dt * 2 + ks2) * 2 + plane) * kWave; }
+
+// N tokens from t0 of the tile and four channels from ch of the operand's rows, transposed, N a multiple of 4.
+template <int N>
+__device__ __forceinline__ void put_transposed(uint4 *to, int tile, int t0, int ch, const f4_t (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        uint2 *at = reinterpret_cast<uint2 *>(to + transposed(ch / 16, tile >> 1, 0) + 16 * ((t0 + i) / 4) + ch % 16) + (tile & 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            h4_t hi, lo;
+            split4(f4_t{v[i][e], v[i + 1][e], v[i + 2][e], v[i + 3][e]}, hi, lo);
+            at[2 * e] = as_u2(hi);
+            at[2 * (e + kWave)] = as_u2(lo);
+        }
+    }
+}
+
+// One workgroup per (chunk, key head): waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query tile; then
+// their products.  The gates of the key head's value heads beside it.
 template <int DK, bool HQ, int KM, typename T>
-__global__ __launch_bounds__(kPrepThreads, 4) void deltanet_prepare_kernel(const DnTokens a, const DnChunks w) {
-    constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1;
-    __shared__ uint4 s_kv[kRowTiles * (kVBlock / 32) * 2 * kWave];  // keys by tokens; then values, transposed
-    __shared__ uint4 s_kt[DT * 2 * 2 * kWave];                      // queries by tokens; then keys, transposed
-    __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
-    __shared__ double s_c[kC];
-    __shared__ float s_beta[kC], s_grown[kC], s_max[8];
-    const int hv = blockIdx.x % a.nv, hk = hv / a.rep, ri = hv % a.rep;
-    const int64_t chunk = blockIdx.x / a.nv;
+__global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const DnTokens a, const DnChunks w) {
+    constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = DK / 16;
+    __shared__ uint4 s_k[kRowTiles * KS * 2 * kWave];  // keys by tokens
+    __shared__ uint4 s_q[DT * 2 * 2 * kWave];          // queries by tokens; then keys, transposed
+    const int hk = blockIdx.x % a.nk;
+    const int64_t chunk = blockIdx.x / a.nk;
     int b, m;
     if (!find_chunk(a, static_cast<int>(chunk), b, m)) return;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int tokens = a.count(b), n0 = a.first(b), tile = wave & 3;
     const bool keys = wave < 4;
-    const T *x0 = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride;
-    const float *ring = reinterpret_cast<const float *>(a.state(b));
-    const uint32_t pos = a.position(b);
-    const int v_base = 2 * a.keyD + hv * a.dv;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 
+    // N tokens and 4 channels per lane, normalised
+    const int ch = 4 * (lane % (DK / 4)), t0 = N * (lane / (DK / 4));
+    f4_t y[N];
+    {
+        const int c = (keys ? a.keyD : 0) + hk * DK + ch, head = a.layout == SWQ_DELTA_SPLIT ? hk * DK + (keys ? a.keyD : 0) : hk * (2 * DK + 2 * a.rep * a.dv) + (keys ? DK : 0);
+        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(a.state(b)), a.position(b), tokens, m * kC + 16 * tile,
+                         t0, head + ch, c, y);
+        uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0) + t0 + 16 * (ch % 16 / 4)) + ch / 16 % 2;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float ss = lanes_sum<DK / 4>(y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3]);
+            y[i] *= kScaleK * __builtin_amdgcn_rsqf(ss + DK * 1e-6f);
+            h4_t hi, lo;
+            split4(y[i], hi, lo);
+            to[2 * i] = as_u2(hi);
+            to[2 * (i + kWave)] = as_u2(lo);
+        }
+    }
+    // a wave reads its own tile back as operands, the queries' before keys take their place
+    asm volatile("" ::: "memory");
+    Op x[KS];
+    auto read_back = [&](const uint4 *from) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x[ks] = {as_h8(from[by_tokens<DK>(tile, ks, 0) + lane]), as_h8(from[by_tokens<DK>(tile, ks, 1) + lane])};
+    };
+    if (!keys) read_back(s_q);
+    lds_barrier();
+    if (keys) {
+        put_transposed(s_q, tile, t0, ch, y);
+        read_back(s_k);
+    } else {
+        uint4 *q = w.q + (chunk * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave + lane;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            q[ks * PL * kWave] = as_u4(x[ks].hi);
+            if (HQ) q[(ks * PL + 1) * kWave] = as_u4(x[ks].lo);
+        }
+    }
+    // k_i.k_j and k_j.q_i of the lower triangle's tiles, as the results lie
+    f4_t *dots = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
+    for (int jt = 0; jt <= tile; ++jt) {
+        f4_t d = zero;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const h8_t kh = as_h8(s_k[by_tokens<DK>(jt, ks, 0) + lane]), kl = as_h8(s_k[by_tokens<DK>(jt, ks, 1) + lane]);
+            d = keys ? mfma22(x[ks].hi, x[ks].lo, kh, kl, d) : mfma22(kh, kl, x[ks].hi, x[ks].lo, d);
+        }
+        d *= 1.f / (kScaleK * kScaleK);
+        here(d);
+        dots[jt * kWave] = d;
+    }
     // gates, and their logarithms' sums, in units of log 2
-    if (wave == 0) {
-        const int t = min(m * kC + lane, tokens - 1);
+    for (int r = wave; r < a.rep; r += kPrepThreads / kWave) {
+        const int hv = hk * a.rep + r, t = min(m * kC + lane, tokens - 1);
         const T *ba = static_cast<const T *>(a.ba) + (n0 + static_cast<int64_t>(t)) * a.ba_stride;
         const bool is = m * kC + lane < tokens;
         const float log_g = -expf(a.a_log[hv]) * softplus_acc(dn_load(ba, ba_at(a, hv, 1)) + a.dt_bias[hv]);
@@ -271,173 +358,142 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_prepare_kernel(const
             const double up = __shfl_up(c, d, kWave);
             if (lane >= d) c += up;
         }
-        s_c[lane] = c;
-        s_beta[lane] = is ? sigmoid_acc(dn_load(ba, ba_at(a, hv, 0))) : 0.f;
-        const float grown = __builtin_amdgcn_exp2f(static_cast<float>(c));
-        s_grown[lane] = grown;
         const double last = __shfl(c, kWave - 1, kWave);
-        float *decay = w.decay + (chunk * a.nv + hv) * 2 * kC;
-        decay[lane] = grown;
-        decay[kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(last - c));
+        const int64_t head = chunk * a.nv + hv;
+        w.sums[head * kC + lane] = c;
+        w.beta[head * kC + lane] = is ? sigmoid_acc(dn_load(ba, ba_at(a, hv, 0))) : 0.f;
+        w.decay[head * 2 * kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(c));
+        w.decay[head * 2 * kC + kC + lane] = kScaleE * __builtin_amdgcn_exp2f(static_cast<float>(last - c));
     }
+    lds_barrier();
+    uint4 *k_to = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave);
+#pragma unroll
+    for (int i = 0; i < DT * 2 * 2 * kWave / kPrepThreads; ++i) k_to[i * kPrepThreads + tid] = s_q[i * kPrepThreads + tid];
+}
 
-    auto kv_at = [&](int t, int ks, int plane) { return ((t * KS + ks) * 2 + plane) * kWave; };
-    auto kt_at = [&](int dt, int ks, int plane) { return ((dt * 2 + ks) * 2 + plane) * kWave; };
-    // four tokens of four channels of a tile, transposed: `token` of the tile, `ch` of the operand's rows
-    auto put_transposed = [&](uint4 *to, int token, int ch, const f4_t *v) {
+// One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.
+template <int DK, bool HQ, int KM, typename T>
+__global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const DnTokens a, const DnChunks w) {
+    constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = kVBlock / 16;
+    __shared__ uint4 s_v[kVBlock / 16 * 2 * 2 * kWave];  // values, transposed
+    __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
+    __shared__ float s_max[4];
+    const int hv = blockIdx.x % a.nv, hk = hv / a.rep;
+    const int64_t chunk = blockIdx.x / a.nv, head = chunk * a.nv + hv;
+    int b, m;
+    if (!find_chunk(a, static_cast<int>(chunk), b, m)) return;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
+    const int tokens = a.count(b), n0 = a.first(b), tile = wave & 3;
+    const bool keys = wave < 4;
+    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+    const double *c = w.sums + head * kC;
+    const float *beta = w.beta + head * kC, *decay = w.decay + head * 2 * kC;
+    const f4_t *dots = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
+
+    const int ch = 4 * (lane % (kVBlock / 4)), t0 = N * (lane / (kVBlock / 4));
+    f4_t v[N];
+    auto values = [&](int c0) {  // columns c0 .. of this wave's tile, and their largest
+        const int off = min(c0 + ch, a.dv - 4), v_at = a.layout == SWQ_DELTA_SPLIT ? 2 * a.keyD + hv * a.dv : hk * (2 * DK + 2 * a.rep * a.dv) + 2 * DK + (hv - hk * a.rep) * a.dv;
+        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(a.state(b)), a.position(b), tokens, m * kC + 16 * tile,
+                         t0, v_at + off, 2 * a.keyD + hv * a.dv + off, v);
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[i][e]));
+        most = wave_max_all(most);
+        if (lane == 0) s_max[tile] = most;
+    };
+    // e^(c_i - c_j) is a row's share times a column's about the tile's first row, both at most 1; within the diagonal
+    // tile it is taken as it is
+    auto pow2 = [](double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); };
+    const double mid = c[16 * tile];
+    if (keys) {
+        double ci[4];
+        float bi[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            h4_t hi, lo;
-            split4(f4_t{v[0][e], v[1][e], v[2][e], v[3][e]}, hi, lo);
-            uint2 *at = reinterpret_cast<uint2 *>(to + kt_at(ch / 16, tile >> 1, 0) + 16 * (token / 4) + ch % 16 + e) + (tile & 1);
-            at[0] = as_u2(hi);
-            at[2 * kWave] = as_u2(lo);
+            ci[e] = c[16 * tile + 4 * g + e];
+            bi[e] = beta[16 * tile + 4 * g + e];
         }
-    };
-
-    // keys and queries, normalised: N tokens and 4 channels per lane
-    constexpr int N = DK / 16;
-    const int ch = 4 * (lane % (DK / 4)), t0 = N * (lane / (DK / 4));
-    f4_t y[N];
-    {
-        const int c = (keys ? a.keyD : 0) + hk * DK + ch;
-        conv_tile<KM, N>(a, x0, ring, pos, tokens, m * kC + 16 * tile + t0, mixed_at(a, c), c, y);
-        uint4 *to = keys ? s_kv : s_kt;
+        for (int jt = 0; jt < tile; ++jt) {
+            f4_t d = dots[jt * kWave] * pow2(mid - c[16 * jt + col]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float ss = y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3];
-            ss = segment_sum(ss, DK / 4);
-            y[i] *= 1.0f / __fsqrt_rn(ss + DK * 1e-6f);
-            h4_t hi, lo;
-            split4(y[i], hi, lo);
-            uint2 *at = reinterpret_cast<uint2 *>(to + kv_at(tile, ch / 32, 0) + t0 + i + 16 * (ch % 16 / 4)) + ch / 16 % 2;
-            at[0] = as_u2(hi);
-            at[2 * kWave] = as_u2(lo);
-        }
-    }
-    // a wave reads its own tile back as operands, the queries' before keys take their place
-    asm volatile("" ::: "memory");
-    Op x[KS];
-    auto read_back = [&](const uint4 *from) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x[ks] = {as_h8(from[kv_at(tile, ks, 0) + lane]), as_h8(from[kv_at(tile, ks, 1) + lane])};
-    };
-    if (!keys) read_back(s_kt);
-    lds_barrier();
-    if (keys) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) put_transposed(s_kt, t0 + i, ch, y + i);
-        read_back(s_kv);
-    } else if (ri == 0) {
-        uint4 *q = w.q + (chunk * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave + lane;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            q[ks * PL * kWave] = as_u4(x[ks].hi);
-            if (HQ) q[(ks * PL + 1) * kWave] = as_u4(x[ks].lo);
-        }
-    }
-
-    // k_i.k_j and k_j.q_i of the lower triangle's tiles
-    auto fade = [&](int i, int j) { return __builtin_amdgcn_exp2f(static_cast<float>(s_c[i] - s_c[j])); };
-    if (keys) {
-        for (int jt = 0; jt <= tile; ++jt) {
-            Acc acc;
-            acc.clear();
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) acc.add(x[ks].hi, x[ks].lo, as_h8(s_kv[kv_at(jt, ks, 0) + lane]), as_h8(s_kv[kv_at(jt, ks, 1) + lane]));
-            f4_t d = acc.sum();
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 16 * tile + 4 * g + e, j = 16 * jt + col;
-                d[e] = i > j ? d[e] * s_beta[i] * fade(i, j) : 0.f;
-            }
+            for (int e = 0; e < 4; ++e) d[e] *= bi[e] * pow2(ci[e] - mid);
             tri_put(s_t + tri(tile, jt), d, lane);
         }
+        f4_t d = dots[tile * kWave];
+        const double cj = c[16 * tile + col];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = 4 * g + e > col ? d[e] * bi[e] * pow2(ci[e] - cj) : 0.f;
+        tri_put(s_t + tri(tile, tile), d, lane);
         // the diagonal block's inverse, by the wave that has just written it
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         tri_invert(s_t + tri(tile, tile), lane);
     } else {
-        uint4 *p = w.p + (chunk * a.nv + hv) * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave + lane;
-        for (int ks2 = 0; ks2 <= tile / 2; ++ks2) {
+        const double ci = c[16 * tile + col];
+        const float row = kScaleP * pow2(ci - mid);
+        uint4 *p = w.p + head * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave + lane;
+#pragma unroll
+        for (int ks2 = 0; ks2 < 2; ++ks2) {
             f4_t d[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int jt = 2 * ks2 + half;
-                d[half] = zero;
-                if (jt > tile) continue;
-                Acc acc;
-                acc.clear();
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const h8_t kh = as_h8(s_kv[kv_at(jt, ks, 0) + lane]);
-                    if constexpr (HQ) acc.add(kh, as_h8(s_kv[kv_at(jt, ks, 1) + lane]), x[ks].hi, x[ks].lo);
-                    else acc.main = mfma16(kh, x[ks].hi, acc.main);
-                }
-                d[half] = HQ ? acc.sum() : acc.main;
+                d[half] = dots[min(jt, tile) * kWave];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 16 * tile + col, j = 16 * jt + 4 * g + e;
-                    d[half][e] = i >= j ? d[half][e] * fade(i, j) : 0.f;
+                    const int j = 16 * jt + 4 * g + e;
+                    const float share = jt < tile ? row * pow2(mid - c[j]) : kScaleP * pow2(ci - c[j]);
+                    d[half][e] = 16 * tile + col >= j ? d[half][e] * share : 0.f;
                 }
             }
             const Op o = op_of(d[0], d[1]);
             p[ks2 * PL * kWave] = as_u4(o.hi);
             if (HQ) p[(ks2 * PL + 1) * kWave] = as_u4(o.lo);
         }
-    }
-    lds_barrier();
-
-    // T below the diagonal blocks, while waves 4 to 7 have the values
-    constexpr int VN = kVBlock / 16;
-    const int vch = 4 * (lane % (kVBlock / 4)), vt0 = VN * (lane / (kVBlock / 4));
-    f4_t v[VN];
-    auto values = [&](int c0) {  // columns c0 .. of this wave's tile, and their largest
-        float most = 0.f;
-        const int c = v_base + min(c0 + vch, a.dv - 4);
-        conv_tile<KM, VN>(a, x0, ring, pos, tokens, m * kC + 16 * tile + vt0, mixed_at(a, c), c, v);
-#pragma unroll
-        for (int i = 0; i < VN; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[i][e]));
-        most = wave_max_all(most);
-        if (lane == 0) s_max[wave] = most;
-    };
-    if (keys) {
-        if (wave < 2) {
-            const int i = 2 * wave + 1, j = 2 * wave;
-            const f4_t t = tri_mul(s_t + tri(i, j), s_t + tri(j, j), lane, zero);
-            tri_put(s_t + tri(i, j), -tri_mul(s_t + tri(i, i), t, lane, zero), lane);
-        }
-    } else {
         values(0);
     }
     lds_barrier();
-    float vmax = fmaxf(fmaxf(s_max[4], s_max[5]), fmaxf(s_max[6], s_max[7]));
-    float v_inv;
+
+    // T below the diagonal blocks, 16 x 16 and then 32 x 32, while waves 4 to 7 put the values
+    float vmax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), v_inv;
     float v_scale = scale_of(vmax, v_inv);
     auto put_values = [&]() {
 #pragma unroll
-        for (int i = 0; i < VN; ++i) v[i] *= v_scale;
-#pragma unroll
-        for (int i = 0; i < VN; i += 4) put_transposed(s_kv, vt0 + i, vch, v + i);
+        for (int i = 0; i < N; ++i) v[i] *= v_scale;
+        put_transposed(s_v, tile, t0, ch, v);
     };
+    float low[2][2][4];  // blocks (2 .. 3, 0 .. 1) of A as operands, before another wave's results take their places
     if (wave < 2) {
-        // columns of the lower left 32 x 32 part
-        const int q = wave;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) low[i][j][s] = tri_a(s_t + tri(2 + i, j), lane, s);
+        const int i = 2 * wave + 1, j = 2 * wave;
+        const f4_t t = tri_mul(s_t + tri(i, j), s_t + tri(j, j), lane, zero);
+        tri_put(s_t + tri(i, j), -tri_mul(s_t + tri(i, i), t, lane, zero), lane);
+    } else if (!keys) {
+        put_values();
+    }
+    lds_barrier();
+    if (wave < 2) {
+        const int q = wave;  // a column of blocks
         f4_t x2 = zero, x3 = zero;
-        for (int s = q; s < 2; ++s) {
-            x2 = tri_mul(s_t + tri(2, s), s_t + tri(s, q), lane, x2);
-            x3 = tri_mul(s_t + tri(3, s), s_t + tri(s, q), lane, x3);
+        for (int j = q; j < 2; ++j) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float t = tri_b(s_t + tri(j, q), lane, s);
+                x2 = mfma4(j ? low[0][1][s] : low[0][0][s], t, x2);
+                x3 = mfma4(j ? low[1][1][s] : low[1][0][s], t, x3);
+            }
         }
-        const f4_t t2 = -tri_mul(s_t + tri(2, 2), x2, lane, zero);
-        const f4_t t3 = -tri_mul(s_t + tri(3, 3), x3, lane, tri_mul(s_t + tri(3, 2), x2, lane, zero));
-        // the blocks are read by this wave (and, of the first column, by the other) until here
-        lds_barrier();
-        tri_put(s_t + tri(2, q), t2, lane);
-        tri_put(s_t + tri(3, q), t3, lane);
-    } else {
-        if (!keys) put_values();
-        lds_barrier();
+        here(x2);
+        here(x3);
+        tri_put(s_t + tri(2, q), -tri_mul(s_t + tri(2, 2), x2, lane, zero), lane);
+        tri_put(s_t + tri(3, q), -tri_mul(s_t + tri(3, 3), x3, lane, tri_mul(s_t + tri(3, 2), x2, lane, zero)), lane);
     }
     lds_barrier();
 
@@ -449,52 +505,43 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_prepare_kernel(const
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int jt = 2 * ks2 + half, j = 16 * jt + 4 * g;
-            u[half] = jt <= tile ? *reinterpret_cast<const f4_t *>(s_t + tri(tile, jt) + col * kTriRow + 4 * g) : zero;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                u[half][e] *= s_beta[j + e];
-                e_u[half][e] = u[half][e] * s_grown[j + e];
-            }
+            u[half] = *reinterpret_cast<const f4_t *>(s_t + tri(tile, min(jt, tile)) + col * kTriRow + 4 * g) * (jt <= tile ? kScaleT : 0.f);
+            u[half] *= load4(beta + j);
+            e_u[half] = u[half] * load4(decay + j);
         }
         tu[ks2] = op_of(u[0], u[1]);
         tw[ks2] = op_of(e_u[0], e_u[1]);
     }
-    const int half_of = wave >> 2, last = tile / 2;  // contraction steps past `last` are zeros
+    const int half_of = wave >> 2;
     {
-        uint4 *to = w.w + (chunk * a.nv + hv) * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
-        uint4 *k_to = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave) + lane;
+        uint4 *to = w.w + head * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
+        const uint4 *k = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave) + lane;
 #pragma unroll
         for (int i = 0; i < KS / 2; ++i) {
             const int ks = half_of * (KS / 2) + i;
-            f4_t d[2];
+            f4_t d[2] = {zero, zero};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int dt = 2 * ks + half;
-                Acc acc;
-                acc.clear();
-                for (int ks2 = 0; ks2 < 2; ++ks2) {
-                    const uint4 kh = s_kt[kt_at(dt, ks2, 0) + lane], kl = s_kt[kt_at(dt, ks2, 1) + lane];
-                    if (ks2 <= last) acc.add(as_h8(kh), as_h8(kl), tw[ks2].hi, tw[ks2].lo);
-                    if (ri == 0 && (dt & 3) == tile) {
-                        k_to[(dt * 2 + ks2) * 2 * kWave] = kh;
-                        k_to[((dt * 2 + ks2) * 2 + 1) * kWave] = kl;
-                    }
-                }
-                d[half] = acc.sum();
-            }
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int ks2 = 0; ks2 < 2; ++ks2)
+                    d[half] = mfma22(as_h8(k[transposed(2 * ks + half, ks2, 0)]), as_h8(k[transposed(2 * ks + half, ks2, 1)]), tw[ks2].hi, tw[ks2].lo, d[half]);
             const Op o = op_of(d[0], d[1]);
             to[ks * 2 * kWave] = as_u4(o.hi);
             to[(ks * 2 + 1) * kWave] = as_u4(o.lo);
         }
     }
-    f4_t *u_to = w.u + (chunk * a.nv + hv) * (a.dv / 16 * kRowTiles * kWave) + lane;
+    f4_t *u_to = w.u + head * (a.dv / 16 * kRowTiles * kWave) + lane;
     for (int c0 = 0;;) {
-        for (int i = half_of; i < kVBlock / 16 && c0 + 16 * i < a.dv; i += 2) {
-            Acc acc;
-            acc.clear();
-            for (int ks2 = 0; ks2 <= last; ++ks2)
-                acc.add(tu[ks2].hi, tu[ks2].lo, as_h8(s_kv[kt_at(i, ks2, 0) + lane]), as_h8(s_kv[kt_at(i, ks2, 1) + lane]));
-            u_to[((c0 / 16 + i) * kRowTiles + tile) * kWave] = acc.sum() * v_inv;
+#pragma unroll
+        for (int i = 0; i < kVBlock / 32; ++i) {
+            const int ct = 2 * i + half_of;
+            f4_t d = zero;
+#pragma unroll
+            for (int ks2 = 0; ks2 < 2; ++ks2)
+                d = mfma22(tu[ks2].hi, tu[ks2].lo, as_h8(s_v[transposed(ct, ks2, 0) + lane]), as_h8(s_v[transposed(ct, ks2, 1) + lane]), d);
+            d *= v_inv * (1.f / kScaleT);
+            here(d);
+            if (c0 + 16 * ct < a.dv) u_to[((c0 / 16 + ct) * kRowTiles + tile) * kWave] = d;
         }
         c0 += kVBlock;
         if (c0 >= a.dv) break;
@@ -502,13 +549,13 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_prepare_kernel(const
         lds_barrier();
         if (!keys) values(c0);
         lds_barrier();
-        const float now = fmaxf(fmaxf(s_max[4], s_max[5]), fmaxf(s_max[6], s_max[7]));
+        const float now = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
         vmax = fmaxf(vmax, now);
         v_scale = scale_of(now, v_inv);
         if (!keys) put_values();
         lds_barrier();
     }
-    if (tid == 0) w.vmax[chunk * a.nv + hv] = vmax;
+    if (tid == 0) w.vmax[head] = vmax;
 }
 
 // One workgroup per (sequence, value head, CT * 16 columns of the state).  Waves 0 to 3 hold the state's rows and make
@@ -607,12 +654,11 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
             const bool more = m + 1 < chunks;
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                Acc acc;
-                acc.clear();
+                f4_t acc = zero;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
-                    acc.add(as_h8(wr[ks][0]), as_h8(wr[ks][1]), as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]), as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]));
-                const f4_t d = ur[c] * scale - acc.sum();
+                    acc = mfma22(as_h8(wr[ks][0]), as_h8(wr[ks][1]), as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]), as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), acc);
+                const f4_t d = ur[c] * scale - acc * (1.f / (kScaleT * kScaleK));
                 h4_t hi, lo;
                 split4(d, hi, lo);
                 reinterpret_cast<uint2 *>(s_d + ((c * 2 + tile / 2) * PL) * kWave + lane)[tile & 1] = as_u2(hi);
@@ -635,12 +681,9 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
                     for (int p = 0; p < 2; ++p) e[ks2][p] = as_h8(s_e[((c * 2 + ks2) * 2 + p) * kWave + lane]);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    Acc acc;
-                    acc.main = st[t][c] * keep;
-                    acc.cross = zero;
+                    st[t][c] *= keep;
 #pragma unroll
-                    for (int ks2 = 0; ks2 < 2; ++ks2) acc.add(as_h8(kr[t][ks2][0]), as_h8(kr[t][ks2][1]), e[ks2][0], e[ks2][1]);
-                    st[t][c] = acc.sum();
+                    for (int ks2 = 0; ks2 < 2; ++ks2) st[t][c] = mfma22(as_h8(kr[t][ks2][0]), as_h8(kr[t][ks2][1]), e[ks2][0], e[ks2][1], st[t][c]);
                 }
             }
             kp += more ? k_step : 0;
@@ -658,7 +701,6 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
         const float *dp = w.decay + (first * a.nv + hv) * 2 * kC;
         const int64_t q_step = static_cast<int64_t>(a.nk) * kRowTiles * KS * PL * kWave, p_step = static_cast<int64_t>(a.nv) * kRowTiles * 2 * PL * kWave,
                       d_step = static_cast<int64_t>(a.nv) * 2 * kC;
-        const int last = tile / 2;
         uint4 qr[KS][PL], pr[2][PL];
         f4_t grown;
         auto load_q = [&]() {
@@ -672,11 +714,11 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) pr[ks2][p] = ks2 <= last ? pp[(ks2 * PL + p) * kWave] : make_uint4(0, 0, 0, 0);
+                for (int p = 0; p < PL; ++p) pr[ks2][p] = pp[(ks2 * PL + p) * kWave];
         };
         load_q();
         load_p();
-        const float back = inverse / __fsqrt_rn(static_cast<float>(DK));
+        const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
         float *o = w.o + (n0 + 16 * tile + 4 * g) * a.nv * a.dv + hv * a.dv + c0 + col;
         for (int m = 0; m < chunks; ++m) {
             lds_barrier();
@@ -684,15 +726,14 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
             f4_t part[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                Acc acc;
-                acc.clear();
+                part[c] = zero;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const h8_t sh = as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]);
-                    if constexpr (HQ) acc.add(as_h8(qr[ks][0]), as_h8(qr[ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]));
-                    else acc.main = mfma16(as_h8(qr[ks][0]), sh, acc.main);
+                    if constexpr (HQ) part[c] = mfma22(as_h8(qr[ks][0]), as_h8(qr[ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), part[c]);
+                    else part[c] = mfma16(as_h8(qr[ks][0]), sh, part[c]);
                 }
-                part[c] = (HQ ? acc.sum() : acc.main) * grown;
+                part[c] *= grown;
             }
             qp += more ? q_step : 0;
             dp += more ? d_step : 0;
@@ -700,16 +741,14 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                Acc acc;
-                acc.main = part[c];
-                acc.cross = zero;
+                f4_t v = part[c];
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
                     const h8_t dh = as_h8(s_d[((c * 2 + ks2) * PL) * kWave + lane]);
-                    if constexpr (HQ) acc.add(as_h8(pr[ks2][0]), as_h8(pr[ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]));
-                    else acc.main = mfma16(as_h8(pr[ks2][0]), dh, acc.main);
+                    if constexpr (HQ) v = mfma22(as_h8(pr[ks2][0]), as_h8(pr[ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v);
+                    else v = mfma16(as_h8(pr[ks2][0]), dh, v);
                 }
-                f4_t v = (HQ ? acc.sum() : acc.main) * back;
+                v *= back;
                 here(v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -752,7 +791,7 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
             const f4_t nw = {a.norm_w[e], a.norm_w[e + 1], a.norm_w[e + 2], a.norm_w[e + 3]};
             f4_t y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = v[i][k] * (sc * nw[k]) * silu_acc(z[i][k]);
+            for (int k = 0; k < 4; ++k) y[k] = v[i][k] * (sc * nw[k]) * silu_hw(z[i][k]);
             if (a.out_f32) {
                 *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at + e) = y;
             } else {
@@ -777,7 +816,7 @@ int planes_of(const DnTokens &a, bool in_f32) { return in_f32 || a.out_f32 ? 2 :
 
 // Parts of the workspace, at 256-byte boundaries; o only where the outputs are no f32.
 struct Parts {
-    size_t k, q, w, p, u, decay, vmax, o, total;
+    size_t k, q, w, p, u, decay, sums, beta, vmax, dots, o, total;
 };
 Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int64_t tokens, int planes, bool with_o) {
     Parts s{};
@@ -787,18 +826,25 @@ Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int6
     s.p = dn_align(cap * nv * kC * kC * planes * 2);
     s.u = dn_align(cap * nv * dv * kC * 4);
     s.decay = dn_align(cap * nv * 2 * kC * 4);
+    s.sums = dn_align(cap * nv * kC * 8);
+    s.beta = dn_align(cap * nv * kC * 4);
     s.vmax = dn_align(cap * nv * 4);
+    s.dots = dn_align(cap * nk * 2 * 10 * 256 * 4);
     s.o = with_o ? dn_align(tokens * nv * dv * 4) : 0;
-    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.vmax + s.o;
+    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.sums + s.beta + s.vmax + s.dots + s.o;
     return s;
 }
 int64_t cap_of(int64_t sequences, int64_t tokens) { return tokens / kC + sequences; }
 
+template <int DK, bool HQ, int KM, typename T>
+void launch_prepare_km(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    hipLaunchKernelGGL((deltanet_keys_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nk)), dim3(kPrepThreads), 0, s, a, w);
+    hipLaunchKernelGGL((deltanet_solve_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nv)), dim3(kPrepThreads), 0, s, a, w);
+}
 template <int DK, bool HQ, typename T>
 void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    const dim3 grid(static_cast<uint32_t>(w.cap * a.nv)), block(kPrepThreads);
-    if (a.K <= 4) hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, 4, T>), grid, block, 0, s, a, w);
-    else hipLaunchKernelGGL((deltanet_prepare_kernel<DK, HQ, 8, T>), grid, block, 0, s, a, w);
+    if (a.K <= 4) launch_prepare_km<DK, HQ, 4, T>(a, w, s);
+    else launch_prepare_km<DK, HQ, 8, T>(a, w, s);
 }
 
 template <int DK, bool HQ>
@@ -859,7 +905,10 @@ void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_
     w.p = reinterpret_cast<uint4 *>(take(parts.p));
     w.u = reinterpret_cast<f4_t *>(take(parts.u));
     w.decay = reinterpret_cast<float *>(take(parts.decay));
+    w.sums = reinterpret_cast<double *>(take(parts.sums));
+    w.beta = reinterpret_cast<float *>(take(parts.beta));
     w.vmax = reinterpret_cast<float *>(take(parts.vmax));
+    w.dots = reinterpret_cast<f4_t *>(take(parts.dots));
     w.o = a.out_f32 ? static_cast<float *>(a.out) : reinterpret_cast<float *>(p);
     if (w.planes == 2) launch<true>(a, w, in_f32, s);
     else launch<false>(a, w, in_f32, s);

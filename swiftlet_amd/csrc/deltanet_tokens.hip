@@ -316,7 +316,7 @@ extern "C" int swq_deltanet_tokens(const swq_deltanet_layer *l, const swq_deltan
     a.eps = l->norm_eps;
     hipStream_t s = static_cast<hipStream_t>(stream);
     // chunks are loaded and stored four elements at a time
-    const bool four = !misaligned(qkvz, 4 * in) && a.qkvz_stride % 4 == 0 && !misaligned(out, a.out_f32 ? 16 : 8) && !misaligned(a.conv_w, 16);
+    const bool four = !misaligned(qkvz, 4 * in) && a.qkvz_stride % 4 == 0 && a.qkvz_stride < 1 << 24 && !misaligned(out, a.out_f32 ? 16 : 8) && !misaligned(a.conv_w, 16);
     if (a.max_tokens >= kChunksFrom && four && deltanet_chunks_take(l)) launch_deltanet_chunks(a, dtype == SWQ_F32, ws, s);
     else if (dtype == SWQ_F32) launch_tokens_dk<float>(a, s);
     else launch_tokens_dk<uint16_t>(a, s);
