@@ -573,7 +573,7 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
     const int tokens = a.count(b);
     uint8_t *slot = a.state(b);
     if (tokens <= 0 || !slot) return;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
     const int chunks = (tokens + kC - 1) / kC, tile = wave & 3;
     const int64_t n0 = a.first(b), first = chunk_base(a, b);
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
@@ -613,64 +613,64 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
                 reinterpret_cast<uint2 *>(s_s + ((c * KS + dt / 2) * 2 + 1) * kWave + lane)[dt & 1] = as_u2(lo);
             }
     };
+    // What a chunk brings is in flight for two chunks before it is used: with one, the chain waited for memory (1.66 us a
+    // chunk).  Chunks that do not exist are loaded as the last one again.
+    auto chunk_at = [&](int m) { return first + min(m, chunks - 1); };
     if (wave < 4) {
-        const uint4 *wp = w.w + (first * a.nv + hv) * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
-        const f4_t *up = w.u + ((first * a.nv + hv) * (a.dv / 16) + c0 / 16) * kRowTiles * kWave + tile * kWave + lane;
-        const uint4 *kp = w.k + (first * a.nk + hk) * (4 * DT * 2 * 2 * kWave) + wave * DT * 2 * 2 * kWave + lane;
-        const float *dp = w.decay + (first * a.nv + hv) * 2 * kC;
-        const int64_t w_step = static_cast<int64_t>(a.nv) * kRowTiles * KS * 2 * kWave, u_step = static_cast<int64_t>(a.nv) * (a.dv / 16) * kRowTiles * kWave,
-                      k_step = static_cast<int64_t>(a.nk) * 4 * DT * 2 * 2 * kWave, d_step = static_cast<int64_t>(a.nv) * 2 * kC;
-        uint4 wr[KS][2], kr[DT][2][2];
-        f4_t ur[CT], late;
-        float grown;
-        auto load_w = [&]() {
+        uint4 wr[2][KS][2], kr[2][DT][2][2];
+        f4_t ur[2][CT], late[2];
+        float grown[2];
+        auto load_w = [&](int s, int m) {
+            const int64_t head = chunk_at(m) * a.nv + hv;
+            const uint4 *wp = w.w + head * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave;
+            const f4_t *up = w.u + (head * (a.dv / 16) + c0 / 16) * kRowTiles * kWave + tile * kWave;
+            const float *dp = w.decay + head * 2 * kC;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) wr[ks][p] = wp[(ks * 2 + p) * kWave];
+                for (int p = 0; p < 2; ++p) wr[s][ks][p] = wp[(ks * 2 + p) * kWave + lane];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) ur[c] = up[c * kRowTiles * kWave];
-            late = *reinterpret_cast<const f4_t *>(dp + kC + 16 * tile + 4 * g);
-            grown = dp[kC - 1];
+            for (int c = 0; c < CT; ++c) ur[s][c] = up[c * kRowTiles * kWave + lane];
+            late[s] = load4(dp + kC + 16 * tile + 4 * g);
+            grown[s] = dp[kC - 1];
         };
-        auto load_k = [&]() {
+        auto load_k = [&](int s, int m) {
+            const uint4 *kp = w.k + (chunk_at(m) * a.nk + hk) * (4 * DT * 2 * 2 * kWave) + wave * DT * 2 * 2 * kWave;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) kr[t][ks2][p] = kp[((t * 2 + ks2) * 2 + p) * kWave];
+                    for (int p = 0; p < 2; ++p) kr[s][t][ks2][p] = kp[((t * 2 + ks2) * 2 + p) * kWave + lane];
         };
-        load_w();
-        load_k();
+        load_w(0, 0);
+        load_k(0, 0);
+        load_w(1, 1);
+        load_k(1, 1);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int c = 0; c < CT; ++c) st[t][c] *= scale;
         put_state();
-        for (int m = 0; m < chunks; ++m) {
+        auto turn = [&](int s, int m) {
             lds_barrier();
-            const float keep = grown;
-            const bool more = m + 1 < chunks;
+            const float keep = grown[s];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 f4_t acc = zero;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
-                    acc = mfma22(as_h8(wr[ks][0]), as_h8(wr[ks][1]), as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]), as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), acc);
-                const f4_t d = ur[c] * scale - acc * (1.f / (kScaleT * kScaleK));
+                    acc = mfma22(as_h8(wr[s][ks][0]), as_h8(wr[s][ks][1]), as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]), as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), acc);
+                const f4_t d = ur[s][c] * scale - acc * (1.f / (kScaleT * kScaleK));
                 h4_t hi, lo;
                 split4(d, hi, lo);
                 reinterpret_cast<uint2 *>(s_d + ((c * 2 + tile / 2) * PL) * kWave + lane)[tile & 1] = as_u2(hi);
                 if (HQ) reinterpret_cast<uint2 *>(s_d + ((c * 2 + tile / 2) * PL + 1) * kWave + lane)[tile & 1] = as_u2(lo);
-                split4(d * late, hi, lo);
+                split4(d * late[s], hi, lo);
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + tile / 2) * 2) * kWave + lane)[tile & 1] = as_u2(hi);
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + tile / 2) * 2 + 1) * kWave + lane)[tile & 1] = as_u2(lo);
             }
-            wp += more ? w_step : 0;
-            up += more ? u_step : 0;
-            dp += more ? d_step : 0;
-            load_w();
+            load_w(s, m + 2);
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
@@ -683,12 +683,15 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
                 for (int t = 0; t < DT; ++t) {
                     st[t][c] *= keep;
 #pragma unroll
-                    for (int ks2 = 0; ks2 < 2; ++ks2) st[t][c] = mfma22(as_h8(kr[t][ks2][0]), as_h8(kr[t][ks2][1]), e[ks2][0], e[ks2][1], st[t][c]);
+                    for (int ks2 = 0; ks2 < 2; ++ks2) st[t][c] = mfma22(as_h8(kr[s][t][ks2][0]), as_h8(kr[s][t][ks2][1]), e[ks2][0], e[ks2][1], st[t][c]);
                 }
             }
-            kp += more ? k_step : 0;
-            load_k();
+            load_k(s, m + 2);
             put_state();
+        };
+        for (int m = 0; m < chunks; m += 2) {
+            turn(0, m);
+            if (m + 1 < chunks) turn(1, m + 1);
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t)
@@ -696,33 +699,31 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
             for (int c = 0; c < CT; ++c)
                 *reinterpret_cast<f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (wave * DT + t)) = st[t][c] * inverse;
     } else {
-        const uint4 *qp = w.q + (first * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave + lane;
-        const uint4 *pp = w.p + (first * a.nv + hv) * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave + lane;
-        const float *dp = w.decay + (first * a.nv + hv) * 2 * kC;
-        const int64_t q_step = static_cast<int64_t>(a.nk) * kRowTiles * KS * PL * kWave, p_step = static_cast<int64_t>(a.nv) * kRowTiles * 2 * PL * kWave,
-                      d_step = static_cast<int64_t>(a.nv) * 2 * kC;
-        uint4 qr[KS][PL], pr[2][PL];
-        f4_t grown;
-        auto load_q = [&]() {
+        uint4 qr[2][KS][PL], pr[2][2][PL];
+        f4_t grown[2];
+        auto load_q = [&](int s, int m) {
+            const uint4 *qp = w.q + (chunk_at(m) * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) qr[ks][p] = qp[(ks * PL + p) * kWave];
-            grown = *reinterpret_cast<const f4_t *>(dp + 16 * tile + 4 * g);
+                for (int p = 0; p < PL; ++p) qr[s][ks][p] = qp[(ks * PL + p) * kWave + lane];
+            grown[s] = load4(w.decay + (chunk_at(m) * a.nv + hv) * 2 * kC + 16 * tile + 4 * g);
         };
-        auto load_p = [&]() {
+        auto load_p = [&](int s, int m) {
+            const uint4 *pp = w.p + (chunk_at(m) * a.nv + hv) * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave;
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) pr[ks2][p] = pp[(ks2 * PL + p) * kWave];
+                for (int p = 0; p < PL; ++p) pr[s][ks2][p] = pp[(ks2 * PL + p) * kWave + lane];
         };
-        load_q();
-        load_p();
+        load_q(0, 0);
+        load_p(0, 0);
+        load_q(1, 1);
+        load_p(1, 1);
         const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
         float *o = w.o + (n0 + 16 * tile + 4 * g) * a.nv * a.dv + hv * a.dv + c0 + col;
-        for (int m = 0; m < chunks; ++m) {
+        auto turn = [&](int s, int m) {
             lds_barrier();
-            const bool more = m + 1 < chunks;
             f4_t part[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
@@ -730,14 +731,12 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const h8_t sh = as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]);
-                    if constexpr (HQ) part[c] = mfma22(as_h8(qr[ks][0]), as_h8(qr[ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), part[c]);
-                    else part[c] = mfma16(as_h8(qr[ks][0]), sh, part[c]);
+                    if constexpr (HQ) part[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), part[c]);
+                    else part[c] = mfma16(as_h8(qr[s][ks][0]), sh, part[c]);
                 }
-                part[c] *= grown;
+                part[c] *= grown[s];
             }
-            qp += more ? q_step : 0;
-            dp += more ? d_step : 0;
-            load_q();
+            load_q(s, m + 2);
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
@@ -745,8 +744,8 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
                     const h8_t dh = as_h8(s_d[((c * 2 + ks2) * PL) * kWave + lane]);
-                    if constexpr (HQ) v = mfma22(as_h8(pr[ks2][0]), as_h8(pr[ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v);
-                    else v = mfma16(as_h8(pr[ks2][0]), dh, v);
+                    if constexpr (HQ) v = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v);
+                    else v = mfma16(as_h8(pr[s][ks2][0]), dh, v);
                 }
                 v *= back;
                 here(v);
@@ -754,49 +753,70 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
                 for (int e = 0; e < 4; ++e)
                     if (m * kC + 16 * tile + 4 * g + e < tokens) o[static_cast<int64_t>(m * kC + e) * a.nv * a.dv + 16 * c] = v[e];
             }
-            pp += more ? p_step : 0;
-            load_p();
+            load_p(s, m + 2);
+        };
+        for (int m = 0; m < chunks; m += 2) {
+            turn(0, m);
+            if (m + 1 < chunks) turn(1, m + 1);
         }
     }
 }
 
 // The gated norm of a chunk's outputs, and the ring's rows of a sequence's last one.  `parts` workgroups share a chunk;
-// a row (token, value head) has `lanes` lanes of 4 values, up to 4 times.
-template <typename T>
-__global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w, int parts, int lanes) {
+// a row (token, value head) has L lanes, of 4 values or as many times 4 as it takes.  Four rows per lane, all their loads
+// in flight at once.
+template <int L, typename T>
+__global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w, int parts) {
+    constexpr int U = L == kWave ? 4 : 1, R = L == kWave ? 1 : 4;  // runs of 4 values per lane, and rows
     const int part = blockIdx.x % parts;
     int b, m;
     if (!find_chunk(a, static_cast<int>(blockIdx.x / parts), b, m)) return;
-    const int tid = threadIdx.x, tokens = a.count(b), lane = tid % lanes, here = min(tokens - m * kC, kC);
+    const int tid = threadIdx.x, tokens = a.count(b), lane = tid % L, rows = min(tokens - m * kC, kC) * a.nv;
     const int64_t n0 = a.first(b) + static_cast<int64_t>(m) * kC;
     const T *x = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride;
-    for (int row = part * (kFinishThreads / lanes) + tid / lanes; row < here * a.nv; row += parts * (kFinishThreads / lanes)) {
-        const int t = row / a.nv, hv = row % a.nv;
-        const int64_t at = (n0 + t) * a.nv * a.dv + hv * a.dv;
-        f4_t v[4], z[4];
-        float ss = 0.f;
+    for (int row0 = part * (kFinishThreads / L) * R + tid / L; row0 < rows; row0 += parts * (kFinishThreads / L) * R) {
+        f4_t v[R][U];
+        Four<T> z[R][U];
+        int64_t at[R];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = 4 * (lane + i * lanes);
-            if (e >= a.dv) continue;
-            v[i] = load4(w.o + at + e);
-            z[i] = load4(x + t * a.qkvz_stride + z_at(a, hv, e));
-            ss += v[i][0] * v[i][0] + v[i][1] * v[i][1] + v[i][2] * v[i][2] + v[i][3] * v[i][3];
+        for (int r = 0; r < R; ++r) {
+            const int row = min(row0 + r * (kFinishThreads / L), rows - 1), t = row / a.nv, hv = row - t * a.nv;
+            at[r] = (n0 + t) * a.nv * a.dv + hv * a.dv;
+            const T *zr = x + t * a.qkvz_stride + z_at(a, hv, 0);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int e = min(4 * (lane + i * L), a.dv - 4);
+                v[r][i] = load4(w.o + at[r] + e);
+                z[r][i].load(zr + e);
+            }
         }
-        const float sc = 1.0f / __fsqrt_rn(segment_sum(ss, lanes) / static_cast<float>(a.dv) + a.eps);
+        f4_t nw[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = 4 * (lane + i * lanes);
-            if (e >= a.dv) continue;
-            const f4_t nw = {a.norm_w[e], a.norm_w[e + 1], a.norm_w[e + 2], a.norm_w[e + 3]};
-            f4_t y;
+        for (int i = 0; i < U; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = v[i][k] * (sc * nw[k]) * silu_hw(z[i][k]);
-            if (a.out_f32) {
-                *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at + e) = y;
-            } else {
-                const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at + e) = make_uint2(lo, hi);
+            for (int k = 0; k < 4; ++k) nw[i][k] = a.norm_w[min(4 * (lane + i * L), a.dv - 4) + k];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (4 * (lane + i * L) < a.dv) ss += v[r][i][0] * v[r][i][0] + v[r][i][1] * v[r][i][1] + v[r][i][2] * v[r][i][2] + v[r][i][3] * v[r][i][3];
+            const float sc = 1.0f / __fsqrt_rn(segment_sum(ss, L) / static_cast<float>(a.dv) + a.eps);
+            if (row0 + r * (kFinishThreads / L) >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int e = 4 * (lane + i * L);
+                if (e >= a.dv) continue;
+                const f4_t zi = z[r][i].get();
+                f4_t y;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = v[r][i][k] * (sc * nw[i][k]) * silu_hw(zi[k]);
+                if (a.out_f32) {
+                    *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at[r] + e) = y;
+                } else {
+                    const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at[r] + e) = make_uint2(lo, hi);
+                }
             }
         }
     }
@@ -854,6 +874,20 @@ void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1, HQ>), dim3(static_cast<uint32_t>(units * groups)), dim3(kChainThreads), 0, s, a, w, groups);
 }
 
+template <int L, typename T>
+void launch_finish_lanes(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    // as many workgroups to a chunk as go round once
+    const int rows = kFinishThreads / L * (L == kWave ? 1 : 4), parts = std::min((kC * a.nv + rows - 1) / rows, 64);
+    hipLaunchKernelGGL((deltanet_finish_kernel<L, T>), dim3(static_cast<uint32_t>(w.cap) * parts), dim3(kFinishThreads), 0, s, a, w, parts);
+}
+template <typename T>
+void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    if (a.dv <= 16) launch_finish_lanes<4, T>(a, w, s);
+    else if (a.dv <= 64) launch_finish_lanes<16, T>(a, w, s);
+    else if (a.dv <= 128) launch_finish_lanes<32, T>(a, w, s);
+    else launch_finish_lanes<kWave, T>(a, w, s);
+}
+
 template <bool HQ>
 void launch(const DnTokens &a, const DnChunks &w, bool in_f32, hipStream_t s) {
     if (a.dk == 64) {
@@ -865,12 +899,8 @@ void launch(const DnTokens &a, const DnChunks &w, bool in_f32, hipStream_t s) {
         else launch_prepare<128, HQ, uint16_t>(a, w, s);
         launch_chain<128, HQ>(a, w, s);
     }
-    int lanes = 4;
-    while (lanes < kWave && 4 * lanes < a.dv) lanes *= 2;
-    const int parts = std::max(1, std::min(32, kC * a.nv * lanes / kFinishThreads / 8));
-    const dim3 grid(static_cast<uint32_t>(w.cap) * parts), block(kFinishThreads);
-    if (in_f32) hipLaunchKernelGGL(deltanet_finish_kernel<float>, grid, block, 0, s, a, w, parts, lanes);
-    else hipLaunchKernelGGL(deltanet_finish_kernel<uint16_t>, grid, block, 0, s, a, w, parts, lanes);
+    if (in_f32) launch_finish<float>(a, w, s);
+    else launch_finish<uint16_t>(a, w, s);
 }
 
 }  // namespace
@@ -881,7 +911,7 @@ bool deltanet_chunks_take(const swq_deltanet_layer *l) {
 
 bool deltanet_chunks_fit(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
     const int64_t most = 1LL << 23, chunks = cap_of(sequences, tokens), heads = (sequences * l->num_key_heads + 7) * (l->num_value_heads / l->num_key_heads);
-    return chunks * std::max(l->num_value_heads, 32) < most && heads * (l->value_head_dim / 16) < most;
+    return chunks * std::max(l->num_value_heads, 64) < most && heads * (l->value_head_dim / 16) < most;
 }
 
 size_t deltanet_chunks_bytes(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
