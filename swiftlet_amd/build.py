@@ -43,7 +43,7 @@ def sources() -> list[Path]:
 # VGPRs: scales, softmax and rescaling work on them by VALU right after each
 # product, and results in AGPRs would each cost a copy back.
 FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-              for name in ("moe_prefill.hip", "attention_q4_step.hip", "attention_q4_prefill.hip")}
+              for name in ("moe_prefill.hip", "attention_q4_step.hip", "attention_q4_prefill.hip", "deltanet_chunks.hip")}
 
 
 def _compile(src: Path) -> Path:

@@ -8,8 +8,8 @@
 // which is the token after token recurrence written out.  Four launches:
 //   keys     per (chunk, key head), all chunks at once: convolution and norms of k and q, k.k and k.q, gates;
 //   solve    per (chunk, value head), all chunks at once: convolution of v, A, T, W, U, P;
-//   chain    per (sequence, value head, 16 to 64 columns of S), chunk after chunk: d, o, S;
-//   finish   the gated norm, and the ring's rows.
+//   chain    per (sequence, value head, 16 or 32 columns of S), chunk after chunk: d, o, S;
+//   finish   all chunks at once: the gated norm, and the ring's rows.
 //
 // Numbers.  f32 numbers meet on the f16 matrix cores as two f16 numbers each, x = hi + lo, and three products (hi hi, hi
 // lo, lo hi): 22 bits of what is large enough for lo to be a normal f16 number, 2^-25 of 1 below.  Powers of two keep
@@ -25,6 +25,7 @@
 // results lie: position j of lane group g is element 16 (j / 4) + 4 g + j % 4 of 32.  Every result then is the next
 // product's operand after rounding alone, and all operands lie in the workspace as lanes load them, 16 bytes each.
 #include <algorithm>
+#include <cstdlib>
 
 #include "deltanet.hpp"
 #include "route.hpp"
@@ -39,7 +40,7 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr int kC = kDnChunk;
 constexpr int kRowTiles = kC / 16;
 constexpr int kPrepThreads = 512;
-constexpr int kChainThreads = 512;
+constexpr int kChainThreads = 768;
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
 // What operands are multiplied by; of d times e^(c_last - c), so that its product with k has S's own.
@@ -100,19 +101,40 @@ __device__ __forceinline__ float scale_of(float m, float &inverse) {
     return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
 
-// The chunk's place: sequence b, chunk m of it.  Sequence b has its chunks from first(b) / 64 + b on, so that those of
-// no two sequences meet where starts rise, and none lies past cap wherever starts point.
+// Sequence b has its chunks from first(b) / 64 + b on, so that those of no two sequences meet where starts rise, and none
+// lies past cap wherever starts point.
 __device__ __forceinline__ int chunk_base(const DnTokens &a, int b) { return a.first(b) / kC + b; }
-__device__ __forceinline__ bool find_chunk(const DnTokens &a, int chunk, int &b, int &m) {
+
+// A chunk: of sequence b the m-th, the sequence's first token, how many it has, tokens before them, its state.
+struct Chunk {
+    int b, m, n0, tokens;
+    uint32_t pos;
+    uint8_t *state;
+};
+// Whether the chunk exists.  Each lane loads all of a sequence, so that one of them is found in one round trip.
+__device__ __forceinline__ bool find_chunk(const DnTokens &a, int chunk, Chunk &c) {
     const int lane = threadIdx.x & (kWave - 1);
-    int below = 0;
+    int n0 = 0, tokens = 0, slot = -1, pos = 0;
+    c.b = -1;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
-        const bool is = b0 + lane < a.B && chunk_base(a, min(b0 + lane, a.B - 1)) <= chunk;
-        below += __builtin_popcountll(__ballot(is));
+        const int b = min(b0 + lane, a.B - 1);
+        const int n = a.first(b), t = a.count(b), s = a.slot ? a.slot[b] : b, p = a.positions[b];
+        const bool is = b0 + lane < a.B && n / kC + b <= chunk;
+        const uint64_t all = __ballot(is);
+        if (all == 0) continue;
+        const int from = 63 - __builtin_clzll(all);  // the last that starts no later
+        c.b = b0 + from;
+        n0 = __builtin_amdgcn_readlane(n, from);
+        tokens = __builtin_amdgcn_readlane(t, from);
+        slot = __builtin_amdgcn_readlane(s, from);
+        pos = __builtin_amdgcn_readlane(p, from);
     }
-    b = max(below - 1, 0);
-    m = chunk - chunk_base(a, b);
-    return m >= 0 && m < (a.count(b) + kC - 1) / kC && a.state(b) != nullptr;
+    c.m = chunk - (n0 / kC + c.b);
+    c.n0 = n0;
+    c.tokens = tokens;
+    c.pos = static_cast<uint32_t>(max(pos, 0));
+    c.state = slot >= 0 && slot < a.slots ? a.states + slot * a.slot_bytes : nullptr;
+    return c.b >= 0 && c.m < (tokens + kC - 1) / kC && c.state != nullptr;
 }
 
 __device__ __forceinline__ f4_t load4(const float *p) { return *reinterpret_cast<const f4_t *>(p); }
@@ -142,15 +164,19 @@ struct Four<uint16_t> {
     }
 };
 
-// Sum over 16 or 32 consecutive lanes, to each of them.
+// Sum over 16, 32 or 64 consecutive lanes, to each of them.
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
     v += dpp<0xB1, 0xF, true>(v);   // quad_perm [1,0,3,2]
     v += dpp<0x4E, 0xF, true>(v);   // quad_perm [2,3,0,1]
     v += dpp<0x141, 0xF, true>(v);  // row_half_mirror
     v += dpp<0x140, 0xF, true>(v);  // row_mirror
-    if constexpr (LANES == 32) {
+    if constexpr (LANES >= 32) {
         const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LANES == 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
         v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
     return v;
@@ -287,10 +313,11 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     __shared__ uint4 s_q[DT * 2 * 2 * kWave];          // queries by tokens; then keys, transposed
     const int hk = blockIdx.x % a.nk;
     const int64_t chunk = blockIdx.x / a.nk;
-    int b, m;
-    if (!find_chunk(a, static_cast<int>(chunk), b, m)) return;
+    Chunk it;
+    if (!find_chunk(a, static_cast<int>(chunk), it)) return;
+    const int m = it.m, tokens = it.tokens, n0 = it.n0;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int tokens = a.count(b), n0 = a.first(b), tile = wave & 3;
+    const int tile = wave & 3;
     const bool keys = wave < 4;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 
@@ -299,7 +326,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     f4_t y[N];
     {
         const int c = (keys ? a.keyD : 0) + hk * DK + ch, head = a.layout == SWQ_DELTA_SPLIT ? hk * DK + (keys ? a.keyD : 0) : hk * (2 * DK + 2 * a.rep * a.dv) + (keys ? DK : 0);
-        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(a.state(b)), a.position(b), tokens, m * kC + 16 * tile,
+        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
                          t0, head + ch, c, y);
         uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0) + t0 + 16 * (ch % 16 / 4)) + ch / 16 % 2;
 #pragma unroll
@@ -380,21 +407,25 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     __shared__ float s_max[4];
     const int hv = blockIdx.x % a.nv, hk = hv / a.rep;
     const int64_t chunk = blockIdx.x / a.nv, head = chunk * a.nv + hv;
-    int b, m;
-    if (!find_chunk(a, static_cast<int>(chunk), b, m)) return;
+    Chunk it;
+    if (!find_chunk(a, static_cast<int>(chunk), it)) return;
+    const int m = it.m, tokens = it.tokens, n0 = it.n0;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
-    const int tokens = a.count(b), n0 = a.first(b), tile = wave & 3;
+    const int tile = wave & 3;
     const bool keys = wave < 4;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
     const double *c = w.sums + head * kC;
     const float *beta = w.beta + head * kC, *decay = w.decay + head * 2 * kC;
-    const f4_t *dots = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
+    const f4_t *dots_at = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
+    f4_t dots[kRowTiles];
+#pragma unroll
+    for (int jt = 0; jt < kRowTiles; ++jt) dots[jt] = dots_at[min(jt, tile) * kWave];
 
     const int ch = 4 * (lane % (kVBlock / 4)), t0 = N * (lane / (kVBlock / 4));
     f4_t v[N];
     auto values = [&](int c0) {  // columns c0 .. of this wave's tile, and their largest
         const int off = min(c0 + ch, a.dv - 4), v_at = a.layout == SWQ_DELTA_SPLIT ? 2 * a.keyD + hv * a.dv : hk * (2 * DK + 2 * a.rep * a.dv) + 2 * DK + (hv - hk * a.rep) * a.dv;
-        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(a.state(b)), a.position(b), tokens, m * kC + 16 * tile,
+        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
                          t0, v_at + off, 2 * a.keyD + hv * a.dv + off, v);
         float most = 0.f;
 #pragma unroll
@@ -416,13 +447,15 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
             ci[e] = c[16 * tile + 4 * g + e];
             bi[e] = beta[16 * tile + 4 * g + e];
         }
-        for (int jt = 0; jt < tile; ++jt) {
-            f4_t d = dots[jt * kWave] * pow2(mid - c[16 * jt + col]);
+#pragma unroll
+        for (int jt = 0; jt < kRowTiles - 1; ++jt) {
+            if (jt >= tile) continue;
+            f4_t d = dots[jt] * pow2(mid - c[16 * jt + col]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] *= bi[e] * pow2(ci[e] - mid);
             tri_put(s_t + tri(tile, jt), d, lane);
         }
-        f4_t d = dots[tile * kWave];
+        f4_t d = dots[kRowTiles - 1];  // the diagonal tile in any wave
         const double cj = c[16 * tile + col];
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = 4 * g + e > col ? d[e] * bi[e] * pow2(ci[e] - cj) : 0.f;
@@ -431,6 +464,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         tri_invert(s_t + tri(tile, tile), lane);
     } else {
+        values(0);
         const double ci = c[16 * tile + col];
         const float row = kScaleP * pow2(ci - mid);
         uint4 *p = w.p + head * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave + lane;
@@ -440,7 +474,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int jt = 2 * ks2 + half;
-                d[half] = dots[min(jt, tile) * kWave];
+                d[half] = dots[jt];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = 16 * jt + 4 * g + e;
@@ -452,7 +486,6 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
             p[ks2 * PL * kWave] = as_u4(o.hi);
             if (HQ) p[(ks2 * PL + 1) * kWave] = as_u4(o.lo);
         }
-        values(0);
     }
     lds_barrier();
 
@@ -495,6 +528,18 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         tri_put(s_t + tri(2, q), -tri_mul(s_t + tri(2, 2), x2, lane, zero), lane);
         tri_put(s_t + tri(3, q), -tri_mul(s_t + tri(3, 3), x3, lane, tri_mul(s_t + tri(3, 2), x2, lane, zero)), lane);
     }
+    const int half_of = wave >> 2;
+    const uint4 *k_at = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave) + lane;
+    uint4 k[2][2][2];
+    auto load_k = [&](int ks) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int ks2 = 0; ks2 < 2; ++ks2)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) k[half][ks2][p] = k_at[transposed(2 * ks + half, ks2, p)];
+    };
+    load_k(half_of * (KS / 2));
     lds_barrier();
 
     // T's rows as operands: 8 of T_ij times b_j (and e^c_j) for i of this wave's tile
@@ -512,23 +557,19 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         tu[ks2] = op_of(u[0], u[1]);
         tw[ks2] = op_of(e_u[0], e_u[1]);
     }
-    const int half_of = wave >> 2;
-    {
-        uint4 *to = w.w + head * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
-        const uint4 *k = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave) + lane;
+    uint4 *w_to = w.w + head * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
 #pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-            const int ks = half_of * (KS / 2) + i;
-            f4_t d[2] = {zero, zero};
+    for (int i = 0; i < KS / 2; ++i) {
+        const int ks = half_of * (KS / 2) + i;
+        f4_t d[2] = {zero, zero};
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int ks2 = 0; ks2 < 2; ++ks2)
-                    d[half] = mfma22(as_h8(k[transposed(2 * ks + half, ks2, 0)]), as_h8(k[transposed(2 * ks + half, ks2, 1)]), tw[ks2].hi, tw[ks2].lo, d[half]);
-            const Op o = op_of(d[0], d[1]);
-            to[ks * 2 * kWave] = as_u4(o.hi);
-            to[(ks * 2 + 1) * kWave] = as_u4(o.lo);
-        }
+            for (int ks2 = 0; ks2 < 2; ++ks2) d[half] = mfma22(as_h8(k[half][ks2][0]), as_h8(k[half][ks2][1]), tw[ks2].hi, tw[ks2].lo, d[half]);
+        if (i + 1 < KS / 2) load_k(ks + 1);
+        const Op o = op_of(d[0], d[1]);
+        w_to[ks * 2 * kWave] = as_u4(o.hi);
+        w_to[(ks * 2 + 1) * kWave] = as_u4(o.lo);
     }
     f4_t *u_to = w.u + head * (a.dv / 16 * kRowTiles * kWave) + lane;
     for (int c0 = 0;;) {
@@ -558,36 +599,41 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     if (tid == 0) w.vmax[head] = vmax;
 }
 
-// One workgroup per (sequence, value head, CT * 16 columns of the state).  Waves 0 to 3 hold the state's rows and make
-// d and the next state; waves 4 to 7 make the outputs, off the chain from chunk to chunk.
+// One workgroup per (sequence, value head, CT * 16 columns of the state), three quarters of waves at three tasks: waves 0 to
+// 3 make d of a quarter of the chunk's tokens each, waves 4 to 7 the next state, of whose rows they hold a quarter each, and
+// waves 8 to 11 the outputs, off the chain from chunk to chunk.  While one kind computes, the others have their loads
+// and stores issued.
 template <int DK, int CT, bool HQ>
-__global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnTokens a, const DnChunks w, int groups) {
+__global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const DnTokens a, const DnChunks w, int groups) {
     constexpr int KS = DK / 32, DT = DK / 64, PL = HQ ? 2 : 1;  // DT: row tiles of the state per wave
     __shared__ uint4 s_s[CT * KS * 2 * kWave], s_d[CT * 2 * PL * kWave], s_e[CT * 2 * 2 * kWave];
-    __shared__ float s_max[8];
+    __shared__ float s_max[kChainThreads / kWave];
     // workgroups of one key head on one XCD (they are handed out round robin): its L2 then has what they share
     const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
     const int unit = rest / (groups * a.rep) * 8 + xcd, within = rest % (groups * a.rep);
     if (unit >= a.B * a.nk) return;
-    const int b = unit / a.nk, hk = unit % a.nk, hv = hk * a.rep + within / groups, c0 = within % groups * CT * 16;
+    const int b = unit / a.nk, hk = unit % a.nk, hv = hk * a.rep + within / groups, ct0 = within % groups * CT;
     const int tokens = a.count(b);
     uint8_t *slot = a.state(b);
     if (tokens <= 0 || !slot) return;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
-    const int chunks = (tokens + kC - 1) / kC, tile = wave & 3;
-    const int64_t n0 = a.first(b), first = chunk_base(a, b);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), part = wave & 3;
+    const uint32_t lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
+    const int chunks = (tokens + kC - 1) / kC, cts = a.dv / 16;
+    const int64_t n0 = a.first(b), first = chunk_base(a, b), head0 = first * a.nv + hv, key0 = first * a.nk + hk;
+    const int64_t decay_step = static_cast<int64_t>(a.nv) * 2 * kC;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+    const bool rows = wave / 4 == 1;  // of the state
 
     // the state's columns, a lane's 4 rows side by side in memory
     f4_t st[DT][CT];
-    float *state = reinterpret_cast<float *>(slot + a.rec_at) + (static_cast<int64_t>(hv) * a.dv + c0 + col) * DK + 4 * g;
+    float *state = reinterpret_cast<float *>(slot + a.rec_at) + (static_cast<int64_t>(hv) * a.dv + 16 * ct0 + col) * DK + 4 * g;
     float most = 0.f;
-    if (wave < 4) {
+    if (rows) {
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                st[t][c] = *reinterpret_cast<const f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (wave * DT + t));
+                st[t][c] = *reinterpret_cast<const f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (part * DT + t));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(st[t][c][e]));
             }
@@ -597,56 +643,43 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
     if (lane == 0) s_max[wave] = most;
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = fmaxf(most, s_max[i]);
+    for (int i = 0; i < kChainThreads / kWave; ++i) most = fmaxf(most, s_max[i]);
     float inverse;
     const float scale = scale_of(most, inverse);
 
-    auto put_state = [&]() {
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const int dt = wave * DT + t;
-                h4_t hi, lo;
-                split4(st[t][c], hi, lo);
-                reinterpret_cast<uint2 *>(s_s + ((c * KS + dt / 2) * 2) * kWave + lane)[dt & 1] = as_u2(hi);
-                reinterpret_cast<uint2 *>(s_s + ((c * KS + dt / 2) * 2 + 1) * kWave + lane)[dt & 1] = as_u2(lo);
-            }
-    };
-    // What a chunk brings is in flight for two chunks before it is used: with one, the chain waited for memory (1.66 us a
-    // chunk).  Chunks that do not exist are loaded as the last one again.
-    auto chunk_at = [&](int m) { return first + min(m, chunks - 1); };
-    if (wave < 4) {
-        uint4 wr[2][KS][2], kr[2][DT][2][2];
-        f4_t ur[2][CT], late[2];
+    // What a chunk brings is in flight for more than a chunk before it is used.  Chunks that do not exist are loaded as the
+    // last one again: no branch.
+    if (rows) {
+        uint4 kr[2][DT][2][2];
         float grown[2];
-        auto load_w = [&](int s, int m) {
-            const int64_t head = chunk_at(m) * a.nv + hv;
-            const uint4 *wp = w.w + head * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave;
-            const f4_t *up = w.u + (head * (a.dv / 16) + c0 / 16) * kRowTiles * kWave + tile * kWave;
-            const float *dp = w.decay + head * 2 * kC;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) wr[s][ks][p] = wp[(ks * 2 + p) * kWave + lane];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) ur[s][c] = up[c * kRowTiles * kWave + lane];
-            late[s] = load4(dp + kC + 16 * tile + 4 * g);
-            grown[s] = dp[kC - 1];
-        };
-        auto load_k = [&](int s, int m) {
-            const uint4 *kp = w.k + (chunk_at(m) * a.nk + hk) * (4 * DT * 2 * 2 * kWave) + wave * DT * 2 * 2 * kWave;
+        const uint4 *k_at = w.k + key0 * (4 * DT * 2 * 2 * kWave) + part * DT * 2 * 2 * kWave;
+        const float *decay_at = w.decay + head0 * 2 * kC + kC - 1;
+        const int64_t k_step = static_cast<int64_t>(a.nk) * 4 * DT * 2 * 2 * kWave;
+        auto load = [&](int s, bool more) {
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) kr[s][t][ks2][p] = kp[((t * 2 + ks2) * 2 + p) * kWave + lane];
+                    for (int p = 0; p < 2; ++p) kr[s][t][ks2][p] = k_at[((t * 2 + ks2) * 2 + p) * kWave + lane];
+            grown[s] = *decay_at;
+            k_at += more ? k_step : 0;
+            decay_at += more ? decay_step : 0;
         };
-        load_w(0, 0);
-        load_k(0, 0);
-        load_w(1, 1);
-        load_k(1, 1);
+        load(0, 1 < chunks);
+        load(1, 2 < chunks);
+        auto put_state = [&]() {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const int dt = part * DT + t, at = (c * KS + dt / 2) * 2;
+                    h4_t hi, lo;
+                    split4(st[t][c], hi, lo);
+                    reinterpret_cast<uint2 *>(s_s + at * kWave + lane)[dt & 1] = as_u2(hi);
+                    reinterpret_cast<uint2 *>(s_s + (at + 1) * kWave + lane)[dt & 1] = as_u2(lo);
+                }
+        };
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -654,23 +687,8 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
         put_state();
         auto turn = [&](int s, int m) {
             lds_barrier();
+            if (m > 0) load(s ^ 1, m + 2 < chunks);  // in place of the last chunk's
             const float keep = grown[s];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                f4_t acc = zero;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    acc = mfma22(as_h8(wr[s][ks][0]), as_h8(wr[s][ks][1]), as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]), as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), acc);
-                const f4_t d = ur[s][c] * scale - acc * (1.f / (kScaleT * kScaleK));
-                h4_t hi, lo;
-                split4(d, hi, lo);
-                reinterpret_cast<uint2 *>(s_d + ((c * 2 + tile / 2) * PL) * kWave + lane)[tile & 1] = as_u2(hi);
-                if (HQ) reinterpret_cast<uint2 *>(s_d + ((c * 2 + tile / 2) * PL + 1) * kWave + lane)[tile & 1] = as_u2(lo);
-                split4(d * late[s], hi, lo);
-                reinterpret_cast<uint2 *>(s_e + ((c * 2 + tile / 2) * 2) * kWave + lane)[tile & 1] = as_u2(hi);
-                reinterpret_cast<uint2 *>(s_e + ((c * 2 + tile / 2) * 2 + 1) * kWave + lane)[tile & 1] = as_u2(lo);
-            }
-            load_w(s, m + 2);
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
@@ -680,13 +698,18 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
 #pragma unroll
                     for (int p = 0; p < 2; ++p) e[ks2][p] = as_h8(s_e[((c * 2 + ks2) * 2 + p) * kWave + lane]);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    st[t][c] *= keep;
+                for (int t = 0; t < DT; ++t) st[t][c] *= keep;
 #pragma unroll
-                    for (int ks2 = 0; ks2 < 2; ++ks2) st[t][c] = mfma22(as_h8(kr[s][t][ks2][0]), as_h8(kr[s][t][ks2][1]), e[ks2][0], e[ks2][1], st[t][c]);
-                }
+                for (int ks2 = 0; ks2 < 2; ++ks2)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) st[t][c] = mfma16(as_h8(kr[s][t][ks2][p == 0]), e[ks2][p == 1], st[t][c]);
             }
-            load_k(s, m + 2);
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) here(st[t][c]);
             put_state();
         };
         for (int m = 0; m < chunks; m += 2) {
@@ -697,63 +720,118 @@ __global__ __launch_bounds__(kChainThreads) void deltanet_chain_kernel(const DnT
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int c = 0; c < CT; ++c)
-                *reinterpret_cast<f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (wave * DT + t)) = st[t][c] * inverse;
-    } else {
-        uint4 qr[2][KS][PL], pr[2][2][PL];
-        f4_t grown[2];
-        auto load_q = [&](int s, int m) {
-            const uint4 *qp = w.q + (chunk_at(m) * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave;
+                *reinterpret_cast<f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (part * DT + t)) = st[t][c] * inverse;
+    } else if (wave < 4) {
+        uint4 wr[2][KS][2];
+        f4_t ur[2][CT], late[2];
+        const uint4 *w_at = w.w + head0 * (kRowTiles * KS * 2 * kWave) + part * KS * 2 * kWave;
+        const f4_t *u_at = w.u + (head0 * cts + ct0) * kRowTiles * kWave + part * kWave;
+        const float *decay_at = w.decay + head0 * 2 * kC + kC + 16 * part;
+        const int64_t w_step = static_cast<int64_t>(a.nv) * kRowTiles * KS * 2 * kWave, u_step = static_cast<int64_t>(a.nv) * cts * kRowTiles * kWave;
+        auto load = [&](int s, bool more) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) qr[s][ks][p] = qp[(ks * PL + p) * kWave + lane];
-            grown[s] = load4(w.decay + (chunk_at(m) * a.nv + hv) * 2 * kC + 16 * tile + 4 * g);
+                for (int p = 0; p < 2; ++p) wr[s][ks][p] = w_at[(ks * 2 + p) * kWave + lane];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) ur[s][c] = u_at[c * kRowTiles * kWave + lane];
+            late[s] = load4(decay_at + 4 * g);
+            w_at += more ? w_step : 0;
+            u_at += more ? u_step : 0;
+            decay_at += more ? decay_step : 0;
         };
-        auto load_p = [&](int s, int m) {
-            const uint4 *pp = w.p + (chunk_at(m) * a.nv + hv) * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave;
+        load(0, 1 < chunks);
+        load(1, 2 < chunks);
+        auto turn = [&](int s, int m) {
+            lds_barrier();
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                // a sum for each kind of product: one after another of the same sum would wait for each other
+                f4_t sum[3] = {zero, zero, zero};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) sum[p] = mfma16(as_h8(wr[s][ks][p == 0]), as_h8(s_s[((c * KS + ks) * 2 + (p == 1)) * kWave + lane]), sum[p]);
+                const f4_t d = ur[s][c] * scale - (sum[2] + (sum[1] + sum[0])) * (1.f / (kScaleT * kScaleK));
+                h4_t hi, lo;
+                split4(d * late[s], hi, lo);
+                reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2) * kWave + lane)[part & 1] = as_u2(hi);
+                reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2 + 1) * kWave + lane)[part & 1] = as_u2(lo);
+                split4(d, hi, lo);
+                reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * PL) * kWave + lane)[part & 1] = as_u2(hi);
+                if (HQ) reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * PL + 1) * kWave + lane)[part & 1] = as_u2(lo);
+            }
+            lds_barrier();
+            load(s, m + 3 < chunks);
+        };
+        for (int m = 0; m < chunks; m += 2) {
+            turn(0, m);
+            if (m + 1 < chunks) turn(1, m + 1);
+        }
+    } else {
+        uint4 qr[2][KS][PL], pr[2][2][PL];
+        f4_t grown[2];
+        const uint4 *q_at = w.q + key0 * (kRowTiles * KS * PL * kWave) + part * KS * PL * kWave, *p_at = w.p + head0 * (kRowTiles * 2 * PL * kWave) + part * 2 * PL * kWave;
+        const float *decay_at = w.decay + head0 * 2 * kC + 16 * part;
+        const int64_t q_step = static_cast<int64_t>(a.nk) * kRowTiles * KS * PL * kWave, p_step = static_cast<int64_t>(a.nv) * kRowTiles * 2 * PL * kWave;
+        auto load_q = [&](int s, bool more) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int p = 0; p < PL; ++p) qr[s][ks][p] = q_at[(ks * PL + p) * kWave + lane];
+            grown[s] = load4(decay_at + 4 * g);
+            q_at += more ? q_step : 0;
+            decay_at += more ? decay_step : 0;
+        };
+        auto load_p = [&](int s, bool more) {
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) pr[s][ks2][p] = pp[(ks2 * PL + p) * kWave + lane];
+                for (int p = 0; p < PL; ++p) pr[s][ks2][p] = p_at[(ks2 * PL + p) * kWave + lane];
+            p_at += more ? p_step : 0;
         };
-        load_q(0, 0);
-        load_p(0, 0);
-        load_q(1, 1);
-        load_p(1, 1);
+        load_q(0, 1 < chunks);
+        load_p(0, 1 < chunks);
+        load_q(1, 2 < chunks);
+        load_p(1, 2 < chunks);
         const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
-        float *o = w.o + (n0 + 16 * tile + 4 * g) * a.nv * a.dv + hv * a.dv + c0 + col;
+        const int64_t row = static_cast<int64_t>(a.nv) * a.dv;
+        float *o = w.o + (n0 + 16 * part + 4 * g) * row + hv * a.dv + 16 * ct0 + col;
         auto turn = [&](int s, int m) {
             lds_barrier();
-            f4_t part[CT];
+            f4_t v[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                part[c] = zero;
+                v[c] = zero;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const h8_t sh = as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]);
-                    if constexpr (HQ) part[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), part[c]);
-                    else part[c] = mfma16(as_h8(qr[s][ks][0]), sh, part[c]);
+                    if constexpr (HQ) v[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), v[c]);
+                    else v[c] = mfma16(as_h8(qr[s][ks][0]), sh, v[c]);
                 }
-                part[c] *= grown[s];
+                v[c] *= grown[s];
             }
-            load_q(s, m + 2);
             lds_barrier();
+            load_q(s, m + 3 < chunks);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                f4_t v = part[c];
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
                     const h8_t dh = as_h8(s_d[((c * 2 + ks2) * PL) * kWave + lane]);
-                    if constexpr (HQ) v = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v);
-                    else v = mfma16(as_h8(pr[s][ks2][0]), dh, v);
+                    if constexpr (HQ) v[c] = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v[c]);
+                    else v[c] = mfma16(as_h8(pr[s][ks2][0]), dh, v[c]);
                 }
-                v *= back;
-                here(v);
+                v[c] *= back;
+                here(v[c]);
+            }
+            load_p(s, m + 3 < chunks);
+            const int left = tokens - m * kC - 16 * part - 4 * static_cast<int>(g);
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (m * kC + 16 * tile + 4 * g + e < tokens) o[static_cast<int64_t>(m * kC + e) * a.nv * a.dv + 16 * c] = v[e];
-            }
-            load_p(s, m + 2);
+                    if (e < left) o[e * row + 16 * c] = v[c][e];
+            o += kC * row;
         };
         for (int m = 0; m < chunks; m += 2) {
             turn(0, m);
@@ -769,10 +847,11 @@ template <int L, typename T>
 __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w, int parts) {
     constexpr int U = L == kWave ? 4 : 1, R = L == kWave ? 1 : 4;  // runs of 4 values per lane, and rows
     const int part = blockIdx.x % parts;
-    int b, m;
-    if (!find_chunk(a, static_cast<int>(blockIdx.x / parts), b, m)) return;
-    const int tid = threadIdx.x, tokens = a.count(b), lane = tid % L, rows = min(tokens - m * kC, kC) * a.nv;
-    const int64_t n0 = a.first(b) + static_cast<int64_t>(m) * kC;
+    Chunk it;
+    if (!find_chunk(a, static_cast<int>(blockIdx.x / parts), it)) return;
+    const int m = it.m, tokens = it.tokens;
+    const int tid = threadIdx.x, lane = tid % L, rows = min(tokens - m * kC, kC) * a.nv;
+    const int64_t n0 = it.n0 + static_cast<int64_t>(m) * kC;
     const T *x = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride;
     for (int row0 = part * (kFinishThreads / L) * R + tid / L; row0 < rows; row0 += parts * (kFinishThreads / L) * R) {
         f4_t v[R][U];
@@ -821,13 +900,12 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
         }
     }
     if ((m + 1) * kC < tokens) return;
-    float *ring = reinterpret_cast<float *>(a.state(b));
-    const uint32_t pos = a.position(b);
-    const T *first = static_cast<const T *>(a.qkvz) + a.first(b) * a.qkvz_stride;
+    float *ring = reinterpret_cast<float *>(it.state);
+    const T *first = static_cast<const T *>(a.qkvz) + it.n0 * a.qkvz_stride;
     for (int ch = part * kFinishThreads + tid; ch < a.convD; ch += parts * kFinishThreads) {
         const int at = mixed_at(a, ch);
         for (int i = max(tokens - a.K, 0); i < tokens; ++i)
-            ring[static_cast<int64_t>((pos + static_cast<uint32_t>(i)) % a.K) * a.convD + ch] = dn_load(first, i * a.qkvz_stride + at);
+            ring[static_cast<int64_t>((it.pos + static_cast<uint32_t>(i)) % a.K) * a.convD + ch] = dn_load(first, i * a.qkvz_stride + at);
     }
 }
 
@@ -867,13 +945,6 @@ void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     else launch_prepare_km<DK, HQ, 8, T>(a, w, s);
 }
 
-template <int DK, bool HQ>
-void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
-    const int groups = a.dv / 16;
-    hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1, HQ>), dim3(static_cast<uint32_t>(units * groups)), dim3(kChainThreads), 0, s, a, w, groups);
-}
-
 template <int L, typename T>
 void launch_finish_lanes(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     // as many workgroups to a chunk as go round once
@@ -888,30 +959,38 @@ void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     else launch_finish_lanes<kWave, T>(a, w, s);
 }
 
-template <bool HQ>
-void launch(const DnTokens &a, const DnChunks &w, bool in_f32, hipStream_t s) {
-    if (a.dk == 64) {
-        if (in_f32) launch_prepare<64, HQ, float>(a, w, s);
-        else launch_prepare<64, HQ, uint16_t>(a, w, s);
-        launch_chain<64, HQ>(a, w, s);
-    } else {
-        if (in_f32) launch_prepare<128, HQ, float>(a, w, s);
-        else launch_prepare<128, HQ, uint16_t>(a, w, s);
-        launch_chain<128, HQ>(a, w, s);
-    }
-    if (in_f32) launch_finish<float>(a, w, s);
-    else launch_finish<uint16_t>(a, w, s);
+template <int DK, bool HQ>
+void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
+    const int cts = a.dv / 16;
+    int ct = 1;
+    if (const char *e = getenv("CTS")) ct = atoi(e) + 1;
+    const dim3 grid(static_cast<uint32_t>(units * (cts / ct))), block(kChainThreads);
+    if (ct == 1) hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1, HQ>), grid, block, 0, s, a, w, cts / ct);
+    else hipLaunchKernelGGL((deltanet_chain_kernel<DK, 2, HQ>), grid, block, 0, s, a, w, cts / ct);
+}
+
+template <int DK, bool HQ, typename T>
+void launch(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    launch_prepare<DK, HQ, T>(a, w, s);
+    launch_chain<DK, HQ>(a, w, s);
+    launch_finish<T>(a, w, s);
+}
+template <bool HQ, typename T>
+void launch_dk(const DnTokens &a, const DnChunks &w, hipStream_t s) {
+    if (a.dk == 64) launch<64, HQ, T>(a, w, s);
+    else launch<128, HQ, T>(a, w, s);
 }
 
 }  // namespace
 
 bool deltanet_chunks_take(const swq_deltanet_layer *l) {
-    return (l->key_head_dim == 64 || l->key_head_dim == 128) && l->value_head_dim % 16 == 0;
+    return (l->key_head_dim == 64 || l->key_head_dim == 128) && l->value_head_dim % 16 == 0 && l->value_head_dim <= 256;
 }
 
 bool deltanet_chunks_fit(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
     const int64_t most = 1LL << 23, chunks = cap_of(sequences, tokens), heads = (sequences * l->num_key_heads + 7) * (l->num_value_heads / l->num_key_heads);
-    return chunks * std::max(l->num_value_heads, 64) < most && heads * (l->value_head_dim / 16) < most;
+    return chunks * std::max(l->num_value_heads, 64) < most && 2 * heads * (l->value_head_dim / 16) < most;
 }
 
 size_t deltanet_chunks_bytes(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
@@ -940,8 +1019,9 @@ void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_
     w.vmax = reinterpret_cast<float *>(take(parts.vmax));
     w.dots = reinterpret_cast<f4_t *>(take(parts.dots));
     w.o = a.out_f32 ? static_cast<float *>(a.out) : reinterpret_cast<float *>(p);
-    if (w.planes == 2) launch<true>(a, w, in_f32, s);
-    else launch<false>(a, w, in_f32, s);
+    if (in_f32) launch_dk<true, float>(a, w, s);
+    else if (w.planes == 2) launch_dk<true, uint16_t>(a, w, s);
+    else launch_dk<false, uint16_t>(a, w, s);
 }
 
 }  // namespace swq
