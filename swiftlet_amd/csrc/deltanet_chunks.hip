@@ -38,12 +38,17 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDnChunk;
+#ifndef SPAN
+#define SPAN 32
+#endif
+constexpr int kSpan = SPAN;
 constexpr int kRowTiles = kC / 16;
 constexpr int kPrepThreads = 512;
 constexpr int kChainThreads = 768;
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
 // What operands are multiplied by; of d times e^(c_last - c), so that its product with k has S's own.
+constexpr float kHalfO = 1.f / 256.f;  // of outputs as f16 numbers
 constexpr float kScaleK = 256.f, kScaleT = 16.f, kScaleP = 256.f, kScaleE = 1.f / kScaleK;
 
 // The workspace: operands of every (chunk, key head) and (chunk, value head).
@@ -55,9 +60,13 @@ struct DnChunks {
     float *beta;           // [chunk][nv][64]
     float *vmax;           // [chunk][nv]
     f4_t *dots;            // [chunk][nk][2][10][64]: k_i.k_j and k_j.q_i, tiles of the lower triangle
-    float *o;              // [N][nv * dv]: the outputs before their norm
+    // the outputs before their norm, as the results lie, [chunk][nv][dv / 16][4][64] lanes: f32 with two planes; else f16
+    // and in the chain's scale, which its inverse ends
+    void *o;
+    float *back;           // [chunk][nv][dv / 16]
     int32_t cap;           // chunks that there is room for
     int32_t planes;
+    int32_t chunk0, span;  // a launch's chunks: those of a sequence from chunk0 on, span at most
 };
 
 __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -101,9 +110,10 @@ __device__ __forceinline__ float scale_of(float m, float &inverse) {
     return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
 
-// Sequence b has its chunks from first(b) / 64 + b on, so that those of no two sequences meet where starts rise, and none
-// lies past cap wherever starts point.
-__device__ __forceinline__ int chunk_base(const DnTokens &a, int b) { return a.first(b) / kC + b; }
+// Sequence b has its chunks' places in the workspace from first(b) / 64 + b on, so that those of no two sequences meet where
+// starts rise, and none lies past cap wherever starts point.  A long prompt alone goes a span of chunks at a time, in the
+// same places again.
+__device__ __forceinline__ int chunk_base(const DnTokens &a, int b) { return a.B == 1 ? 0 : a.first(b) / kC + b; }
 
 // A chunk: of sequence b the m-th, the sequence's first token, how many it has, tokens before them, its state.
 struct Chunk {
@@ -112,14 +122,14 @@ struct Chunk {
     uint8_t *state;
 };
 // Whether the chunk exists.  Each lane loads all of a sequence, so that one of them is found in one round trip.
-__device__ __forceinline__ bool find_chunk(const DnTokens &a, int chunk, Chunk &c) {
+__device__ __forceinline__ bool find_chunk(const DnTokens &a, const DnChunks &w, int chunk, Chunk &c) {
     const int lane = threadIdx.x & (kWave - 1);
     int n0 = 0, tokens = 0, slot = -1, pos = 0;
     c.b = -1;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
         const int b = min(b0 + lane, a.B - 1);
         const int n = a.first(b), t = a.count(b), s = a.slot ? a.slot[b] : b, p = a.positions[b];
-        const bool is = b0 + lane < a.B && n / kC + b <= chunk;
+        const bool is = b0 + lane < a.B && (a.B == 1 || n / kC + b <= chunk);
         const uint64_t all = __ballot(is);
         if (all == 0) continue;
         const int from = 63 - __builtin_clzll(all);  // the last that starts no later
@@ -129,7 +139,7 @@ __device__ __forceinline__ bool find_chunk(const DnTokens &a, int chunk, Chunk &
         slot = __builtin_amdgcn_readlane(s, from);
         pos = __builtin_amdgcn_readlane(p, from);
     }
-    c.m = chunk - (n0 / kC + c.b);
+    c.m = chunk - (a.B == 1 ? 0 : n0 / kC + c.b) + w.chunk0;
     c.n0 = n0;
     c.tokens = tokens;
     c.pos = static_cast<uint32_t>(max(pos, 0));
@@ -283,23 +293,29 @@ __device__ __forceinline__ void tri_invert(float *blk, int lane) {
     }
 }
 
-// Where a lane puts or finds operands of a tile by tokens, [tile][contraction step][plane], and transposed.
+// Where operands of a tile lie in LDS, by tokens [tile][contraction step][plane] and transposed [row tile][tokens / 32][plane], 64
+// places of 16 bytes each.  Operands are read with lane l's at place l but for the low bits of its row, which are mixed
+// with what sets lanes apart that write at once: 16 of them would meet in a bank.
 template <int DK>
 __device__ __forceinline__ constexpr int by_tokens(int tile, int ks, int plane) { return ((tile * (DK / 32) + ks) * 2 + plane) * kWave; }
+__device__ __forceinline__ constexpr int token_place(int ks, int token, int g) { return 16 * g + (token ^ (4 * ks + g)); }
 __device__ __forceinline__ constexpr int transposed(int dt, int ks2, int plane) { return ((dt * 2 + ks2) * 2 + plane) * kWave; }
+__device__ __forceinline__ constexpr int row_place(int dt, int row, int g) { return 16 * g + (row ^ (dt & 3)); }
 
 // N tokens from t0 of the tile and four channels from ch of the operand's rows, transposed, N a multiple of 4.
 template <int N>
 __device__ __forceinline__ void put_transposed(uint4 *to, int tile, int t0, int ch, const f4_t (&v)[N]) {
+    const int dt = ch / 16;
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-        uint2 *at = reinterpret_cast<uint2 *>(to + transposed(ch / 16, tile >> 1, 0) + 16 * ((t0 + i) / 4) + ch % 16) + (tile & 1);
+        uint2 *at = reinterpret_cast<uint2 *>(to + transposed(dt, tile >> 1, 0)) + (tile & 1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             h4_t hi, lo;
             split4(f4_t{v[i][e], v[i + 1][e], v[i + 2][e], v[i + 3][e]}, hi, lo);
-            at[2 * e] = as_u2(hi);
-            at[2 * (e + kWave)] = as_u2(lo);
+            const int place = row_place(dt, ch % 16 + e, (t0 + i) / 4);
+            at[2 * place] = as_u2(hi);
+            at[2 * (place + kWave)] = as_u2(lo);
         }
     }
 }
@@ -314,7 +330,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     const int hk = blockIdx.x % a.nk;
     const int64_t chunk = blockIdx.x / a.nk;
     Chunk it;
-    if (!find_chunk(a, static_cast<int>(chunk), it)) return;
+    if (!find_chunk(a, w, static_cast<int>(chunk), it)) return;
     const int m = it.m, tokens = it.tokens, n0 = it.n0;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int tile = wave & 3;
@@ -328,15 +344,16 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         const int c = (keys ? a.keyD : 0) + hk * DK + ch, head = a.layout == SWQ_DELTA_SPLIT ? hk * DK + (keys ? a.keyD : 0) : hk * (2 * DK + 2 * a.rep * a.dv) + (keys ? DK : 0);
         conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
                          t0, head + ch, c, y);
-        uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0) + t0 + 16 * (ch % 16 / 4)) + ch / 16 % 2;
+        uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0)) + ch / 16 % 2;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float ss = lanes_sum<DK / 4>(y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3]);
             y[i] *= kScaleK * __builtin_amdgcn_rsqf(ss + DK * 1e-6f);
             h4_t hi, lo;
             split4(y[i], hi, lo);
-            to[2 * i] = as_u2(hi);
-            to[2 * (i + kWave)] = as_u2(lo);
+            const int place = token_place(ch / 32, t0 + i, ch % 16 / 4);
+            to[2 * place] = as_u2(hi);
+            to[2 * (place + kWave)] = as_u2(lo);
         }
     }
     // a wave reads its own tile back as operands, the queries' before keys take their place
@@ -344,7 +361,10 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     Op x[KS];
     auto read_back = [&](const uint4 *from) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x[ks] = {as_h8(from[by_tokens<DK>(tile, ks, 0) + lane]), as_h8(from[by_tokens<DK>(tile, ks, 1) + lane])};
+        for (int ks = 0; ks < KS; ++ks) {
+            const int place = token_place(ks, lane & 15, lane >> 4);
+            x[ks] = {as_h8(from[by_tokens<DK>(tile, ks, 0) + place]), as_h8(from[by_tokens<DK>(tile, ks, 1) + place])};
+        }
     };
     if (!keys) read_back(s_q);
     lds_barrier();
@@ -365,7 +385,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         f4_t d = zero;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const h8_t kh = as_h8(s_k[by_tokens<DK>(jt, ks, 0) + lane]), kl = as_h8(s_k[by_tokens<DK>(jt, ks, 1) + lane]);
+            const int place = token_place(ks, lane & 15, lane >> 4);
+            const h8_t kh = as_h8(s_k[by_tokens<DK>(jt, ks, 0) + place]), kl = as_h8(s_k[by_tokens<DK>(jt, ks, 1) + place]);
             d = keys ? mfma22(x[ks].hi, x[ks].lo, kh, kl, d) : mfma22(kh, kl, x[ks].hi, x[ks].lo, d);
         }
         d *= 1.f / (kScaleK * kScaleK);
@@ -395,7 +416,10 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     lds_barrier();
     uint4 *k_to = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave);
 #pragma unroll
-    for (int i = 0; i < DT * 2 * 2 * kWave / kPrepThreads; ++i) k_to[i * kPrepThreads + tid] = s_q[i * kPrepThreads + tid];
+    for (int i = 0; i < DT * 2 * 2 * kWave / kPrepThreads; ++i) {
+        const int part = i * (kPrepThreads / kWave) + wave;  // four to a row tile
+        k_to[part * kWave + lane] = s_q[part * kWave + row_place(part / 4, lane & 15, lane >> 4)];
+    }
 }
 
 // One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.
@@ -405,10 +429,12 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     __shared__ uint4 s_v[kVBlock / 16 * 2 * 2 * kWave];  // values, transposed
     __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
     __shared__ float s_max[4];
-    const int hv = blockIdx.x % a.nv, hk = hv / a.rep;
-    const int64_t chunk = blockIdx.x / a.nv, head = chunk * a.nv + hv;
+    // a key head's value heads on one XCD (workgroups are handed out round robin), which they share dots and keys in
+    const uint32_t unit = blockIdx.x / 8 / a.rep * 8 + blockIdx.x % 8;
+    const int hk = unit % a.nk, hv = hk * a.rep + blockIdx.x / 8 % a.rep;
+    const int64_t chunk = unit / a.nk, head = chunk * a.nv + hv;
     Chunk it;
-    if (!find_chunk(a, static_cast<int>(chunk), it)) return;
+    if (chunk >= w.cap || !find_chunk(a, w, static_cast<int>(chunk), it)) return;
     const int m = it.m, tokens = it.tokens, n0 = it.n0;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
     const int tile = wave & 3;
@@ -579,7 +605,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
             f4_t d = zero;
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
-                d = mfma22(tu[ks2].hi, tu[ks2].lo, as_h8(s_v[transposed(ct, ks2, 0) + lane]), as_h8(s_v[transposed(ct, ks2, 1) + lane]), d);
+                d = mfma22(tu[ks2].hi, tu[ks2].lo, as_h8(s_v[transposed(ct, ks2, 0) + row_place(ct, col, g)]), as_h8(s_v[transposed(ct, ks2, 1) + row_place(ct, col, g)]), d);
             d *= v_inv * (1.f / kScaleT);
             here(d);
             if (c0 + 16 * ct < a.dv) u_to[((c0 / 16 + ct) * kRowTiles + tile) * kWave] = d;
@@ -613,13 +639,13 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
     const int unit = rest / (groups * a.rep) * 8 + xcd, within = rest % (groups * a.rep);
     if (unit >= a.B * a.nk) return;
     const int b = unit / a.nk, hk = unit % a.nk, hv = hk * a.rep + within / groups, ct0 = within % groups * CT;
-    const int tokens = a.count(b);
+    const int tokens = a.count(b) - w.chunk0 * kC;
     uint8_t *slot = a.state(b);
     if (tokens <= 0 || !slot) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), part = wave & 3;
     const uint32_t lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
-    const int chunks = (tokens + kC - 1) / kC, cts = a.dv / 16;
-    const int64_t n0 = a.first(b), first = chunk_base(a, b), head0 = first * a.nv + hv, key0 = first * a.nk + hk;
+    const int chunks = min((tokens + kC - 1) / kC, w.span), cts = a.dv / 16;
+    const int64_t first = chunk_base(a, b), head0 = first * a.nv + hv, key0 = first * a.nk + hk;
     const int64_t decay_step = static_cast<int64_t>(a.nv) * 2 * kC;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
     const bool rows = wave / 4 == 1;  // of the state
@@ -795,8 +821,11 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
         load_q(1, 2 < chunks);
         load_p(1, 2 < chunks);
         const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
-        const int64_t row = static_cast<int64_t>(a.nv) * a.dv;
-        float *o = w.o + (n0 + 16 * part + 4 * g) * row + hv * a.dv + 16 * ct0 + col;
+        const int64_t o0 = (head0 * cts + ct0) * kRowTiles * kWave + part * kWave + lane;
+        f4_t *o = static_cast<f4_t *>(w.o) + o0;
+        uint2 *o_half = static_cast<uint2 *>(w.o) + o0;
+        float *back_at = w.back + head0 * cts + ct0 + lane;
+        const int64_t o_step = static_cast<int64_t>(a.nv) * cts * kRowTiles * kWave;
         auto turn = [&](int s, int m) {
             lds_barrier();
             f4_t v[CT];
@@ -821,17 +850,17 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
                     if constexpr (HQ) v[c] = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v[c]);
                     else v[c] = mfma16(as_h8(pr[s][ks2][0]), dh, v[c]);
                 }
-                v[c] *= back;
-                here(v[c]);
+                v[c] *= HQ ? back : kHalfO;
             }
             load_p(s, m + 3 < chunks);
-            const int left = tokens - m * kC - 16 * part - 4 * static_cast<int>(g);
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < left) o[e * row + 16 * c] = v[c][e];
-            o += kC * row;
+            for (int c = 0; c < CT; ++c) {
+                if (HQ) o[c * kRowTiles * kWave] = v[c];
+                else o_half[c * kRowTiles * kWave] = as_u2(__builtin_convertvector(v[c], h4_t));
+            }
+            o += o_step;
+            o_half += o_step;
+            if (!HQ && part == 0 && lane < CT) back_at[static_cast<int64_t>(m) * a.nv * cts] = back * (1.f / kHalfO);
         };
         for (int m = 0; m < chunks; m += 2) {
             turn(0, m);
@@ -840,83 +869,80 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
     }
 }
 
-// The gated norm of a chunk's outputs, and the ring's rows of a sequence's last one.  `parts` workgroups share a chunk;
-// a row (token, value head) has L lanes, of 4 values or as many times 4 as it takes.  Four rows per lane, all their loads
-// in flight at once.
-template <int L, typename T>
-__global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w, int parts) {
-    constexpr int U = L == kWave ? 4 : 1, R = L == kWave ? 1 : 4;  // runs of 4 values per lane, and rows
-    const int part = blockIdx.x % parts;
+// One workgroup per (chunk, value head): the gated norm, and the ring's rows of a sequence's last chunk.  CW * 32 columns at
+// most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.
+template <int CW, bool HQ, typename T>
+__global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w) {
+    constexpr int L = CW * 8, ROWS = kFinishThreads / L, R = kC / ROWS, kRow = CW * 32 + 4;
+    __shared__ __align__(16) float s_o[kC * kRow];
+    const int hv = blockIdx.x % a.nv, hk = hv / a.rep, ri = hv - hk * a.rep;
+    const int64_t chunk = blockIdx.x / a.nv, head = chunk * a.nv + hv;
     Chunk it;
-    if (!find_chunk(a, static_cast<int>(blockIdx.x / parts), it)) return;
-    const int m = it.m, tokens = it.tokens;
-    const int tid = threadIdx.x, lane = tid % L, rows = min(tokens - m * kC, kC) * a.nv;
+    if (!find_chunk(a, w, static_cast<int>(chunk), it)) return;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g = lane >> 4, cts = a.dv / 16;
+    const int m = it.m, tokens = it.tokens, here_tokens = min(tokens - m * kC, kC);
     const int64_t n0 = it.n0 + static_cast<int64_t>(m) * kC;
-    const T *x = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride;
-    for (int row0 = part * (kFinishThreads / L) * R + tid / L; row0 < rows; row0 += parts * (kFinishThreads / L) * R) {
-        f4_t v[R][U];
-        Four<T> z[R][U];
-        int64_t at[R];
+
+    // output gates and the norm's weights, as they will be used
+    const int e = min(4 * (tid % L), a.dv - 4), row0 = tid / L;
+    const bool real = 4 * (tid % L) < a.dv;
+    const T *zr = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride + z_at(a, hv, 0) + e;
+    Four<T> z[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = min(row0 + r * (kFinishThreads / L), rows - 1), t = row / a.nv, hv = row - t * a.nv;
-            at[r] = (n0 + t) * a.nv * a.dv + hv * a.dv;
-            const T *zr = x + t * a.qkvz_stride + z_at(a, hv, 0);
+    for (int i = 0; i < R; ++i) z[i].load(zr + min(row0 + i * ROWS, here_tokens - 1) * a.qkvz_stride);
+    f4_t nw;
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int e = min(4 * (lane + i * L), a.dv - 4);
-                v[r][i] = load4(w.o + at[r] + e);
-                z[r][i].load(zr + e);
-            }
-        }
-        f4_t nw[U];
+    for (int k = 0; k < 4; ++k) nw[k] = a.norm_w[e + k];
+    const int64_t o0 = head * cts * kRowTiles * kWave + lane;
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+    for (int i = 0; i < CW * 2 * kRowTiles * kWave / kFinishThreads; ++i) {
+        const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
+        f4_t o;
+        if (HQ) o = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
+        else o = __builtin_convertvector(__builtin_bit_cast(h4_t, static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave]), f4_t) * w.back[head * cts + ct];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) nw[i][k] = a.norm_w[min(4 * (lane + i * L), a.dv - 4) + k];
+        for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[k];
+    }
+    lds_barrier();
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float ss = 0.f;
+    for (int i = 0; i < R; ++i) {
+        const int t = row0 + i * ROWS;
+        const f4_t o = *reinterpret_cast<const f4_t *>(s_o + t * kRow + e);
+        const float ss = real ? o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3] : 0.f;
+        const float sc = __builtin_amdgcn_rsqf(lanes_sum<L>(ss) / static_cast<float>(a.dv) + a.eps);
+        const f4_t zi = z[i].get();
+        f4_t y;
 #pragma unroll
-            for (int i = 0; i < U; ++i)
-                if (4 * (lane + i * L) < a.dv) ss += v[r][i][0] * v[r][i][0] + v[r][i][1] * v[r][i][1] + v[r][i][2] * v[r][i][2] + v[r][i][3] * v[r][i][3];
-            const float sc = 1.0f / __fsqrt_rn(segment_sum(ss, L) / static_cast<float>(a.dv) + a.eps);
-            if (row0 + r * (kFinishThreads / L) >= rows) continue;
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int e = 4 * (lane + i * L);
-                if (e >= a.dv) continue;
-                const f4_t zi = z[r][i].get();
-                f4_t y;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = v[r][i][k] * (sc * nw[i][k]) * silu_hw(zi[k]);
-                if (a.out_f32) {
-                    *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at[r] + e) = y;
-                } else {
-                    const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at[r] + e) = make_uint2(lo, hi);
-                }
-            }
+        for (int k = 0; k < 4; ++k) y[k] = o[k] * (sc * nw[k]) * silu_hw(zi[k]);
+        if (t >= here_tokens || !real) continue;
+        const int64_t at = ((n0 + t) * a.nv + hv) * a.dv + e;
+        if (a.out_f32) {
+            *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at) = y;
+        } else {
+            const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(lo, hi);
         }
     }
     if ((m + 1) * kC < tokens) return;
+    // the ring: this head's values, and with the first value head of a key head its queries and keys
     float *ring = reinterpret_cast<float *>(it.state);
-    const T *first = static_cast<const T *>(a.qkvz) + it.n0 * a.qkvz_stride;
-    for (int ch = part * kFinishThreads + tid; ch < a.convD; ch += parts * kFinishThreads) {
-        const int at = mixed_at(a, ch);
-        for (int i = max(tokens - a.K, 0); i < tokens; ++i)
-            ring[static_cast<int64_t>((it.pos + static_cast<uint32_t>(i)) % a.K) * a.convD + ch] = dn_load(first, i * a.qkvz_stride + at);
+    const T *last = static_cast<const T *>(a.qkvz) + (it.n0 + static_cast<int64_t>(tokens) - 1) * a.qkvz_stride;
+    const int channels = a.dv + (ri == 0 ? 2 * a.dk : 0), rows = min(tokens, a.K);
+    for (int i = tid; i < channels * rows; i += kFinishThreads) {
+        const int back = i / channels, c = i - back * channels;
+        const int ch = c < a.dv ? 2 * a.keyD + hv * a.dv + c : hk * a.dk + (c - a.dv) % a.dk + (c - a.dv >= a.dk ? a.keyD : 0);
+        ring[static_cast<int64_t>((it.pos + static_cast<uint32_t>(tokens - 1 - back)) % a.K) * a.convD + ch] = dn_load(last - back * a.qkvz_stride, mixed_at(a, ch));
     }
 }
 
 // Whether outputs are made of two planes: unless projections and outputs are bf16.
 int planes_of(const DnTokens &a, bool in_f32) { return in_f32 || a.out_f32 ? 2 : 1; }
 
-// Parts of the workspace, at 256-byte boundaries; o only where the outputs are no f32.
+// Parts of the workspace, at 256-byte boundaries.
 struct Parts {
-    size_t k, q, w, p, u, decay, sums, beta, vmax, dots, o, total;
+    size_t k, q, w, p, u, decay, sums, beta, vmax, dots, o, back, total;
 };
-Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int64_t tokens, int planes, bool with_o) {
+Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int planes) {
     Parts s{};
     s.k = dn_align(cap * nk * dk * kC * 2 * 2);
     s.q = dn_align(cap * nk * dk * kC * planes * 2);
@@ -928,16 +954,20 @@ Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int6
     s.beta = dn_align(cap * nv * kC * 4);
     s.vmax = dn_align(cap * nv * 4);
     s.dots = dn_align(cap * nk * 2 * 10 * 256 * 4);
-    s.o = with_o ? dn_align(tokens * nv * dv * 4) : 0;
-    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.sums + s.beta + s.vmax + s.dots + s.o;
+    s.o = dn_align(cap * nv * dv * kC * 2 * planes);
+    s.back = dn_align(cap * nv * (dv / 16) * 4);
+    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.sums + s.beta + s.vmax + s.dots + s.o + s.back;
     return s;
 }
-int64_t cap_of(int64_t sequences, int64_t tokens) { return tokens / kC + sequences; }
+// Chunks that have places in the workspace: for one sequence those of a span.
+int64_t cap_of(int64_t sequences, int64_t tokens) {
+    return sequences == 1 ? std::min<int64_t>((tokens + kC - 1) / kC, kSpan) : tokens / kC + sequences;
+}
 
 template <int DK, bool HQ, int KM, typename T>
 void launch_prepare_km(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     hipLaunchKernelGGL((deltanet_keys_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nk)), dim3(kPrepThreads), 0, s, a, w);
-    hipLaunchKernelGGL((deltanet_solve_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nv)), dim3(kPrepThreads), 0, s, a, w);
+    hipLaunchKernelGGL((deltanet_solve_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>((w.cap * a.nk + 7) / 8 * 8 * a.rep)), dim3(kPrepThreads), 0, s, a, w);
 }
 template <int DK, bool HQ, typename T>
 void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
@@ -945,18 +975,12 @@ void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     else launch_prepare_km<DK, HQ, 8, T>(a, w, s);
 }
 
-template <int L, typename T>
-void launch_finish_lanes(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    // as many workgroups to a chunk as go round once
-    const int rows = kFinishThreads / L * (L == kWave ? 1 : 4), parts = std::min((kC * a.nv + rows - 1) / rows, 64);
-    hipLaunchKernelGGL((deltanet_finish_kernel<L, T>), dim3(static_cast<uint32_t>(w.cap) * parts), dim3(kFinishThreads), 0, s, a, w, parts);
-}
-template <typename T>
+template <bool HQ, typename T>
 void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    if (a.dv <= 16) launch_finish_lanes<4, T>(a, w, s);
-    else if (a.dv <= 64) launch_finish_lanes<16, T>(a, w, s);
-    else if (a.dv <= 128) launch_finish_lanes<32, T>(a, w, s);
-    else launch_finish_lanes<kWave, T>(a, w, s);
+    const dim3 grid(static_cast<uint32_t>(w.cap * a.nv)), block(kFinishThreads);
+    if (a.dv <= 64) hipLaunchKernelGGL((deltanet_finish_kernel<2, HQ, T>), grid, block, 0, s, a, w);
+    else if (a.dv <= 128) hipLaunchKernelGGL((deltanet_finish_kernel<4, HQ, T>), grid, block, 0, s, a, w);
+    else hipLaunchKernelGGL((deltanet_finish_kernel<8, HQ, T>), grid, block, 0, s, a, w);
 }
 
 template <int DK, bool HQ>
@@ -974,7 +998,7 @@ template <int DK, bool HQ, typename T>
 void launch(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     launch_prepare<DK, HQ, T>(a, w, s);
     launch_chain<DK, HQ>(a, w, s);
-    launch_finish<T>(a, w, s);
+    launch_finish<HQ, T>(a, w, s);
 }
 template <bool HQ, typename T>
 void launch_dk(const DnTokens &a, const DnChunks &w, hipStream_t s) {
@@ -990,18 +1014,18 @@ bool deltanet_chunks_take(const swq_deltanet_layer *l) {
 
 bool deltanet_chunks_fit(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
     const int64_t most = 1LL << 23, chunks = cap_of(sequences, tokens), heads = (sequences * l->num_key_heads + 7) * (l->num_value_heads / l->num_key_heads);
-    return chunks * std::max(l->num_value_heads, 64) < most && 2 * heads * (l->value_head_dim / 16) < most;
+    return chunks * l->num_value_heads < most && 2 * heads * (l->value_head_dim / 16) < most;
 }
 
 size_t deltanet_chunks_bytes(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
-    return parts_of(l->num_key_heads, l->num_value_heads, l->key_head_dim, l->value_head_dim, cap_of(sequences, tokens), tokens, 2, true).total;
+    return parts_of(l->num_key_heads, l->num_value_heads, l->key_head_dim, l->value_head_dim, cap_of(sequences, tokens), 2).total;
 }
 
 void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_t s) {
     DnChunks w{};
     w.cap = static_cast<int32_t>(cap_of(a.B, a.N));
     w.planes = planes_of(a, in_f32);
-    const Parts parts = parts_of(a.nk, a.nv, a.dk, a.dv, w.cap, a.N, w.planes, !a.out_f32);
+    const Parts parts = parts_of(a.nk, a.nv, a.dk, a.dv, w.cap, w.planes);
     uint8_t *p = static_cast<uint8_t *>(ws);
     auto take = [&](size_t n) {
         uint8_t *at = p;
@@ -1018,10 +1042,16 @@ void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_
     w.beta = reinterpret_cast<float *>(take(parts.beta));
     w.vmax = reinterpret_cast<float *>(take(parts.vmax));
     w.dots = reinterpret_cast<f4_t *>(take(parts.dots));
-    w.o = a.out_f32 ? static_cast<float *>(a.out) : reinterpret_cast<float *>(p);
-    if (in_f32) launch_dk<true, float>(a, w, s);
-    else if (w.planes == 2) launch_dk<true, uint16_t>(a, w, s);
-    else launch_dk<false, uint16_t>(a, w, s);
+    w.o = take(parts.o);
+    w.back = reinterpret_cast<float *>(take(parts.back));
+    const int chunks = a.B == 1 ? (a.max_tokens + kC - 1) / kC : 1;  // of a sequence alone
+    w.span = a.B == 1 ? kSpan : INT32_MAX;
+    for (w.chunk0 = 0; w.chunk0 < chunks; w.chunk0 += kSpan) {
+        if (a.B == 1) w.cap = std::min(chunks - w.chunk0, kSpan);
+        if (in_f32) launch_dk<true, float>(a, w, s);
+        else if (w.planes == 2) launch_dk<true, uint16_t>(a, w, s);
+        else launch_dk<false, uint16_t>(a, w, s);
+    }
 }
 
 }  // namespace swq
