@@ -310,9 +310,9 @@ typedef struct swq_deltanet_batch {
 } swq_deltanet_batch;
 
 /* Workspace bytes of swq_deltanet_tokens for calls of up to batch->sequences
- * sequences, batch->tokens tokens and batch->max_tokens of one sequence.  Of
- * starts and slot only whether they are NULL is read, of positions nothing.  0
- * on bad input. */
+ * sequences, batch->tokens tokens and batch->max_tokens of one sequence (starts
+ * NULL: tokens / sequences).  Of starts and slot only whether they are NULL is
+ * read, of positions nothing.  0 on bad input. */
 size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch);
 
 /* swq_deltanet_step for the tokens of many sequences, prompts or one token

@@ -65,13 +65,16 @@ struct DnTokens {
     void *out;                   // [N][nv * dv]
     const int32_t *starts, *positions, *slot;
     int32_t B, N, max_tokens, slots;
+    int32_t least, most;         // tokens of the sequences that a launch takes
     int32_t nk, nv, dk, dv, K, layout, rep, keyD, convD;
     int32_t out_f32;
     float eps;
 
     __device__ __forceinline__ int first(int b) const { return starts ? min(max(starts[b], 0), N) : b * max_tokens; }
+    // Tokens of sequence b, 0 if the launch does not take it.
     __device__ __forceinline__ int count(int b) const {
-        return starts ? min(max(min(starts[b + 1], N) - first(b), 0), max_tokens) : max_tokens;
+        const int n = starts ? min(max(min(starts[b + 1], N) - first(b), 0), max_tokens) : max_tokens;
+        return n >= least && n <= most ? n : 0;
     }
     // The sequence's state, or null for one that is left out.
     __device__ __forceinline__ uint8_t *state(int b) const {

@@ -25,7 +25,6 @@
 // results lie: position j of lane group g is element 16 (j / 4) + 4 g + j % 4 of 32.  Every result then is the next
 // product's operand after rounding alone, and all operands lie in the workspace as lanes load them, 16 bytes each.
 #include <algorithm>
-#include <cstdlib>
 
 #include "deltanet.hpp"
 #include "route.hpp"
@@ -38,13 +37,14 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDnChunk;
-#ifndef SPAN
-#define SPAN 32
-#endif
-constexpr int kSpan = SPAN;
+// Chunks of a prompt alone that go through all launches before the next do, 200 MB of operands at 32 value heads of
+// 128, which the caches hold from one launch to the next.  4,096 (16,384) tokens: spans of 16 251 us (1,031), 32 221
+// (860), 64 245 (946), the whole prompt at once 245 (954).
+constexpr int kSpan = 32;
 constexpr int kRowTiles = kC / 16;
 constexpr int kPrepThreads = 512;
 constexpr int kChainThreads = 768;
+constexpr int kCus = 256;  // a workgroup of the chain takes one
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
 // What operands are multiplied by; of d times e^(c_last - c), so that its product with k has S's own.
@@ -986,9 +986,9 @@ void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
 template <int DK, bool HQ>
 void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
-    const int cts = a.dv / 16;
-    int ct = 1;
-    if (const char *e = getenv("CTS")) ct = atoi(e) + 1;
+    // 32 columns to a workgroup where those of 16 would not find a CU each: at 32 value heads of 128 four prompts of 1,000
+    // tokens in all take 138 us instead of 155, but one of 4,096 231 instead of 221
+    const int cts = a.dv / 16, ct = cts % 2 == 0 && static_cast<int64_t>(a.B) * a.nv * cts > kCus ? 2 : 1;
     const dim3 grid(static_cast<uint32_t>(units * (cts / ct))), block(kChainThreads);
     if (ct == 1) hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1, HQ>), grid, block, 0, s, a, w, cts / ct);
     else hipLaunchKernelGGL((deltanet_chain_kernel<DK, 2, HQ>), grid, block, 0, s, a, w, cts / ct);

@@ -147,6 +147,46 @@ def test_sizes_of_values(size):
     check(c, c.run())
 
 
+@pytest.mark.parametrize("lengths", [[64, 4, 5, 0, 3, 12, 1, 2, 11, 13], [4, 4, 12], [11, 11, 3]], ids=str)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_short_ones_beside_long_ones(lengths, dtype):
+    c = Batch(BIG, lengths, dtype, seed=18, K=3)
+    check(c, c.run())
+
+
+@pytest.mark.parametrize("heads,tokens,most", [(SMALL, 2048, None), (SMALL, 2049, None), (SMALL, 4160, None), (SMALL, 6200, 4100), ((1, 2, 128, 16), 5000, None)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_long_prompt(heads, tokens, most, dtype):
+    """A prompt alone passes through the workspace 2,048 tokens at a time."""
+    c = Batch(heads, [tokens], dtype, seed=tokens)
+    out = torch.full((tokens, c.val), 7.0, dtype=c.dtype, device="cuda")
+    c.run(max_tokens=most or tokens, out=out)
+    assert bool((out[most or tokens:] == 7).all())
+    if most:
+        out[most:] = 0
+    check(c, out, lengths=[most or tokens])
+
+
+def test_one_long_prompt_captured():
+    c = Batch(SMALL, [4500], "bf16", True, seed=19)
+    out = torch.empty((4500, c.val), dtype=torch.bfloat16, device="cuda")
+    c.run(out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(out=out)
+    for n in (4500, 2100, 30, 4500):  # of the captured call's tokens
+        c.starts[1] = n
+        c.states.copy_(c.before)
+        want = c.run(out=torch.empty_like(out))[:n].clone()
+        states = c.states.clone()
+        c.states.copy_(c.before)
+        c.ws.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:n], want) and torch.equal(c.states, states), n
+    check(c, out)
+
+
 def test_long():
     c = Batch(SMALL, [2500, 1, 700], "bf16", True, seed=12)
     check(c, c.run())
