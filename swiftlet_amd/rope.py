@@ -70,7 +70,7 @@ class RopeGPU:
         """cos and sin, f32 [n, rotary_dims / 2, 2]: of positions (int32 device [n]), or of first .. first + count - 1."""
         torch = _torch()
         n = count if positions is None else positions.numel()
-        if n is None or (count is not None and count != n):
+        if n is None or n < 0 or (count is not None and count != n):
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "rope_table: count")
         if out is None:
             if stream is not None and _elsewhere(stream):
@@ -97,34 +97,34 @@ class RopeGPU:
             out = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
         if not xs or len(out) != len(xs) or (norm_weights is not None and len(norm_weights) != len(xs)):
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
-        at, (N, _, hd) = _here(table, "rope"), _shape(xs[0])
+        at, dtype, shape = _here(table, "rope"), xs[0].dtype, xs[0].shape
+        if len(shape) != 3:
+            raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
+        N, _, hd = shape
         parts = (RopeHeads * len(xs))()
-        for i, (x, y) in enumerate(zip(xs, out)):
-            for t in (x, y):
-                if t.get_device() != at:
-                    raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "rope: not on the table's device")
-                if t.dtype != xs[0].dtype:
-                    raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, "rope: tensors of two types")
-                if _shape(t) != (N, x.shape[1], hd) or (t.stride(2) != 1 and hd > 1):
-                    raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
-            if (N > 1 and y.stride(0) == 0) or (x.shape[1] > 1 and y.stride(1) == 0):
+        for part, x, y, w in zip(parts, xs, out, norm_weights or (None,) * len(xs)):
+            shape = x.shape
+            if x.get_device() != at or y.get_device() != at:
+                raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "rope: not on the table's device")
+            if x.dtype != dtype or y.dtype != dtype:
+                raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, "rope: tensors of two types")
+            if len(shape) != 3 or shape[0] != N or shape[2] != hd or y.shape != shape:
+                raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
+            heads, (part.token_stride, part.head_stride, e), (to, ho, eo) = shape[1], x.stride(), y.stride()
+            if hd > 1 and (e != 1 or eo != 1):
+                raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
+            if (to == 0 and N > 1) or (ho == 0 and heads > 1):
                 raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: out")
-            w = norm_weights[i] if norm_weights is not None else None
-            if w is not None and w.numel() != hd:
-                raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: norm_weights")
-            parts[i] = RopeHeads(x.data_ptr(), y.data_ptr(), x.stride(0), x.stride(1), y.stride(0), y.stride(1),
-                                 _ptr(w, hd, "rope: norm_weights", at, torch.float32), x.shape[1], 0)
-        if table.dim() != 3 or tuple(table.shape[1:]) != (self.rot // 2, 2):
+            if w is not None:
+                if w.numel() != hd:
+                    raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: norm_weights")
+                part.norm_weight = _ptr(w, hd, "rope: norm_weights", at, torch.float32)
+            part.x, part.out, part.heads, part.out_token_stride, part.out_head_stride = x.data_ptr(), y.data_ptr(), heads, to, ho
+        if table.shape[1:] != (self.rot // 2, 2):
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: table")
         check(self.lib.swq_rope(parts, len(xs), N, hd, self.rot, self._layout, int(inverse), eps, _ptr(table, 1, "rope: table", at, torch.float32),
                                 len(table), _ptr(rows, N, "rope: rows", at, torch.int32), _code(xs[0], "rope"), _stream_handle(stream)), "rope")
         return out
-
-
-def _shape(t):
-    if t.dim() != 3:
-        raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
-    return tuple(t.shape)
 
 
 def _here(t, what):
