@@ -263,3 +263,88 @@ def test_what_is_not_finite_stays_with_its_head():
     a, b = c.block.states_views(states)[1], c.views()[1]
     a[int(c.slots[0]), 1] = b[int(c.slots[0]), 1] = 0
     assert torch.equal(a, b)
+
+
+def test_two_captured_calls_share_a_workspace():
+    """Two calls in graphs of their own, one after another on a stream, in the same workspace."""
+    a, b = Batch(SMALL, [130, 2], seed=20), Batch(SMALL, [2, 70], seed=21)
+    wants = []
+    for c in (a, b):
+        wants.append((c.run(), c.states.clone()))
+        c.states.copy_(c.before)
+    ws = a.block.new_batch_workspace(2, 132)
+    outs, graphs = [torch.empty_like(w[0]) for w in wants], []
+    torch.cuda.synchronize()
+    for c, out in zip((a, b), outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.block.prefill(c.qkvz, c.ba, c.states, c.positions, ws, starts=c.starts, slots=c.slots, max_tokens=max(c.lengths), out=out)
+        graphs.append(graph)
+    for _ in range(3):
+        for c, graph in zip((a, b), graphs):
+            c.states.copy_(c.before)
+            graph.replay()
+        torch.cuda.synchronize()
+        for c, out, (want, states) in zip((a, b), outs, wants):
+            assert torch.equal(out, want) and torch.equal(c.states, states)
+            out.zero_()
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    cs = [Batch(SMALL, [300, 5, 1], "bf16", seed=22 + i) for i in range(2)]
+    wants = []
+    for c in cs:
+        wants.append((c.run(), c.states.clone()))
+        c.states.copy_(c.before)
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        outs = [c.run(stream=s) for c, s in zip(cs, streams)]
+        torch.cuda.synchronize()
+        for c, out, (want, states) in zip(cs, outs, wants):
+            assert torch.equal(out, want) and torch.equal(c.states, states)
+            c.states.copy_(c.before)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("split", [False, True], ids=["interleaved", "split"])
+def test_rows_that_no_wide_load_fits(split):
+    """Projections that start off a multiple of 8 bytes and outputs likewise: token after token, the same results."""
+    c = Batch(SMALL, [90, 2], "bf16", split, seed=24)
+    wide = torch.empty(c.qkvz.numel() + 1, dtype=torch.bfloat16, device="cuda")
+    rows = wide[1:].view(c.qkvz.shape)
+    rows.copy_(c.qkvz)
+    out = torch.empty(92 * c.val + 1, dtype=torch.bfloat16, device="cuda")[1:].view(92, c.val)
+    c.qkvz = rows
+    check(c, c.run(out=out))
+
+
+def test_starts_that_do_not_rise():
+    """Nor end with the rows; slots of nobody, positions below 0: taken as no tokens or as 0, nothing out of bounds."""
+    c = Batch(SMALL, [70, 20, 30], seed=25)
+    c.starts.copy_(torch.tensor([-5, 90, 20, 4000], dtype=torch.int32))
+    c.positions.copy_(torch.tensor([-7, 3, 2 ** 31 - 1], dtype=torch.int32))
+    c.slots[1] = -2 ** 31
+    out = c.run(max_tokens=120)
+    assert bool(torch.isfinite(out).all())
+    n = c.block.slot_bytes
+    used = {int(c.slots[0]), int(c.slots[2])}
+    for j in range(5):
+        if j not in used:
+            assert torch.equal(c.states[j * n:(j + 1) * n], c.before[j * n:(j + 1) * n])
+
+
+def test_refusals_in_python():
+    from swiftlet_amd._lib import SwqError
+    c = Batch(SMALL, [70, 1], seed=26)
+    good = dict(qkvz=c.qkvz, ba=c.ba, states=c.states, positions=c.positions, ws=c.ws, starts=c.starts, slots=c.slots, max_tokens=70)
+    y = torch.empty((71, c.val), device="cuda")
+    for kw in (dict(qkvz=c.qkvz.half()), dict(qkvz=c.qkvz.bfloat16()), dict(qkvz=c.qkvz[:, :-1]), dict(qkvz=c.qkvz.cpu()), dict(qkvz=c.qkvz[:70]), dict(ba=c.ba[:70]),
+               dict(ba=c.ba[:, :-1]), dict(ba=c.ba.cpu()), dict(states=c.states.float()), dict(states=c.states.cpu()),
+               dict(states=c.states[:c.block.slot_bytes - 1]), dict(positions=c.positions.long()), dict(positions=c.positions.cpu()), dict(ws=c.ws[:256]), dict(ws=c.ws.cpu()),
+               dict(ws=c.ws[1:]), dict(starts=c.starts[:2]), dict(starts=c.starts.long()), dict(slots=c.slots[:1]), dict(slots=c.slots.cpu()),
+               dict(starts=None), dict(max_tokens=-1), dict(out=y[:70]), dict(out=y.half()), dict(out=y.cpu())):
+        with pytest.raises(SwqError):
+            c.block.prefill(**{**good, **kw})
+    torch.cuda.synchronize()
+    assert torch.equal(c.states, c.before)

@@ -10,6 +10,7 @@ import math
 import pytest
 import torch
 
+from swiftlet_amd._lib import SwqError
 from swiftlet_amd.rope import RopeGPU, RopeScaling
 
 pytestmark = pytest.mark.gpu
@@ -137,6 +138,46 @@ def test_strides_and_in_place(hd, rot, layout, dtype):
     r.apply([k], table, out=[k])
     check(k, was[..., 3:3 + hd], table, None, layout, rot)
     assert torch.equal(wide[..., :3], was[..., :3]) and torch.equal(wide[..., 3 + hd:], was[..., 3 + hd:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("N,heads,hd,rot", [(4100, [16, 2], 256, 64), (2500, [48, 8], 128, 128)])
+def test_outputs_beyond_the_caches(N, heads, hd, rot, layout, dtype):
+    """More than 32 MB of results, into tensors of their own and in place between what stays."""
+    g, xs = inputs(N, heads, hd + 16, dtype, seed=7)
+    r = RopeGPU(rot, 1e6, layout)
+    table, w = r.table(count=N), 1 + 0.1 * torch.randn(hd, generator=g, device="cuda")
+    heads_of = [x[..., :hd] for x in xs]
+    want = [x.clone() for x in xs]
+    outs = r.apply(heads_of, table, norm_weights=[w, None])
+    for x, y, n in zip(heads_of, outs, (w, None)):
+        check(y, x, table, None, layout, rot, n)
+    r.apply(heads_of, table, norm_weights=[w, None], out=heads_of)
+    for x, y, was in zip(heads_of, outs, want):
+        assert torch.equal(x, y)
+    assert all(torch.equal(x[..., hd:], was[..., hd:]) for x, was in zip(xs, want))
+
+
+def test_refusals_in_python():
+    r = RopeGPU(64, 1e6)
+    table, x = r.table(count=5), torch.zeros((5, 4, 128), device="cuda")
+    w, y = torch.ones(128, device="cuda"), torch.empty_like(x)
+    for kw in (dict(xs=[]), dict(xs=[x] * 5), dict(xs=[x[0]]), dict(xs=[x, x[:4]]), dict(xs=[x, x[..., :64]]), dict(xs=[x, x.bfloat16()]), dict(xs=[x.half()]),
+               dict(xs=[x.transpose(1, 2)]), dict(xs=[x.cpu()]), dict(xs=[x, x], out=[y]), dict(out=[y[..., :64]]), dict(out=[y[:, :1].expand(5, 4, 128)]),
+               dict(out=[y[:1].expand(5, 4, 128)]), dict(out=[y.bfloat16()]), dict(out=[y.cpu()]), dict(norm_weights=[]), dict(norm_weights=[w[:64]]),
+               dict(norm_weights=[w.bfloat16()]), dict(norm_weights=[w.cpu()]), dict(table=table[:4]), dict(table=table[:, :16]), dict(table=table.cpu()),
+               dict(table=table.double()), dict(table=table[::2]), dict(table=table[0]), dict(rows=torch.zeros(4, dtype=torch.int32, device="cuda")),
+               dict(rows=torch.zeros(5, dtype=torch.int64, device="cuda")), dict(rows=torch.zeros(5, dtype=torch.int32))):
+        with pytest.raises(SwqError):
+            r.apply(**{**dict(xs=[x], table=table), **kw})
+    at = torch.zeros(5, dtype=torch.int32, device="cuda")
+    for kw in (dict(), dict(positions=at, count=4), dict(positions=at.long()), dict(positions=at.cpu()), dict(positions=at[::2]), dict(count=-1),
+               dict(count=5, out=torch.empty((4, 32, 2), device="cuda")), dict(count=5, out=torch.empty((5, 32, 2))),
+               dict(count=5, out=torch.empty((5, 32, 2), device="cuda", dtype=torch.bfloat16)), dict(count=5, out=torch.empty((10, 32, 2), device="cuda")[::2])):
+        with pytest.raises(SwqError):
+            r.table(**kw)
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
