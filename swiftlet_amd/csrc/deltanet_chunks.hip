@@ -47,9 +47,11 @@ constexpr int kChainThreads = 768;
 constexpr int kCus = 256;  // a workgroup of the chain takes one
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
-// What operands are multiplied by; of d times e^(c_last - c), so that its product with k has S's own.
-constexpr float kHalfO = 1.f / 256.f;  // of outputs as f16 numbers
-constexpr float kScaleK = 256.f, kScaleT = 16.f, kScaleP = 256.f, kScaleE = 1.f / kScaleK;
+// What operands are multiplied by.  Of d e^(c_last - c): so that its product with k has S's own, which leaves both far
+// enough above 2^-14 for their low parts: with 256 and 1 / 256 the states of 4,096 tokens were off by 7e-6, with 16 by
+// 5e-7, with 8 by 3e-7, and outputs of f32 by 2e-7.  P's is q's, as their products meet in a sum.
+constexpr float kScaleK = 8.f, kScaleT = 16.f, kScaleP = kScaleK, kScaleE = 1.f / kScaleK;
+constexpr float kHalfO = 1.f / kScaleK;  // of outputs as f16 numbers
 
 // The workspace: operands of every (chunk, key head) and (chunk, value head).
 struct DnChunks {

@@ -133,6 +133,23 @@ def test_types_mixed(dtype, out_dtype):
     check(c, c.run(out=out))
 
 
+@pytest.mark.parametrize("heads", [BIG, SMALL], ids=str)
+@pytest.mark.parametrize("lengths,dtype", [([77], "f32"), ([64], "f32"), ([1000], "bf16"), ([300, 5], "bf16")], ids=str)
+def test_states_and_f32_outputs_keep_22_bits(heads, lengths, dtype):
+    """In the 2-norm.  Factors of products are off by 2^-23, their low parts' product of 2^-24 is left out: 2.5 * 2^-23
+    a product; a state comes through four in a row (k.k to T, T k to W, W S to d, k d): 10 * 2^-23 = 1.2e-6 at most, and an
+    output through one more at its side."""
+    c = Batch(heads, lengths, dtype, seed=27)
+    out = c.run()
+    want, _, rec = c.oracle()
+    norm = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+    for j in c.slots.tolist():
+        print(f"state {norm(c.views()[1][j], rec[j]):.2e}", flush=True)
+        assert norm(c.views()[1][j], rec[j]) < 1.2e-6
+    if dtype == "f32":
+        assert norm(out, want) < 1.5e-6
+
+
 @pytest.mark.parametrize("decay", [-12.0, 3.0, 6.0, 100.0])
 def test_decays(decay):
     """From heads that forget next to nothing to heads that forget everything at once."""
