@@ -54,6 +54,8 @@ __device__ __forceinline__ void dn_store_as(void *p, int is_f32, int64_t i, floa
     else static_cast<uint16_t *>(p)[i] = dn_bf16(v);
 }
 
+constexpr int kCus = 256;
+
 // A layer and the tokens of one swq_deltanet_tokens call.  What comes from device memory is clamped where it is
 // read, so that no value of it leads out of a buffer.
 struct DnTokens {

@@ -44,7 +44,6 @@ constexpr int kSpan = 32;
 constexpr int kRowTiles = kC / 16;
 constexpr int kPrepThreads = 512;
 constexpr int kChainThreads = 768;
-constexpr int kCus = 256;  // a workgroup of the chain takes one
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
 // What operands are multiplied by.  Of d e^(c_last - c): so that its product with k has S's own, which leaves both far

@@ -3,7 +3,7 @@
 // (QwenCPUModel.swift:371-496); the state's layout too, so that a sequence may go on with either call.
 //
 // Token after token: one workgroup per (sequence, value head).  The head's matrix [dv][dk] is loaded once, stays in
-// registers over the sequence's tokens (its first 128 rows at dk 128; others pass through memory) and is stored once;
+// registers over the sequence's tokens (its first 128 rows, 64 at dk 256; others pass through memory) and is stored once;
 // the convolution's rows stay in registers as well, and the next token's inputs are in flight while one is computed.
 #include <algorithm>
 
@@ -26,16 +26,18 @@ __device__ __forceinline__ float lds_sum_sq(const float *v, int n, int lane) {
 // WIDE: kernels of up to 8 rows and any number of channels per head; else 4 rows and a channel per thread, as
 // the usual heads of 128 have.  Kernels shorter than that have zero weights in front, which change no bit of
 // the sums.  ONE: no sequence brings more than a token, and the ring takes its row here (a
-// workgroup then overwrites no row that another still reads; with more tokens it would).
-template <int DK, bool WIDE, bool ONE, typename T>
-__global__ __launch_bounds__(kTokThreads) void deltanet_tokens_kernel(const DnTokens a) {
+// workgroup then overwrites no row that another still reads; with more tokens it would).  MANY: registers for two
+// workgroups to a CU, where there are more workgroups than CUs: 64 single tokens at 32 heads of 128 take 51 us instead of 56 (290
+// MB: 5.7 TB/s), 32 sequences of 4 55 instead of 69; one of 8 would take 29 instead of 27.
+template <int DK, bool WIDE, bool ONE, bool MANY, typename T>
+__global__ __launch_bounds__(kTokThreads, MANY ? 4 : 2) void deltanet_tokens_kernel(const DnTokens a) {
     constexpr int C4 = DK / 4;          // float4 chunks per state row
-    constexpr int G = C4 < 4 ? C4 : 4;  // lanes per row
+    constexpr int G = C4 < 4 ? C4 : C4 > 32 ? 8 : 4;  // lanes per row
     constexpr int CPL = C4 / G;         // chunks per lane
     constexpr int RPW = kWave / G;      // rows per wave and pass
     constexpr int KM = WIDE ? kDnMaxConv : 4;                                           // rows of the convolution
     constexpr int MC = WIDE ? (2 * DK + kDnMaxDv + kTokThreads - 1) / kTokThreads : 1;  // channels per thread
-    __shared__ float s_q[DK], s_k[DK];
+    __shared__ __align__(16) float s_q[DK], s_k[DK];
     __shared__ float s_v[kDnMaxDv], s_o[kDnMaxDv];
     __shared__ float s_gb[2];
     const int b = blockIdx.x / a.nv, hv = blockIdx.x % a.nv, hk = hv / a.rep, ri = hv % a.rep;
@@ -130,34 +132,33 @@ __global__ __launch_bounds__(kTokThreads) void deltanet_tokens_kernel(const DnTo
         const float g = s_gb[0], beta = s_gb[1];
 
         // 3. recurrence: G lanes per row, chunk m of lane j is chunk j + G * m of the row
-        float4 qv[CPL], kv[CPL];
-#pragma unroll
-        for (int m = 0; m < CPL; ++m) {
-            const int e = 4 * (gl + G * m);
-            qv[m] = make_float4(s_q[e] * scq * (inv * inv), s_q[e + 1] * scq * (inv * inv), s_q[e + 2] * scq * (inv * inv),
-                                s_q[e + 3] * scq * (inv * inv));
-            kv[m] = make_float4(s_k[e] * sck * inv, s_k[e + 1] * sck * inv, s_k[e + 2] * sck * inv, s_k[e + 3] * sck * inv);
-        }
+        auto part = [&](const float *from, int m, float by, float and_by) {
+            const float4 x = *reinterpret_cast<const float4 *>(from + 4 * (gl + G * m));
+            return make_float4(x.x * by * and_by, x.y * by * and_by, x.z * by * and_by, x.w * by * and_by);
+        };
         auto turn = [&](float4(&s)[CPL], int row) {
             float mem = 0.f;
 #pragma unroll
             for (int m = 0; m < CPL; ++m) {
+                const float4 k = part(s_k, m, sck, inv);
                 s[m].x *= g;
                 s[m].y *= g;
                 s[m].z *= g;
                 s[m].w *= g;
-                mem += s[m].x * kv[m].x + s[m].y * kv[m].y + s[m].z * kv[m].z + s[m].w * kv[m].w;
+                mem += s[m].x * k.x + s[m].y * k.y + s[m].z * k.z + s[m].w * k.w;
             }
             mem = segment_sum(mem, G);
             const float delta = (s_v[row] - mem) * beta;
+            if constexpr (MANY) asm volatile("" ::: "memory");  // read again, for fewer registers
             float o = 0.f;
 #pragma unroll
             for (int m = 0; m < CPL; ++m) {
-                s[m].x += kv[m].x * delta;
-                s[m].y += kv[m].y * delta;
-                s[m].z += kv[m].z * delta;
-                s[m].w += kv[m].w * delta;
-                o += s[m].x * qv[m].x + s[m].y * qv[m].y + s[m].z * qv[m].z + s[m].w * qv[m].w;
+                const float4 k = part(s_k, m, sck, inv), q = part(s_q, m, scq, inv * inv);
+                s[m].x += k.x * delta;
+                s[m].y += k.y * delta;
+                s[m].z += k.z * delta;
+                s[m].w += k.w * delta;
+                o += s[m].x * q.x + s[m].y * q.y + s[m].z * q.z + s[m].w * q.w;
             }
             o = segment_sum(o, G);
             if (gl == 0) s_o[row] = o;
@@ -206,14 +207,12 @@ __global__ __launch_bounds__(kRingThreads) void deltanet_ring_kernel(const DnTok
 template <int DK, typename T>
 void launch_tokens(const DnTokens &a, hipStream_t s) {
     const dim3 grid(a.B * a.nv), block(kTokThreads);
-    const bool one = a.max_tokens == 1;
-    if (a.K <= 4 && 2 * a.dk + a.dv <= kTokThreads) {
-        if (one) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, true, T>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, false, T>), grid, block, 0, s, a);
-    } else {
-        if (one) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, true, true, T>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((deltanet_tokens_kernel<DK, true, false, T>), grid, block, 0, s, a);
-    }
+    const bool one = a.max_tokens == 1, wide = a.K > 4 || 2 * a.dk + a.dv > kTokThreads, many = a.B * a.nv > kCus;
+    if (wide && one) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, true, true, false, T>), grid, block, 0, s, a);
+    else if (wide) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, true, false, false, T>), grid, block, 0, s, a);
+    else if (one) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, true, true, T>), grid, block, 0, s, a);
+    else if (many) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, false, true, T>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, false, false, T>), grid, block, 0, s, a);
     if (!one) {
         const int parts = (a.convD + kRingThreads - 1) / kRingThreads;
         hipLaunchKernelGGL(deltanet_ring_kernel<T>, dim3(a.B * parts), dim3(kRingThreads), 0, s, a, parts);
