@@ -68,6 +68,7 @@ struct DnChunks {
     int32_t cap;           // chunks that there is room for
     int32_t planes;
     int32_t chunk0, span;  // a launch's chunks: those of a sequence from chunk0 on, span at most
+    int32_t least;         // tokens of a sequence that comes through here
 };
 
 __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -870,7 +871,8 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
     }
 }
 
-// One workgroup per (chunk, value head): the gated norm, and the ring's rows of a sequence's last chunk.  CW * 32 columns at
+// One workgroup per (chunk, value head): the gated norm, and the ring's rows of a sequence's last chunk, also of one that has
+// gone token after token.  CW * 32 columns at
 // most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.
 template <int CW, bool HQ, typename T>
 __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w) {
@@ -884,44 +886,46 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
     const int m = it.m, tokens = it.tokens, here_tokens = min(tokens - m * kC, kC);
     const int64_t n0 = it.n0 + static_cast<int64_t>(m) * kC;
 
-    // output gates and the norm's weights, as they will be used
-    const int e = min(4 * (tid % L), a.dv - 4), row0 = tid / L;
-    const bool real = 4 * (tid % L) < a.dv;
-    const T *zr = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride + z_at(a, hv, 0) + e;
-    Four<T> z[R];
+    if (tokens >= w.least) {
+        // output gates and the norm's weights, as they will be used
+        const int e = min(4 * (tid % L), a.dv - 4), row0 = tid / L;
+        const bool real = 4 * (tid % L) < a.dv;
+        const T *zr = static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride + z_at(a, hv, 0) + e;
+        Four<T> z[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) z[i].load(zr + min(row0 + i * ROWS, here_tokens - 1) * a.qkvz_stride);
-    f4_t nw;
+        for (int i = 0; i < R; ++i) z[i].load(zr + min(row0 + i * ROWS, here_tokens - 1) * a.qkvz_stride);
+        f4_t nw;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) nw[k] = a.norm_w[e + k];
-    const int64_t o0 = head * cts * kRowTiles * kWave + lane;
+        for (int k = 0; k < 4; ++k) nw[k] = a.norm_w[e + k];
+        const int64_t o0 = head * cts * kRowTiles * kWave + lane;
 #pragma unroll
-    for (int i = 0; i < CW * 2 * kRowTiles * kWave / kFinishThreads; ++i) {
-        const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
-        f4_t o;
-        if (HQ) o = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
-        else o = __builtin_convertvector(__builtin_bit_cast(h4_t, static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave]), f4_t) * w.back[head * cts + ct];
+        for (int i = 0; i < CW * 2 * kRowTiles * kWave / kFinishThreads; ++i) {
+            const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
+            f4_t o;
+            if (HQ) o = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
+            else o = __builtin_convertvector(__builtin_bit_cast(h4_t, static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave]), f4_t) * w.back[head * cts + ct];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[k];
-    }
-    lds_barrier();
+            for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[k];
+        }
+        lds_barrier();
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int t = row0 + i * ROWS;
-        const f4_t o = *reinterpret_cast<const f4_t *>(s_o + t * kRow + e);
-        const float ss = real ? o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3] : 0.f;
-        const float sc = __builtin_amdgcn_rsqf(lanes_sum<L>(ss) / static_cast<float>(a.dv) + a.eps);
-        const f4_t zi = z[i].get();
-        f4_t y;
+        for (int i = 0; i < R; ++i) {
+            const int t = row0 + i * ROWS;
+            const f4_t o = *reinterpret_cast<const f4_t *>(s_o + t * kRow + e);
+            const float ss = real ? o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3] : 0.f;
+            const float sc = __builtin_amdgcn_rsqf(lanes_sum<L>(ss) / static_cast<float>(a.dv) + a.eps);
+            const f4_t zi = z[i].get();
+            f4_t y;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = o[k] * (sc * nw[k]) * silu_hw(zi[k]);
-        if (t >= here_tokens || !real) continue;
-        const int64_t at = ((n0 + t) * a.nv + hv) * a.dv + e;
-        if (a.out_f32) {
-            *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at) = y;
-        } else {
-            const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(lo, hi);
+            for (int k = 0; k < 4; ++k) y[k] = o[k] * (sc * nw[k]) * silu_hw(zi[k]);
+            if (t >= here_tokens || !real) continue;
+            const int64_t at = ((n0 + t) * a.nv + hv) * a.dv + e;
+            if (a.out_f32) {
+                *reinterpret_cast<f4_t *>(static_cast<float *>(a.out) + at) = y;
+            } else {
+                const uint32_t lo = dn_bf16(y[0]) | static_cast<uint32_t>(dn_bf16(y[1])) << 16, hi = dn_bf16(y[2]) | static_cast<uint32_t>(dn_bf16(y[3])) << 16;
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(lo, hi);
+            }
         }
     }
     if ((m + 1) * kC < tokens) return;
@@ -999,7 +1003,9 @@ template <int DK, bool HQ, typename T>
 void launch(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     launch_prepare<DK, HQ, T>(a, w, s);
     launch_chain<DK, HQ>(a, w, s);
-    launch_finish<HQ, T>(a, w, s);
+    DnTokens all = a;
+    all.least = 1;
+    launch_finish<HQ, T>(all, w, s);
 }
 template <bool HQ, typename T>
 void launch_dk(const DnTokens &a, const DnChunks &w, hipStream_t s) {
@@ -1026,6 +1032,7 @@ void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_
     DnChunks w{};
     w.cap = static_cast<int32_t>(cap_of(a.B, a.N));
     w.planes = planes_of(a, in_f32);
+    w.least = a.least;
     const Parts parts = parts_of(a.nk, a.nv, a.dk, a.dv, w.cap, w.planes);
     uint8_t *p = static_cast<uint8_t *>(ws);
     auto take = [&](size_t n) {

@@ -213,7 +213,7 @@ void launch_tokens(const DnTokens &a, hipStream_t s) {
     else if (one) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, true, true, T>), grid, block, 0, s, a);
     else if (many) hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, false, true, T>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((deltanet_tokens_kernel<DK, false, false, false, T>), grid, block, 0, s, a);
-    if (!one) {
+    if (!one && a.most == INT32_MAX) {  // else deltanet_chunks.hip's last launch does it
         const int parts = (a.convD + kRingThreads - 1) / kRingThreads;
         hipLaunchKernelGGL(deltanet_ring_kernel<T>, dim3(a.B * parts), dim3(kRingThreads), 0, s, a, parts);
     }
