@@ -252,11 +252,12 @@ int check_sizes(const swq_deltanet_layer *l, const swq_deltanet_batch *b) {
 // Most tokens of one sequence.
 int most_tokens(const swq_deltanet_batch *b) { return b->starts ? std::min(b->max_tokens, b->tokens) : b->tokens / b->sequences; }
 
-// From so many tokens of a sequence on, those of a batch go a chunk at a time.  At 32 value heads of 128 a sequence of 8
-// (12, 16) takes 27 us (36, 46) token after token and 35 us in chunks; 32 of them 110 (150, 192) and 154 (160, 165).
-constexpr int kChunksFrom = 12;
+// From so many tokens of a sequence on, those of a batch go a chunk at a time; from more where workgroups are as many as
+// CUs, which token after token keeps busy.  At 32 value heads of 128, 1 sequence of 8 (12, 16) takes 28 us (38, 49) token after
+// token and 34 us in chunks, 4 of them 29 (38, 49) and 43, 8 of 16 (24) 50 (71) and 63, 32 of them 137 (195) and 164.
+constexpr int kChunksFrom = 12, kChunksFromMany = 20;
 // Beside a sequence of so many, those of up to kFew go token after token all the same, in launches of their own: with one of
-// 600 tokens, 31 of 1 (4, 8) take 113 us (143, 183) so and 199 (202, 207) in chunks, but a single one of 8 87 and 59.
+// 600 tokens, 31 of 1 (4) take 106 us (125) so and 199 (202) in chunks, but a single one of 1 65 and 59, of 8 87 and 60.
 constexpr int kFew = 4;
 
 bool misaligned(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
@@ -320,7 +321,7 @@ extern "C" int swq_deltanet_tokens(const swq_deltanet_layer *l, const swq_deltan
     hipStream_t s = static_cast<hipStream_t>(stream);
     // chunks are loaded and stored four elements at a time
     const bool four = !misaligned(qkvz, 4 * in) && a.qkvz_stride % 4 == 0 && a.qkvz_stride < 1 << 24 && !misaligned(out, a.out_f32 ? 16 : 8) && !misaligned(a.conv_w, 16);
-    const bool chunks = a.max_tokens >= kChunksFrom && four && deltanet_chunks_take(l);
+    const bool chunks = a.max_tokens >= (a.B * a.nv < kCus ? kChunksFrom : kChunksFromMany) && four && deltanet_chunks_take(l);
     // where no sequence can be of another length, nothing is launched for the short ones
     a.least = 1;
     a.most = !chunks ? INT32_MAX : a.B > 1 && a.starts ? kFew : 0;

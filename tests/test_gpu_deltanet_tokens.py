@@ -164,7 +164,7 @@ def test_sizes_of_values(size):
     check(c, c.run())
 
 
-@pytest.mark.parametrize("lengths", [[64, 4, 5, 0, 3, 12, 1, 2, 11, 13], [4, 4, 12], [11, 11, 3]], ids=str)
+@pytest.mark.parametrize("lengths", [[64, 4, 5, 0, 3, 12, 1, 2, 11, 13], [4, 4, 12], [11, 11, 3], [19, 1, 5, 4, 2, 0, 18, 12, 13], [20, 1, 5, 4, 2, 0, 18, 12, 13]], ids=str)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_short_ones_beside_long_ones(lengths, dtype):
     c = Batch(BIG, lengths, dtype, seed=18, K=3)
