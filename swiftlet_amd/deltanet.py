@@ -19,9 +19,12 @@ def _row_stride(t, rows, width, what, device):
     """Elements between the rows of a tensor [rows, width] (or wider) whose rows are contiguous."""
     if t.get_device() != device:
         raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": not on the block's device")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.stride(1) != 1 or (rows > 1 and t.stride(0) < width):
+    if t.dim() != 2:
         raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
-    return t.stride(0) if rows > 1 else 0
+    (n, w), (row, element) = t.shape, t.stride()
+    if n != rows or w < width or element != 1 or (rows > 1 and row < width):
+        raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
+    return row if rows > 1 else 0
 
 
 class DeltaNetGPU:
@@ -53,7 +56,9 @@ class DeltaNetGPU:
             layout=layout, norm_eps=eps, reserved=0, conv_weight=self.conv_weight.data_ptr(),
             a_log=self.a_log.data_ptr(), dt_bias=self.dt_bias.data_ptr(), norm_weight=self.norm_weight.data_ptr())
         self._projs = DescArray()
-        self._scratch = self.lib.swq_deltanet_scratch_floats(ctypes.byref(self._c))
+        self._ref = ctypes.byref(self._c)
+        self._scratch = self.lib.swq_deltanet_scratch_floats(self._ref)
+        self._slot_bytes = self.lib.swq_deltanet_slot_bytes(self._ref)
 
     @property
     def state_bytes(self) -> int:
@@ -77,7 +82,9 @@ class DeltaNetGPU:
 
     @property
     def slot_bytes(self) -> int:
-        return self.lib.swq_deltanet_slot_bytes(ctypes.byref(self._c))
+        if self._slot_bytes == 0:
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "deltanet_slot_bytes")
+        return self._slot_bytes
 
     def new_states(self, slots: int):
         """Fresh states (zeros) of `slots` sequences, as a flat uint8 device tensor."""
@@ -118,23 +125,24 @@ class DeltaNetGPU:
                 with torch.cuda.stream(stream):
                     return self.prefill(qkvz, ba, states, positions, ws, starts, slots, max_tokens)
             out = torch.empty((qkvz.shape[0], self.value_dim), dtype=qkvz.dtype, device=qkvz.device)
-        what, at, B, N = "deltanet_tokens", self.conv_weight.get_device(), positions.numel(), qkvz.shape[0]
+        at, B, N, dtype, i32, u8 = self.conv_weight.get_device(), positions.numel(), len(qkvz), qkvz.dtype, torch.int32, torch.uint8
         if at < 0 or at != torch.cuda.current_device():
-            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, what + ": the block is not on the current device")
-        if ba.dtype != qkvz.dtype:
-            raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, what + ": ba")
+            raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "deltanet_tokens: the block is not on the current device")
+        if ba.dtype != dtype:
+            raise SwqError(_lib.SWQ_ERR_UNSUPPORTED_DTYPE, "deltanet_tokens: ba")
         if out.numel() != N * self.value_dim:
-            raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what + ": out")
-        b = DeltaNetBatch(B, N, max_tokens or max(N, 1), states.numel() // self.slot_bytes,
-                          _ptr(starts, B + 1, what + ": starts", at, torch.int32),
-                          _ptr(positions, 1, what + ": positions", at, torch.int32),
-                          _ptr(slots, B, what + ": slots", at, torch.int32),
-                          _row_stride(qkvz, N, self.conv_dim + self.value_dim, what + ": qkvz", at),
-                          _row_stride(ba, N, 2 * self.nv, what + ": ba", at), 0)
+            raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "deltanet_tokens: out")
+        states_bytes = states.numel()
+        b = DeltaNetBatch(B, N, max_tokens or max(N, 1), states_bytes // self.slot_bytes,
+                          None if starts is None else _ptr(starts, B + 1, "deltanet_tokens: starts", at, i32),
+                          _ptr(positions, 1, "deltanet_tokens: positions", at, i32),
+                          None if slots is None else _ptr(slots, B, "deltanet_tokens: slots", at, i32),
+                          _row_stride(qkvz, N, self.conv_dim + self.value_dim, "deltanet_tokens: qkvz", at),
+                          _row_stride(ba, N, 2 * self.nv, "deltanet_tokens: ba", at), 0)
         check(self.lib.swq_deltanet_tokens(
-            ctypes.byref(self._c), ctypes.byref(b), qkvz.data_ptr(), ba.data_ptr(), _code(qkvz, what),
-            _ptr(states, 1, what + ": states", at, torch.uint8), states.numel(), _ptr(out, 0, what + ": out", at), _code(out, what),
-            _ptr(ws, 1, what + ": ws", at, torch.uint8), ws.numel(), _stream_handle(stream)), what)
+            self._ref, ctypes.byref(b), qkvz.data_ptr(), ba.data_ptr(), _code(qkvz, "deltanet_tokens"),
+            _ptr(states, 1, "deltanet_tokens: states", at, u8), states_bytes, _ptr(out, 0, "deltanet_tokens: out", at),
+            _code(out, "deltanet_tokens"), _ptr(ws, 1, "deltanet_tokens: ws", at, u8), ws.numel(), _stream_handle(stream)), "deltanet_tokens")
         return out
 
     def step_batch(self, qkvz, ba, states, positions, ws, slots=None, out=None, stream=None):
