@@ -312,7 +312,9 @@ typedef struct swq_deltanet_batch {
 /* Workspace bytes of swq_deltanet_tokens for calls of up to batch->sequences
  * sequences, batch->tokens tokens and batch->max_tokens of one sequence (starts
  * NULL: tokens / sequences).  Of starts and slot only whether they are NULL is
- * read, of positions nothing.  0 on bad input. */
+ * read, of positions nothing.  Prompts: it grows with the tokens of several
+ * sequences (80 KB each at 32 value heads of 128), up to 2,048 of one alone.
+ * 0 on bad input. */
 size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch);
 
 /* swq_deltanet_step for the tokens of many sequences, prompts or one token

@@ -323,7 +323,8 @@ __device__ __forceinline__ void put_transposed(uint4 *to, int tile, int t0, int 
 }
 
 // One workgroup per (chunk, key head): waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query tile; then
-// their products.  The gates of the key head's value heads beside it.
+// their products.  The gates of the key head's value heads beside it.  32 chunks of 16 heads of 128 take 17 us: one round of
+// two workgroups to a CU, so what bounds it is its own chain of loads, convolution, norms and products.
 template <int DK, bool HQ, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const DnTokens a, const DnChunks w) {
     constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = DK / 16;
@@ -424,7 +425,9 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     }
 }
 
-// One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.
+// One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.  32 chunks of
+// 32 heads of 128 take 42 us: two rounds of two workgroups to a CU (128 registers; with 4 waves and twice the columns each
+// they spill: 53), 10 to 16 thousand clocks up to the inverted diagonal blocks, 5 for the others, 4 each for W and U.
 template <int DK, bool HQ, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const DnTokens a, const DnChunks w) {
     constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = kVBlock / 16;
@@ -630,7 +633,9 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 // One workgroup per (sequence, value head, CT * 16 columns of the state), three quarters of waves at three tasks: waves 0 to
 // 3 make d of a quarter of the chunk's tokens each, waves 4 to 7 the next state, of whose rows they hold a quarter each, and
 // waves 8 to 11 the outputs, off the chain from chunk to chunk.  While one kind computes, the others have their loads
-// and stores issued.
+// and stores issued.  A chunk takes 1.2 us at 256 workgroups (its products and barriers alone 0.8): each reads its head's
+// operands for itself, 19 TB/s from the L2s in all, of 22 to 28 that loads alone reach.  Outputs in a launch of their own,
+// from S and d stored per chunk, took 145 us instead of 109 for 64 chunks.
 template <int DK, int CT, bool HQ>
 __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const DnTokens a, const DnChunks w, int groups) {
     constexpr int KS = DK / 32, DT = DK / 64, PL = HQ ? 2 : 1;  // DT: row tiles of the state per wave
@@ -873,7 +878,8 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
 
 // One workgroup per (chunk, value head): the gated norm, and the ring's rows of a sequence's last chunk, also of one that has
 // gone token after token.  CW * 32 columns at
-// most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.
+// most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.  32
+// chunks of 32 heads of 128 take 16 us for 34 MB: one round of workgroups, loads and stores in turn.
 template <int CW, bool HQ, typename T>
 __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w) {
     constexpr int L = CW * 8, ROWS = kFinishThreads / L, R = kC / ROWS, kRow = CW * 32 + 4;
@@ -991,7 +997,7 @@ void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
 template <int DK, bool HQ>
 void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
-    // 32 columns to a workgroup where those of 16 would not find a CU each: at 32 value heads of 128 four prompts of 1,000
+    // 32 columns to a workgroup where those of 16 would not find a CU each: at 32 value heads of 128 four prompts of 2,500
     // tokens in all take 138 us instead of 155, but one of 4,096 231 instead of 221
     const int cts = a.dv / 16, ct = cts % 2 == 0 && static_cast<int64_t>(a.B) * a.nv * cts > kCus ? 2 : 1;
     const dim3 grid(static_cast<uint32_t>(units * (cts / ct))), block(kChainThreads);
