@@ -1,4 +1,4 @@
-"""The gated DeltaNet block over the tokens of many sequences, in 64 bits — TEST INFRASTRUCTURE ONLY, the checker of
+"""The gated DeltaNet block over the tokens of many sequences, in 64 bits — TEST INFRASTRUCTURE ONLY, what is held against
 swq_deltanet_tokens: QwenCPUModel.deltaNetForward's formulas (QwenCPUModel.swift:371-496) token after token, as
 deltanet_ref.deltanet_core has them in 32 bits.  torch, on any device."""
 

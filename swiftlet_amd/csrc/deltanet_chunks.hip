@@ -438,9 +438,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     const uint32_t unit = blockIdx.x / 8 / a.rep * 8 + blockIdx.x % 8;
     const int hk = unit % a.nk, hv = hk * a.rep + blockIdx.x / 8 % a.rep;
     const int64_t chunk = unit / a.nk, head = chunk * a.nv + hv;
-    Chunk it;
-    if (chunk >= w.cap || !find_chunk(a, w, static_cast<int>(chunk), it)) return;
-    const int m = it.m, tokens = it.tokens, n0 = it.n0;
+    if (chunk >= w.cap) return;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), col = lane & 15, g = lane >> 4;
     const int tile = wave & 3;
     const bool keys = wave < 4;
@@ -451,6 +449,10 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     f4_t dots[kRowTiles];
 #pragma unroll
     for (int jt = 0; jt < kRowTiles; ++jt) dots[jt] = dots_at[min(jt, tile) * kWave];
+    asm volatile("" ::: "memory");  // in flight while the chunk is looked up
+    Chunk it;
+    if (!find_chunk(a, w, static_cast<int>(chunk), it)) return;
+    const int m = it.m, tokens = it.tokens, n0 = it.n0;
 
     const int ch = 4 * (lane % (kVBlock / 4)), t0 = N * (lane / (kVBlock / 4));
     f4_t v[N];
@@ -886,9 +888,25 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
     __shared__ __align__(16) float s_o[kC * kRow];
     const int hv = blockIdx.x % a.nv, hk = hv / a.rep, ri = hv - hk * a.rep;
     const int64_t chunk = blockIdx.x / a.nv, head = chunk * a.nv + hv;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g = lane >> 4, cts = a.dv / 16;
+    constexpr int PARTS = CW * 2 * kRowTiles * kWave / kFinishThreads;
+    f4_t o[PARTS];
+    uint2 o_half[PARTS];
+    float back[PARTS];
+    const int64_t o0 = head * cts * kRowTiles * kWave + lane;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
+        if (HQ) {
+            o[i] = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
+        } else {
+            o_half[i] = static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
+            back[i] = w.back[head * cts + ct];
+        }
+    }
+    asm volatile("" ::: "memory");  // in flight while the chunk is looked up
     Chunk it;
     if (!find_chunk(a, w, static_cast<int>(chunk), it)) return;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g = lane >> 4, cts = a.dv / 16;
     const int m = it.m, tokens = it.tokens, here_tokens = min(tokens - m * kC, kC);
     const int64_t n0 = it.n0 + static_cast<int64_t>(m) * kC;
 
@@ -903,27 +921,24 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
         f4_t nw;
 #pragma unroll
         for (int k = 0; k < 4; ++k) nw[k] = a.norm_w[e + k];
-        const int64_t o0 = head * cts * kRowTiles * kWave + lane;
 #pragma unroll
-        for (int i = 0; i < CW * 2 * kRowTiles * kWave / kFinishThreads; ++i) {
+        for (int i = 0; i < PARTS; ++i) {
             const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
-            f4_t o;
-            if (HQ) o = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
-            else o = __builtin_convertvector(__builtin_bit_cast(h4_t, static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave]), f4_t) * w.back[head * cts + ct];
+            if (!HQ) o[i] = __builtin_convertvector(__builtin_bit_cast(h4_t, o_half[i]), f4_t) * back[i];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[k];
+            for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[i][k];
         }
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int t = row0 + i * ROWS;
-            const f4_t o = *reinterpret_cast<const f4_t *>(s_o + t * kRow + e);
-            const float ss = real ? o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3] : 0.f;
+            const f4_t ot = *reinterpret_cast<const f4_t *>(s_o + t * kRow + e);
+            const float ss = real ? ot[0] * ot[0] + ot[1] * ot[1] + ot[2] * ot[2] + ot[3] * ot[3] : 0.f;
             const float sc = __builtin_amdgcn_rsqf(lanes_sum<L>(ss) / static_cast<float>(a.dv) + a.eps);
             const f4_t zi = z[i].get();
             f4_t y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = o[k] * (sc * nw[k]) * silu_hw(zi[k]);
+            for (int k = 0; k < 4; ++k) y[k] = ot[k] * (sc * nw[k]) * silu_hw(zi[k]);
             if (t >= here_tokens || !real) continue;
             const int64_t at = ((n0 + t) * a.nv + hv) * a.dv + e;
             if (a.out_f32) {
@@ -940,9 +955,9 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
     const T *last = static_cast<const T *>(a.qkvz) + (it.n0 + static_cast<int64_t>(tokens) - 1) * a.qkvz_stride;
     const int channels = a.dv + (ri == 0 ? 2 * a.dk : 0), rows = min(tokens, a.K);
     for (int i = tid; i < channels * rows; i += kFinishThreads) {
-        const int back = i / channels, c = i - back * channels;
+        const int ago = i / channels, c = i - ago * channels;
         const int ch = c < a.dv ? 2 * a.keyD + hv * a.dv + c : hk * a.dk + (c - a.dv) % a.dk + (c - a.dv >= a.dk ? a.keyD : 0);
-        ring[static_cast<int64_t>((it.pos + static_cast<uint32_t>(tokens - 1 - back)) % a.K) * a.convD + ch] = dn_load(last - back * a.qkvz_stride, mixed_at(a, ch));
+        ring[static_cast<int64_t>((it.pos + static_cast<uint32_t>(tokens - 1 - ago)) % a.K) * a.convD + ch] = dn_load(last - ago * a.qkvz_stride, mixed_at(a, ch));
     }
 }
 
