@@ -426,7 +426,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
 }
 
 // One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.  32 chunks of
-// 32 heads of 128 take 42 us: two rounds of two workgroups to a CU (128 registers; with 4 waves and twice the columns each
+// 32 heads of 128 take 40 us: two rounds of two workgroups to a CU (128 registers; with 4 waves and twice the columns each
 // they spill: 53), 10 to 16 thousand clocks up to the inverted diagonal blocks, 5 for the others, 4 each for W and U.
 template <int DK, bool HQ, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const DnTokens a, const DnChunks w) {

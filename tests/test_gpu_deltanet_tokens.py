@@ -365,3 +365,36 @@ def test_refusals_in_python():
             c.block.prefill(**{**good, **kw})
     torch.cuda.synchronize()
     assert torch.equal(c.states, c.before)
+
+
+def test_offsets_past_32_bits():
+    """A prompt of more than 2^31 elements: the bits of the same in two calls, whose second begins with a span of its own;
+    states more than 4 GB apart."""
+    c = Batch(BIG, [16], "bf16", seed=28)
+    T, cut, slots = 180000, 86 * 2048, 2100
+    assert T * (c.conv + c.val) > 2 ** 31 and (slots - 1) * c.block.slot_bytes > 2 ** 32
+    g = torch.Generator(device="cuda").manual_seed(29)
+    qkvz = torch.randn((4500, c.conv + c.val), generator=g, device="cuda").bfloat16().repeat(T // 4500, 1)
+    ba = torch.randn((T, 64), generator=g, device="cuda").bfloat16()
+    states = torch.zeros(slots * c.block.slot_bytes, dtype=torch.uint8, device="cuda")
+    last, first = (torch.tensor([n], dtype=torch.int32, device="cuda") for n in (slots - 1, 0))
+    ws, at = c.block.new_batch_workspace(1, T), torch.zeros(1, dtype=torch.int32, device="cuda")
+    whole = c.block.prefill(qkvz, ba, states, at, ws, slots=last)
+    parts = [c.block.prefill(qkvz[:cut], ba[:cut], states, at, ws, slots=first), c.block.prefill(qkvz[cut:], ba[cut:], states, at + cut, ws, slots=first)]
+    assert torch.equal(whole[:cut], parts[0]) and torch.equal(whole[cut:], parts[1])
+    n = c.block.slot_bytes
+    assert torch.equal(states[:n], states[-n:]) and bool(states[:n].any())
+    assert not bool(states[n:2 * n].any()) and not bool(states[-2 * n:-n].any())
+    one = c.block.step_batch(qkvz[-1:], ba[-1:], states, at + T, ws, slots=last)
+    assert torch.equal(one, c.block.step_batch(qkvz[-1:], ba[-1:], states, at + T, ws, slots=first))
+    rows = qkvz[[0, T - 1]]
+    far = qkvz.as_strided(rows.shape, ((T - 1) * rows.shape[1], 1))
+    states[-n:].copy_(states[:n])
+    assert torch.equal(c.block.prefill(far, ba[:2], states, at, ws, slots=last), c.block.prefill(rows, ba[:2], states, at, ws, slots=first))
+    assert torch.equal(states[:n], states[-n:])
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 200])
+def test_more_sequences_than_lanes(B):
+    c = Batch((1, 2, 64, 32), [(37 * i) % 90 if i % 7 else 0 for i in range(B)], "f32", True, seed=B)
+    check(c, c.run())
