@@ -62,6 +62,10 @@ class RopeGPU:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "RopeGPU: rope_type " + str(kind))
         scaling = None
         if _KINDS[kind] != _lib.SWQ_ROPE_PLAIN:
+            # what would change the angles or the magnitude and is not in RopeScaling
+            odd = [k for k, plain in (("mscale", None), ("mscale_all_dim", None), ("truncate", True)) if sc.get(k, plain) not in (None, plain)]
+            if odd:
+                raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "RopeGPU: " + ", ".join(odd))
             scaling = RopeScaling(kind, float(sc["factor"]), int(sc.get("original_max_position_embeddings", c.get("max_position_embeddings", 0))),
                                   float(sc.get("beta_fast", 32.0)), float(sc.get("beta_slow", 1.0)), sc.get("attention_factor"))
         return cls(int(c["head_dim"] * part), theta, scaling=scaling, device=device)

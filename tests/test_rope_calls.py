@@ -94,6 +94,11 @@ def test_config():
     assert (r.rot, r.theta, r.scaling) == (64, 5e6, RopeScaling("yarn", 2.0, 8192, 16.0, 1.0, 1.5))
     with pytest.raises(_lib.SwqError):
         RopeGPU.from_config({**base, "rope_scaling": {"rope_type": "something"}}, device="cpu")
+    yarn = {"rope_type": "yarn", "factor": 4.0}
+    for odd in ({"mscale": 1.0}, {"mscale_all_dim": 0.7}, {"truncate": False}):
+        with pytest.raises(_lib.SwqError):
+            RopeGPU.from_config({**base, "rope_scaling": {**yarn, **odd}}, device="cpu")
+    assert RopeGPU.from_config({**base, "rope_scaling": {**yarn, "truncate": True, "mscale": None}}, device="cpu").scaling == RopeScaling("yarn", 4.0, 4096)
     with pytest.raises(_lib.SwqError):
         RopeGPU(64, 1e6, layout="other")
     with pytest.raises(_lib.SwqError):
