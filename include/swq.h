@@ -322,13 +322,12 @@ size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, cons
  * dtype (SWQ_F32 / SWQ_BF16), in the layer's layout; out [tokens][nv*dv] of
  * out_dtype.  Each sequence goes on from its state, which is updated in place
  * (f32): the results of as many swq_deltanet_step calls, up to the order of f32
- * sums (prompts: products of 22 bits; for outputs alone, where they and the
- * projections are bf16, of 11).  The same call gives the same bits again.  Any
- * layer that swq_deltanet_step takes; key heads of 64 or 128 with value heads of
- * a multiple of 16 up to 256, rows at multiples of 4 elements and aligned to 4,
- * take prompts 64 tokens at a time, others token after token.  No output overlaps
- * an input or the workspace.  states and workspace: 256-byte aligned; the
- * workspace needs no preparation. */
+ * sums (prompts: products of 22 bits), bf16 outputs rounded once.  The same call
+ * gives the same bits again.  Any layer that swq_deltanet_step takes; key heads
+ * of 64 or 128 with value heads of a multiple of 16 up to 256, rows at multiples
+ * of 4 elements and aligned to 4, take prompts 64 tokens at a time, others token
+ * after token.  No output overlaps an input or the workspace.  states and
+ * workspace: 256-byte aligned; the workspace needs no preparation. */
 int swq_deltanet_tokens(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch, const void *qkvz,
                         const void *ba, int dtype, void *states, size_t states_bytes, void *out, int out_dtype,
                         void *ws, size_t ws_bytes, void *stream);

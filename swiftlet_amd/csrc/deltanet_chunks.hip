@@ -17,8 +17,8 @@
 // nothing) and take fixed ones.  v, d and S have no bound: one per (sequence, head, columns), from the largest v and
 // S, brings them to 32 .. 64, from where S grows by sqrt(tokens) at most, so past f16's largest only after 2^20
 // tokens that all agree.  Sums are f32, c is summed and subtracted in 64 bits, and T is made by f32
-// substitution and f32 matrix instructions.  Where projections and out are bf16, q S and P d take the high parts alone:
-// their terms are off by 2^-12, an eighth of what the projections' own rounding makes them.
+// substitution and f32 matrix instructions.  That holds whatever the types of the projections and of out: bf16 outputs are
+// the f32 ones rounded once.
 //
 // Layout.  A matrix instruction's result has a lane's 4 numbers in consecutive rows of one column; its operands have 8
 // numbers along the contraction.  The order of a contraction is free, so operands take the order in which two
@@ -50,23 +50,18 @@ constexpr int kVBlock = 128;  // columns of v that are prepared at once
 // enough above 2^-14 for their low parts: with 256 and 1 / 256 the states of 4,096 tokens were off by 7e-6, with 16 by
 // 5e-7, with 8 by 3e-7, and outputs of f32 by 2e-7.  P's is q's, as their products meet in a sum.
 constexpr float kScaleK = 8.f, kScaleT = 16.f, kScaleP = kScaleK, kScaleE = 1.f / kScaleK;
-constexpr float kHalfO = 1.f / kScaleK;  // of outputs as f16 numbers
 
 // The workspace: operands of every (chunk, key head) and (chunk, value head).
 struct DnChunks {
-    uint4 *k, *q, *w, *p;  // f16 operands; k, w two planes, q, p `planes`
+    uint4 *k, *q, *w, *p;  // f16 operands, two planes each
     f4_t *u;               // [chunk][nv][dv / 16][4][64]
     float *decay;          // [chunk][nv][2][64]: e^c_i and kScaleE e^(c_last - c_i)
     double *sums;          // [chunk][nv][64]: c, in units of log 2
     float *beta;           // [chunk][nv][64]
     float *vmax;           // [chunk][nv]
     f4_t *dots;            // [chunk][nk][2][10][64]: k_i.k_j and k_j.q_i, tiles of the lower triangle
-    // the outputs before their norm, as the results lie, [chunk][nv][dv / 16][4][64] lanes: f32 with two planes; else f16
-    // and in the chain's scale, which its inverse ends
-    void *o;
-    float *back;           // [chunk][nv][dv / 16]
+    f4_t *o;               // the outputs before their norm, as the results lie: [chunk][nv][dv / 16][4][64]
     int32_t cap;           // chunks that there is room for
-    int32_t planes;
     int32_t chunk0, span;  // a launch's chunks: those of a sequence from chunk0 on, span at most
     int32_t least;         // tokens of a sequence that comes through here
 };
@@ -325,9 +320,9 @@ __device__ __forceinline__ void put_transposed(uint4 *to, int tile, int t0, int 
 // One workgroup per (chunk, key head): waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query tile; then
 // their products.  The gates of the key head's value heads beside it.  32 chunks of 16 heads of 128 take 17 us: one round of
 // two workgroups to a CU, so what bounds it is its own chain of loads, convolution, norms and products.
-template <int DK, bool HQ, int KM, typename T>
+template <int DK, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const DnTokens a, const DnChunks w) {
-    constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = DK / 16;
+    constexpr int KS = DK / 32, DT = DK / 16, N = DK / 16;
     __shared__ uint4 s_k[kRowTiles * KS * 2 * kWave];  // keys by tokens
     __shared__ uint4 s_q[DT * 2 * 2 * kWave];          // queries by tokens; then keys, transposed
     const int hk = blockIdx.x % a.nk;
@@ -375,11 +370,11 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         put_transposed(s_q, tile, t0, ch, y);
         read_back(s_k);
     } else {
-        uint4 *q = w.q + (chunk * a.nk + hk) * (kRowTiles * KS * PL * kWave) + tile * KS * PL * kWave + lane;
+        uint4 *q = w.q + (chunk * a.nk + hk) * (kRowTiles * KS * 2 * kWave) + tile * KS * 2 * kWave + lane;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            q[ks * PL * kWave] = as_u4(x[ks].hi);
-            if (HQ) q[(ks * PL + 1) * kWave] = as_u4(x[ks].lo);
+            q[ks * 2 * kWave] = as_u4(x[ks].hi);
+            q[(ks * 2 + 1) * kWave] = as_u4(x[ks].lo);
         }
     }
     // k_i.k_j and k_j.q_i of the lower triangle's tiles, as the results lie
@@ -428,9 +423,9 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
 // One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.  32 chunks of
 // 32 heads of 128 take 40 us: two rounds of two workgroups to a CU (128 registers; with 4 waves and twice the columns each
 // they spill: 53), 10 to 16 thousand clocks up to the inverted diagonal blocks, 5 for the others, 4 each for W and U.
-template <int DK, bool HQ, int KM, typename T>
+template <int DK, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const DnTokens a, const DnChunks w) {
-    constexpr int KS = DK / 32, DT = DK / 16, PL = HQ ? 2 : 1, N = kVBlock / 16;
+    constexpr int KS = DK / 32, DT = DK / 16, N = kVBlock / 16;
     __shared__ uint4 s_v[kVBlock / 16 * 2 * 2 * kWave];  // values, transposed
     __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
     __shared__ float s_max[4];
@@ -500,7 +495,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         values(0);
         const double ci = c[16 * tile + col];
         const float row = kScaleP * pow2(ci - mid);
-        uint4 *p = w.p + head * (kRowTiles * 2 * PL * kWave) + tile * 2 * PL * kWave + lane;
+        uint4 *p = w.p + head * (kRowTiles * 2 * 2 * kWave) + tile * 2 * 2 * kWave + lane;
 #pragma unroll
         for (int ks2 = 0; ks2 < 2; ++ks2) {
             f4_t d[2];
@@ -516,8 +511,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
                 }
             }
             const Op o = op_of(d[0], d[1]);
-            p[ks2 * PL * kWave] = as_u4(o.hi);
-            if (HQ) p[(ks2 * PL + 1) * kWave] = as_u4(o.lo);
+            p[ks2 * 2 * kWave] = as_u4(o.hi);
+            p[(ks2 * 2 + 1) * kWave] = as_u4(o.lo);
         }
     }
     lds_barrier();
@@ -638,10 +633,10 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 // and stores issued.  A chunk takes 1.2 us at 256 workgroups (its products and barriers alone 0.8): each reads its head's
 // operands for itself, 19 TB/s from the L2s in all, of 22 to 28 that loads alone reach.  Outputs in a launch of their own,
 // from S and d stored per chunk, took 145 us instead of 109 for 64 chunks.
-template <int DK, int CT, bool HQ>
+template <int DK, int CT>
 __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const DnTokens a, const DnChunks w, int groups) {
-    constexpr int KS = DK / 32, DT = DK / 64, PL = HQ ? 2 : 1;  // DT: row tiles of the state per wave
-    __shared__ uint4 s_s[CT * KS * 2 * kWave], s_d[CT * 2 * PL * kWave], s_e[CT * 2 * 2 * kWave];
+    constexpr int KS = DK / 32, DT = DK / 64;  // DT: row tiles of the state per wave
+    __shared__ uint4 s_s[CT * KS * 2 * kWave], s_d[CT * 2 * 2 * kWave], s_e[CT * 2 * 2 * kWave];
     __shared__ float s_max[kChainThreads / kWave];
     // workgroups of one key head on one XCD (they are handed out round robin): its L2 then has what they share
     const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
@@ -793,8 +788,8 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2) * kWave + lane)[part & 1] = as_u2(hi);
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2 + 1) * kWave + lane)[part & 1] = as_u2(lo);
                 split4(d, hi, lo);
-                reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * PL) * kWave + lane)[part & 1] = as_u2(hi);
-                if (HQ) reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * PL + 1) * kWave + lane)[part & 1] = as_u2(lo);
+                reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * 2) * kWave + lane)[part & 1] = as_u2(hi);
+                reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * 2 + 1) * kWave + lane)[part & 1] = as_u2(lo);
             }
             lds_barrier();
             load(s, m + 3 < chunks);
@@ -804,16 +799,16 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
             if (m + 1 < chunks) turn(1, m + 1);
         }
     } else {
-        uint4 qr[2][KS][PL], pr[2][2][PL];
+        uint4 qr[2][KS][2], pr[2][2][2];
         f4_t grown[2];
-        const uint4 *q_at = w.q + key0 * (kRowTiles * KS * PL * kWave) + part * KS * PL * kWave, *p_at = w.p + head0 * (kRowTiles * 2 * PL * kWave) + part * 2 * PL * kWave;
+        const uint4 *q_at = w.q + key0 * (kRowTiles * KS * 2 * kWave) + part * KS * 2 * kWave, *p_at = w.p + head0 * (kRowTiles * 2 * 2 * kWave) + part * 2 * 2 * kWave;
         const float *decay_at = w.decay + head0 * 2 * kC + 16 * part;
-        const int64_t q_step = static_cast<int64_t>(a.nk) * kRowTiles * KS * PL * kWave, p_step = static_cast<int64_t>(a.nv) * kRowTiles * 2 * PL * kWave;
+        const int64_t q_step = static_cast<int64_t>(a.nk) * kRowTiles * KS * 2 * kWave, p_step = static_cast<int64_t>(a.nv) * kRowTiles * 2 * 2 * kWave;
         auto load_q = [&](int s, bool more) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) qr[s][ks][p] = q_at[(ks * PL + p) * kWave + lane];
+                for (int p = 0; p < 2; ++p) qr[s][ks][p] = q_at[(ks * 2 + p) * kWave + lane];
             grown[s] = load4(decay_at + 4 * g);
             q_at += more ? q_step : 0;
             decay_at += more ? decay_step : 0;
@@ -822,7 +817,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-                for (int p = 0; p < PL; ++p) pr[s][ks2][p] = p_at[(ks2 * PL + p) * kWave + lane];
+                for (int p = 0; p < 2; ++p) pr[s][ks2][p] = p_at[(ks2 * 2 + p) * kWave + lane];
             p_at += more ? p_step : 0;
         };
         load_q(0, 1 < chunks);
@@ -830,10 +825,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
         load_q(1, 2 < chunks);
         load_p(1, 2 < chunks);
         const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
-        const int64_t o0 = (head0 * cts + ct0) * kRowTiles * kWave + part * kWave + lane;
-        f4_t *o = static_cast<f4_t *>(w.o) + o0;
-        uint2 *o_half = static_cast<uint2 *>(w.o) + o0;
-        float *back_at = w.back + head0 * cts + ct0 + lane;
+        f4_t *o = w.o + (head0 * cts + ct0) * kRowTiles * kWave + part * kWave + lane;
         const int64_t o_step = static_cast<int64_t>(a.nv) * cts * kRowTiles * kWave;
         auto turn = [&](int s, int m) {
             lds_barrier();
@@ -844,8 +836,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const h8_t sh = as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]);
-                    if constexpr (HQ) v[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][PL - 1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), v[c]);
-                    else v[c] = mfma16(as_h8(qr[s][ks][0]), sh, v[c]);
+                    v[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), v[c]);
                 }
                 v[c] *= grown[s];
             }
@@ -855,21 +846,15 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
             for (int c = 0; c < CT; ++c) {
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
-                    const h8_t dh = as_h8(s_d[((c * 2 + ks2) * PL) * kWave + lane]);
-                    if constexpr (HQ) v[c] = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][PL - 1]), dh, as_h8(s_d[((c * 2 + ks2) * PL + PL - 1) * kWave + lane]), v[c]);
-                    else v[c] = mfma16(as_h8(pr[s][ks2][0]), dh, v[c]);
+                    const h8_t dh = as_h8(s_d[((c * 2 + ks2) * 2) * kWave + lane]);
+                    v[c] = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][1]), dh, as_h8(s_d[((c * 2 + ks2) * 2 + 1) * kWave + lane]), v[c]);
                 }
-                v[c] *= HQ ? back : kHalfO;
+                v[c] *= back;
             }
             load_p(s, m + 3 < chunks);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if (HQ) o[c * kRowTiles * kWave] = v[c];
-                else o_half[c * kRowTiles * kWave] = as_u2(__builtin_convertvector(v[c], h4_t));
-            }
+            for (int c = 0; c < CT; ++c) o[c * kRowTiles * kWave] = v[c];
             o += o_step;
-            o_half += o_step;
-            if (!HQ && part == 0 && lane < CT) back_at[static_cast<int64_t>(m) * a.nv * cts] = back * (1.f / kHalfO);
         };
         for (int m = 0; m < chunks; m += 2) {
             turn(0, m);
@@ -882,7 +867,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
 // gone token after token.  CW * 32 columns at
 // most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.  32
 // chunks of 32 heads of 128 take 16 us for 34 MB: one round of workgroups, loads and stores in turn.
-template <int CW, bool HQ, typename T>
+template <int CW, typename T>
 __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w) {
     constexpr int L = CW * 8, ROWS = kFinishThreads / L, R = kC / ROWS, kRow = CW * 32 + 4;
     __shared__ __align__(16) float s_o[kC * kRow];
@@ -891,18 +876,11 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
     const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g = lane >> 4, cts = a.dv / 16;
     constexpr int PARTS = CW * 2 * kRowTiles * kWave / kFinishThreads;
     f4_t o[PARTS];
-    uint2 o_half[PARTS];
-    float back[PARTS];
     const int64_t o0 = head * cts * kRowTiles * kWave + lane;
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
         const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
-        if (HQ) {
-            o[i] = static_cast<const f4_t *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
-        } else {
-            o_half[i] = static_cast<const uint2 *>(w.o)[o0 + (ct * kRowTiles + rt) * kWave];
-            back[i] = w.back[head * cts + ct];
-        }
+        o[i] = w.o[o0 + (ct * kRowTiles + rt) * kWave];
     }
     asm volatile("" ::: "memory");  // in flight while the chunk is looked up
     Chunk it;
@@ -924,7 +902,6 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
             const int at = i * (kFinishThreads / kWave) + tid / kWave, ct = min(at / kRowTiles, cts - 1), rt = at % kRowTiles;
-            if (!HQ) o[i] = __builtin_convertvector(__builtin_bit_cast(h4_t, o_half[i]), f4_t) * back[i];
 #pragma unroll
             for (int k = 0; k < 4; ++k) s_o[(16 * rt + 4 * g + k) * kRow + 16 * ct + col] = o[i][k];
         }
@@ -961,28 +938,24 @@ __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const D
     }
 }
 
-// Whether outputs are made of two planes: unless projections and outputs are bf16.
-int planes_of(const DnTokens &a, bool in_f32) { return in_f32 || a.out_f32 ? 2 : 1; }
-
 // Parts of the workspace, at 256-byte boundaries.
 struct Parts {
-    size_t k, q, w, p, u, decay, sums, beta, vmax, dots, o, back, total;
+    size_t k, q, w, p, u, decay, sums, beta, vmax, dots, o, total;
 };
-Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap, int planes) {
+Parts parts_of(int64_t nk, int64_t nv, int64_t dk, int64_t dv, int64_t cap) {
     Parts s{};
     s.k = dn_align(cap * nk * dk * kC * 2 * 2);
-    s.q = dn_align(cap * nk * dk * kC * planes * 2);
+    s.q = dn_align(cap * nk * dk * kC * 2 * 2);
     s.w = dn_align(cap * nv * dk * kC * 2 * 2);
-    s.p = dn_align(cap * nv * kC * kC * planes * 2);
+    s.p = dn_align(cap * nv * kC * kC * 2 * 2);
     s.u = dn_align(cap * nv * dv * kC * 4);
     s.decay = dn_align(cap * nv * 2 * kC * 4);
     s.sums = dn_align(cap * nv * kC * 8);
     s.beta = dn_align(cap * nv * kC * 4);
     s.vmax = dn_align(cap * nv * 4);
     s.dots = dn_align(cap * nk * 2 * 10 * 256 * 4);
-    s.o = dn_align(cap * nv * dv * kC * 2 * planes);
-    s.back = dn_align(cap * nv * (dv / 16) * 4);
-    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.sums + s.beta + s.vmax + s.dots + s.o + s.back;
+    s.o = dn_align(cap * nv * dv * kC * 4);
+    s.total = s.k + s.q + s.w + s.p + s.u + s.decay + s.sums + s.beta + s.vmax + s.dots + s.o;
     return s;
 }
 // Chunks that have places in the workspace: for one sequence those of a span.
@@ -990,48 +963,48 @@ int64_t cap_of(int64_t sequences, int64_t tokens) {
     return sequences == 1 ? std::min<int64_t>((tokens + kC - 1) / kC, kSpan) : tokens / kC + sequences;
 }
 
-template <int DK, bool HQ, int KM, typename T>
+template <int DK, int KM, typename T>
 void launch_prepare_km(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    hipLaunchKernelGGL((deltanet_keys_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nk)), dim3(kPrepThreads), 0, s, a, w);
-    hipLaunchKernelGGL((deltanet_solve_kernel<DK, HQ, KM, T>), dim3(static_cast<uint32_t>((w.cap * a.nk + 7) / 8 * 8 * a.rep)), dim3(kPrepThreads), 0, s, a, w);
+    hipLaunchKernelGGL((deltanet_keys_kernel<DK, KM, T>), dim3(static_cast<uint32_t>(w.cap * a.nk)), dim3(kPrepThreads), 0, s, a, w);
+    hipLaunchKernelGGL((deltanet_solve_kernel<DK, KM, T>), dim3(static_cast<uint32_t>((w.cap * a.nk + 7) / 8 * 8 * a.rep)), dim3(kPrepThreads), 0, s, a, w);
 }
-template <int DK, bool HQ, typename T>
+template <int DK, typename T>
 void launch_prepare(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    if (a.K <= 4) launch_prepare_km<DK, HQ, 4, T>(a, w, s);
-    else launch_prepare_km<DK, HQ, 8, T>(a, w, s);
+    if (a.K <= 4) launch_prepare_km<DK, 4, T>(a, w, s);
+    else launch_prepare_km<DK, 8, T>(a, w, s);
 }
 
-template <bool HQ, typename T>
+template <typename T>
 void launch_finish(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const dim3 grid(static_cast<uint32_t>(w.cap * a.nv)), block(kFinishThreads);
-    if (a.dv <= 64) hipLaunchKernelGGL((deltanet_finish_kernel<2, HQ, T>), grid, block, 0, s, a, w);
-    else if (a.dv <= 128) hipLaunchKernelGGL((deltanet_finish_kernel<4, HQ, T>), grid, block, 0, s, a, w);
-    else hipLaunchKernelGGL((deltanet_finish_kernel<8, HQ, T>), grid, block, 0, s, a, w);
+    if (a.dv <= 64) hipLaunchKernelGGL((deltanet_finish_kernel<2, T>), grid, block, 0, s, a, w);
+    else if (a.dv <= 128) hipLaunchKernelGGL((deltanet_finish_kernel<4, T>), grid, block, 0, s, a, w);
+    else hipLaunchKernelGGL((deltanet_finish_kernel<8, T>), grid, block, 0, s, a, w);
 }
 
-template <int DK, bool HQ>
+template <int DK>
 void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
     // 32 columns to a workgroup where those of 16 would not find a CU each: at 32 value heads of 128 four prompts of 2,500
     // tokens in all take 138 us instead of 155, but one of 4,096 231 instead of 221
     const int cts = a.dv / 16, ct = cts % 2 == 0 && static_cast<int64_t>(a.B) * a.nv * cts > kCus ? 2 : 1;
     const dim3 grid(static_cast<uint32_t>(units * (cts / ct))), block(kChainThreads);
-    if (ct == 1) hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1, HQ>), grid, block, 0, s, a, w, cts / ct);
-    else hipLaunchKernelGGL((deltanet_chain_kernel<DK, 2, HQ>), grid, block, 0, s, a, w, cts / ct);
+    if (ct == 1) hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1>), grid, block, 0, s, a, w, cts / ct);
+    else hipLaunchKernelGGL((deltanet_chain_kernel<DK, 2>), grid, block, 0, s, a, w, cts / ct);
 }
 
-template <int DK, bool HQ, typename T>
+template <int DK, typename T>
 void launch(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    launch_prepare<DK, HQ, T>(a, w, s);
-    launch_chain<DK, HQ>(a, w, s);
+    launch_prepare<DK, T>(a, w, s);
+    launch_chain<DK>(a, w, s);
     DnTokens all = a;
     all.least = 1;
-    launch_finish<HQ, T>(all, w, s);
+    launch_finish<T>(all, w, s);
 }
-template <bool HQ, typename T>
+template <typename T>
 void launch_dk(const DnTokens &a, const DnChunks &w, hipStream_t s) {
-    if (a.dk == 64) launch<64, HQ, T>(a, w, s);
-    else launch<128, HQ, T>(a, w, s);
+    if (a.dk == 64) launch<64, T>(a, w, s);
+    else launch<128, T>(a, w, s);
 }
 
 }  // namespace
@@ -1046,15 +1019,14 @@ bool deltanet_chunks_fit(const swq_deltanet_layer *l, int64_t sequences, int64_t
 }
 
 size_t deltanet_chunks_bytes(const swq_deltanet_layer *l, int64_t sequences, int64_t tokens) {
-    return parts_of(l->num_key_heads, l->num_value_heads, l->key_head_dim, l->value_head_dim, cap_of(sequences, tokens), 2).total;
+    return parts_of(l->num_key_heads, l->num_value_heads, l->key_head_dim, l->value_head_dim, cap_of(sequences, tokens)).total;
 }
 
 void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_t s) {
     DnChunks w{};
     w.cap = static_cast<int32_t>(cap_of(a.B, a.N));
-    w.planes = planes_of(a, in_f32);
     w.least = a.least;
-    const Parts parts = parts_of(a.nk, a.nv, a.dk, a.dv, w.cap, w.planes);
+    const Parts parts = parts_of(a.nk, a.nv, a.dk, a.dv, w.cap);
     uint8_t *p = static_cast<uint8_t *>(ws);
     auto take = [&](size_t n) {
         uint8_t *at = p;
@@ -1071,15 +1043,13 @@ void launch_deltanet_chunks(const DnTokens &a, bool in_f32, void *ws, hipStream_
     w.beta = reinterpret_cast<float *>(take(parts.beta));
     w.vmax = reinterpret_cast<float *>(take(parts.vmax));
     w.dots = reinterpret_cast<f4_t *>(take(parts.dots));
-    w.o = take(parts.o);
-    w.back = reinterpret_cast<float *>(take(parts.back));
+    w.o = reinterpret_cast<f4_t *>(take(parts.o));
     const int chunks = a.B == 1 ? (a.max_tokens + kC - 1) / kC : 1;  // of a sequence alone
     w.span = a.B == 1 ? kSpan : INT32_MAX;
     for (w.chunk0 = 0; w.chunk0 < chunks; w.chunk0 += kSpan) {
         if (a.B == 1) w.cap = std::min(chunks - w.chunk0, kSpan);
-        if (in_f32) launch_dk<true, float>(a, w, s);
-        else if (w.planes == 2) launch_dk<true, uint16_t>(a, w, s);
-        else launch_dk<false, uint16_t>(a, w, s);
+        if (in_f32) launch_dk<float>(a, w, s);
+        else launch_dk<uint16_t>(a, w, s);
     }
 }
 
