@@ -322,8 +322,11 @@ size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, cons
  * dtype (SWQ_F32 / SWQ_BF16), in the layer's layout; out [tokens][nv*dv] of
  * out_dtype.  Each sequence goes on from its state, which is updated in place
  * (f32): the results of as many swq_deltanet_step calls, up to the order of f32
- * sums (prompts: products of 22 bits), bf16 outputs rounded once.  The same call
- * gives the same bits again.  Any layer that swq_deltanet_step takes; key heads
+ * sums (prompts: products of 22 bits), bf16 outputs rounded once.  In prompts
+ * those bits are of numbers down to 10^-6 (sequences of more than 16,384 tokens
+ * beside others: 10^-5) of the largest value or number of its state that a head
+ * of a sequence has in the call, and what is 10^-7 (10^-6) of it is off by some
+ * 1e-5 of itself.  The same call gives the same bits again.  Any layer that swq_deltanet_step takes; key heads
  * of 64 or 128 with value heads of a multiple of 16 up to 256, rows at multiples
  * of 4 elements and aligned to 4, take prompts 64 tokens at a time, others token
  * after token.  No output overlaps an input or the workspace.  states and

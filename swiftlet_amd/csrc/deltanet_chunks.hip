@@ -11,12 +11,15 @@
 //   chain    per (sequence, value head, 16 or 32 columns of S), chunk after chunk: d, o, S;
 //   finish   all chunks at once: the gated norm, and the ring's rows.
 //
-// Numbers.  f32 numbers meet on the f16 matrix cores as two f16 numbers each, x = hi + lo, and three products (hi hi, hi
-// lo, lo hi): 22 bits of what is large enough for lo to be a normal f16 number, 2^-25 of 1 below.  Powers of two keep
-// them there.  k, q, P and T are bounded by 1 and W by 8 (|k|, |q| <= 1 and b, g <= 1: a step of the rule lengthens
-// nothing) and take fixed ones.  v, d and S have no bound: one per (sequence, head, columns), from the largest v and
-// S, brings them to 32 .. 64, from where S grows by sqrt(tokens) at most, so past f16's largest only after 2^20
-// tokens that all agree.  Sums are f32, c is summed and subtracted in 64 bits, and T is made by f32
+// Numbers.  f32 numbers meet on the f16 matrix cores as two f16 numbers each, x = hi + lo / 2048, and three products (hi
+// hi, hi lo, lo hi; those with a lo are summed apart): 22 bits.  lo is 2048 times what hi leaves, as large as hi, so it
+// keeps its bits wherever hi is a normal f16 number, and below that 2^-36 of 1 remains.  Powers of two bring numbers to the top
+// of that range.  k, q, P and T are bounded by 1 and W by 8 (|k|, |q| <= 1 and b, g <= 1: a step of the rule lengthens
+// nothing) and take fixed ones.  v, d and S have no bound.  In T (b v) each chunk's v are brought below 2^15, beside which
+// numbers down to 2^-28 of the largest keep 22 bits.  In the chain one power per (sequence, head, columns), from the largest v
+// and S, leaves room for what S can become: the writes of n tokens add at most their largest times sqrt(n) to its norm.
+// For 64 tokens numbers down to 2^-24 of the largest keep 22 bits, for 2,048 down to 2^-22, for 2^20 2^-17; smaller
+// ones lose a bit with each power of two.  Sums are f32, c is summed and subtracted in 64 bits, and T is made by f32
 // substitution and f32 matrix instructions.  That holds whatever the types of the projections and of out: bf16 outputs are
 // the f32 ones rounded once.
 //
@@ -46,16 +49,15 @@ constexpr int kPrepThreads = 512;
 constexpr int kChainThreads = 768;
 constexpr int kFinishThreads = 256;
 constexpr int kVBlock = 128;  // columns of v that are prepared at once
-// What operands are multiplied by.  Of d e^(c_last - c): so that its product with k has S's own, which leaves both far
-// enough above 2^-14 for their low parts: with 256 and 1 / 256 the states of 4,096 tokens were off by 7e-6, with 16 by
-// 5e-7, with 8 by 3e-7, and outputs of f32 by 2e-7.  P's is q's, as their products meet in a sum.
-constexpr float kScaleK = 8.f, kScaleT = 16.f, kScaleP = kScaleK, kScaleE = 1.f / kScaleK;
+// What low parts are multiplied by, and T, W, P and q as operands: decays make the entries of T, W and P small beside 1 where
+// the numbers they meet may be large; q's is P's, as their products meet in a sum.  W stays below 2^14.
+constexpr float kLow = 2048.f, kScaleT = 2048.f;
 
 // The workspace: operands of every (chunk, key head) and (chunk, value head).
 struct DnChunks {
     uint4 *k, *q, *w, *p;  // f16 operands, two planes each
     f4_t *u;               // [chunk][nv][dv / 16][4][64]
-    float *decay;          // [chunk][nv][2][64]: e^c_i and kScaleE e^(c_last - c_i)
+    float *decay;          // [chunk][nv][2][64]: e^c_i and e^(c_last - c_i)
     double *sums;          // [chunk][nv][64]: c, in units of log 2
     float *beta;           // [chunk][nv][64]
     float *vmax;           // [chunk][nv]
@@ -78,7 +80,7 @@ __device__ __forceinline__ void here(f4_t &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void split4(f4_t x, h4_t &hi, h4_t &lo) {
     hi = __builtin_convertvector(x, h4_t);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) lo[e] = static_cast<_Float16>(fmaf(static_cast<float>(hi[e]), -1.0f, x[e]));
+    for (int e = 0; e < 4; ++e) lo[e] = static_cast<_Float16>(kLow * fmaf(static_cast<float>(hi[e]), -1.0f, x[e]));
 }
 __device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ h8_t as_h8(uint4 u) { return __builtin_bit_cast(h8_t, u); }
@@ -95,14 +97,25 @@ __device__ __forceinline__ Op op_of(f4_t a, f4_t b) {
     split4(b, bh, bl);
     return {join(ah, bh), join(al, bl)};
 }
-// c + a b in 22 bits.
-__device__ __forceinline__ f4_t mfma22(h8_t ah, h8_t al, h8_t bh, h8_t bl, f4_t c) { return mfma16(ah, bh, mfma16(ah, bl, mfma16(al, bh, c))); }
+// A sum of products in 22 bits: of high parts, and of those that have a low part.
+struct Sum {
+    f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ f4_t get() const {
+        f4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(lo[e], 1.f / kLow, hi[e]);
+        return v;
+    }
+};
+__device__ __forceinline__ void mfma22(h8_t ah, h8_t al, h8_t bh, h8_t bl, Sum &c) {
+    c.lo = mfma16(ah, bl, mfma16(al, bh, c.lo));
+    c.hi = mfma16(ah, bh, c.hi);
+}
 
-// A power of two that brings m to 32 .. 64, and its inverse; 32 where m is 0 or no number.
-__device__ __forceinline__ float scale_of(float m, float &inverse) {
-    int e = static_cast<int>((__float_as_uint(m) >> 23) & 255u) - 5;
-    if (e >= 250 || !(m > 0.f)) e = 122;
-    e = max(e, 2);
+// A power of two that brings m to 2^top .. 2^(top + 1), and its inverse; 1 where m is 0 or no number.
+__device__ __forceinline__ float scale_of(float m, int top, float &inverse) {
+    int e = static_cast<int>((__float_as_uint(m) >> 23) & 255u);
+    e = e == 255 || !(m > 0.f) ? 127 : max(e - top, 1);
     inverse = __uint_as_float(static_cast<uint32_t>(e) << 23);
     return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
@@ -333,7 +346,6 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int tile = wave & 3;
     const bool keys = wave < 4;
-    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 
     // N tokens and 4 channels per lane, normalised
     const int ch = 4 * (lane % (DK / 4)), t0 = N * (lane / (DK / 4));
@@ -346,7 +358,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float ss = lanes_sum<DK / 4>(y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3]);
-            y[i] *= kScaleK * __builtin_amdgcn_rsqf(ss + DK * 1e-6f);
+            y[i] *= (keys ? 1.f : kScaleT) * __builtin_amdgcn_rsqf(ss + DK * 1e-6f);
             h4_t hi, lo;
             split4(y[i], hi, lo);
             const int place = token_place(ch / 32, t0 + i, ch % 16 / 4);
@@ -380,14 +392,15 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     // k_i.k_j and k_j.q_i of the lower triangle's tiles, as the results lie
     f4_t *dots = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
     for (int jt = 0; jt <= tile; ++jt) {
-        f4_t d = zero;
+        Sum sum;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int place = token_place(ks, lane & 15, lane >> 4);
             const h8_t kh = as_h8(s_k[by_tokens<DK>(jt, ks, 0) + place]), kl = as_h8(s_k[by_tokens<DK>(jt, ks, 1) + place]);
-            d = keys ? mfma22(x[ks].hi, x[ks].lo, kh, kl, d) : mfma22(kh, kl, x[ks].hi, x[ks].lo, d);
+            if (keys) mfma22(x[ks].hi, x[ks].lo, kh, kl, sum);
+            else mfma22(kh, kl, x[ks].hi, x[ks].lo, sum);
         }
-        d *= 1.f / (kScaleK * kScaleK);
+        f4_t d = sum.get() * (keys ? 1.f : 1.f / kScaleT);
         here(d);
         dots[jt * kWave] = d;
     }
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         w.sums[head * kC + lane] = c;
         w.beta[head * kC + lane] = is ? sigmoid_acc(dn_load(ba, ba_at(a, hv, 0))) : 0.f;
         w.decay[head * 2 * kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(c));
-        w.decay[head * 2 * kC + kC + lane] = kScaleE * __builtin_amdgcn_exp2f(static_cast<float>(last - c));
+        w.decay[head * 2 * kC + kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(last - c));
     }
     lds_barrier();
     uint4 *k_to = w.k + (chunk * a.nk + hk) * (DT * 2 * 2 * kWave);
@@ -494,7 +507,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     } else {
         values(0);
         const double ci = c[16 * tile + col];
-        const float row = kScaleP * pow2(ci - mid);
+        const float row = kScaleT * pow2(ci - mid);
         uint4 *p = w.p + head * (kRowTiles * 2 * 2 * kWave) + tile * 2 * 2 * kWave + lane;
 #pragma unroll
         for (int ks2 = 0; ks2 < 2; ++ks2) {
@@ -506,7 +519,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = 16 * jt + 4 * g + e;
-                    const float share = jt < tile ? row * pow2(mid - c[j]) : kScaleP * pow2(ci - c[j]);
+                    const float share = jt < tile ? row * pow2(mid - c[j]) : kScaleT * pow2(ci - c[j]);
                     d[half][e] = 16 * tile + col >= j ? d[half][e] * share : 0.f;
                 }
             }
@@ -519,7 +532,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 
     // T below the diagonal blocks, 16 x 16 and then 32 x 32, while waves 4 to 7 put the values
     float vmax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), v_inv;
-    float v_scale = scale_of(vmax, v_inv);
+    float v_scale = scale_of(vmax, 14, v_inv);
     auto put_values = [&]() {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] *= v_scale;
@@ -589,13 +602,13 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 #pragma unroll
     for (int i = 0; i < KS / 2; ++i) {
         const int ks = half_of * (KS / 2) + i;
-        f4_t d[2] = {zero, zero};
+        Sum d[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2) d[half] = mfma22(as_h8(k[half][ks2][0]), as_h8(k[half][ks2][1]), tw[ks2].hi, tw[ks2].lo, d[half]);
+            for (int ks2 = 0; ks2 < 2; ++ks2) mfma22(as_h8(k[half][ks2][0]), as_h8(k[half][ks2][1]), tw[ks2].hi, tw[ks2].lo, d[half]);
         if (i + 1 < KS / 2) load_k(ks + 1);
-        const Op o = op_of(d[0], d[1]);
+        const Op o = op_of(d[0].get(), d[1].get());
         w_to[ks * 2 * kWave] = as_u4(o.hi);
         w_to[(ks * 2 + 1) * kWave] = as_u4(o.lo);
     }
@@ -604,11 +617,11 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 #pragma unroll
         for (int i = 0; i < kVBlock / 32; ++i) {
             const int ct = 2 * i + half_of;
-            f4_t d = zero;
+            Sum sum;
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2)
-                d = mfma22(tu[ks2].hi, tu[ks2].lo, as_h8(s_v[transposed(ct, ks2, 0) + row_place(ct, col, g)]), as_h8(s_v[transposed(ct, ks2, 1) + row_place(ct, col, g)]), d);
-            d *= v_inv * (1.f / kScaleT);
+                mfma22(tu[ks2].hi, tu[ks2].lo, as_h8(s_v[transposed(ct, ks2, 0) + row_place(ct, col, g)]), as_h8(s_v[transposed(ct, ks2, 1) + row_place(ct, col, g)]), sum);
+            f4_t d = sum.get() * (v_inv * (1.f / kScaleT));
             here(d);
             if (c0 + 16 * ct < a.dv) u_to[((c0 / 16 + ct) * kRowTiles + tile) * kWave] = d;
         }
@@ -620,7 +633,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         lds_barrier();
         const float now = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
         vmax = fmaxf(vmax, now);
-        v_scale = scale_of(now, v_inv);
+        v_scale = scale_of(now, 14, v_inv);
         if (!keys) put_values();
         lds_barrier();
     }
@@ -674,8 +687,9 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < kChainThreads / kWave; ++i) most = fmaxf(most, s_max[i]);
+    // (1 + sqrt(dk + n)) times the largest, with n tokens' writes, stays below f16's largest
     float inverse;
-    const float scale = scale_of(most, inverse);
+    const float scale = scale_of(most, 14 - (33 - __builtin_clz(min(tokens, chunks * kC) + DK - 1)) / 2, inverse);
 
     // What a chunk brings is in flight for more than a chunk before it is used.  Chunks that do not exist are loaded as the
     // last one again: no branch.
@@ -729,12 +743,22 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
                     for (int p = 0; p < 2; ++p) e[ks2][p] = as_h8(s_e[((c * 2 + ks2) * 2 + p) * kWave + lane]);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) st[t][c] *= keep;
+                f4_t low[DT];
+#pragma unroll
+                for (int t = 0; t < DT; ++t) low[t] = zero;
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
                     for (int p = 0; p < 3; ++p)
 #pragma unroll
-                        for (int t = 0; t < DT; ++t) st[t][c] = mfma16(as_h8(kr[s][t][ks2][p == 0]), e[ks2][p == 1], st[t][c]);
+                        for (int t = 0; t < DT; ++t) {
+                            f4_t &to = p < 2 ? low[t] : st[t][c];
+                            to = mfma16(as_h8(kr[s][t][ks2][p == 0]), e[ks2][p == 1], to);
+                        }
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) st[t][c][x] = fmaf(low[t][x], 1.f / kLow, st[t][c][x]);
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t)
@@ -782,13 +806,13 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int p = 0; p < 3; ++p) sum[p] = mfma16(as_h8(wr[s][ks][p == 0]), as_h8(s_s[((c * KS + ks) * 2 + (p == 1)) * kWave + lane]), sum[p]);
-                const f4_t d = ur[s][c] * scale - (sum[2] + (sum[1] + sum[0])) * (1.f / (kScaleT * kScaleK));
+                const f4_t d = ur[s][c] * scale - Sum{sum[2], sum[1] + sum[0]}.get() * (1.f / kScaleT);
                 h4_t hi, lo;
                 split4(d * late[s], hi, lo);
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2) * kWave + lane)[part & 1] = as_u2(hi);
                 reinterpret_cast<uint2 *>(s_e + ((c * 2 + part / 2) * 2 + 1) * kWave + lane)[part & 1] = as_u2(lo);
                 split4(d, hi, lo);
-                reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * 2) * kWave + lane)[part & 1] = as_u2(hi);
+                reinterpret_cast<uint2 *>(s_d + (c * 2 + part / 2) * 2 * kWave + lane)[part & 1] = as_u2(hi);
                 reinterpret_cast<uint2 *>(s_d + ((c * 2 + part / 2) * 2 + 1) * kWave + lane)[part & 1] = as_u2(lo);
             }
             lds_barrier();
@@ -824,7 +848,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
         load_p(0, 1 < chunks);
         load_q(1, 2 < chunks);
         load_p(1, 2 < chunks);
-        const float back = inverse / (kScaleK * __fsqrt_rn(static_cast<float>(DK)));
+        const float back = inverse / (kScaleT * __fsqrt_rn(static_cast<float>(DK)));
         f4_t *o = w.o + (head0 * cts + ct0) * kRowTiles * kWave + part * kWave + lane;
         const int64_t o_step = static_cast<int64_t>(a.nv) * cts * kRowTiles * kWave;
         auto turn = [&](int s, int m) {
@@ -832,24 +856,25 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
             f4_t v[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                v[c] = zero;
+                Sum sum;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const h8_t sh = as_h8(s_s[((c * KS + ks) * 2) * kWave + lane]);
-                    v[c] = mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), v[c]);
+                    const h8_t sh = as_h8(s_s[(c * KS + ks) * 2 * kWave + lane]);
+                    mfma22(as_h8(qr[s][ks][0]), as_h8(qr[s][ks][1]), sh, as_h8(s_s[((c * KS + ks) * 2 + 1) * kWave + lane]), sum);
                 }
-                v[c] *= grown[s];
+                v[c] = sum.get() * grown[s];
             }
             lds_barrier();
             load_q(s, m + 3 < chunks);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
+                Sum sum{v[c]};
 #pragma unroll
                 for (int ks2 = 0; ks2 < 2; ++ks2) {
-                    const h8_t dh = as_h8(s_d[((c * 2 + ks2) * 2) * kWave + lane]);
-                    v[c] = mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][1]), dh, as_h8(s_d[((c * 2 + ks2) * 2 + 1) * kWave + lane]), v[c]);
+                    const h8_t dh = as_h8(s_d[(c * 2 + ks2) * 2 * kWave + lane]);
+                    mfma22(as_h8(pr[s][ks2][0]), as_h8(pr[s][ks2][1]), dh, as_h8(s_d[((c * 2 + ks2) * 2 + 1) * kWave + lane]), sum);
                 }
-                v[c] *= back;
+                v[c] = sum.get() * back;
             }
             load_p(s, m + 3 < chunks);
 #pragma unroll
