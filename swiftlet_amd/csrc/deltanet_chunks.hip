@@ -410,8 +410,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         const T *ba = static_cast<const T *>(a.ba) + (n0 + static_cast<int64_t>(t)) * a.ba_stride;
         const bool is = m * kC + lane < tokens;
         const float log_g = -expf(a.a_log[hv]) * softplus_acc(dn_load(ba, ba_at(a, hv, 1)) + a.dt_bias[hv]);
-        // below 2^-149 a decay is 0 like any other, and sums stay exact beside it
-        double c = is ? 1.4426950408889634 * static_cast<double>(fmaxf(log_g, -110.f)) : 0.0;
+        // below 2^-149 a decay is 0 like any other, and sums stay exact beside it; one that is no number stays none
+        double c = is ? 1.4426950408889634 * static_cast<double>(log_g < -110.f ? -110.f : log_g) : 0.0;
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
             const double up = __shfl_up(c, d, kWave);
