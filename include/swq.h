@@ -326,11 +326,15 @@ size_t swq_deltanet_tokens_workspace_bytes(const swq_deltanet_layer *layer, cons
  * those bits are of numbers down to 10^-6 (sequences of more than 16,384 tokens
  * beside others: 10^-5) of the largest value or number of its state that a head
  * of a sequence has in the call, and what is 10^-7 (10^-6) of it is off by some
- * 1e-5 of itself.  The same call gives the same bits again.  Any layer that swq_deltanet_step takes; key heads
- * of 64 or 128 with value heads of a multiple of 16 up to 256, rows at multiples
- * of 4 elements and aligned to 4, take prompts 64 tokens at a time, others token
- * after token.  No output overlaps an input or the workspace.  states and
- * workspace: 256-byte aligned; the workspace needs no preparation. */
+ * 1e-5 of itself.  What is not finite in a token leaves earlier tokens, other
+ * heads and other sequences as they are; from that token on its head's outputs
+ * are not finite, and of the head's state at least the rows that it reaches
+ * (queries: their own token's outputs alone).  The same call gives the same bits
+ * again.  Any layer that swq_deltanet_step takes; key heads of 64 or 128 with
+ * value heads of a multiple of 16 up to 256, rows at multiples of 4 elements and
+ * aligned to 4, take prompts 64 tokens at a time, others token after token.  No
+ * output overlaps an input or the workspace.  states and workspace: 256-byte
+ * aligned; the workspace needs no preparation. */
 int swq_deltanet_tokens(const swq_deltanet_layer *layer, const swq_deltanet_batch *batch, const void *qkvz,
                         const void *ba, int dtype, void *states, size_t states_bytes, void *out, int out_dtype,
                         void *ws, size_t ws_bytes, void *stream);

@@ -23,6 +23,11 @@
 // substitution and f32 matrix instructions.  That holds whatever the types of the projections and of out: bf16 outputs are
 // the f32 ones rounded once.
 //
+// What is not finite.  0 times it is no 0, and the triangles above T's and P's diagonals would carry it to earlier tokens.
+// So keys, gates and values that are not finite are taken as 0 (log g: g = 1), and e^c is NaN from the first such token of
+// a chunk on: outputs of that token and all after it are, and S is from the chunk's end on, as a whole where
+// one value alone would spoil its row.  Queries reach their own token's outputs alone and need nothing.
+//
 // Layout.  A matrix instruction's result has a lane's 4 numbers in consecutive rows of one column; its operands have 8
 // numbers along the contraction.  The order of a contraction is free, so operands take the order in which two
 // results lie: position j of lane group g is element 16 (j / 4) + 4 g + j % 4 of 32.  Every result then is the next
@@ -57,7 +62,7 @@ constexpr float kLow = 2048.f, kScaleT = 2048.f;
 struct DnChunks {
     uint4 *k, *q, *w, *p;  // f16 operands, two planes each
     f4_t *u;               // [chunk][nv][dv / 16][4][64]
-    float *decay;          // [chunk][nv][2][64]: e^c_i and e^(c_last - c_i)
+    float *decay;          // [chunk][nv][2][64]: e^c_i, NaN from the first token with anything not finite on, and e^(c_last - c_i)
     double *sums;          // [chunk][nv][64]: c, in units of log 2
     float *beta;           // [chunk][nv][64]
     float *vmax;           // [chunk][nv]
@@ -156,6 +161,10 @@ __device__ __forceinline__ bool find_chunk(const DnTokens &a, const DnChunks &w,
     c.state = slot >= 0 && slot < a.slots ? a.states + slot * a.slot_bytes : nullptr;
     return c.b >= 0 && c.m < (tokens + kC - 1) / kC && c.state != nullptr;
 }
+
+// The bits of |v|; those of what is not finite are kNotFinite or more.
+constexpr uint32_t kNotFinite = 0x7F800000u;
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 __device__ __forceinline__ f4_t load4(const float *p) { return *reinterpret_cast<const f4_t *>(p); }
 __device__ __forceinline__ f4_t load4(const uint16_t *p) {
@@ -338,6 +347,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     constexpr int KS = DK / 32, DT = DK / 16, N = DK / 16;
     __shared__ uint4 s_k[kRowTiles * KS * 2 * kWave];  // keys by tokens
     __shared__ uint4 s_q[DT * 2 * 2 * kWave];          // queries by tokens; then keys, transposed
+    __shared__ int s_bad[kRowTiles];                   // the first token of each tile whose key is not finite, or kC
     const int hk = blockIdx.x % a.nk;
     const int64_t chunk = blockIdx.x / a.nk;
     Chunk it;
@@ -354,11 +364,33 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         const int c = (keys ? a.keyD : 0) + hk * DK + ch, head = a.layout == SWQ_DELTA_SPLIT ? hk * DK + (keys ? a.keyD : 0) : hk * (2 * DK + 2 * a.rep * a.dv) + (keys ? DK : 0);
         conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
                          t0, head + ch, c, y);
-        uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0)) + ch / 16 % 2;
+        float most = 0.f;  // of the sums: what is not finite makes them so
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float ss = lanes_sum<DK / 4>(y[i][0] * y[i][0] + y[i][1] * y[i][1] + y[i][2] * y[i][2] + y[i][3] * y[i][3]);
             y[i] *= (keys ? 1.f : kScaleT) * __builtin_amdgcn_rsqf(ss + DK * 1e-6f);
+            most = fmaxf(most, ss < INFINITY ? 0.f : 1.f);
+        }
+        if (keys) {
+            int bad = kC;
+            if (__any(most > 0.f)) {
+#pragma unroll
+                for (int i = N - 1; i >= 0; --i) {
+                    float odd = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd += abs_bits(y[i][e]) >= kNotFinite ? 1.f : 0.f;
+                    if (lanes_sum<DK / 4>(odd) > 0.f) {
+                        y[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+                        bad = 16 * tile + t0 + i;
+                    }
+                }
+                for (int d = 1; d < kWave; d <<= 1) bad = min(bad, __shfl_xor(bad, d, kWave));
+            }
+            if (lane == 0) s_bad[tile] = bad;
+        }
+        uint2 *to = reinterpret_cast<uint2 *>((keys ? s_k : s_q) + by_tokens<DK>(tile, ch / 32, 0)) + ch / 16 % 2;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             h4_t hi, lo;
             split4(y[i], hi, lo);
             const int place = token_place(ch / 32, t0 + i, ch % 16 / 4);
@@ -409,9 +441,12 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         const int hv = hk * a.rep + r, t = min(m * kC + lane, tokens - 1);
         const T *ba = static_cast<const T *>(a.ba) + (n0 + static_cast<int64_t>(t)) * a.ba_stride;
         const bool is = m * kC + lane < tokens;
-        const float log_g = -expf(a.a_log[hv]) * softplus_acc(dn_load(ba, ba_at(a, hv, 1)) + a.dt_bias[hv]);
-        // below 2^-149 a decay is 0 like any other, and sums stay exact beside it; one that is no number stays none
-        double c = is ? 1.4426950408889634 * static_cast<double>(log_g < -110.f ? -110.f : log_g) : 0.0;
+        const float log_g = -expf(a.a_log[hv]) * softplus_acc(dn_load(ba, ba_at(a, hv, 1)) + a.dt_bias[hv]), b = sigmoid_acc(dn_load(ba, ba_at(a, hv, 0)));
+        const bool none = log_g != log_g || b != b;
+        const uint64_t nones = __ballot(is && none);
+        const int bad = min(min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3])), nones ? __builtin_ctzll(nones) : kC);
+        // below 2^-149 a decay is 0 like any other, and sums stay exact beside it
+        double c = is && !none ? 1.4426950408889634 * static_cast<double>(fmaxf(log_g, -110.f)) : 0.0;
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
             const double up = __shfl_up(c, d, kWave);
@@ -420,8 +455,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
         const double last = __shfl(c, kWave - 1, kWave);
         const int64_t head = chunk * a.nv + hv;
         w.sums[head * kC + lane] = c;
-        w.beta[head * kC + lane] = is ? sigmoid_acc(dn_load(ba, ba_at(a, hv, 0))) : 0.f;
-        w.decay[head * 2 * kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(c));
+        w.beta[head * kC + lane] = is && !none ? b : 0.f;
+        w.decay[head * 2 * kC + lane] = lane < bad ? __builtin_amdgcn_exp2f(static_cast<float>(c)) : NAN;
         w.decay[head * 2 * kC + kC + lane] = __builtin_amdgcn_exp2f(static_cast<float>(last - c));
     }
     lds_barrier();
@@ -442,6 +477,7 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     __shared__ uint4 s_v[kVBlock / 16 * 2 * 2 * kWave];  // values, transposed
     __shared__ __align__(16) float s_t[10 * 16 * kTriRow];
     __shared__ float s_max[4];
+    __shared__ int s_bad[4];  // the first token of each tile that has a value which is not finite, or kC
     // a key head's value heads on one XCD (workgroups are handed out round robin), which they share dots and keys in
     const uint32_t unit = blockIdx.x / 8 / a.rep * 8 + blockIdx.x % 8;
     const int hk = unit % a.nk, hv = hk * a.rep + blockIdx.x / 8 % a.rep;
@@ -452,7 +488,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     const bool keys = wave < 4;
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
     const double *c = w.sums + head * kC;
-    const float *beta = w.beta + head * kC, *decay = w.decay + head * 2 * kC;
+    const float *beta = w.beta + head * kC;
+    float *decay = w.decay + head * 2 * kC;
     const f4_t *dots_at = w.dots + (chunk * a.nk + hk) * (2 * 10 * kWave) + (keys ? 0 : 10 * kWave) + tile * (tile + 1) / 2 * kWave + lane;
     f4_t dots[kRowTiles];
 #pragma unroll
@@ -468,13 +505,33 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         const int off = min(c0 + ch, a.dv - 4), v_at = a.layout == SWQ_DELTA_SPLIT ? 2 * a.keyD + hv * a.dv : hk * (2 * DK + 2 * a.rep * a.dv) + 2 * DK + (hv - hk * a.rep) * a.dv;
         conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
                          t0, v_at + off, 2 * a.keyD + hv * a.dv + off, v);
-        float most = 0.f;
+        uint32_t most = 0;
+        auto largest = [&]() {
+            most = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[i][e]));
-        most = wave_max_all(most);
-        if (lane == 0) s_max[tile] = most;
+                for (int e = 0; e < 4; ++e) most = max(most, abs_bits(v[i][e]));
+        };
+        largest();
+        int bad = kC;
+        if (__any(most >= kNotFinite)) {
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (abs_bits(v[i][e]) >= kNotFinite) {
+                        v[i][e] = 0.f;
+                        bad = 16 * tile + t0 + i;
+                    }
+            for (int d = 1; d < kWave; d <<= 1) bad = min(bad, __shfl_xor(bad, d, kWave));
+            largest();
+        }
+        const float m = wave_max_all(__uint_as_float(most));
+        if (lane == 0) {
+            s_max[tile] = m;
+            s_bad[tile] = c0 ? min(bad, s_bad[tile]) : bad;
+        }
     };
     // e^(c_i - c_j) is a row's share times a column's about the tile's first row, both at most 1; within the diagonal
     // tile it is taken as it is
@@ -593,7 +650,10 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
             const int jt = 2 * ks2 + half, j = 16 * jt + 4 * g;
             u[half] = *reinterpret_cast<const f4_t *>(s_t + tri(tile, min(jt, tile)) + col * kTriRow + 4 * g) * (jt <= tile ? kScaleT : 0.f);
             u[half] *= load4(beta + j);
-            e_u[half] = u[half] * load4(decay + j);
+            f4_t grown = load4(decay + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) grown[e] = fmaxf(grown[e], 0.f);  // 0 for NaN, whose tokens T has zeros for in earlier rows
+            e_u[half] = u[half] * grown;
         }
         tu[ks2] = op_of(u[0], u[1]);
         tw[ks2] = op_of(e_u[0], e_u[1]);
@@ -638,6 +698,11 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
         lds_barrier();
     }
     if (tid == 0) w.vmax[head] = vmax;
+    const int bad = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
+    if (bad < kC) {
+        lds_barrier();  // all waves have used what they read of it
+        if (tid >= bad && tid < kC) decay[tid] = NAN;
+    }
 }
 
 // One workgroup per (sequence, value head, CT * 16 columns of the state), three quarters of waves at three tasks: waves 0 to
@@ -678,7 +743,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
             for (int c = 0; c < CT; ++c) {
                 st[t][c] = *reinterpret_cast<const f4_t *>(state + static_cast<int64_t>(16 * c) * DK + 16 * (part * DT + t));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(st[t][c][e]));
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, abs_bits(st[t][c][e]) < kNotFinite ? fabsf(st[t][c][e]) : 0.f);
             }
     }
     for (int i = tid; i < chunks; i += kChainThreads) most = fmaxf(most, w.vmax[(first + i) * a.nv + hv]);
