@@ -214,8 +214,9 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // Convolution and silu of a tile of 16 tokens, N of them per lane from `tau` on (places in the sequence) and 4 mixed channels
 // from ch on, whose elements lie at `at`: a row's channels side by side over the lanes, a token's earlier rows in
 // registers.  Zeros for tokens that the sequence does not have.  tau0: the wave's first token.  KM: rows of the kernel that
-// are held, 4 or 8; shorter kernels have zero weights in front.
-template <int KM, int N, typename T>
+// are held, 4 or 8; shorter kernels have zero weights in front.  SHORT: and zeros for the rows that meet them, which may be
+// not finite and no business of the token's.
+template <int KM, int N, bool SHORT, typename T>
 __device__ __forceinline__ void conv_tile(const DnTokens &a, const T *x, const float *ring, uint32_t pos, int tokens, int tau0, int t0, int at, int ch,
                                           f4_t (&y)[N]) {
     Four<T> rows[N + KM - 1];
@@ -254,19 +255,23 @@ __device__ __forceinline__ void conv_tile(const DnTokens &a, const T *x, const f
             if (tau + j < KM - 1)
                 win[j + 1] = j >= KM - a.K ? load4(ring + static_cast<int64_t>((pos + static_cast<uint32_t>(tau + 1 + j - (KM - a.K))) % a.K) * a.convD + ch) : f4_t{0.f, 0.f, 0.f, 0.f};
     }
+    auto taps = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
-        for (int j = 0; j < KM - 1; ++j) win[j] = win[j + 1];
-        win[KM - 1] = rows[i + KM - 1].get();
-        f4_t acc = w[0] * win[0];
+            for (int j = 0; j < KM - 1; ++j) win[j] = win[j + 1];
+            win[KM - 1] = rows[i + KM - 1].get();
+            f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 1; j < KM; ++j)
+            for (int j = 0; j < KM; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = fmaf(w[j][e], win[j][e], acc[e]);
+                for (int e = 0; e < 4; ++e) acc[e] = fmaf(w[j][e], j >= j0 ? win[j][e] : 0.f, acc[e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[i][e] = tau + i < tokens ? silu_hw(acc[e]) : 0.f;
-    }
+            for (int e = 0; e < 4; ++e) y[i][e] = tau + i < tokens ? silu_hw(acc[e]) : 0.f;
+        }
+    };
+    if (!SHORT || a.K == KM) taps(0);
+    else taps(KM - a.K);
 }
 
 // Block (row tile, column tile) of a lower triangular matrix of 4 x 4 blocks of 16 x 16, rows 20 apart.
@@ -362,8 +367,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
     f4_t y[N];
     {
         const int c = (keys ? a.keyD : 0) + hk * DK + ch, head = a.layout == SWQ_DELTA_SPLIT ? hk * DK + (keys ? a.keyD : 0) : hk * (2 * DK + 2 * a.rep * a.dv) + (keys ? DK : 0);
-        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
-                         t0, head + ch, c, y);
+        conv_tile<KM, N, true>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens,
+                               m * kC + 16 * tile, t0, head + ch, c, y);
         float most = 0.f;  // of the sums: what is not finite makes them so
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -503,8 +508,9 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
     f4_t v[N];
     auto values = [&](int c0) {  // columns c0 .. of this wave's tile, and their largest
         const int off = min(c0 + ch, a.dv - 4), v_at = a.layout == SWQ_DELTA_SPLIT ? 2 * a.keyD + hv * a.dv : hk * (2 * DK + 2 * a.rep * a.dv) + 2 * DK + (hv - hk * a.rep) * a.dv;
-        conv_tile<KM, N>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens, m * kC + 16 * tile,
-                         t0, v_at + off, 2 * a.keyD + hv * a.dv + off, v);
+        // from the first value that is not finite on the head gives none, so it does not matter how far a shorter kernel carries it
+        conv_tile<KM, N, false>(a, static_cast<const T *>(a.qkvz) + n0 * a.qkvz_stride, reinterpret_cast<const float *>(it.state), it.pos, tokens,
+                                m * kC + 16 * tile, t0, v_at + off, 2 * a.keyD + hv * a.dv + off, v);
         uint32_t most = 0;
         auto largest = [&]() {
             most = 0;

@@ -24,8 +24,8 @@ __device__ __forceinline__ float lds_sum_sq(const float *v, int n, int lane) {
 }
 
 // WIDE: kernels of up to 8 rows and any number of channels per head; else 4 rows and a channel per thread, as
-// the usual heads of 128 have.  Kernels shorter than that have zero weights in front, which change no bit of
-// the sums.  ONE: no sequence brings more than a token, and the ring takes its row here (a
+// the usual heads of 128 have.  Kernels shorter than that have zero weights in front, and zeros for the rows that meet
+// them, which change no bit of the sums.  ONE: no sequence brings more than a token, and the ring takes its row here (a
 // workgroup then overwrites no row that another still reads; with more tokens it would).  MANY: registers for two
 // workgroups to a CU, where there are more workgroups than CUs: 64 single tokens at 32 heads of 128 take 51 us instead of 56 (290
 // MB: 5.7 TB/s), 32 sequences of 4 55 instead of 69; one of 8 would take 29 instead of 27.
@@ -115,8 +115,7 @@ __global__ __launch_bounds__(kTokThreads, MANY ? 4 : 2) void deltanet_tokens_ker
             (t < DK ? s_q[t] : t < 2 * DK ? s_k[t - DK] : s_v[t - 2 * DK]) = silu_acc(acc);
             if constexpr (!ONE) {
 #pragma unroll
-                for (int j = 0; j + 1 < KM - 1; ++j) hist[c][j] = hist[c][j + 1];
-                hist[c][KM - 2] = xc[c];
+                for (int j = 0; j < KM - 1; ++j) hist[c][j] = j < KM - a.K ? 0.f : j < KM - 2 ? hist[c][j + 1] : xc[c];
             }
         }
         // 2. gates

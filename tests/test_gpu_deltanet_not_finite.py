@@ -180,10 +180,15 @@ def test_keys(at, value):
 
 @pytest.mark.parametrize("value", [INF, NAN])
 @pytest.mark.parametrize("at", [0, 30, 63, 64, 140])
-@pytest.mark.parametrize("K", [4])
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 6])
 def test_queries(at, value, K):
     """A query is of its own token and of the K - 1 after it, whose convolution it is in."""
     of_key_head(Batch(SMALL, [150, 20], split=True, seed=48, K=K), 7, at, value)
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 6])
+def test_queries_token_after_token(K):
+    of_key_head(Batch(SMALL, [10, 3], split=True, seed=49, K=K), 7, 4, NAN)
 
 
 @pytest.mark.parametrize("heads", [SMALL, BIG, (1, 2, 128, 256)], ids=str)
