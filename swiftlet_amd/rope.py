@@ -62,8 +62,11 @@ class RopeGPU:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "RopeGPU: rope_type " + str(kind))
         scaling = None
         if _KINDS[kind] != _lib.SWQ_ROPE_PLAIN:
+            sc = {k: v for k, v in sc.items() if v is not None}
+            if "factor" not in sc:
+                raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "RopeGPU: rope_type " + str(kind) + " without a factor")
             # what would change the angles or the magnitude and is not in RopeScaling
-            odd = [k for k, plain in (("mscale", None), ("mscale_all_dim", None), ("truncate", True)) if sc.get(k, plain) not in (None, plain)]
+            odd = [k for k, plain in (("mscale", None), ("mscale_all_dim", None), ("truncate", True)) if sc.get(k, plain) != plain]
             if odd:
                 raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "RopeGPU: " + ", ".join(odd))
             scaling = RopeScaling(kind, float(sc["factor"]), int(sc.get("original_max_position_embeddings", c.get("max_position_embeddings", 0))),
