@@ -12,7 +12,7 @@ import ctypes
 
 from . import _lib
 from ._lib import SWQ_DELTA_INTERLEAVED, SWQ_DELTA_SPLIT, DeltaNetBatch, DeltaNetLayer, SwqError, check
-from .engine import DescArray, GPULinear, HipEngine, _code, _elsewhere, _norm_arg, _ptr, _stream_handle, _torch, own_launches
+from .engine import DescArray, GPULinear, HipEngine, _code, _elsewhere, _i32, _norm_arg, _ptr, _stream_handle, _torch, own_launches
 
 
 def _row_stride(t, rows, width, what, device):
@@ -25,6 +25,11 @@ def _row_stride(t, rows, width, what, device):
     if n != rows or w < width or element != 1 or (rows > 1 and row < width):
         raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, what)
     return row if rows > 1 else 0
+
+
+def _most(max_tokens, tokens):
+    """The most tokens of one sequence, no more than the call has."""
+    return max(min(max_tokens or tokens, tokens), -1) or 1
 
 
 class DeltaNetGPU:
@@ -105,7 +110,8 @@ class DeltaNetGPU:
         `max_tokens` of one sequence (any number of the call's if not given)."""
         torch = _torch()
         tokens = sequences if tokens is None else tokens
-        b = DeltaNetBatch(sequences=sequences, tokens=tokens, max_tokens=max_tokens or max(tokens, 1), slots=sequences, starts=1)
+        b = DeltaNetBatch(sequences=_i32(sequences, "deltanet_tokens: sequences"), tokens=_i32(tokens, "deltanet_tokens: tokens"),
+                          max_tokens=_most(max_tokens, tokens), slots=sequences, starts=1)
         n = self.lib.swq_deltanet_tokens_workspace_bytes(ctypes.byref(self._c), ctypes.byref(b))
         if n == 0:
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "deltanet_tokens_workspace_bytes")
@@ -133,7 +139,7 @@ class DeltaNetGPU:
         if out.numel() != N * self.value_dim:
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "deltanet_tokens: out")
         states_bytes = states.numel()
-        b = DeltaNetBatch(B, N, max_tokens or max(N, 1), states_bytes // self.slot_bytes,
+        b = DeltaNetBatch(B, _i32(N, "deltanet_tokens: tokens"), _most(max_tokens, N), _i32(states_bytes // self.slot_bytes, "deltanet_tokens: states"),
                           None if starts is None else _ptr(starts, B + 1, "deltanet_tokens: starts", at, i32),
                           _ptr(positions, 1, "deltanet_tokens: positions", at, i32),
                           None if slots is None else _ptr(slots, B, "deltanet_tokens: slots", at, i32),

@@ -72,6 +72,13 @@ def _ptr(t, count, what, device, dtype=None):
     return t.data_ptr()
 
 
+def _i32(n, what):
+    """A count that the C interface takes in 32 bits, which ctypes would cut to size without a word."""
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise SwqError(_lib.SWQ_ERR_LIMIT, what)
+    return n
+
+
 class DescArray:
     """The descriptors of several linears as one C array, rebuilt when one of them changed."""
 

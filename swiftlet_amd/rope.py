@@ -9,7 +9,7 @@ from dataclasses import dataclass
 
 from . import _lib
 from ._lib import SWQ_ROPE_HALF, SWQ_ROPE_INTERLEAVED, RopeHeads, RopeScalingDesc, SwqError, check
-from .engine import _code, _elsewhere, _ptr, _stream_handle, _torch
+from .engine import _code, _elsewhere, _i32, _ptr, _stream_handle, _torch
 
 _KINDS = {"none": _lib.SWQ_ROPE_PLAIN, "default": _lib.SWQ_ROPE_PLAIN, "linear": _lib.SWQ_ROPE_LINEAR, "ntk": _lib.SWQ_ROPE_NTK,
           "yarn": _lib.SWQ_ROPE_YARN}
@@ -79,6 +79,7 @@ class RopeGPU:
         n = count if positions is None else positions.numel()
         if n is None or n < 0 or (count is not None and count != n):
             raise SwqError(_lib.SWQ_ERR_INVALID_ARGUMENT, "rope_table: count")
+        _i32(n, "rope_table: count")
         if out is None:
             if stream is not None and _elsewhere(stream):
                 with torch.cuda.stream(stream):
@@ -108,6 +109,7 @@ class RopeGPU:
         if len(shape) != 3:
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: tensors")
         N, _, hd = shape
+        _i32(N, "rope: tokens")
         parts = (RopeHeads * len(xs))()
         for part, x, y, w in zip(parts, xs, out, norm_weights or (None,) * len(xs)):
             shape = x.shape
@@ -130,7 +132,7 @@ class RopeGPU:
         if table.shape[1:] != (self.rot // 2, 2):
             raise SwqError(_lib.SWQ_ERR_BAD_SHAPE, "rope: table")
         check(self.lib.swq_rope(parts, len(xs), N, hd, self.rot, self._layout, int(inverse), eps, _ptr(table, 1, "rope: table", at, torch.float32),
-                                len(table), _ptr(rows, N, "rope: rows", at, torch.int32), _code(xs[0], "rope"), _stream_handle(stream)), "rope")
+                                _i32(len(table), "rope: table"), _ptr(rows, N, "rope: rows", at, torch.int32), _code(xs[0], "rope"), _stream_handle(stream)), "rope")
         return out
 
 
