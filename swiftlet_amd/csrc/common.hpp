@@ -141,6 +141,13 @@ __device__ __forceinline__ float wave_sum(float v) { return segment_sum(v, kWave
 // __syncthreads would wait for them too).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Values that are in their registers before any branch that follows.  The compiler counts the wait states from a matrix
+// instruction to the first use of its result over the branch's longer way alone where both meet again, and on the
+// shorter one the last elements were used before they were there (errors of 1e-4 now and then).  For the first values that
+// are made of a result, where a branch follows.
+typedef float matrix_f4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void here(matrix_f4_t &v) { asm volatile("" : "+v"(v)); }
+
 __device__ __forceinline__ float wave_max(float v) {
     for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
     return v;

@@ -28,6 +28,9 @@
 // a chunk on: outputs of that token and all after it are, and S is from the chunk's end on, as a whole where
 // one value alone would spoil its row.  Queries reach their own token's outputs alone and need nothing.
 //
+// No branch stands between a matrix instruction and its result's first use (see `here`): chunks that do not exist are
+// loaded as the last one again.
+//
 // Layout.  A matrix instruction's result has a lane's 4 numbers in consecutive rows of one column; its operands have 8
 // numbers along the contraction.  The order of a contraction is free, so operands take the order in which two
 // results lie: position j of lane group g is element 16 (j / 4) + 4 g + j % 4 of 32.  Every result then is the next
@@ -75,12 +78,6 @@ struct DnChunks {
 
 __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4_t mfma4(float a, float b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-
-// Values that are in their registers before any branch that follows.  The compiler counts the wait states from a matrix
-// instruction to the first use of its result over the branch's longer way alone where both meet again, and on the
-// shorter one the last elements were used before they were there; so no branch stands between the two, and chunks
-// that do not exist are loaded as the last one again.
-__device__ __forceinline__ void here(f4_t &v) { asm volatile("" : "+v"(v)); }
 
 __device__ __forceinline__ void split4(f4_t x, h4_t &hi, h4_t &lo) {
     hi = __builtin_convertvector(x, h4_t);

@@ -721,6 +721,7 @@ __global__ __launch_bounds__(kPfThreads) void pf_gemm(const GemmArgs a) {
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[mt][j][r] = fmaf(sc[j], c[r], acc[mt][j][r]);
+                if constexpr (MT > 1) here(acc[mt][j]);
             }
         }
     };
@@ -1011,6 +1012,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(4)))
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[mt][j][r] = fmaf(sc[j], c[r], acc[mt][j][r]);
+                if constexpr (MT > 1) here(acc[mt][j]);
             }
         }
     };
