@@ -27,8 +27,9 @@ __device__ __forceinline__ float lds_sum_sq(const float *v, int n, int lane) {
 // the usual heads of 128 have.  Kernels shorter than that have zero weights in front, and zeros for the rows that meet
 // them, which change no bit of the sums.  ONE: no sequence brings more than a token, and the ring takes its row here (a
 // workgroup then overwrites no row that another still reads; with more tokens it would).  MANY: registers for two
-// workgroups to a CU, where there are more workgroups than CUs: 64 single tokens at 32 heads of 128 take 51 us instead of 56 (290
-// MB: 5.7 TB/s), 32 sequences of 4 55 instead of 69; one of 8 would take 29 instead of 27.
+// workgroups to a CU, where there are more workgroups than CUs: 64 single tokens at 32 heads of 128 take 51 us instead of 56
+// (the same states again, in part from the caches; 64 where they change, 4.3 TB/s), 32 sequences of 4 55 instead of 69; one of 8
+// would take 29 instead of 27.  Several tokens spill 4 registers so, 6 at dk 256.
 template <int DK, bool WIDE, bool ONE, bool MANY, typename T>
 __global__ __launch_bounds__(kTokThreads, MANY ? 4 : 2) void deltanet_tokens_kernel(const DnTokens a) {
     constexpr int C4 = DK / 4;          // float4 chunks per state row
@@ -252,11 +253,12 @@ int check_sizes(const swq_deltanet_layer *l, const swq_deltanet_batch *b) {
 int most_tokens(const swq_deltanet_batch *b) { return b->starts ? std::min(b->max_tokens, b->tokens) : b->tokens / b->sequences; }
 
 // From so many tokens of a sequence on, those of a batch go a chunk at a time; from more where workgroups are as many as
-// CUs, which token after token keeps busy.  At 32 value heads of 128, 1 sequence of 8 (12, 16) takes 28 us (38, 49) token after
-// token and 34 us in chunks, 4 of them 29 (38, 49) and 43, 8 of 16 (24) 50 (71) and 63, 32 of them 137 (195) and 164.
-constexpr int kChunksFrom = 12, kChunksFromMany = 20;
+// CUs, which token after token keeps busy.  At 32 value heads of 128 (bf16), 1 sequence of 8 (12, 16) takes 28 us (38, 49) token
+// after token and 34 us in chunks, 4 of them 28 (38, 47) and 46, 8 of 16 (24) 50 (71) and 67, 32 of them 138 (195) and 187 (196).
+constexpr int kChunksFrom = 12, kChunksFromMany = 24;
 // Beside a sequence of so many, those of up to kFew go token after token all the same, in launches of their own: with one of
-// 600 tokens, 31 of 1 (4) take 106 us (125) so and 199 (202) in chunks, but a single one of 1 65 and 59, of 8 87 and 60.
+// 600 tokens, 31 of 1 (4) take 116 us (134) so and 223 (232) in chunks, but a single one of 1 69 and 63, of 8 88 and 64.
+// Of 8 tokens 8 (31) would take 99 (162) so and 103 (239) in chunks, where they go: the rule does not count them.
 constexpr int kFew = 4;
 
 bool misaligned(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }

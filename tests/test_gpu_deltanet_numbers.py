@@ -28,6 +28,13 @@ def test_bf16_outputs_are_the_f32_ones_rounded(heads, lengths):
     assert torch.equal(c.states, states)
 
 
+@pytest.mark.parametrize("most", [23, 24])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_both_sides_of_where_many_go_in_chunks(most, dtype):
+    c = Batch(BIG, [most, 1, 5, 4, 2, 0, 18, 12, 13], dtype, split=True, seed=36)
+    close(c, c.run())
+
+
 def close(c, out):
     """Every row of every head over the size of its terms, every head's state over its own size."""
     want, _, rec = c.oracle()
