@@ -113,7 +113,9 @@ _OWN_STEP = AttentionGPU.step
 def attention_from_checkpoint(ckpt, layer: int, config: dict, max_positions: int = 4096, device="cuda",
                               stream=None) -> AttentionGPU:
     """Layer `layer`'s self_attn block from a checkpoint; rope settings as
-    QwenConfig reads them (QwenConfig.swift:80-88, :115)."""
+    QwenConfig reads them (QwenConfig.swift:80-88, :115): plain angles, also
+    where the config names a scaling (RopeGPU.from_config reads it, for
+    AttentionQ4GPU's rope_table)."""
     torch = _torch()
     p = f"model.layers.{layer}.self_attn."
     c = config.get("text_config", config)

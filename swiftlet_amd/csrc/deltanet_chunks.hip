@@ -48,9 +48,10 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDnChunk;
-// Chunks of a prompt alone that go through all launches before the next do, 200 MB of operands at 32 value heads of
-// 128, which the caches hold from one launch to the next.  4,096 (16,384) tokens: spans of 16 251 us (1,031), 32 221
-// (860), 64 245 (946), the whole prompt at once 245 (954).
+// Chunks of a prompt alone that go through all launches before the next do, 163 MB of operands at 16 key and 32 value heads
+// of 128, which the caches hold from one launch to the next.  4,096 (16,384) tokens: spans of 16 277 us (1,129), 32 251
+// (966), 64 303 (1,195), the whole prompt at once 303 (1,116).  It was found at these heads and does not follow others': 8
+// value heads of 128 bring 41 MB.
 constexpr int kSpan = 32;
 constexpr int kRowTiles = kC / 16;
 constexpr int kPrepThreads = 512;
@@ -117,7 +118,7 @@ __device__ __forceinline__ void mfma22(h8_t ah, h8_t al, h8_t bh, h8_t bl, Sum &
 // A power of two that brings m to 2^top .. 2^(top + 1), and its inverse; 1 where m is 0 or no number.
 __device__ __forceinline__ float scale_of(float m, int top, float &inverse) {
     int e = static_cast<int>((__float_as_uint(m) >> 23) & 255u);
-    e = e == 255 || !(m > 0.f) ? 127 : max(e - top, 1);
+    e = e == 255 || !(m > 0.f) ? 127 : min(max(e - top, 1), 253);
     inverse = __uint_as_float(static_cast<uint32_t>(e) << 23);
     return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
@@ -342,7 +343,7 @@ __device__ __forceinline__ void put_transposed(uint4 *to, int tile, int t0, int 
 }
 
 // One workgroup per (chunk, key head): waves 0 to 3 take a key tile of 16 tokens each, waves 4 to 7 a query tile; then
-// their products.  The gates of the key head's value heads beside it.  32 chunks of 16 heads of 128 take 17 us: one round of
+// their products.  The gates of the key head's value heads beside it.  32 chunks of 16 heads of 128 take 19 us: one round of
 // two workgroups to a CU, so what bounds it is its own chain of loads, convolution, norms and products.
 template <int DK, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const DnTokens a, const DnChunks w) {
@@ -471,8 +472,8 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_keys_kernel(const Dn
 }
 
 // One workgroup per (chunk, value head): waves 0 to 3 make A and T, waves 4 to 7 P and the values; then all W and U.  32 chunks of
-// 32 heads of 128 take 40 us: two rounds of two workgroups to a CU (128 registers; with 4 waves and twice the columns each
-// they spill: 53), 10 to 16 thousand clocks up to the inverted diagonal blocks, 5 for the others, 4 each for W and U.
+// 32 heads of 128 take 42 us: two rounds of two workgroups to a CU (128 registers, of which 10 to 17 are spilled, 50 to 57 with
+// kernels of 5 to 8 rows; 4 waves with twice the columns each spill more: 53 when this took 40), 10 to 16 thousand clocks up to the inverted diagonal blocks, 5 for the others, 4 each for W and U.
 template <int DK, int KM, typename T>
 __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const DnTokens a, const DnChunks w) {
     constexpr int KS = DK / 32, DT = DK / 16, N = kVBlock / 16;
@@ -711,9 +712,9 @@ __global__ __launch_bounds__(kPrepThreads, 4) void deltanet_solve_kernel(const D
 // One workgroup per (sequence, value head, CT * 16 columns of the state), three quarters of waves at three tasks: waves 0 to
 // 3 make d of a quarter of the chunk's tokens each, waves 4 to 7 the next state, of whose rows they hold a quarter each, and
 // waves 8 to 11 the outputs, off the chain from chunk to chunk.  While one kind computes, the others have their loads
-// and stores issued.  A chunk takes 1.2 us at 256 workgroups (its products and barriers alone 0.8): each reads its head's
-// operands for itself, 19 TB/s from the L2s in all, of 22 to 28 that loads alone reach.  Outputs in a launch of their own,
-// from S and d stored per chunk, took 145 us instead of 109 for 64 chunks.
+// and stores issued.  A chunk takes 1.4 us at 256 workgroups: each reads its head's operands for itself, 20 TB/s from the
+// L2s in all, of 22 to 28 that loads alone reach.  Outputs in a launch of their own, from S and d stored per chunk, took 145
+// us instead of 109 for 64 chunks (both with outputs of 11 bits, which are 22 now).
 template <int DK, int CT>
 __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const DnTokens a, const DnChunks w, int groups) {
     constexpr int KS = DK / 32, DT = DK / 64;  // DT: row tiles of the state per wave
@@ -959,7 +960,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void deltanet_chain_kernel(const 
 // One workgroup per (chunk, value head): the gated norm, and the ring's rows of a sequence's last chunk, also of one that has
 // gone token after token.  CW * 32 columns at
 // most, CW * 8 lanes of 4 columns to a token; the outputs come as the matrix instructions leave them, and through LDS.  32
-// chunks of 32 heads of 128 take 16 us for 34 MB: one round of workgroups, loads and stores in turn.
+// chunks of 32 heads of 128 take 18 us for 67 MB: one round of workgroups, loads and stores in turn.
 template <int CW, typename T>
 __global__ __launch_bounds__(kFinishThreads) void deltanet_finish_kernel(const DnTokens a, const DnChunks w) {
     constexpr int L = CW * 8, ROWS = kFinishThreads / L, R = kC / ROWS, kRow = CW * 32 + 4;
@@ -1079,7 +1080,7 @@ template <int DK>
 void launch_chain(const DnTokens &a, const DnChunks &w, hipStream_t s) {
     const int64_t units = (static_cast<int64_t>(a.B) * a.nk + 7) / 8 * 8 * a.rep;
     // 32 columns to a workgroup where those of 16 would not find a CU each: at 32 value heads of 128 four prompts of 2,500
-    // tokens in all take 138 us instead of 155, but one of 4,096 231 instead of 221
+    // tokens in all take 154 us instead of 178, but one of 4,096 257 instead of 244
     const int cts = a.dv / 16, ct = cts % 2 == 0 && static_cast<int64_t>(a.B) * a.nv * cts > kCus ? 2 : 1;
     const dim3 grid(static_cast<uint32_t>(units * (cts / ct))), block(kChainThreads);
     if (ct == 1) hipLaunchKernelGGL((deltanet_chain_kernel<DK, 1>), grid, block, 0, s, a, w, cts / ct);
